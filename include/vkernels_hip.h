@@ -665,6 +665,85 @@ int vk_hip_dequant_weight_tile(const uint8_t* packed, const uint8_t* scale,
                                int32_t stride_scale_n, int32_t stride_scale_k,
                                int32_t fast, void* stream);
 
+/* ---- The key-value cache of a decode step (additive) --------------------------------
+ *
+ * A paged cache: k_cache and v_cache [num_pages, Hkv, page_size, D] with D values of a
+ * position in a row (contiguous) and strides in elements for the other three, the same
+ * for both; block_table [B, table_width] int32 (rows table_stride apart) names the page
+ * of every page_size positions of a sequence, seq_lens [B] int32 how many it has.
+ * Position j of sequence b is slot j % page_size of page block_table[b][j / page_size].
+ * An entry outside [0, num_pages) is no page: nothing is written there, and the attention
+ * leaves its positions out.  Pages may be of any size; what is stored at positions beyond
+ * a sequence's length may be anything, NaN included.
+ *
+ * D is a multiple of 16 up to 256, rows start on 16 bytes (base addresses and strides),
+ * query heads Hq = G * Hkv, heads G g .. G g + G - 1 share key/value head g.
+ */
+enum {
+  VK_HIP_KV_BF16 = 0,     /* bf16 cache, bf16 queries and results */
+  VK_HIP_KV_F16 = 1,      /* fp16 cache, fp16 queries and results */
+  VK_HIP_KV_FP8_BF16 = 2, /* E4M3 cache (value = code * scale of its head), bf16 queries and results */
+  VK_HIP_KV_FP8_F16 = 3   /* the same with fp16 queries and results */
+};
+
+/* New rows into the cache.  k, v [tokens, Hkv, D] in the query type, strides in elements.
+ * seq_lens count the new tokens.  query_start [B + 1] int32: the new tokens of sequence b
+ * are query_start[b] .. query_start[b + 1] - 1 and go to its last positions; NULL: one
+ * token for each sequence (tokens == B; a sequence of length 0 takes none).  Positions
+ * outside the table are skipped.  8-bit caches: the code nearest to value / scale[head]
+ * (ties to even), the largest finite one beyond +-448; k_scale, v_scale [Hkv], NULL for
+ * the other kinds. */
+int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_cache,
+                           const int32_t* block_table, const int32_t* seq_lens,
+                           const int32_t* query_start, const float* k_scale, const float* v_scale,
+                           int kind, int B, int tokens, int Hkv, int D, int num_pages, int page_size,
+                           int table_width, int table_stride, int64_t k_stride_t, int64_t k_stride_h,
+                           int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
+                           int64_t head_stride, int64_t slot_stride, void* stream);
+
+/* Attention of one new token of every sequence over its cache: q [B, Hq, D] (strides in
+ * elements), out [B, Hq, D] contiguous, lse [B, Hq] fp32 or NULL.
+ *   s_j = scale * k_scale[g] * q_h . k_j, then softcap * tanh(s_j / softcap) if softcap > 0,
+ *   over the positions j in [max(0, L - window), L) (window <= 0: from 0), L = seq_lens[b]
+ *   cut to max_len;  Z = sum_j e^{s_j} + e^{sinks[h]} (sinks [Hq] or NULL),
+ *   out_h = v_scale[g] * sum_j e^{s_j} v_j / Z,  lse_h = log Z.
+ * A row that nothing is left of, or whose every score is -inf, gives 0 and lse -inf (the
+ * sink, where there is one).  weight_sums (or NULL): element [b][g][j] (strides in elements)
+ * grows by the sum over the heads h of g of e^{s_j} / Z.  max_len: at least every length,
+ * at most table_width * page_size; launches and workspace follow it, not the lengths.
+ * The workspace (16-byte aligned) of vk_hip_paged_attention_workspace_bytes is scratch of
+ * this call alone; 0 bytes: none is needed.  Deterministic: no atomics. */
+size_t vk_hip_paged_attention_workspace_bytes(int B, int Hkv, int G, int D, int max_len, int window,
+                                              int counted);
+int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cache,
+                           const int32_t* block_table, const int32_t* seq_lens, const float* sinks,
+                           const float* k_scale, const float* v_scale, void* out, float* lse,
+                           float* weight_sums, int kind, int B, int Hkv, int G, int D, int num_pages,
+                           int page_size, int table_width, int table_stride, int max_len, int window,
+                           float scale, float softcap, int64_t q_stride_b, int64_t q_stride_h,
+                           int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                           int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Eviction: a sequence of more than `budget` positions (its length cut to max_len) keeps
+ * its first keep_first and last keep_last positions and of the others the
+ * budget - keep_first - keep_last with the largest weight_sums, in every key/value head by
+ * itself (NaN counts as largest, ties go to the lowest position).  Their rows move, in
+ * order, to positions 0 .. budget - 1 of the same pages, in place; rows beyond stay as
+ * they are.  sums_out [B, Hkv, positions] gets the kept sums, and 0 from budget up to the
+ * old length; it is weight_sums itself (with its strides) or an array that does not
+ * overlap it.  new_lens [B] = min(length, budget); kept [B, Hkv, budget] int32 the old
+ * positions in order, -1 beyond the new length.  A shorter sequence keeps all it has
+ * (its sums are copied).  The pages of a sequence that is cut have to be its own.
+ * elem_bytes: 1 or 2, a value of the cache. */
+int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
+                          const int32_t* seq_lens, const float* weight_sums, float* sums_out,
+                          int32_t* new_lens, int32_t* kept, int elem_bytes, int B, int Hkv, int D,
+                          int num_pages, int page_size, int table_width, int table_stride, int max_len,
+                          int budget, int keep_first, int keep_last, int64_t page_stride,
+                          int64_t head_stride, int64_t slot_stride, int64_t sums_stride_b,
+                          int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,7 +26,7 @@ LIB = PKG / "libvkernels_hip.so"
 
 SOURCES = ["moe_route.hip", "moe_align.hip", "moe_dequant.hip", "moe_gemm.hip", "moe_prefill.hip", "static_scratch.hip",
            "moe_tuning.cpp", "moe_stages.hip",
-           "hip_capi.cpp"]
+           "hip_capi.cpp", "paged_attention.hip", "kv_cache.hip", "kv_capi.cpp"]
 
 # -packed-fp32-ops off: hipcc must not form packed fp32 arithmetic.
 # No fast-math: the router relies on IEEE division and un-contracted arithmetic.

@@ -1,0 +1,776 @@
+// paged_attention.hip — the attention of one new token over a paged key-value cache.
+//
+// For a query head h on key/value head g and the positions j that it sees,
+//   s_j = scale k_scale_g q_h . k_j   (c tanh(s_j / c) with a softcap c),
+//   out_h = v_scale_g (sum_j e^{s_j} v_j) / (sum_j e^{s_j} + e^{sink_h}),
+// in one pass over keys and values: a running reference m (at least the maximum less 8 in
+// powers of two), the sum of 2^{s log2 e - m} and the weighted sum of the values, both
+// rescaled when m rises; partial results with references m_p join as sum_p 2^{m_p - m} (.).
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "paged_attention.hpp"
+
+namespace vk {
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_inff();
+// The reference of the exponentials is moved when the scores pass it by more than 2^8: weights of
+// up to 256 cost no accuracy, and few tiles then have to rescale what they have summed.
+constexpr float kSlack = 8.0f;
+
+// The 16-bit type that the matrix instructions multiply in.
+struct Bf16 {
+  typedef __bf16 T;
+  typedef __attribute__((ext_vector_type(8))) __bf16 V8;
+  typedef __attribute__((ext_vector_type(2))) __bf16 V2;
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ V2 of_fp8(uint32_t codes, bool high) {
+    return high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true)
+                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false);
+  }
+};
+struct F16 {
+  typedef _Float16 T;
+  typedef __attribute__((ext_vector_type(8))) _Float16 V8;
+  typedef __attribute__((ext_vector_type(2))) _Float16 V2;
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ V2 of_fp8(uint32_t codes, bool high) {
+    return high ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true)
+                : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false);
+  }
+};
+
+template <class M>
+__device__ __forceinline__ typename M::V8 as_v8(u32x4 x) {
+  union { u32x4 u; typename M::V8 v; } c;
+  c.u = x;
+  return c.v;
+}
+
+// 8 E4M3 codes -> 8 values (exact in either type).
+template <class M>
+__device__ __forceinline__ typename M::V8 fp8x8(uint32_t lo, uint32_t hi) {
+  union { typename M::V2 p[4]; typename M::V8 v; } c;
+  c.p[0] = M::of_fp8(lo, false);
+  c.p[1] = M::of_fp8(lo, true);
+  c.p[2] = M::of_fp8(hi, false);
+  c.p[3] = M::of_fp8(hi, true);
+  return c.v;
+}
+
+// Maximum / sum over the four lanes l % 16, + 16, + 32, + 48 that hold a head's column.
+__device__ __forceinline__ float over_column_max(float x) {
+  const uint32_t u = __float_as_uint(x);
+  u32x2 s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+  s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float over_column_sum(float x) {
+  const uint32_t u = __float_as_uint(x);
+  u32x2 s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+  s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// log of a row's sum ll 2^ref (a sink alone is handed back as it is).
+__device__ __forceinline__ float log_of_sum(float ref, float ll, const float* sink) {
+  if (ll == 0.0f) return kNegInf;
+  if (sink != nullptr && ll == 1.0f && ref == *sink * kLog2e) return *sink;
+  return ref * kLn2 + logf(ll);
+}
+__device__ __forceinline__ float or_zero(float m) { return m == kNegInf ? 0.0f : m; }
+
+// What a work item (16 heads of one sequence) sees of its cache.
+struct Span {
+  int start;   // first position, rounded down to 16
+  int lo, len; // positions [lo, len)
+  int units;   // of kPaUnit positions from `start`; at least one
+};
+__device__ __forceinline__ Span span_of(int len, int max_len, int window) {
+  Span s;
+  s.len = min(max(len, 0), max_len);
+  s.lo = window > 0 ? max(0, s.len - window) : 0;
+  s.start = s.lo & ~15;
+  s.units = max(1, (s.len - s.start + kPaUnit - 1) / kPaUnit);
+  return s;
+}
+
+struct KernelArgs {
+  PagedAttentionArgs a;
+  PagedAttentionPlan p;
+  uint32_t page_magic;   // position / page_size = (position * magic) >> (32 + shift)
+  int page_shift;        // -1: pages of one position
+};
+
+__device__ __forceinline__ int page_of(const KernelArgs& A, int pos) {
+  return A.page_shift < 0 ? pos : (int)(__umulhi((uint32_t)pos, A.page_magic) >> A.page_shift);
+}
+
+// The units of all items in order (sequence, head item, unit), cut into equal shares.
+struct Share {
+  int first, last;   // units of this workgroup
+  int per;           // units of a share
+  int b, unit0;      // the sequence that `first` lies in, and its first unit
+};
+
+// Every workgroup finds its share by itself from the lengths: a thread adds up the units
+// of B / 256 sequences, a scan over the threads, and the thread that holds `first` walks on.
+__device__ bool find_share(const KernelArgs& A, Share* sh, int* lds) {
+  const PagedAttentionArgs& a = A.a;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int heads = a.Hkv * A.p.head_tiles;
+  const int per = (a.B + 255) / 256;
+  int mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int b = t * per + i;
+    if (b < a.B) mine += span_of(a.lens[b], a.max_len, a.window).units;
+  }
+  int scan = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int up = __shfl_up(scan, d);
+    if (lane >= d) scan += up;
+  }
+  if (lane == 63) lds[wave] = scan;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kPaWaves; ++w) {
+    if (w < wave) before += lds[w];
+    total += lds[w];
+  }
+  total *= heads;
+  const int share = max(A.p.min_units, (total + A.p.workgroups - 1) / A.p.workgroups);
+  const int first = (int)blockIdx.x * share;
+  if (first >= total) return false;   // (uniform over the workgroup)
+  int at = (before + scan - mine) * heads;
+  if (first >= at && first < at + mine * heads) {
+    int b = t * per;
+    for (;; ++b) {
+      const int units = span_of(a.lens[b], a.max_len, a.window).units * heads;
+      if (first < at + units) break;
+      at += units;
+    }
+    lds[4] = b;
+    lds[5] = at;
+  }
+  __syncthreads();
+  sh->first = first;
+  sh->last = min(total, first + share);
+  sh->per = share;
+  sh->b = lds[4];
+  sh->unit0 = lds[5];
+  return true;
+}
+
+template <class M, bool FP8, int DP>
+struct Tile {
+  static constexpr int kElem = FP8 ? 1 : 2;
+  static constexpr int kRowBytes = DP * kElem;
+  // 16-byte pieces of a value row, rounded up to a power of two: lanes that load a row
+  static constexpr int kPieces = kRowBytes <= 64 ? 4 : kRowBytes <= 128 ? 8 : kRowBytes <= 256 ? 16 : 32;
+  static constexpr int kRowsPerLoad = 64 / kPieces;
+  static constexpr int kVLoads = kPaWaveRows / kRowsPerLoad;
+  static constexpr int kPitch = kPieces * 16;            // bytes of a row in LDS
+  static constexpr int kKLoads = kRowBytes / 64;         // 64 bytes of 16 rows each
+  static constexpr int kSteps = DP / 32;                 // MFMAs over the head's width
+  static constexpr int kOutPitch = DP + 4;               // floats of a head's sums in LDS
+  static constexpr int kWaveLds = kPaWaveRows * kPitch > kPaHeads * kOutPitch * 4
+                                      ? kPaWaveRows * kPitch : kPaHeads * kOutPitch * 4;
+};
+
+template <class M, bool FP8, int DP, bool P16>
+__global__ __launch_bounds__(256) void paged_attention_kernel(const KernelArgs A) {
+  typedef Tile<M, FP8, DP> L;
+  typedef typename M::V8 V8;
+  const PagedAttentionArgs& a = A.a;
+  __shared__ __attribute__((aligned(16))) char lds[kPaWaves * L::kWaveLds];
+  __shared__ float wave_m[kPaWaves][kPaHeads], wave_l[kPaWaves][kPaHeads];
+  __shared__ int share_lds[8];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int item_heads = a.Hkv * A.p.head_tiles;
+  char* const my_lds = lds + wave * L::kWaveLds;
+
+  Share sh;
+  int item_in_b = 0;
+  if (A.p.workgroups > 0) {
+    if (!find_share(A, &sh, share_lds)) return;
+  } else {
+    sh.first = 0;
+    sh.b = blockIdx.x / item_heads;
+    item_in_b = blockIdx.x % item_heads;
+  }
+  Span span = span_of(a.lens[sh.b], a.max_len, a.window);
+  int unit_at;         // unit of the item that the segment begins with
+  int left;            // units of the share that are left
+  if (A.p.workgroups > 0) {
+    const int in_b = sh.first - sh.unit0;
+    item_in_b = in_b / span.units;
+    unit_at = in_b % span.units;
+    left = sh.last - sh.first;
+  } else {
+    unit_at = 0;
+    left = span.units;
+  }
+  int b = sh.b;
+  int item_unit0 = A.p.workgroups > 0 ? sh.first - unit_at : 0;   // the item's first unit
+
+  const int64_t slot_bytes = a.slot_stride * L::kElem, page_bytes = a.page_stride * L::kElem;
+  while (left > 0) {
+    const int units = min(left, span.units - unit_at);
+    const int g = item_in_b / A.p.head_tiles, head0 = (item_in_b % A.p.head_tiles) * kPaHeads;
+    const int heads = min(kPaHeads, a.G - head0);
+    const int32_t* const pages = a.table + (int64_t)b * a.table_stride;
+    const char* const kbase = (const char*)a.k_cache + (int64_t)g * a.head_stride * L::kElem;
+    const char* const vbase = (const char*)a.v_cache + (int64_t)g * a.head_stride * L::kElem;
+
+    // The queries as the MFMA's second operand: lane (col, quad) holds head col and, of
+    // every 32 values, the 8 at 8 quad (of an 8-bit cache: of every 64 the 16 at 16 quad,
+    // in two operands; the keys below are dealt out alike).
+    V8 q[L::kSteps];
+    {
+      const char* row = (const char*)a.q + ((int64_t)b * a.q_stride_b + (int64_t)(g * a.G + head0 + col) * a.q_stride_h) * 2;
+#pragma unroll
+      for (int i = 0; i < L::kSteps; ++i) {
+        const int d = FP8 ? (i / 2) * 64 + quad * 16 + (i % 2) * 8 : i * 32 + quad * 8;
+        u32x4 x = {0, 0, 0, 0};
+        if (col < heads && d < a.D) x = *(const u32x4*)(row + d * 2);
+        q[i] = as_v8<M>(x);
+      }
+    }
+    const float k_scale = a.k_scale != nullptr ? a.k_scale[g] : 1.0f;
+    const float to_log2 = a.scale * k_scale * kLog2e;
+    const float cap_in = a.softcap > 0.0f ? 2.0f * a.scale * k_scale * kLog2e / a.softcap : 0.0f;
+    const float cap_out = a.softcap * kLog2e;
+
+    f32x4 acc[DP / 16];
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    float m = kNegInf, l = 0.0f;
+
+    u32x4 kreg[2][L::kKLoads], vreg[L::kVLoads];
+    // Of the tile that is loaded: which positions count (one page id per 16 positions where
+    // pages are multiples of 16 long, else one per lane).
+    int page0 = -1, page1 = -1;      // P16
+    int64_t row_at = 0;              // else: bytes from the cache's start to position lane % 32
+    bool row_ok = false;
+
+    const int begin = span.start + unit_at * kPaUnit + wave * kPaWaveRows;
+    const int end = span.start + (unit_at + units) * kPaUnit;
+
+    auto find_pages = [&](int pos0) {
+      if constexpr (P16) {
+        const int i0 = page_of(A, pos0), i1 = page_of(A, pos0 + 16);
+        page0 = pos0 < span.len ? pages[i0] : -1;
+        page1 = pos0 + 16 < span.len ? pages[i1] : -1;
+        if ((uint32_t)page0 >= (uint32_t)a.num_pages) page0 = -1;
+        if ((uint32_t)page1 >= (uint32_t)a.num_pages) page1 = -1;
+      } else {
+        const int pos = pos0 + (lane & 31);
+        row_ok = pos >= span.lo && pos < span.len;
+        int page = 0, in_table = 0;
+        if (row_ok) {
+          in_table = page_of(A, pos);
+          page = pages[in_table];
+          row_ok = (uint32_t)page < (uint32_t)a.num_pages;
+          if (!row_ok) page = 0;
+        }
+        row_at = row_ok ? (int64_t)page * page_bytes + (int64_t)(pos - in_table * a.page_size) * slot_bytes : 0;
+      }
+    };
+    // Where a row of the loaded tile lies (generic pages), from the lane that looked it up.
+    auto row_from = [&](int row) -> int64_t {
+      const int lo = __shfl((int)(uint32_t)row_at, row);
+      const int hi = __shfl((int)(row_at >> 32), row);
+      return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+    };
+    auto load_k = [&](int pos0) {
+      if constexpr (P16) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int p0 = pos0 + 16 * t;
+          const int page = max(t == 0 ? page0 : page1, 0);
+          const int slot = t == 0 ? p0 - page_of(A, p0) * a.page_size : p0 - page_of(A, p0) * a.page_size;
+          const char* base = kbase + (int64_t)page * page_bytes + (int64_t)slot * slot_bytes;
+          const uint32_t at = (uint32_t)col * (uint32_t)slot_bytes + quad * 16;
+#pragma unroll
+          for (int i = 0; i < L::kKLoads; ++i) {
+            u32x4 x = {0, 0, 0, 0};
+            if (DP * L::kElem == a.D * L::kElem || i * 64 + quad * 16 < a.D * L::kElem)
+              x = *(const u32x4*)(base + at + i * 64);
+            kreg[t][i] = x;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const char* base = kbase + row_from(16 * t + col) + quad * 16;
+#pragma unroll
+          for (int i = 0; i < L::kKLoads; ++i) {
+            u32x4 x = {0, 0, 0, 0};
+            if (i * 64 + quad * 16 < a.D * L::kElem) x = *(const u32x4*)(base + i * 64);
+            kreg[t][i] = x;
+          }
+        }
+      }
+    };
+    auto load_v = [&](int pos0) {
+      const int piece = lane % L::kPieces, sub = lane / L::kPieces;
+      const bool mine = piece * 16 < a.D * L::kElem;
+      if constexpr (P16) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int p0 = pos0 + 16 * t;
+          const int page = max(t == 0 ? page0 : page1, 0);
+          const int slot = p0 - page_of(A, p0) * a.page_size;
+          const char* base = vbase + (int64_t)page * page_bytes + (int64_t)slot * slot_bytes;
+#pragma unroll
+          for (int i = 0; i < L::kVLoads / 2; ++i) {
+            const uint32_t at = (uint32_t)(i * L::kRowsPerLoad + sub) * (uint32_t)slot_bytes + piece * 16;
+            u32x4 x = {0, 0, 0, 0};
+            if (mine) x = *(const u32x4*)(base + at);
+            vreg[t * (L::kVLoads / 2) + i] = x;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < L::kVLoads; ++i) {
+          const char* base = vbase + row_from(i * L::kRowsPerLoad + sub) + piece * 16;
+          u32x4 x = {0, 0, 0, 0};
+          if (mine) x = *(const u32x4*)base;
+          vreg[i] = x;
+        }
+      }
+    };
+
+    if (begin < end) {
+      find_pages(begin);
+      load_k(begin);
+      load_v(begin);
+    }
+    for (int pos0 = begin; pos0 < end; pos0 += kPaUnit) {
+      const bool more = pos0 + kPaUnit < end;
+      // which of the 8 positions of this lane count, and which value rows it loaded do
+      bool whole;
+      uint32_t rows;        // bit r: position pos0 + r counts
+      if constexpr (P16) {
+        whole = pos0 >= span.lo && pos0 + 32 <= span.len && page0 >= 0 && page1 >= 0;
+        rows = 0xFFFFFFFFu;
+        if (!whole) {
+          if (page0 < 0) rows &= 0xFFFF0000u;
+          if (page1 < 0) rows &= 0x0000FFFFu;
+          const int n = span.len - pos0, skip = span.lo - pos0;
+          if (n < 32) rows &= n <= 0 ? 0u : (1u << n) - 1u;
+          if (skip > 0) rows &= skip >= 32 ? 0u : ~0u << skip;
+        }
+      } else {
+        rows = (uint32_t)__ballot(row_ok);
+        whole = rows == 0xFFFFFFFFu;
+      }
+
+      f32x4 s[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s[t] = f32x4{0, 0, 0, 0};
+        if constexpr (FP8) {
+#pragma unroll
+          for (int i = 0; i < L::kKLoads; ++i) {
+            s[t] = M::mfma(fp8x8<M>(kreg[t][i][0], kreg[t][i][1]), q[2 * i], s[t]);
+            s[t] = M::mfma(fp8x8<M>(kreg[t][i][2], kreg[t][i][3]), q[2 * i + 1], s[t]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < L::kKLoads; ++i) s[t] = M::mfma(as_v8<M>(kreg[t][i]), q[i], s[t]);
+        }
+      }
+      if (more) {
+        find_pages(pos0 + kPaUnit);
+        load_k(pos0 + kPaUnit);
+      }
+
+      // scores in powers of two
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[t * 4 + r] = s[t][r];
+      if (a.softcap > 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          // c tanh(y / c) = c (1 - 2 / (1 + e^{2 y / c})), and y (1 - z^2 / 3 + 2 z^4 / 15) with
+          // z = y / c below 0.1, where the first form cancels
+          const float z2 = x[i] * cap_in;                       // 2 y / c, in powers of two
+          const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(z2));
+          const float z = z2 * (0.5f * kLn2), zz = z * z;
+          const float small = z * (1.0f - zz * (0.33333334f - zz * 0.13333334f));
+          x[i] = cap_out * (fabsf(z) < 0.1f ? small : big);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= to_log2;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((rows >> (t * 16 + quad * 4 + r)) & 1u)) x[t * 4 + r] = kNegInf;
+      }
+      if (A.p.score_pitch > 0 && col < heads) {
+        float* to = (float*)((char*)a.workspace + A.p.scores_at) +
+                    ((int64_t)(b * a.Hkv + g) * a.G + head0 + col) * A.p.score_pitch + pos0 + quad * 4;
+        if (pos0 + quad * 4 < span.len) *(f32x4*)to = f32x4{x[0], x[1], x[2], x[3]};
+        if (pos0 + 16 + quad * 4 < span.len) *(f32x4*)(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+      top = over_column_max(top);
+      if (__any(top > m + kSlack)) {
+        const float m_new = fmaxf(m, top);
+        const float fix = exp2_fast(m - or_zero(m_new));
+        m = m_new;
+        l *= fix;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) acc[i] *= fix;
+      }
+      const float ref = or_zero(m);
+      // The weights as two 16-bit terms: 16 bits of each weight instead of 8 (the matrix
+      // cores idle otherwise), so that the result is off by its own rounding alone.
+      union { typename M::T e[8]; V8 v; } hi, lo;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p = exp2_fast(x[i] - ref);
+        l += p;
+        hi.e[i] = (typename M::T)p;
+        lo.e[i] = (typename M::T)(p - (float)hi.e[i]);
+      }
+
+      // The values to LDS, row after row (rows that do not count as zeros: what is stored
+      // there may be anything), 32-byte pairs of pieces exchanged by the row so that the
+      // transposed reads below spread over the banks.
+      {
+        const int piece = lane % L::kPieces, sub = lane / L::kPieces;
+#pragma unroll
+        for (int i = 0; i < L::kVLoads; ++i) {
+          const int row = i * L::kRowsPerLoad + sub;
+          if (!whole && !((rows >> row) & 1u)) vreg[i] = u32x4{0, 0, 0, 0};
+          const int turn = FP8 ? (L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 7 & (L::kPieces - 1) : 0)
+                               : 2 * (L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 3 : 0);
+          *(u32x4*)(my_lds + row * L::kPitch + ((piece ^ turn) * 16)) = vreg[i];
+        }
+      }
+      if (more) load_v(pos0 + kPaUnit);
+      // (lanes read what other lanes of their wavefront wrote: LDS keeps the order, and so must the compiler)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+
+      // Weighted values, transposed: rows of the result are the head's width, columns the
+      // heads.  Lane (col, quad) reads value col of every 16 of the positions 4 quad + (0..3)
+      // and 16 + 4 quad + (0..3): the order in which the scores' tile left the weights.
+      if constexpr (FP8) {
+        const int r8 = col >> 1, row = (r8 < 4 ? 0 : 12) + quad * 4 + r8;
+        const int turn = L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 7 & (L::kPieces - 1) : 0;
+        const int at = row * L::kPitch + (col & 1) * 8;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(my_lds + at + ((i ^ turn) * 16)));
+          const V8 v = fp8x8<M>((uint32_t)c[0], (uint32_t)c[1]);
+          acc[i] = M::mfma(v, hi.v, acc[i]);
+          acc[i] = M::mfma(v, lo.v, acc[i]);
+        }
+      } else {
+        const int row = quad * 4 + (col >> 2);
+        const int turn = L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 3 : 0;
+        const int at = row * L::kPitch + (col & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          union { i16x4 h[2]; V8 v; } c;
+          char* const from = my_lds + at + ((i ^ turn) * 32);
+          c.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)from);
+          c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) i16x4*)(from + 16 * L::kPitch));
+          acc[i] = M::mfma(c.v, hi.v, acc[i]);
+          acc[i] = M::mfma(c.v, lo.v, acc[i]);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+
+    // The four wavefronts' sums, joined in LDS.
+    l = over_column_sum(l);
+    if (quad == 0) {
+      wave_m[wave][col] = m;
+      wave_l[wave][col] = l;
+    }
+    if (col < heads) {
+      float* to = (float*)my_lds + col * L::kOutPitch + quad * 4;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) *(f32x4*)(to + i * 16) = acc[i];
+    }
+    __syncthreads();
+    const int item = b * item_heads + item_in_b;
+    const bool begins = unit_at == 0, ends = unit_at + units == span.units;
+    const bool alone = begins && ends;
+    int64_t* const meta = (int64_t*)((char*)a.workspace + A.p.meta_at);
+    if (A.p.workgroups > 0 && begins && threadIdx.x == 0) {
+      const int count = (item_unit0 + span.units - 1) / sh.per - (int)blockIdx.x + 1;
+      meta[item] = ((int64_t)count << 32) | blockIdx.x;
+    }
+    const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
+    const int pairs = a.D / 4;
+    for (int e = threadIdx.x; e < heads * pairs; e += 256) {
+      const int h = e / pairs, d = (e - h * pairs) * 4;
+      float mm = kNegInf;
+#pragma unroll
+      for (int w = 0; w < kPaWaves; ++w) mm = fmaxf(mm, wave_m[w][h]);
+      const int hq = g * a.G + head0 + h;
+      // (a sink is one more score whose value is zero)
+      const float sink = alone && a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
+      mm = fmaxf(mm, sink);
+      const float ref = or_zero(mm);
+      float ll = exp2_fast(sink - ref);
+      f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kPaWaves; ++w) {
+        const float f = exp2_fast(wave_m[w][h] - ref);
+        ll += wave_l[w][h] * f;
+        o += f * *(const f32x4*)((float*)(lds + w * L::kWaveLds) + h * L::kOutPitch + d);
+      }
+      if (alone) {
+        const float inv = (ll == 0.0f ? 0.0f : 1.0f / ll) * (a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
+        typename M::T* to = (typename M::T*)a.out + ((int64_t)b * a.Hkv * a.G + hq) * a.D + d;
+        union { typename M::T e[4]; u32x2 u; } r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r.e[j] = (typename M::T)(o[j] * inv);
+        *(u32x2*)to = r.u;
+        if (d == 0) {
+          if (a.lse != nullptr) a.lse[(int64_t)b * a.Hkv * a.G + hq] = log_of_sum(ref, ll, a.sinks != nullptr ? a.sinks + hq : nullptr);
+          if (A.p.score_pitch > 0)
+            ((f32x2*)((char*)a.workspace + A.p.stats_at))[(int64_t)b * a.Hkv * a.G + hq] = f32x2{ref, ll};
+        }
+      } else {
+        float* part = (float*)((char*)a.workspace + A.p.part_at) + ((int64_t)slot * kPaHeads + h) * DP + d;
+        *(f32x4*)part = o;
+        if (d == 0) ((f32x2*)((char*)a.workspace + A.p.ml_at))[slot * kPaHeads + h] = f32x2{mm, ll};
+      }
+    }
+
+    left -= units;
+    item_unit0 += span.units;
+    unit_at = 0;
+    if (left > 0 && ++item_in_b == item_heads) {
+      item_in_b = 0;
+      ++b;
+      span = span_of(a.lens[b], a.max_len, a.window);
+    }
+    if (left > 0) __syncthreads();   // (the sums are read before the next item's values come)
+  }
+}
+
+// Reference and sum of a head over the partial results of its item, the sink included; every
+// lane of the wavefront gets them.  `first`: the workgroup whose share begins the item.
+__device__ __forceinline__ f32x2 joined_stats(const f32x2* ml, int first, int count, int h, float sink) {
+  const int lane = threadIdx.x & 63;
+  float m = sink;
+  for (int p = lane; p < count; p += 64) m = fmaxf(m, ml[(2 * (first + p) + (p == 0 ? 1 : 0)) * kPaHeads + h][0]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+  const float ref = or_zero(m);
+  float l = lane == 0 ? exp2_fast(sink - ref) : 0.0f;
+  for (int p = lane; p < count; p += 64) {
+    const f32x2 x = ml[(2 * (first + p) + (p == 0 ? 1 : 0)) * kPaHeads + h];
+    l += x[1] * exp2_fast(x[0] - ref);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  return f32x2{ref, l};
+}
+
+// Joins the items that several workgroups had a share of (a workgroup per head: blocks below
+// `join_blocks`) and adds up the weights that the positions received (the other blocks: 1024
+// positions of a key/value head each).
+template <class M>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const KernelArgs A, int padded, int join_blocks,
+                                                                   int chunks) {
+  const PagedAttentionArgs& a = A.a;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t* const meta = (const int64_t*)((const char*)a.workspace + A.p.meta_at);
+  const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at);
+  const int Hq = a.Hkv * a.G;
+  __shared__ float o_lds[kPaWaves][256];
+  __shared__ f32x2 stats[64];
+  if ((int)blockIdx.x < join_blocks) {
+    const int b = blockIdx.x / Hq, hq = blockIdx.x % Hq;
+    const int g = hq / a.G, hg = hq % a.G, h = hg % kPaHeads;
+    const int64_t mt = meta[((int64_t)b * a.Hkv + g) * A.p.head_tiles + hg / kPaHeads];
+    const int first = (int)(uint32_t)mt, count = (int)(mt >> 32);
+    if (count <= 1) return;
+    const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
+    const f32x2 st = joined_stats(ml, first, count, h, sink);
+    const float* const part = (const float*)((const char*)a.workspace + A.p.part_at) + (int64_t)h * padded;
+    f32x4 o = {0, 0, 0, 0};
+    // a wavefront takes every fourth partial result; a lane four of up to 256 values
+    if (lane * 4 < a.D) {
+#pragma unroll 4
+      for (int p = wave; p < count; p += kPaWaves) {
+        const int slot = 2 * (first + p) + (p == 0 ? 1 : 0);
+        const float f = exp2_fast(ml[slot * kPaHeads + h][0] - st[0]);
+        o += f * *(const f32x4*)(part + (int64_t)slot * kPaHeads * padded + lane * 4);
+      }
+      *(f32x4*)&o_lds[wave][lane * 4] = o;
+    }
+    __syncthreads();
+    const float inv = (st[1] == 0.0f ? 0.0f : 1.0f / st[1]) * (a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
+    const int d = threadIdx.x;
+    if (d < a.D) {
+      const float sum = (o_lds[0][d] + o_lds[1][d]) + (o_lds[2][d] + o_lds[3][d]);
+      ((typename M::T*)a.out)[((int64_t)b * Hq + hq) * a.D + d] = (typename M::T)(sum * inv);
+    }
+    if (threadIdx.x == 0 && a.lse != nullptr)
+      a.lse[(int64_t)b * Hq + hq] = log_of_sum(st[0], st[1], a.sinks != nullptr ? a.sinks + hq : nullptr);
+    return;
+  }
+  const int block = blockIdx.x - join_blocks;
+  const int bg = block / chunks, b = bg / a.Hkv, g = bg % a.Hkv;
+  const Span span = span_of(a.lens[b], a.max_len, a.window);
+  const int at = span.start + (block % chunks) * kPaSumsChunk;
+  if (at >= span.len) return;
+  const int pos = at + threadIdx.x * 4;
+  const float* const scores = (const float*)((const char*)a.workspace + A.p.scores_at) +
+                              (int64_t)bg * a.G * A.p.score_pitch + pos;
+  float sum[4] = {0, 0, 0, 0};
+  for (int h0 = 0; h0 < a.G; h0 += 64) {
+    const int n = min(64, a.G - h0);
+    __syncthreads();
+    for (int i = wave; i < n; i += kPaWaves) {
+      const int hg = h0 + i, hq = g * a.G + hg;
+      const int64_t mt = A.p.workgroups > 0 ? meta[(int64_t)bg * A.p.head_tiles + hg / kPaHeads] : 0;
+      const int first = (int)(uint32_t)mt, count = (int)(mt >> 32);
+      f32x2 st;
+      if (count <= 1)
+        st = ((const f32x2*)((const char*)a.workspace + A.p.stats_at))[(int64_t)b * Hq + hq];
+      else
+        st = joined_stats(ml, first, count, hg % kPaHeads, a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf);
+      if (lane == 0) stats[i] = f32x2{st[0], st[1] == 0.0f ? 0.0f : 1.0f / st[1]};
+    }
+    __syncthreads();
+    if (pos < span.len) {
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const f32x4 x = *(const f32x4*)(scores + (int64_t)(h0 + i) * A.p.score_pitch);
+        const f32x2 st = stats[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += exp2_fast(x[j] - st[0]) * st[1];
+      }
+    }
+  }
+  float* const to = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)g * a.sums_stride_h + pos;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (pos + j >= span.lo && pos + j < span.len) to[j] += sum[j];
+}
+
+int padded_width(int D, bool fp8) {
+  if (D <= 64) return 64;
+  if (D <= 96 && !fp8) return 96;
+  return D <= 128 ? 128 : D <= 192 ? 192 : 256;
+}
+
+template <class M, bool FP8, int DP>
+void launch_width(const KernelArgs& A, hipStream_t stream) {
+  const dim3 grid(A.p.workgroups > 0 ? A.p.workgroups : A.p.items), block(256);
+  if (A.a.page_size % 16 == 0)
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true>), grid, block, 0, stream, A);
+  else
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false>), grid, block, 0, stream, A);
+}
+
+template <class M, bool FP8>
+void launch_kind(const KernelArgs& A, hipStream_t stream) {
+  const int padded = padded_width(A.a.D, FP8);
+  switch (padded) {
+    case 64: launch_width<M, FP8, 64>(A, stream); break;
+    case 96: if constexpr (!FP8) launch_width<M, FP8, 96>(A, stream); break;
+    case 128: launch_width<M, FP8, 128>(A, stream); break;
+    case 192: launch_width<M, FP8, 192>(A, stream); break;
+    default: launch_width<M, FP8, 256>(A, stream); break;
+  }
+  const int join_blocks = A.p.workgroups > 0 ? A.a.B * A.a.Hkv * A.a.G : 0;
+  const int seen = A.a.window > 0 && A.a.window + 16 < A.a.max_len ? A.a.window + 16 : A.a.max_len;
+  const int chunks = (seen + kPaSumsChunk - 1) / kPaSumsChunk;
+  const int blocks = join_blocks + (A.a.sums != nullptr ? A.a.B * A.a.Hkv * chunks : 0);
+  if (blocks > 0)
+    hipLaunchKernelGGL((paged_attention_join_kernel<M>), dim3(blocks), dim3(256), 0, stream, A, padded, join_blocks,
+                       chunks);
+}
+
+}  // namespace
+
+PagedAttentionPlan paged_attention_plan(int B, int Hkv, int G, int D, int max_len, int window, bool counted) {
+  PagedAttentionPlan p{};
+  p.head_tiles = (G + kPaHeads - 1) / kPaHeads;
+  p.items = B * Hkv * p.head_tiles;
+  const int seen = window > 0 && window + 16 < max_len ? window + 16 : max_len;
+  const int units = (seen + kPaUnit - 1) / kPaUnit;
+  p.min_units = 2;
+  p.workgroups = units > 4 ? 768 : 0;
+  size_t at = 0;
+  auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+  if (p.workgroups > 0) {
+    const size_t slots = 2 * (size_t)p.workgroups;
+    p.meta_at = part((size_t)p.items * 8);
+    p.ml_at = part(slots * kPaHeads * 8);
+    p.part_at = part(slots * kPaHeads * 256 * 4);
+  }
+  if (counted) {
+    p.stats_at = part((size_t)B * Hkv * G * 8);
+    p.score_pitch = (max_len + 15) / 16 * 16;
+    p.scores_at = part((size_t)B * Hkv * G * p.score_pitch * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t stream) {
+  KernelArgs A{};
+  A.a = a;
+  A.p = paged_attention_plan(a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.sums != nullptr);
+  // n / d for n < 2^31 as a product: with l = ceil(log2 d), m = floor(2^(31 + l) / d) + 1 is off by
+  // at most 2^l / 2^(31 + l), so floor(n m / 2^(31 + l)) = floor(n / d)
+  if (a.page_size == 1) {
+    A.page_shift = -1;
+  } else {
+    int l = 0;
+    while ((1ll << l) < a.page_size) ++l;
+    A.page_magic = (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)a.page_size + 1);
+    A.page_shift = l - 1;
+  }
+  switch (kind) {
+    case kKvBf16: launch_kind<Bf16, false>(A, stream); break;
+    case kKvF16: launch_kind<F16, false>(A, stream); break;
+    case kKvFp8Bf16: launch_kind<Bf16, true>(A, stream); break;
+    default: launch_kind<F16, true>(A, stream); break;
+  }
+}
+
+}  // namespace vk

@@ -1,0 +1,213 @@
+"""The key-value cache of a decode step on torch device tensors: append, the attention of one
+new token over the paged cache, and eviction by accumulated attention weight.
+
+A cache is two tensors [pages, Hkv, page_size, D] of any strides with D contiguous (a cache that is
+[pages, page_size, Hkv, D] in memory goes in as its ``transpose(1, 2)``), bf16, fp16 or
+float8_e4m3fn with a float32 scale for each head.  ``block_table`` [B, W] int32 names the page of
+every page_size positions of a sequence, ``seq_lens`` [B] int32 how many positions it has.  Every
+call is enqueued on the current stream of the tensors' device, with no host synchronisation; what it
+writes besides its arguments comes from torch's allocator, so calls on several streams do not share
+scratch and a call can be captured in a graph.
+
+The entry points are additive: the reference keeps its cache outside this path.  Everything runs in
+``libvkernels_hip.so``; there is no fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .vllm_experts import VK_OK, last_error, load_libvkernels_hip
+
+__all__ = ["kv_cache_append", "kv_cache_evict", "paged_attention"]
+
+_P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+
+# VK_HIP_KV_*: (type of the cache, type of the queries)
+_KINDS = {
+    (torch.bfloat16, torch.bfloat16): 0,
+    (torch.float16, torch.float16): 1,
+    (torch.float8_e4m3fn, torch.bfloat16): 2,
+    (torch.float8_e4m3fn, torch.float16): 3,
+}
+
+_fns: dict = {}
+
+
+def _fn(name):
+    fn = _fns.get(name)
+    if fn is None:
+        lib = load_libvkernels_hip()
+        argtypes, restype = {
+            "vk_hip_kv_cache_append": ([_P] * 9 + [_I] * 9 + [_L] * 7 + [_P], _I),
+            "vk_hip_paged_attention_workspace_bytes": ([_I] * 7, _Z),
+            "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
+            "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P], _I),
+        }[name]
+        try:
+            fn = getattr(lib, name)
+        except AttributeError:
+            raise RuntimeError(f"{name} not found in libvkernels_hip.so") from None
+        fn.argtypes, fn.restype = argtypes, restype
+        _fns[name] = fn
+    return fn
+
+
+def _done(status, name):
+    if status != VK_OK:
+        raise RuntimeError(f"{name} failed with status {status}: {last_error(load_libvkernels_hip())}")
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _cache_args(k_cache, v_cache, block_table, seq_lens):
+    """Checks of what every operator takes: (pages, Hkv, page_size, D, strides, B, table width)."""
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be [pages, Hkv, page_size, D] alike")
+    strides = k_cache.stride()
+    _need(k_cache.dtype == v_cache.dtype and strides == v_cache.stride() and strides[3] == 1,
+          "k_cache and v_cache must have one type and the same strides, rows of D values contiguous")
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
+          "block_table must be int32 [B, W] with contiguous rows")
+    B, W = block_table.shape
+    _need(seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.shape[0] == B and
+          (seq_lens.stride(0) == 1 or B <= 1), "seq_lens must be int32 [B], contiguous")
+    dev = k_cache.device
+    _need(dev.type == "cuda" and v_cache.device == dev and block_table.device == dev and seq_lens.device == dev,
+          "the cache, block_table and seq_lens must be on one device")
+    return k_cache.shape, strides, B, W
+
+
+def _head_vector(t, n, name, dev):
+    if t is None:
+        return None
+    _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous() and t.device == dev,
+          f"{name} must be {n} contiguous float32 values on the cache's device")
+    return t.data_ptr()
+
+
+def _rows(t):
+    """`t` [n, heads, D], or a copy of it where its rows do not start on 16 bytes."""
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _on(dev):
+    """The raw current stream of the device; the calling thread's device has to be that one."""
+    _need(dev.index == torch.cuda.current_device(), "the tensors' device must be the current device")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_start=None, k_scale=None, v_scale=None):
+    """New tokens' keys and values [tokens, Hkv, D] into the pages.
+
+    ``seq_lens`` count the new tokens.  ``query_start`` [B + 1] int32: the new tokens of sequence b are
+    query_start[b] .. query_start[b + 1] - 1 and go to its last positions; None: one token for each
+    sequence (a sequence of length 0 takes none).  Positions whose page is outside [0, pages) are
+    skipped.  An 8-bit cache holds the codes nearest to value / scale of the head (``k_scale``,
+    ``v_scale`` [Hkv]), the largest finite code beyond +-448."""
+    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
+    dev = k_cache.device
+    _need(k.dim() == 3 and k.shape[1:] == (Hkv, D) and v.shape == k.shape and v.dtype == k.dtype,
+          "k and v must be [tokens, Hkv, D] alike")
+    _need(k.device == dev and v.device == dev, "k and v must be on the cache's device")
+    kind = _KINDS.get((k_cache.dtype, k.dtype))
+    _need(kind is not None, f"no cache of {k_cache.dtype} takes rows of {k.dtype}")
+    if query_start is not None:
+        _need(query_start.dtype == torch.int32 and query_start.numel() == B + 1 and query_start.is_contiguous() and
+              query_start.device == dev, "query_start must be int32 [B + 1] on the cache's device")
+    else:
+        _need(k.shape[0] == B, "without query_start there is one token for each sequence")
+    k, v = _rows(k), _rows(v)
+    ks, vs = k.stride(), v.stride()
+    _done(_fn("vk_hip_kv_cache_append")(
+        k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        None if query_start is None else query_start.data_ptr(), _head_vector(k_scale, Hkv, "k_scale", dev),
+        _head_vector(v_scale, Hkv, "v_scale", dev), kind, B, k.shape[0], Hkv, D, pages, ps, W,
+        max(block_table.stride(0), W), ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2], _on(dev)),
+        "vk_hip_kv_cache_append")
+
+
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, softcap=0.0,
+                    sinks=None, k_scale=None, v_scale=None, weight_sums=None, return_lse=False, out=None):
+    """Attention of one new token of every sequence, q [B, Hq, D], over its cached positions.
+
+    Query heads G g .. G g + G - 1 read key/value head g (G = Hq / Hkv).  ``scale`` defaults to
+    D ** -0.5; ``window`` > 0 leaves the last so many positions; ``softcap`` c > 0 bounds the scores by
+    c tanh(s / c); ``sinks`` [Hq] float32 are scores whose value is zero.  ``max_len`` bounds every
+    length (default: what the table holds; a longer sequence is cut to it): the launch and its
+    workspace follow it, so a tight bound is worth giving.  ``weight_sums`` [B, Hkv, positions]
+    float32: every position's weights, summed over the heads of the group, are added to it.
+    Returns out [B, Hq, D], or (out, lse [B, Hq] float32).  A row that nothing is left of is 0, its
+    lse -inf (its sink, where there is one)."""
+    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
+    dev = k_cache.device
+    _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == D and q.shape[1] % Hkv == 0 and q.shape[1] > 0,
+          "q must be [B, Hq, D] with Hq a multiple of the cache's heads")
+    _need(q.device == dev, "q must be on the cache's device")
+    Hq = q.shape[1]
+    kind = _KINDS.get((k_cache.dtype, q.dtype))
+    _need(kind is not None, f"no cache of {k_cache.dtype} takes queries of {q.dtype}")
+    max_len = W * ps if max_len is None else max_len
+    q = _rows(q)
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
+              "out must be contiguous and like q")
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    sums, sums_b, sums_h = None, 0, 0
+    if weight_sums is not None:
+        _need(weight_sums.dtype == torch.float32 and weight_sums.dim() == 3 and weight_sums.shape[:2] == (B, Hkv) and
+              weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.device == dev,
+              "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
+        sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
+    size = _fn("vk_hip_paged_attention_workspace_bytes")(B, Hkv, Hq // Hkv, D, max_len, window, sums is not None)
+    workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    qs = q.stride()
+    _done(_fn("vk_hip_paged_attention")(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        _head_vector(sinks, Hq, "sinks", dev), _head_vector(k_scale, Hkv, "k_scale", dev),
+        _head_vector(v_scale, Hkv, "v_scale", dev), out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind,
+        B, Hkv, Hq // Hkv, D, pages, ps, W, max(block_table.stride(0), W), max_len, window,
+        D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1], strides[0], strides[1], strides[2],
+        sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size, _on(dev)),
+        "vk_hip_paged_attention")
+    return (out, lse) if return_lse else out
+
+
+def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget, *, keep_first=0, keep_last=0,
+                   max_len=None, sums_out=None):
+    """Cuts every sequence of more than ``budget`` positions to that many, in place.
+
+    Each key/value head keeps the first ``keep_first`` and last ``keep_last`` positions and, of the
+    others, those with the largest ``weight_sums`` [B, Hkv, positions] (NaN counts as largest, ties go
+    to the lowest position); their rows move in order to positions 0 .. budget - 1.  The sums move
+    along, with zeros from the budget up to the old length: in place, or to ``sums_out``.
+    Returns (new_lens [B] int32, kept [B, Hkv, budget] int32: the old positions, -1 beyond the new
+    length).  The pages of a sequence that is cut must be its own; those behind its new length are
+    free afterwards.  Rows keep the position encoding they were stored with."""
+    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
+    dev = k_cache.device
+    max_len = W * ps if max_len is None else max_len
+    sums_out = weight_sums if sums_out is None else sums_out
+    for name, t in (("weight_sums", weight_sums), ("sums_out", sums_out)):
+        _need(t.dtype == torch.float32 and t.dim() == 3 and t.shape[:2] == (B, Hkv) and t.shape[2] >= max_len and
+              t.stride(2) == 1 and t.device == dev,
+              f"{name} must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
+    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+    kept = torch.empty((B, Hkv, max(budget, 0)), dtype=torch.int32, device=dev)
+    ss, so = weight_sums.stride(), sums_out.stride()
+    _done(_fn("vk_hip_kv_cache_evict")(
+        k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), weight_sums.data_ptr(),
+        sums_out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), k_cache.element_size(), B, Hkv, D, pages, ps, W,
+        max(block_table.stride(0), W), max_len, budget, keep_first, keep_last, strides[0], strides[1], strides[2],
+        ss[0], ss[1], so[0], so[1], _on(dev)), "vk_hip_kv_cache_evict")
+    return new_lens, kept
