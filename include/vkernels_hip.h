@@ -735,14 +735,17 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
  * overlap it.  new_lens [B] = min(length, budget); kept [B, Hkv, budget] int32 the old
  * positions in order, -1 beyond the new length.  A shorter sequence keeps all it has
  * (its sums are copied).  The pages of a sequence that is cut have to be its own.
- * elem_bytes: 1 or 2, a value of the cache. */
+ * elem_bytes: 1 or 2, a value of the cache.  The workspace of
+ * vk_hip_kv_cache_evict_workspace_bytes (4-byte aligned) is scratch of this call alone. */
+size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int budget);
 int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
                           const int32_t* seq_lens, const float* weight_sums, float* sums_out,
                           int32_t* new_lens, int32_t* kept, int elem_bytes, int B, int Hkv, int D,
                           int num_pages, int page_size, int table_width, int table_stride, int max_len,
                           int budget, int keep_first, int keep_last, int64_t page_stride,
                           int64_t head_stride, int64_t slot_stride, int64_t sums_stride_b,
-                          int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* stream);
+                          int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -21,7 +21,8 @@ ATTEND = dict(q=P, k_cache=P, v_cache=P, block_table=P, seq_lens=P, sinks=None, 
 EVICT = dict(k_cache=P, v_cache=P, block_table=P, seq_lens=P, weight_sums=P, sums_out=P, new_lens=2 * P, kept=P,
              elem_bytes=2, B=4, Hkv=2, D=64, num_pages=8, page_size=16, table_width=4, table_stride=4, max_len=64,
              budget=32, keep_first=4, keep_last=8, page_stride=2048, head_stride=1024, slot_stride=64,
-             sums_stride_b=128, sums_stride_h=64, out_stride_b=128, out_stride_h=64, stream=None)
+             sums_stride_b=128, sums_stride_h=64, out_stride_b=128, out_stride_h=64, workspace=P, workspace_bytes=1 << 40,
+             stream=None)
 CALLS = {"vk_hip_kv_cache_append": APPEND, "vk_hip_paged_attention": ATTEND, "vk_hip_kv_cache_evict": EVICT}
 
 CACHE = [dict(D=0), dict(D=24), dict(D=272), dict(D=-16), dict(Hkv=0), dict(num_pages=0), dict(page_size=0),
@@ -40,7 +41,7 @@ INVALID = {
     "vk_hip_kv_cache_evict": CACHE + [
         dict(weight_sums=None), dict(sums_out=None), dict(new_lens=None), dict(kept=None), dict(max_len=65),
         dict(max_len=-1), dict(budget=0), dict(budget=-3), dict(keep_first=-1), dict(keep_last=-1), dict(keep_first=25),
-        dict(out_stride_b=64), dict(new_lens=P)],
+        dict(out_stride_b=64), dict(new_lens=P), dict(workspace=None), dict(workspace_bytes=4), dict(workspace=P + 2)],
 }
 OTHER = [
     ("vk_hip_kv_cache_append", dict(kind=4), ve.VK_ERROR_UNSUPPORTED),

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "fast_div.hpp"
+
 namespace vk {
 
 struct KvAppendArgs {
@@ -21,6 +23,7 @@ struct KvAppendArgs {
   int64_t page_stride, head_stride, slot_stride;            // elements, of both caches
   int table_stride, table_width, num_pages, page_size;
   int B, tokens, Hkv, D;
+  FastDiv by_page;                                          // (set by the launcher)
 };
 void launch_kv_append(const KvAppendArgs& a, int kind, hipStream_t stream);
 
@@ -37,7 +40,11 @@ struct KvEvictArgs {
   int64_t page_stride, head_stride, slot_stride;            // bytes
   int table_stride, num_pages, page_size, row_bytes;
   int B, Hkv, max_len, budget, keep_first, keep_last;
+  uint32_t* order;          // workspace: for the keys and values of every head a count and a word for each batch
+  int batches;              // of kv_evict_batches
+  FastDiv by_page, by_pieces;                               // (set by the launcher)
 };
+int kv_evict_batches(int budget, int row_bytes);   // of the keys (or values) of a head
 void launch_kv_evict(const KvEvictArgs& a, hipStream_t stream);
 
 }  // namespace vk

@@ -145,13 +145,19 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   return launched(who, before);
 }
 
+size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int budget) {
+  if (elem_bytes <= 0 || B <= 0 || Hkv <= 0 || D < 16 || budget <= 0 || D * (int64_t)elem_bytes > 512) return 0;
+  return 4 * 2 * static_cast<size_t>(B) * Hkv * (1 + vk::kv_evict_batches(budget, D * elem_bytes));
+}
+
 int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
                           const int32_t* seq_lens, const float* weight_sums, float* sums_out,
                           int32_t* new_lens, int32_t* kept, int elem_bytes, int B, int Hkv, int D,
                           int num_pages, int page_size, int table_width, int table_stride, int max_len,
                           int budget, int keep_first, int keep_last, int64_t page_stride,
                           int64_t head_stride, int64_t slot_stride, int64_t sums_stride_b,
-                          int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* stream) {
+                          int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   const char* const who = "vk_hip_kv_cache_evict";
   if (elem_bytes != 1 && elem_bytes != 2) return refuse(VK_ERROR_UNSUPPORTED, who, "elem_bytes must be 1 or 2");
   if (B < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B must not be negative");
@@ -168,8 +174,12 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
     why = "sums_out in place has weight_sums' strides";
   if (why == nullptr && new_lens == seq_lens) why = "new_lens must not be seq_lens";
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  if ((int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2)
+  if ((int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2 ||
+      (int64_t)B * Hkv * vk::kv_evict_batches(budget, D * elem_bytes) > kInt32 / 2)
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many rows for one call");
+  if (workspace == nullptr || !aligned(workspace, 4) ||
+      workspace_bytes < vk_hip_kv_cache_evict_workspace_bytes(elem_bytes, B, Hkv, D, budget))
+    return refuse(VK_ERROR_INVALID_ARGUMENT, who, "a workspace of vk_hip_kv_cache_evict_workspace_bytes is needed");
   vk::KvEvictArgs a{};
   a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
   a.sums = weight_sums; a.sums_out = sums_out; a.new_lens = new_lens; a.kept = kept;
@@ -179,6 +189,8 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
   a.slot_stride = slot_stride * elem_bytes;
   a.table_stride = table_stride; a.num_pages = num_pages; a.page_size = page_size; a.row_bytes = D * elem_bytes;
   a.B = B; a.Hkv = Hkv; a.max_len = max_len; a.budget = budget; a.keep_first = keep_first; a.keep_last = keep_last;
+  a.order = static_cast<uint32_t*>(workspace);
+  a.batches = vk::kv_evict_batches(budget, a.row_bytes);
   const hipError_t before = hipPeekAtLastError();
   vk::launch_kv_evict(a, static_cast<hipStream_t>(stream));
   return launched(who, before);

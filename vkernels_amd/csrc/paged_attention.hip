@@ -9,6 +9,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fast_div.hpp"
 #include "paged_attention.hpp"
 
 namespace vk {
@@ -114,13 +115,10 @@ __device__ __forceinline__ Span span_of(int len, int max_len, int window) {
 struct KernelArgs {
   PagedAttentionArgs a;
   PagedAttentionPlan p;
-  uint32_t page_magic;   // position / page_size = (position * magic) >> (32 + shift)
-  int page_shift;        // -1: pages of one position
+  FastDiv by_page;       // position / page_size
 };
 
-__device__ __forceinline__ int page_of(const KernelArgs& A, int pos) {
-  return A.page_shift < 0 ? pos : (int)(__umulhi((uint32_t)pos, A.page_magic) >> A.page_shift);
-}
+__device__ __forceinline__ int page_of(const KernelArgs& A, int pos) { return divided(pos, A.by_page); }
 
 // The units of all items in order (sequence, head item, unit), cut into equal shares.
 struct Share {
@@ -195,8 +193,16 @@ struct Tile {
                                       ? kPaWaveRows * kPitch : kPaHeads * kOutPitch * 4;
 };
 
-template <class M, bool FP8, int DP, bool P16>
-__global__ __launch_bounds__(256) void paged_attention_kernel(const KernelArgs A) {
+#ifndef OCC64
+#define OCC64 4
+#define OCC128 2
+#define OCC256 1
+#endif
+// Workgroups of a CU (wavefronts of a SIMD), by the registers that a width needs.
+constexpr int residents(int DP) { return DP <= 64 ? OCC64 : DP <= 128 ? OCC128 : OCC256; }
+
+template <class M, bool FP8, int DP, bool P16, bool FULL>
+__global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(const KernelArgs A) {
   typedef Tile<M, FP8, DP> L;
   typedef typename M::V8 V8;
   const PagedAttentionArgs& a = A.a;
@@ -303,62 +309,45 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const KernelArgs A
       const int hi = __shfl((int)(row_at >> 32), row);
       return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
     };
+    // A row of a width below DP: what lies behind its last value is read as zeros (keys) or not
+    // used (values); such lanes read the row's first bytes instead.
+    const int row_bytes = a.D * L::kElem;
+    auto key_piece = [&](const char* row, int i) -> u32x4 {
+      if constexpr (FULL) return *(const u32x4*)(row + quad * 16 + i * 64);
+      const int at = quad * 16 + i * 64;
+      const u32x4 x = *(const u32x4*)(row + (at < row_bytes ? at : 0));
+      return at < row_bytes ? x : u32x4{0, 0, 0, 0};
+    };
+    const int piece = lane % L::kPieces, sub = lane / L::kPieces;
+    const uint32_t value_at = FULL ? piece * 16 : (piece * 16 < row_bytes ? piece * 16 : 0);
+    const uint32_t key_lane = (uint32_t)col * (uint32_t)slot_bytes, value_lane = (uint32_t)sub * (uint32_t)slot_bytes + value_at;
+    auto half_tile = [&](int pos0, int page) -> int64_t {   // bytes to the row of position pos0
+      return (int64_t)max(page, 0) * page_bytes + (int64_t)(pos0 - page_of(A, pos0) * a.page_size) * slot_bytes;
+    };
     auto load_k = [&](int pos0) {
-      if constexpr (P16) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int p0 = pos0 + 16 * t;
-          const int page = max(t == 0 ? page0 : page1, 0);
-          const int slot = t == 0 ? p0 - page_of(A, p0) * a.page_size : p0 - page_of(A, p0) * a.page_size;
-          const char* base = kbase + (int64_t)page * page_bytes + (int64_t)slot * slot_bytes;
-          const uint32_t at = (uint32_t)col * (uint32_t)slot_bytes + quad * 16;
+      for (int t = 0; t < 2; ++t) {
+        const char* row;
+        if constexpr (P16) row = kbase + half_tile(pos0 + 16 * t, t == 0 ? page0 : page1) + key_lane;
+        else row = kbase + row_from(16 * t + col);
 #pragma unroll
-          for (int i = 0; i < L::kKLoads; ++i) {
-            u32x4 x = {0, 0, 0, 0};
-            if (DP * L::kElem == a.D * L::kElem || i * 64 + quad * 16 < a.D * L::kElem)
-              x = *(const u32x4*)(base + at + i * 64);
-            kreg[t][i] = x;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const char* base = kbase + row_from(16 * t + col) + quad * 16;
-#pragma unroll
-          for (int i = 0; i < L::kKLoads; ++i) {
-            u32x4 x = {0, 0, 0, 0};
-            if (i * 64 + quad * 16 < a.D * L::kElem) x = *(const u32x4*)(base + i * 64);
-            kreg[t][i] = x;
-          }
-        }
+        for (int i = 0; i < L::kKLoads; ++i) kreg[t][i] = key_piece(row, i);
       }
     };
     auto load_v = [&](int pos0) {
-      const int piece = lane % L::kPieces, sub = lane / L::kPieces;
-      const bool mine = piece * 16 < a.D * L::kElem;
       if constexpr (P16) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const int p0 = pos0 + 16 * t;
-          const int page = max(t == 0 ? page0 : page1, 0);
-          const int slot = p0 - page_of(A, p0) * a.page_size;
-          const char* base = vbase + (int64_t)page * page_bytes + (int64_t)slot * slot_bytes;
+          const char* rows = vbase + half_tile(pos0 + 16 * t, t == 0 ? page0 : page1);
 #pragma unroll
-          for (int i = 0; i < L::kVLoads / 2; ++i) {
-            const uint32_t at = (uint32_t)(i * L::kRowsPerLoad + sub) * (uint32_t)slot_bytes + piece * 16;
-            u32x4 x = {0, 0, 0, 0};
-            if (mine) x = *(const u32x4*)(base + at);
-            vreg[t * (L::kVLoads / 2) + i] = x;
-          }
+          for (int i = 0; i < L::kVLoads / 2; ++i)
+            vreg[t * (L::kVLoads / 2) + i] =
+                *(const u32x4*)(rows + (int64_t)(i * L::kRowsPerLoad) * slot_bytes + value_lane);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < L::kVLoads; ++i) {
-          const char* base = vbase + row_from(i * L::kRowsPerLoad + sub) + piece * 16;
-          u32x4 x = {0, 0, 0, 0};
-          if (mine) x = *(const u32x4*)base;
-          vreg[i] = x;
-        }
+        for (int i = 0; i < L::kVLoads; ++i)
+          vreg[i] = *(const u32x4*)(vbase + row_from(i * L::kRowsPerLoad + sub) + value_at);
       }
     };
 
@@ -467,7 +456,6 @@ __global__ __launch_bounds__(256) void paged_attention_kernel(const KernelArgs A
       // there may be anything), 32-byte pairs of pieces exchanged by the row so that the
       // transposed reads below spread over the banks.
       {
-        const int piece = lane % L::kPieces, sub = lane / L::kPieces;
 #pragma unroll
         for (int i = 0; i < L::kVLoads; ++i) {
           const int row = i * L::kRowsPerLoad + sub;
@@ -699,10 +687,15 @@ int padded_width(int D, bool fp8) {
 template <class M, bool FP8, int DP>
 void launch_width(const KernelArgs& A, hipStream_t stream) {
   const dim3 grid(A.p.workgroups > 0 ? A.p.workgroups : A.p.items), block(256);
-  if (A.a.page_size % 16 == 0)
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true>), grid, block, 0, stream, A);
+  const bool aligned_pages = A.a.page_size % 16 == 0, full = A.a.D == DP;
+  if (aligned_pages && full)
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, true>), grid, block, 0, stream, A);
+  else if (aligned_pages)
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, false>), grid, block, 0, stream, A);
+  else if (full)
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, true>), grid, block, 0, stream, A);
   else
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false>), grid, block, 0, stream, A);
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, false>), grid, block, 0, stream, A);
 }
 
 template <class M, bool FP8>
@@ -733,7 +726,7 @@ PagedAttentionPlan paged_attention_plan(int B, int Hkv, int G, int D, int max_le
   const int seen = window > 0 && window + 16 < max_len ? window + 16 : max_len;
   const int units = (seen + kPaUnit - 1) / kPaUnit;
   p.min_units = 2;
-  p.workgroups = units > 4 ? 768 : 0;
+  p.workgroups = units > 4 ? 256 * residents(D) : 0;
   size_t at = 0;
   auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   if (p.workgroups > 0) {
@@ -755,16 +748,7 @@ void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t s
   KernelArgs A{};
   A.a = a;
   A.p = paged_attention_plan(a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.sums != nullptr);
-  // n / d for n < 2^31 as a product: with l = ceil(log2 d), m = floor(2^(31 + l) / d) + 1 is off by
-  // at most 2^l / 2^(31 + l), so floor(n m / 2^(31 + l)) = floor(n / d)
-  if (a.page_size == 1) {
-    A.page_shift = -1;
-  } else {
-    int l = 0;
-    while ((1ll << l) < a.page_size) ++l;
-    A.page_magic = (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)a.page_size + 1);
-    A.page_shift = l - 1;
-  }
+  A.by_page = fast_div(a.page_size);
   switch (kind) {
     case kKvBf16: launch_kind<Bf16, false>(A, stream); break;
     case kKvF16: launch_kind<F16, false>(A, stream); break;

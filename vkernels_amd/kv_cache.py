@@ -18,7 +18,7 @@ import ctypes
 
 import torch
 
-from .vllm_experts import VK_OK, last_error, load_libvkernels_hip
+from .vllm_experts import last_error, load_libvkernels_hip
 
 __all__ = ["kv_cache_append", "kv_cache_evict", "paged_attention"]
 
@@ -43,7 +43,8 @@ def _fn(name):
             "vk_hip_kv_cache_append": ([_P] * 9 + [_I] * 9 + [_L] * 7 + [_P], _I),
             "vk_hip_paged_attention_workspace_bytes": ([_I] * 7, _Z),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
-            "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P], _I),
+            "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 5, _Z),
+            "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P, _Z, _P], _I),
         }[name]
         try:
             fn = getattr(lib, name)
@@ -54,9 +55,8 @@ def _fn(name):
     return fn
 
 
-def _done(status, name):
-    if status != VK_OK:
-        raise RuntimeError(f"{name} failed with status {status}: {last_error(load_libvkernels_hip())}")
+def _failed(status, name):
+    raise RuntimeError(f"{name} failed with status {status}: {last_error(load_libvkernels_hip())}")
 
 
 def _need(ok, message):
@@ -64,27 +64,43 @@ def _need(ok, message):
         raise ValueError(message)
 
 
-def _cache_args(k_cache, v_cache, block_table, seq_lens):
-    """Checks of what every operator takes: (pages, Hkv, page_size, D, strides, B, table width)."""
-    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "k_cache and v_cache must be [pages, Hkv, page_size, D] alike")
-    strides = k_cache.stride()
-    _need(k_cache.dtype == v_cache.dtype and strides == v_cache.stride() and strides[3] == 1,
+# The checks are one expression each on the path that is taken (a decode step is short: the host's work per
+# call counts); the functions _explain_* say which part of it did not hold.
+
+def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
+    B = block_table.shape[0]
+    return (len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is k_cache.dtype and strides[3] == 1 and
+            v_cache.stride() == strides and device >= 0 and v_cache.get_device() == device and
+            block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1 and
+            block_table.get_device() == device and seq_lens.dtype is torch.int32 and seq_lens.shape == (B,) and
+            seq_lens.is_contiguous() and seq_lens.get_device() == device and _device() == device)
+
+
+def _explain_cache(k_cache, v_cache, block_table, seq_lens):
+    _need(k_cache.dim() == 4 and k_cache.shape == v_cache.shape,
+          "k_cache and v_cache must be [pages, Hkv, page_size, D] alike")
+    _need(k_cache.dtype == v_cache.dtype and k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1,
           "k_cache and v_cache must have one type and the same strides, rows of D values contiguous")
     _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
           "block_table must be int32 [B, W] with contiguous rows")
-    B, W = block_table.shape
-    _need(seq_lens.dtype == torch.int32 and seq_lens.dim() == 1 and seq_lens.shape[0] == B and
-          (seq_lens.stride(0) == 1 or B <= 1), "seq_lens must be int32 [B], contiguous")
-    dev = k_cache.device
-    _need(dev.type == "cuda" and v_cache.device == dev and block_table.device == dev and seq_lens.device == dev,
-          "the cache, block_table and seq_lens must be on one device")
-    return k_cache.shape, strides, B, W
+    _need(seq_lens.dtype == torch.int32 and seq_lens.shape == block_table.shape[:1] and seq_lens.is_contiguous(),
+          "seq_lens must be int32 [B], contiguous")
+    devices = {t.get_device() for t in (k_cache, v_cache, block_table, seq_lens)}
+    _need(len(devices) == 1 and devices != {-1}, "the cache, block_table and seq_lens must be on one device")
+    _need(devices == {_device()}, "the tensors' device must be the current device")
 
 
-def _head_vector(t, n, name, dev):
-    if t is None:
-        return None
-    _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous() and t.device == dev,
+def _device():
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
+
+
+def _stream(device):
+    """The raw current stream of the device."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _head_vector(t, n, name, device):
+    _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == device,
           f"{name} must be {n} contiguous float32 values on the cache's device")
     return t.data_ptr()
 
@@ -99,12 +115,6 @@ def _rows(t):
     return t
 
 
-def _on(dev):
-    """The raw current stream of the device; the calling thread's device has to be that one."""
-    _need(dev.index == torch.cuda.current_device(), "the tensors' device must be the current device")
-    return torch.cuda.current_stream().cuda_stream
-
-
 def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_start=None, k_scale=None, v_scale=None):
     """New tokens' keys and values [tokens, Hkv, D] into the pages.
 
@@ -113,26 +123,34 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     sequence (a sequence of length 0 takes none).  Positions whose page is outside [0, pages) are
     skipped.  An 8-bit cache holds the codes nearest to value / scale of the head (``k_scale``,
     ``v_scale`` [Hkv]), the largest finite code beyond +-448."""
-    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
-    dev = k_cache.device
-    _need(k.dim() == 3 and k.shape[1:] == (Hkv, D) and v.shape == k.shape and v.dtype == k.dtype,
+    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
+    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
+        _explain_cache(k_cache, v_cache, block_table, seq_lens)
+    pages, Hkv, ps, D = shape
+    B, W = block_table.shape
+    tokens = k.shape[0]
+    _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype,
           "k and v must be [tokens, Hkv, D] alike")
-    _need(k.device == dev and v.device == dev, "k and v must be on the cache's device")
+    _need(k.get_device() == device and v.get_device() == device, "k and v must be on the cache's device")
     kind = _KINDS.get((k_cache.dtype, k.dtype))
-    _need(kind is not None, f"no cache of {k_cache.dtype} takes rows of {k.dtype}")
+    _need(kind is not None, "the cache's type does not take rows of this type")
     if query_start is not None:
-        _need(query_start.dtype == torch.int32 and query_start.numel() == B + 1 and query_start.is_contiguous() and
-              query_start.device == dev, "query_start must be int32 [B + 1] on the cache's device")
+        _need(query_start.dtype is torch.int32 and query_start.numel() == B + 1 and query_start.is_contiguous() and
+              query_start.get_device() == device, "query_start must be int32 [B + 1] on the cache's device")
+        query_start = query_start.data_ptr()
     else:
-        _need(k.shape[0] == B, "without query_start there is one token for each sequence")
+        _need(tokens == B, "without query_start there is one token for each sequence")
     k, v = _rows(k), _rows(v)
     ks, vs = k.stride(), v.stride()
-    _done(_fn("vk_hip_kv_cache_append")(
-        k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        None if query_start is None else query_start.data_ptr(), _head_vector(k_scale, Hkv, "k_scale", dev),
-        _head_vector(v_scale, Hkv, "v_scale", dev), kind, B, k.shape[0], Hkv, D, pages, ps, W,
-        max(block_table.stride(0), W), ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2], _on(dev)),
-        "vk_hip_kv_cache_append")
+    status = _fn("vk_hip_kv_cache_append")(
+        k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+        seq_lens.data_ptr(), query_start,
+        None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
+        None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device), kind, B, tokens, Hkv, D, pages, ps,
+        W, max(block_table.stride(0), W), ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2],
+        _stream(device))
+    if status:
+        _failed(status, "vk_hip_kv_cache_append")
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, softcap=0.0,
@@ -147,39 +165,46 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     float32: every position's weights, summed over the heads of the group, are added to it.
     Returns out [B, Hq, D], or (out, lse [B, Hq] float32).  A row that nothing is left of is 0, its
     lse -inf (its sink, where there is one)."""
-    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
-    dev = k_cache.device
-    _need(q.dim() == 3 and q.shape[0] == B and q.shape[2] == D and q.shape[1] % Hkv == 0 and q.shape[1] > 0,
-          "q must be [B, Hq, D] with Hq a multiple of the cache's heads")
-    _need(q.device == dev, "q must be on the cache's device")
+    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
+    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
+        _explain_cache(k_cache, v_cache, block_table, seq_lens)
+    pages, Hkv, ps, D = shape
+    B, W = block_table.shape
+    _need(q.dim() == 3 and q.get_device() == device, "q must be [B, Hq, D] on the cache's device")
     Hq = q.shape[1]
+    G = Hq // Hkv
+    _need(q.shape == (B, G * Hkv, D) and G > 0, "q must be [B, Hq, D] with Hq a multiple of the cache's heads")
     kind = _KINDS.get((k_cache.dtype, q.dtype))
-    _need(kind is not None, f"no cache of {k_cache.dtype} takes queries of {q.dtype}")
-    max_len = W * ps if max_len is None else max_len
+    _need(kind is not None, "the cache's type does not take queries of this type")
+    if max_len is None:
+        max_len = W * ps
     q = _rows(q)
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((B, Hq, D))
     else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous() and out.device == dev,
+        _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and out.get_device() == device,
               "out must be contiguous and like q")
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
-        _need(weight_sums.dtype == torch.float32 and weight_sums.dim() == 3 and weight_sums.shape[:2] == (B, Hkv) and
-              weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.device == dev,
+        _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3 and weight_sums.shape[:2] == (B, Hkv) and
+              weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.get_device() == device,
               "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
-    size = _fn("vk_hip_paged_attention_workspace_bytes")(B, Hkv, Hq // Hkv, D, max_len, window, sums is not None)
-    workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    size = _fn("vk_hip_paged_attention_workspace_bytes")(B, Hkv, G, D, max_len, window, sums is not None)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     qs = q.stride()
-    _done(_fn("vk_hip_paged_attention")(
+    status = _fn("vk_hip_paged_attention")(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        _head_vector(sinks, Hq, "sinks", dev), _head_vector(k_scale, Hkv, "k_scale", dev),
-        _head_vector(v_scale, Hkv, "v_scale", dev), out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind,
-        B, Hkv, Hq // Hkv, D, pages, ps, W, max(block_table.stride(0), W), max_len, window,
-        D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1], strides[0], strides[1], strides[2],
-        sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size, _on(dev)),
-        "vk_hip_paged_attention")
+        None if sinks is None else _head_vector(sinks, Hq, "sinks", device),
+        None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
+        None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device),
+        out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind, B, Hkv, G, D, pages, ps, W,
+        max(block_table.stride(0), W), max_len, window, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
+        strides[0], strides[1], strides[2], sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size,
+        _stream(device))
+    if status:
+        _failed(status, "vk_hip_paged_attention")
     return (out, lse) if return_lse else out
 
 
@@ -194,20 +219,29 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     Returns (new_lens [B] int32, kept [B, Hkv, budget] int32: the old positions, -1 beyond the new
     length).  The pages of a sequence that is cut must be its own; those behind its new length are
     free afterwards.  Rows keep the position encoding they were stored with."""
-    (pages, Hkv, ps, D), strides, B, W = _cache_args(k_cache, v_cache, block_table, seq_lens)
-    dev = k_cache.device
-    max_len = W * ps if max_len is None else max_len
+    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
+    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
+        _explain_cache(k_cache, v_cache, block_table, seq_lens)
+    pages, Hkv, ps, D = shape
+    B, W = block_table.shape
+    if max_len is None:
+        max_len = W * ps
     sums_out = weight_sums if sums_out is None else sums_out
     for name, t in (("weight_sums", weight_sums), ("sums_out", sums_out)):
-        _need(t.dtype == torch.float32 and t.dim() == 3 and t.shape[:2] == (B, Hkv) and t.shape[2] >= max_len and
-              t.stride(2) == 1 and t.device == dev,
+        _need(t.dtype is torch.float32 and t.dim() == 3 and t.shape[:2] == (B, Hkv) and t.shape[2] >= max_len and
+              t.stride(2) == 1 and t.get_device() == device,
               f"{name} must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
-    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    kept = torch.empty((B, Hkv, max(budget, 0)), dtype=torch.int32, device=dev)
+    new_lens = torch.empty_like(seq_lens)
+    kept = seq_lens.new_empty((B, Hkv, max(budget, 0)))
+    elem = k_cache.element_size()
+    size = _fn("vk_hip_kv_cache_evict_workspace_bytes")(elem, B, Hkv, D, budget)
+    workspace = torch.empty(size, dtype=torch.uint8, device=k_cache.device)
     ss, so = weight_sums.stride(), sums_out.stride()
-    _done(_fn("vk_hip_kv_cache_evict")(
+    status = _fn("vk_hip_kv_cache_evict")(
         k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), weight_sums.data_ptr(),
-        sums_out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), k_cache.element_size(), B, Hkv, D, pages, ps, W,
+        sums_out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), elem, B, Hkv, D, pages, ps, W,
         max(block_table.stride(0), W), max_len, budget, keep_first, keep_last, strides[0], strides[1], strides[2],
-        ss[0], ss[1], so[0], so[1], _on(dev)), "vk_hip_kv_cache_evict")
+        ss[0], ss[1], so[0], so[1], workspace.data_ptr(), size, _stream(device))
+    if status:
+        _failed(status, "vk_hip_kv_cache_evict")
     return new_lens, kept
