@@ -737,7 +737,7 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
  * (its sums are copied).  The pages of a sequence that is cut have to be its own.
  * elem_bytes: 1 or 2, a value of the cache.  The workspace of
  * vk_hip_kv_cache_evict_workspace_bytes (4-byte aligned) is scratch of this call alone. */
-size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int budget);
+size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget);
 int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
                           const int32_t* seq_lens, const float* weight_sums, float* sums_out,
                           int32_t* new_lens, int32_t* kept, int elem_bytes, int B, int Hkv, int D,

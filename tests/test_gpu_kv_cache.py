@@ -380,11 +380,28 @@ def test_evict_ties_zeros_and_odd_values(hip_lib):
     _check_evict(s, sums, 50, 2, 9)
 
 
-def test_evict_long(hip_lib):
-    """More positions than a pass of the selection takes, keys that agree in their leading digits."""
-    s = Setup([20000, 9000], 1, 1, 16, 16, seed=2)
-    sums = 1.0 + torch.rand((2, 1, s.table.shape[1] * 16), device=dev()) * 2e-4
-    _check_evict(s, sums, 4097, 1, 64)
+@pytest.mark.parametrize("budget,first,last", [(4097, 1, 64), (8999, 0, 0), (300, 100, 200), (9001, 9001, 0), (5, 0, 2)])
+@pytest.mark.parametrize("kind", ["close", "spread", "ties", "zero"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_long(hip_lib, budget, first, last, kind, in_place):
+    """Rows that several workgroups share: keys that agree in their leading digits, that do not, few values."""
+    s = Setup([20000, 9000, 100, 8193], 1, 1, 16, 16, seed=2)
+    g = torch.Generator(device=dev()).manual_seed(budget)
+    sums = torch.rand((4, 1, s.table.shape[1] * 16), device=dev(), generator=g)
+    sums = {"close": 1 + 2e-4 * sums, "spread": torch.exp(40 * sums - 20), "ties": (5 * sums).floor(),
+            "zero": 0 * sums}[kind]
+    _check_evict(s, sums, budget, first, last, in_place)
+
+
+@pytest.mark.parametrize("rows,longest", [(129, 9000), (40, 12288), (256, 40000)])
+def test_evict_many_rows(hip_lib, rows, longest):
+    """A workgroup for each of many rows longer than it holds in registers, and the rule's edges."""
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(1, 200, (rows,), generator=g).tolist()
+    lens[0], lens[rows // 2], lens[-1] = longest, 8193, longest - 777
+    s = Setup(lens, 1, 1, 16, 16, seed=2)
+    sums = torch.exp(3 * torch.randn((rows, 1, s.table.shape[1] * 16), device=dev()))
+    _check_evict(s, sums, 150, 3, 40, in_place=True)
 
 
 def test_evict_twice_in_place(hip_lib):

@@ -123,18 +123,11 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
   return x;
 }
 
-// Of the digits counted in `bins` (n of them): the one that the need-th largest key has,
-// found[0], and how many keys of it are still wanted, found[1].
-__device__ void find_digit(uint32_t (*bins)[kBins], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
+// The workgroup's threads hold the counts c of two digits each, from the largest digit down
+// (thread t those of digits n - 1 - 2 t and n - 2 - 2 t).  Finds the digit that the need-th
+// largest key has, found[0], and how many keys of it are still wanted, found[1].
+__device__ void find_digit(const uint32_t (&c)[2], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
   const int t = threadIdx.x, wave = t >> 6;
-  // from the largest digit down: thread t holds the digits n - 1 - 2 t and n - 2 - 2 t
-  uint32_t c[2] = {0, 0};
-  if (2 * t < n) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < kBinCopies; ++k) c[i] += bins[k][n - 1 - 2 * t - i];
-  }
   uint32_t above = wave_scan(c[0] + c[1]);
   if ((t & 63) == 63) scan_lds[wave] = above;
   __syncthreads();
@@ -153,178 +146,343 @@ __device__ void find_digit(uint32_t (*bins)[kBins], int n, uint32_t need, uint32
   __syncthreads();
 }
 
-// One workgroup for the positions of a sequence in a head.  The least key that is kept is
-// found digit by digit (11, 11, 10 bits) from histograms in LDS.  The first pass reads the
-// sums; the second, when the first digit is known, counts what is kept for certain and
-// lists the keys that share the digit in LDS, where the other two digits are found (the
-// sums are read again for those when there are too many such keys).  The last pass writes
-// the kept positions down: every wavefront walks a stretch of its own, from the counts of
-// the ones before it.
-__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvictArgs a) {
-  __shared__ uint32_t bins[kBinCopies][kBins];
-  __shared__ uint32_t listed[kSelectWaves][kListed];
-  __shared__ uint32_t scan_lds[kSelectWaves], sure_of[kSelectWaves], equal_of[kSelectWaves];
-  __shared__ uint32_t found[2], too_many;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, b = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
-  // What orders the workgroups of the compaction behind this, for the keys and the values: a
-  // count of the batches taken, and a word for each batch that has been read.
-  for (int i = t; i < 2 * (1 + a.batches); i += kSelectThreads)
-    a.order[(int64_t)blockIdx.x * 2 * (1 + a.batches) + i] = 0;
-
-  const int len = min(max(a.lens[b], 0), a.max_len);
-  const float* const sums = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)h * a.sums_stride_h;
-  float* const out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
-  int32_t* const kept = a.kept + (int64_t)blockIdx.x * a.budget;
-  if (h == 0 && t == 0) a.new_lens[b] = min(len, a.budget);
-  if (len <= a.budget) {
-    for (int j = t; j < a.budget; j += kSelectThreads) kept[j] = j < len ? j : -1;
-    if (out != sums)
-      for (int j = t; j < len; j += kSelectThreads) out[j] = sums[j];
-    return;
-  }
-  const int lo = a.keep_first, hi = len - a.keep_last;       // positions that have to earn their place
-  const uint32_t places = (uint32_t)(a.budget - a.keep_first - a.keep_last);   // (hi - lo > places)
-  const int stretch = (len + 64 * kSelectWaves - 1) / (64 * kSelectWaves) * 64;
-  const int from = min(len, wave * stretch), to = min(len, from + stretch);
-  // The sums of 1024 positions of the stretch at a time, 16 a lane: all their loads at once, and
-  // none but the first pass's where that is the whole stretch (up to 16384 positions).
-  float x[kSelectLoads];
-  auto load = [&](int j0) {
+// The same from histograms in LDS.
+__device__ void find_digit_lds(uint32_t (*bins)[kBins], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
+  uint32_t c[2] = {0, 0};
+  if (2 * (int)threadIdx.x < n) {
 #pragma unroll
-    for (int i = 0; i < kSelectLoads; ++i) {
-      const int j = j0 + 64 * i + lane;
-      if (j0 + 64 * i < to) x[i] = sums[min(j, to - 1)];
-    }
-  };
-  const bool resident = stretch <= 64 * kSelectLoads;
-  // f(position, is it one, sum) for every position of the stretch, in order; `again`: a pass
-  // behind the first.
-  auto walk = [&](bool again, auto f) {
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < kBinCopies; ++k) c[i] += bins[k][n - 1 - 2 * threadIdx.x - i];
+  }
+  find_digit(c, n, need, scan_lds, found);
+}
+
+// The digits, from the most significant one: their shifts, numbers of values and the bits above.
+__device__ __forceinline__ constexpr int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ constexpr int digit_values(int pass) { return pass == 2 ? 1024 : 2048; }
+
+// A row of sums (a sequence in a head) that is cut, and the stretch of it that a wavefront
+// walks.
+struct SelectRow {
+  int len, lo, hi;      // positions; those in [lo, hi) have to earn their place
+  uint32_t places;      // how many of them do (fewer than there are)
+  const float* sums;
+  int32_t* kept;
+  int from, to;         // the wavefront's stretch
+  int lane;
+  bool resident;        // the stretch is held in registers after the first pass
+
+  // f(position, is it one, sum) for every position of the stretch, in order, 64 at a time; the sums
+  // of 64 kSelectLoads positions are loaded at once, and only by the first pass (`again` false)
+  // where that is the whole stretch.
+  template <class F>
+  __device__ __forceinline__ void walk(float (&x)[kSelectLoads], bool again, F f) const {
     for (int j0 = from; j0 < to; j0 += 64 * kSelectLoads) {
-      if (!again || !resident) load(j0);
+      if (!again || !resident) {
+#pragma unroll
+        for (int i = 0; i < kSelectLoads; ++i)
+          if (j0 + 64 * i < to) x[i] = sums[min(j0 + 64 * i + lane, to - 1)];
+      }
 #pragma unroll
       for (int i = 0; i < kSelectLoads; ++i)
         if (j0 + 64 * i < to) f(j0 + 64 * i + lane, j0 + 64 * i + lane < to, x[i]);
     }
-  };
+  }
+  __device__ __forceinline__ bool earns(int j, bool real) const { return real && j >= lo && j < hi; }
+  __device__ __forceinline__ bool given(int j, bool real) const { return real && (j < lo || j >= hi); }
+};
 
-  uint32_t least = 0, need = places;   // the least key that is kept; of its equals, the first `need` are
+// What a row that is cut and one that is not have in common: true for the first.  `part` of
+// `parts` workgroups of the row, a stretch for each of their wavefronts.
+__device__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, bool first_pass, SelectRow* r) {
+  const int t = threadIdx.x, wave = t >> 6, b = row / a.Hkv, h = row % a.Hkv;
+  r->len = min(max(a.lens[b], 0), a.max_len);
+  r->sums = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)h * a.sums_stride_h;
+  r->kept = a.kept + (int64_t)row * a.budget;
+  r->lane = t & 63;
+  if (first_pass && part == 0) {
+    // What orders the workgroups of the compaction behind this, for the keys and the values: a
+    // count of the batches taken, and a word for each batch that has been read.
+    for (int i = t; i < 2 * (1 + a.batches); i += kSelectThreads) a.order[(int64_t)row * 2 * (1 + a.batches) + i] = 0;
+    if (h == 0 && t == 0) a.new_lens[b] = min(r->len, a.budget);
+    if (r->len <= a.budget) {
+      float* const out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
+      for (int j = t; j < a.budget; j += kSelectThreads) r->kept[j] = j < r->len ? j : -1;
+      if (out != r->sums)
+        for (int j = t; j < r->len; j += kSelectThreads) out[j] = r->sums[j];
+    }
+  }
+  if (r->len <= a.budget) return false;
+  r->lo = a.keep_first;
+  r->hi = r->len - a.keep_last;
+  r->places = (uint32_t)(a.budget - a.keep_first - a.keep_last);
+  const int waves = parts * kSelectWaves;
+  const int stretch = (r->len + 64 * waves - 1) / (64 * waves) * 64;
+  r->from = min(r->len, (part * kSelectWaves + wave) * stretch);
+  r->to = min(r->len, r->from + stretch);
+  r->resident = stretch <= 64 * kSelectLoads;
+  return true;
+}
+
+// The last pass: the wavefront's kept positions, behind the `certain` and `ties` ones before its stretch;
+// of the keys equal to `least` the first `need` of the row are kept.
+__device__ __forceinline__ void write_kept(const SelectRow& r, float (&x)[kSelectLoads], uint32_t least, uint32_t need,
+                                           uint32_t certain, uint32_t ties) {
+  const uint64_t below = (1ull << r.lane) - 1;
+  r.walk(x, true, [&](int j, bool real, float v) {
+    const uint32_t key = order_key(v);
+    const bool middle = r.earns(j, real) && r.places > 0;
+    const bool sure = r.given(j, real) || (middle && key > least), tied = middle && key == least;
+    const uint64_t all_sure = __ballot(sure), all_tied = __ballot(tied);
+    const uint32_t before = ties + (uint32_t)__popcll(all_tied & below);
+    // what was kept before it: the certain ones, and of the equal ones at most `need`
+    if (sure || (tied && before < need))
+      r.kept[certain + (uint32_t)__popcll(all_sure & below) + min(before, need)] = j;
+    certain += (uint32_t)__popcll(all_sure);
+    ties += (uint32_t)__popcll(all_tied);
+  });
+}
+
+// Sums over the workgroup's wavefronts before this one, of a pair of counts.
+__device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, uint32_t (*lds)[kSelectWaves]) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    lds[0][wave] = sure;
+    lds[1][wave] = equal;
+  }
+  __syncthreads();
+  sure = equal = 0;
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    if (w < wave) {
+      sure += lds[0][w];
+      equal += lds[1][w];
+    }
+  }
+}
+
+// One workgroup for a row.  The least key that is kept is found digit by digit (11, 11, 10
+// bits) from histograms in LDS.  The first pass reads the sums; the second, when the first
+// digit is known, counts what is kept for certain and lists the keys that share the digit in
+// LDS, where the other two digits are found (the sums are walked again for those when there
+// are too many such keys).  The last pass writes the kept positions down: every wavefront
+// walks a stretch of its own, from the counts of the ones before it.
+__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvictArgs a) {
+  __shared__ uint32_t bins[kBinCopies][kBins];
+  __shared__ uint32_t listed[kSelectWaves][kListed];
+  __shared__ uint32_t scan_lds[kSelectWaves], counts_lds[2][kSelectWaves];
+  __shared__ uint32_t found[2], too_many;
+  const int t = threadIdx.x, wave = t >> 6;
+  SelectRow r;
+  if (!select_row(a, blockIdx.x, 0, 1, true, &r)) return;
+  float x[kSelectLoads];
+  uint32_t least = 0, need = r.places;   // the least key that is kept; of its equals, the first `need` are
   auto clear_bins = [&] {
     for (int i = t; i < kBinCopies * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
     __syncthreads();
   };
+  auto count = [&](uint32_t digit) { atomicAdd(&bins[wave % kBinCopies][digit], 1u); };
   clear_bins();
-  walk(false, [&](int j, bool real, float v) {
-    if (real && j >= lo && j < hi) atomicAdd(&bins[wave % kBinCopies][order_key(v) >> 21], 1u);
+  r.walk(x, false, [&](int j, bool real, float v) {
+    if (r.earns(j, real)) count(order_key(v) >> 21);
   });
   if (t == 0) too_many = 0;
   __syncthreads();
-  if (places > 0) {
-    find_digit(bins, 2048, places, scan_lds, found);
+  if (r.places > 0) {
+    find_digit_lds(bins, 2048, r.places, scan_lds, found);
     least = found[0] << 21;
     need = found[1];
   }
 
   // what this wavefront's stretch keeps for certain, and its candidates
-  uint32_t sure = 0, n_listed = 0;
-  const uint64_t below = (1ull << lane) - 1;
-  walk(true, [&](int j, bool real, float v) {
+  uint32_t sure = 0, equal = 0, n_listed = 0;
+  const uint64_t below = (1ull << r.lane) - 1;
+  r.walk(x, true, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
-    const bool ends = real && (j < lo || j >= hi), middle = real && !ends && places > 0;
-    sure += (uint32_t)__popcll(__ballot(ends || (middle && key >> 21 > least >> 21)));
+    const bool middle = r.earns(j, real) && r.places > 0;
+    sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key >> 21 > least >> 21)));
     const bool candidate = middle && key >> 21 == least >> 21;
     const uint64_t all = __ballot(candidate);
     const uint32_t at = n_listed + (uint32_t)__popcll(all & below);
     if (candidate && at < kListed) listed[wave][at] = key;
     n_listed += (uint32_t)__popcll(all);
   });
-  uint32_t equal = 0;
-  if (places > 0) {
-    if (lane == 0 && n_listed > kListed) too_many = 1;
+  if (r.places > 0) {
+    if (r.lane == 0 && n_listed > kListed) too_many = 1;
     __syncthreads();
     const bool again = too_many != 0;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-      const int shift = pass == 0 ? 10 : 0, n = pass == 0 ? 2048 : 1024;
-      const uint32_t same = pass == 0 ? 21 : 10;    // the bits above agree
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = digit_shift(pass), n = digit_values(pass);
+      const uint32_t same = pass == 1 ? 21 : 10;    // the bits above agree
       clear_bins();
       if (!again) {
-        for (uint32_t i = lane; i < n_listed; i += 64) {
+        for (uint32_t i = r.lane; i < n_listed; i += 64) {
           const uint32_t key = listed[wave][i];
-          if (key >> same == least >> same) atomicAdd(&bins[wave % kBinCopies][(key >> shift) & (n - 1)], 1u);
+          if (key >> same == least >> same) count((key >> shift) & (n - 1));
         }
       } else {
-        walk(true, [&](int j, bool real, float v) {
+        r.walk(x, true, [&](int j, bool real, float v) {
           const uint32_t key = order_key(v);
-          if (real && j >= lo && j < hi && key >> same == least >> same)
-            atomicAdd(&bins[wave % kBinCopies][(key >> shift) & (n - 1)], 1u);
+          if (r.earns(j, real) && key >> same == least >> same) count((key >> shift) & (n - 1));
         });
       }
       __syncthreads();
-      find_digit(bins, n, need, scan_lds, found);
+      find_digit_lds(bins, n, need, scan_lds, found);
       least |= found[0] << shift;
       need = found[1];
       __syncthreads();
     }
     if (!again) {
       for (uint32_t i0 = 0; i0 < n_listed; i0 += 64) {
-        const bool real = i0 + lane < n_listed;
-        const uint32_t key = real ? listed[wave][i0 + lane] : 0u;
+        const bool real = i0 + r.lane < n_listed;
+        const uint32_t key = real ? listed[wave][i0 + r.lane] : 0u;
         sure += (uint32_t)__popcll(__ballot(real && key > least));
         equal += (uint32_t)__popcll(__ballot(real && key == least));
       }
     } else {
-      walk(true, [&](int j, bool real, float v) {
-        const bool middle = real && j >= lo && j < hi;
+      r.walk(x, true, [&](int j, bool real, float v) {
+        const bool middle = r.earns(j, real);
         const uint32_t key = order_key(v);
         sure += (uint32_t)__popcll(__ballot(middle && key > least && key >> 21 == least >> 21));
         equal += (uint32_t)__popcll(__ballot(middle && key == least));
       });
     }
   }
-  if (lane == 0) {
-    sure_of[wave] = sure;
-    equal_of[wave] = equal;
+  counts_before(sure, equal, counts_lds);
+  write_kept(r, x, least, need, sure, equal);
+}
+
+// Few long rows: `parts` workgroups for each, a launch for each digit.  A workgroup counts the
+// digits of its part and leaves the counts in the workspace; the next launch adds the parts' counts
+// up and goes on from the digit found.  What a part keeps for certain follows from the counts as
+// well, so that the last launch knows where each part's positions begin.
+struct SplitRow {
+  uint32_t* counts;   // [3][parts][kBins]
+  uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] certain ones by those
+};
+__device__ __forceinline__ SplitRow split_row(const KvEvictArgs& a, int row) {
+  const int words = 3 * a.parts * kBins + 4 + 2 * a.parts;
+  uint32_t* const base = a.split + (int64_t)row * words;
+  return SplitRow{base, base + 3 * a.parts * kBins};
+}
+
+// Digit `pass` of the least key from the parts' counts; part 0 leaves what is known behind it, every
+// part what it keeps for certain by this digit.
+__device__ void split_digit(const KvEvictArgs& a, const SplitRow& s, int pass, int part, uint32_t& least, uint32_t& need,
+                            uint32_t* scan_lds, uint32_t* found) {
+  const int t = threadIdx.x, n = digit_values(pass);
+  uint32_t c[2] = {0, 0}, mine[2] = {0, 0};
+  if (2 * t < n) {
+    const uint32_t* const from = s.counts + (int64_t)pass * a.parts * kBins + (n - 2 - 2 * t);
+    for (int p = 0; p < a.parts; ++p) {
+      const uint32_t high = from[p * kBins + 1], low = from[p * kBins];
+      c[0] += high;
+      c[1] += low;
+      if (p == part) {
+        mine[0] = high;
+        mine[1] = low;
+      }
+    }
+  }
+  find_digit(c, n, need, scan_lds, found);
+  const uint32_t digit = found[0];
+  least |= digit << digit_shift(pass);
+  need = found[1];
+  uint32_t sure = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (2 * t < n && (uint32_t)(n - 1 - 2 * t - i) > digit) sure += mine[i];
+  sure = wave_scan(sure);
+  if ((t & 63) == 63) scan_lds[t >> 6] = sure;
+  __syncthreads();
+  if (t == 0 && pass < 2) {
+    uint32_t all = 0;
+    for (int w = 0; w < kSelectWaves; ++w) all += scan_lds[w];
+    s.state[4 + pass * a.parts + part] = all;
+    if (part == 0) {
+      s.state[2 * pass] = least;
+      s.state[2 * pass + 1] = need;
+    }
   }
   __syncthreads();
-  uint32_t n_sure = 0, n_equal = 0;     // kept before this wavefront's stretch
-#pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
-    if (w < wave) {
-      n_sure += sure_of[w];
-      n_equal += equal_of[w];
-    }
+}
+
+template <int PASS>
+__global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const KvEvictArgs a) {
+  __shared__ uint32_t bins[kBinCopies][kBins];
+  __shared__ uint32_t scan_lds[kSelectWaves], found[2];
+  const int t = threadIdx.x, wave = t >> 6, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  SelectRow r;
+  if (!select_row(a, row, part, a.parts, PASS == 0, &r) || r.places == 0) return;
+  const SplitRow s = split_row(a, row);
+  uint32_t least = 0, need = r.places;
+  if constexpr (PASS == 2) {
+    least = s.state[0];
+    need = s.state[1];
   }
-  const bool in_place = out == sums;
-  walk(true, [&](int j, bool real, float v) {
+  for (int i = t; i < kBinCopies * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
+  if constexpr (PASS > 0) split_digit(a, s, PASS - 1, part, least, need, scan_lds, found);
+  __syncthreads();
+  float x[kSelectLoads];
+  r.walk(x, false, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
-    const bool ends = real && (j < lo || j >= hi), middle = real && !ends && places > 0;
-    const bool certain = ends || (middle && key > least), tied = middle && key == least;
-    const uint64_t certain_all = __ballot(certain), tied_all = __ballot(tied);
-    const uint32_t ties = n_equal + (uint32_t)__popcll(tied_all & below);
-    if (certain || (tied && ties < need)) {
-      // what was kept before it: the certain ones, and of the equal ones at most `need`
-      const uint32_t at = n_sure + (uint32_t)__popcll(certain_all & below) + min(ties, need);
-      kept[at] = j;
-      if (!in_place) out[at] = v;
-    }
-    n_sure += (uint32_t)__popcll(certain_all);
-    n_equal += (uint32_t)__popcll(tied_all);
+    constexpr uint32_t same = PASS == 1 ? 21 : 10;
+    if (r.earns(j, real) && (PASS == 0 || key >> same == least >> same))
+      atomicAdd(&bins[wave % kBinCopies][(key >> digit_shift(PASS)) & (digit_values(PASS) - 1)], 1u);
   });
   __syncthreads();
-  if (in_place) {
-    // kept[j] >= j: a chunk's sums are all read before any of them is written
-    for (int j0 = 0; j0 < a.budget; j0 += kSelectThreads) {
-      const int j = j0 + t;
-      float x = 0.0f;
-      if (j < a.budget) x = sums[kept[j]];
-      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      if (j < a.budget) out[j] = x;
-    }
-    __syncthreads();
+  uint32_t* const to = s.counts + ((int64_t)PASS * a.parts + part) * kBins;
+  for (int i = t; i < digit_values(PASS); i += kSelectThreads) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kBinCopies; ++k) n += bins[k][i];
+    to[i] = n;
   }
-  for (int j = a.budget + t; j < len; j += kSelectThreads) out[j] = 0.0f;
+}
+
+__global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const KvEvictArgs a) {
+  __shared__ uint32_t scan_lds[kSelectWaves], counts_lds[2][kSelectWaves], found[2];
+  const int t = threadIdx.x, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  SelectRow r;
+  if (!select_row(a, row, part, a.parts, false, &r)) return;
+  const SplitRow s = split_row(a, row);
+  uint32_t least = 0, need = r.places;
+  uint32_t before_sure = 0, before_equal = 0;      // kept in the parts before this one
+  if (r.places > 0) {
+    least = s.state[2];
+    need = s.state[3];
+    split_digit(a, s, 2, part, least, need, scan_lds, found);
+    const uint32_t digit = least & 1023u;
+    uint32_t sure = 0;
+    for (int p = 0; p < part; ++p) {
+      const uint32_t* const counts = s.counts + ((int64_t)2 * a.parts + p) * kBins;
+      if ((uint32_t)t > digit && t < 1024) sure += counts[t];
+      if (t == 0) sure += s.state[4 + p] + s.state[4 + a.parts + p];
+      before_equal += counts[digit];
+    }
+    sure = wave_scan(sure);
+    if ((t & 63) == 63) scan_lds[t >> 6] = sure;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; ++w) before_sure += scan_lds[w];
+  }
+  // (the ends before this part's stretch are kept as well)
+  const int stretch = (r.len + 64 * a.parts * kSelectWaves - 1) / (64 * a.parts * kSelectWaves) * 64;
+  const int begin = min(r.len, part * kSelectWaves * stretch);
+  before_sure += (uint32_t)(min(begin, r.lo) + max(0, begin - r.hi));
+
+  float x[kSelectLoads];
+  uint32_t sure = 0, equal = 0;
+  r.walk(x, false, [&](int j, bool real, float v) {
+    const uint32_t key = order_key(v);
+    const bool middle = r.earns(j, real) && r.places > 0;
+    sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key > least)));
+    equal += (uint32_t)__popcll(__ballot(middle && key == least));
+  });
+  counts_before(sure, equal, counts_lds);
+  write_kept(r, x, least, need, before_sure + sure, before_equal + equal);
 }
 
 // The compaction.  A batch is 32 KB of rows that become neighbours: the keys or the values
@@ -380,15 +538,28 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
     x[i] = *(const u32x4*)(cache + (there ? (int64_t)src_page[i] * a.page_stride + (int64_t)slot * a.slot_stride : 0) +
                            piece[i] * 16);
   }
+  // The rows' sums go with the keys.
+  const bool with_sums = which == 0;
+  const float* const sums = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)h * a.sums_stride_h;
+  float* const sums_out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
+  float sum[kMovePieces / kMoveThreads];
+  if (with_sums) {
+#pragma unroll
+    for (int i = 0; i < kMovePieces / kMoveThreads; ++i)
+      if (i * kMoveThreads < rows) sum[i] = sums[kept[min(first + i * kMoveThreads + t, last - 1)]];
+  }
   // Every read of the batch has arrived: the rows are in registers, and nobody reads in this
   // kernel what another workgroup writes, so that the words need no cache to be written
   // back or invalidated (relaxed, but seen by the whole card).
   __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (t == 0) __hip_atomic_store(read + batch, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  // earlier batches with a source among the rows first .. last - 1
+  // earlier batches with a source among the rows first .. last - 1 (and, before the sums behind the
+  // last row are cleared, those with a source there)
+  const bool clears = with_sums && batch == a.batches - 1;
   for (int c = t; c < batch; c += kMoveThreads) {
-    if (kept[c * rows] < last && kept[c * rows + rows - 1] >= first)
+    const int c_last = kept[c * rows + rows - 1];
+    if ((kept[c * rows] < last && c_last >= first) || (clears && c_last >= a.budget))
       while (__hip_atomic_load(read + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
   }
   __syncthreads();
@@ -397,6 +568,15 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
     const int slot = dst[i] - divided(dst[i], a.by_page) * a.page_size;
     if (moves[i])
       *(u32x4*)(cache + (int64_t)dst_page[i] * a.page_stride + (int64_t)slot * a.slot_stride + piece[i] * 16) = x[i];
+  }
+  if (with_sums) {
+#pragma unroll
+    for (int i = 0; i < kMovePieces / kMoveThreads; ++i) {
+      const int j = first + i * kMoveThreads + t;
+      if (i * kMoveThreads < rows && i * kMoveThreads + t < rows && j < last) sums_out[j] = sum[i];
+    }
+    if (clears)
+      for (int j = a.budget + t; j < len; j += kMoveThreads) sums_out[j] = 0.0f;
   }
 }
 
@@ -420,12 +600,38 @@ int kv_evict_batches(int budget, int row_bytes) {
   return (budget + rows - 1) / rows;
 }
 
+int kv_evict_parts(int rows, int max_len) {
+  // A workgroup walks a row of 8192 positions in 20 us; below that, and with a row for every CU,
+  // the launches of the split form cost more than they save.
+  if (max_len <= 8192 || rows > 128) return 1;
+  const int most = (max_len + 4095) / 4096;
+  return min(min(256 / rows, most), 16);
+}
+
+size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget) {
+  const size_t order = 2 * (size_t)rows * (1 + kv_evict_batches(budget, row_bytes));
+  const int parts = kv_evict_parts(rows, max_len);
+  return 4 * (order + (parts > 1 ? (size_t)rows * (3 * parts * kBins + 4 + 2 * parts) : 0));
+}
+
 void launch_kv_evict(const KvEvictArgs& args, hipStream_t stream) {
   KvEvictArgs a = args;
+  const int rows = a.B * a.Hkv;
   a.by_page = fast_div(a.page_size);
   a.by_pieces = fast_div(a.row_bytes / 16);
-  hipLaunchKernelGGL(kv_select_kernel, dim3(a.B * a.Hkv), dim3(kSelectThreads), 0, stream, a);
-  hipLaunchKernelGGL(kv_move_kernel, dim3(2 * a.B * a.Hkv * a.batches), dim3(kMoveThreads), 0, stream, a);
+  a.batches = kv_evict_batches(a.budget, a.row_bytes);
+  a.parts = kv_evict_parts(rows, a.max_len);
+  a.split = a.order + 2 * (size_t)rows * (1 + a.batches);
+  if (a.parts == 1) {
+    hipLaunchKernelGGL(kv_select_kernel, dim3(rows), dim3(kSelectThreads), 0, stream, a);
+  } else {
+    const dim3 grid(rows * a.parts), block(kSelectThreads);
+    hipLaunchKernelGGL((kv_select_digit_kernel<0>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((kv_select_digit_kernel<1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((kv_select_digit_kernel<2>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL(kv_select_keep_kernel, grid, block, 0, stream, a);
+  }
+  hipLaunchKernelGGL(kv_move_kernel, dim3(2 * rows * a.batches), dim3(kMoveThreads), 0, stream, a);
 }
 
 }  // namespace vk

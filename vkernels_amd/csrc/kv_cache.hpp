@@ -40,11 +40,15 @@ struct KvEvictArgs {
   int64_t page_stride, head_stride, slot_stride;            // bytes
   int table_stride, num_pages, page_size, row_bytes;
   int B, Hkv, max_len, budget, keep_first, keep_last;
-  uint32_t* order;          // workspace: for the keys and values of every head a count and a word for each batch
-  int batches;              // of kv_evict_batches
-  FastDiv by_page, by_pieces;                               // (set by the launcher)
+  uint32_t* order;          // the workspace: for the keys and values of every head a count and a word for
+                            // each batch; behind it what the split selection leaves between its launches
+  // (set by the launcher)
+  uint32_t* split;
+  int batches, parts;
+  FastDiv by_page, by_pieces;
 };
 int kv_evict_batches(int budget, int row_bytes);   // of the keys (or values) of a head
+size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget);
 void launch_kv_evict(const KvEvictArgs& a, hipStream_t stream);
 
 }  // namespace vk

@@ -145,9 +145,10 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   return launched(who, before);
 }
 
-size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int budget) {
+size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget) {
   if (elem_bytes <= 0 || B <= 0 || Hkv <= 0 || D < 16 || budget <= 0 || D * (int64_t)elem_bytes > 512) return 0;
-  return 4 * 2 * static_cast<size_t>(B) * Hkv * (1 + vk::kv_evict_batches(budget, D * elem_bytes));
+  if (static_cast<int64_t>(B) * Hkv > kInt32) return 0;
+  return vk::kv_evict_workspace_bytes(B * Hkv, D * elem_bytes, max_len, budget);
 }
 
 int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
@@ -178,7 +179,7 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
       (int64_t)B * Hkv * vk::kv_evict_batches(budget, D * elem_bytes) > kInt32 / 2)
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many rows for one call");
   if (workspace == nullptr || !aligned(workspace, 4) ||
-      workspace_bytes < vk_hip_kv_cache_evict_workspace_bytes(elem_bytes, B, Hkv, D, budget))
+      workspace_bytes < vk_hip_kv_cache_evict_workspace_bytes(elem_bytes, B, Hkv, D, max_len, budget))
     return refuse(VK_ERROR_INVALID_ARGUMENT, who, "a workspace of vk_hip_kv_cache_evict_workspace_bytes is needed");
   vk::KvEvictArgs a{};
   a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
@@ -190,7 +191,6 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
   a.table_stride = table_stride; a.num_pages = num_pages; a.page_size = page_size; a.row_bytes = D * elem_bytes;
   a.B = B; a.Hkv = Hkv; a.max_len = max_len; a.budget = budget; a.keep_first = keep_first; a.keep_last = keep_last;
   a.order = static_cast<uint32_t*>(workspace);
-  a.batches = vk::kv_evict_batches(budget, a.row_bytes);
   const hipError_t before = hipPeekAtLastError();
   vk::launch_kv_evict(a, static_cast<hipStream_t>(stream));
   return launched(who, before);

@@ -43,7 +43,7 @@ def _fn(name):
             "vk_hip_kv_cache_append": ([_P] * 9 + [_I] * 9 + [_L] * 7 + [_P], _I),
             "vk_hip_paged_attention_workspace_bytes": ([_I] * 7, _Z),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
-            "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 5, _Z),
+            "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 6, _Z),
             "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P, _Z, _P], _I),
         }[name]
         try:
@@ -234,7 +234,7 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     new_lens = torch.empty_like(seq_lens)
     kept = seq_lens.new_empty((B, Hkv, max(budget, 0)))
     elem = k_cache.element_size()
-    size = _fn("vk_hip_kv_cache_evict_workspace_bytes")(elem, B, Hkv, D, budget)
+    size = _fn("vk_hip_kv_cache_evict_workspace_bytes")(elem, B, Hkv, D, max_len, budget)
     workspace = torch.empty(size, dtype=torch.uint8, device=k_cache.device)
     ss, so = weight_sums.stride(), sums_out.stride()
     status = _fn("vk_hip_kv_cache_evict")(
