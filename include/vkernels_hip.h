@@ -713,7 +713,7 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
  * at most table_width * page_size; launches and workspace follow it, not the lengths.
  * The workspace (16-byte aligned) of vk_hip_paged_attention_workspace_bytes is scratch of
  * this call alone; 0 bytes: none is needed.  Deterministic: no atomics. */
-size_t vk_hip_paged_attention_workspace_bytes(int B, int Hkv, int G, int D, int max_len, int window,
+size_t vk_hip_paged_attention_workspace_bytes(int kind, int B, int Hkv, int G, int D, int max_len, int window,
                                               int counted);
 int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cache,
                            const int32_t* block_table, const int32_t* seq_lens, const float* sinks,

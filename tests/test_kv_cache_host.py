@@ -86,9 +86,9 @@ def test_calls_with_nothing_to_do(lib, name):
 
 def test_workspace_bytes(lib):
     size = kv._fn("vk_hip_paged_attention_workspace_bytes")
-    assert size(0, 8, 4, 64, 1000, 0, 0) == 0
-    assert size(64, 8, 4, 64, 100, 0, 0) == 0              # short calls need none
-    plain, counted = size(64, 8, 4, 128, 8192, 0, 0), size(64, 8, 4, 128, 8192, 0, 1)
+    assert size(0, 0, 8, 4, 64, 1000, 0, 0) == 0
+    assert size(0, 64, 8, 4, 64, 100, 0, 0) == 0              # short calls need none
+    plain, counted = size(0, 64, 8, 4, 128, 8192, 0, 0), size(0, 64, 8, 4, 128, 8192, 0, 1)
     assert 0 < plain < counted
     assert counted >= plain + 4 * 64 * 32 * 8192           # every score is kept
-    assert size(64, 8, 4, 128, 100, 0, 1) >= 4 * 64 * 32 * 100
+    assert size(0, 64, 8, 4, 128, 100, 0, 1) >= 4 * 64 * 32 * 100

@@ -90,9 +90,10 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
   return launched(who, before);
 }
 
-size_t vk_hip_paged_attention_workspace_bytes(int B, int Hkv, int G, int D, int max_len, int window, int counted) {
-  if (B <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0) return 0;
-  return vk::paged_attention_plan(B, Hkv, G, D, max_len, window, counted != 0).bytes;
+size_t vk_hip_paged_attention_workspace_bytes(int kind, int B, int Hkv, int G, int D, int max_len, int window,
+                                              int counted) {
+  if (!known_kind(kind) || B <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0) return 0;
+  return vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, counted != 0).bytes;
 }
 
 int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -126,7 +127,7 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   if ((int64_t)B * Hkv > kInt32 / G ||
       (int64_t)B * Hkv * ((G + vk::kPaHeads - 1) / vk::kPaHeads) > kInt32 / (max_len / vk::kPaUnit + 3) / 2)
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, heads and positions for one call");
-  const vk::PagedAttentionPlan plan = vk::paged_attention_plan(B, Hkv, G, D, max_len, window, weight_sums != nullptr);
+  const vk::PagedAttentionPlan plan = vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, weight_sums != nullptr);
   if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
     return refuse(VK_ERROR_INVALID_ARGUMENT, who,
                   "a workspace of vk_hip_paged_attention_workspace_bytes (16-byte aligned) is needed");

@@ -9,6 +9,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+#include <type_traits>
+
 #include "fast_div.hpp"
 #include "paged_attention.hpp"
 
@@ -27,6 +30,7 @@ constexpr float kNegInf = -__builtin_inff();
 // The reference of the exponentials is moved when the scores pass it by more than 2^8: weights of
 // up to 256 cost no accuracy, and few tiles then have to rescale what they have summed.
 constexpr float kSlack = 8.0f;
+constexpr int kAhead = 4;    // value tiles that are read from LDS ahead of their products
 
 // The 16-bit type that the matrix instructions multiply in.
 struct Bf16 {
@@ -97,6 +101,10 @@ __device__ __forceinline__ float log_of_sum(float ref, float ll, const float* si
 }
 __device__ __forceinline__ float or_zero(float m) { return m == kNegInf ? 0.0f : m; }
 
+// An array of int32 that the kernel only reads: through the scalar cache where the index is uniform.
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+__device__ __forceinline__ ConstInts read_only(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
+
 // What a work item (16 heads of one sequence) sees of its cache.
 struct Span {
   int start;   // first position, rounded down to 16
@@ -110,6 +118,15 @@ __device__ __forceinline__ Span span_of(int len, int max_len, int window) {
   s.start = s.lo & ~15;
   s.units = max(1, (s.len - s.start + kPaUnit - 1) / kPaUnit);
   return s;
+}
+
+// Workgroups of a CU (wavefronts of a SIMD), by the registers that a width needs: the grid is as
+// many as the card holds at once.
+constexpr int residents(int DP) { return DP <= 128 ? 2 : 1; }
+int padded_width(int D, bool fp8) {
+  if (D <= 64) return 64;
+  if (D <= 96 && !fp8) return 96;
+  return D <= 128 ? 128 : D <= 192 ? 192 : 256;
 }
 
 struct KernelArgs {
@@ -127,53 +144,52 @@ struct Share {
   int b, unit0;      // the sequence that `first` lies in, and its first unit
 };
 
-// Every workgroup finds its share by itself from the lengths: a thread adds up the units
-// of B / 256 sequences, a scan over the threads, and the thread that holds `first` walks on.
-__device__ bool find_share(const KernelArgs& A, Share* sh, int* lds) {
+// Inclusive sum over the lanes of a wavefront up to this one.
+__device__ __forceinline__ int lanes_up_to(int x) {
+#define VK_ADD_FROM(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, true)
+  VK_ADD_FROM(0x111, 0xF);   // the lane 1, 2, 4, 8 below, within rows of 16
+  VK_ADD_FROM(0x112, 0xF);
+  VK_ADD_FROM(0x114, 0xF);
+  VK_ADD_FROM(0x118, 0xF);
+  VK_ADD_FROM(0x142, 0xA);   // lane 15 of rows 0 and 2 to rows 1 and 3
+  VK_ADD_FROM(0x143, 0xC);   // lane 31 to rows 2 and 3
+#undef VK_ADD_FROM
+  return x;
+}
+
+// Every wavefront finds its workgroup's share by itself from the lengths: a lane adds up the units of
+// B / 64 sequences, a scan over the lanes finds the lane that holds `first`, which walks on.  (No
+// LDS and no barrier: this is all latency, in front of the first load of a key.)
+__device__ __forceinline__ bool find_share(const KernelArgs& A, Share* sh) {
   const PagedAttentionArgs& a = A.a;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int lane = threadIdx.x & 63;
   const int heads = a.Hkv * A.p.head_tiles;
-  const int per = (a.B + 255) / 256;
+  const int per = (a.B + 63) / 64;
   int mine = 0;
   for (int i = 0; i < per; ++i) {
-    const int b = t * per + i;
+    const int b = lane * per + i;
     if (b < a.B) mine += span_of(a.lens[b], a.max_len, a.window).units;
   }
-  int scan = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int up = __shfl_up(scan, d);
-    if (lane >= d) scan += up;
-  }
-  if (lane == 63) lds[wave] = scan;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kPaWaves; ++w) {
-    if (w < wave) before += lds[w];
-    total += lds[w];
-  }
-  total *= heads;
+  const int scan = lanes_up_to(mine);
+  const int total = __builtin_amdgcn_readlane(scan, 63) * heads;
   const int share = max(A.p.min_units, (total + A.p.workgroups - 1) / A.p.workgroups);
   const int first = (int)blockIdx.x * share;
   if (first >= total) return false;   // (uniform over the workgroup)
-  int at = (before + scan - mine) * heads;
-  if (first >= at && first < at + mine * heads) {
-    int b = t * per;
+  int at = (scan - mine) * heads, b = lane * per;
+  const bool here = first >= at && first < at + mine * heads;
+  if (here && per > 1) {
     for (;; ++b) {
       const int units = span_of(a.lens[b], a.max_len, a.window).units * heads;
       if (first < at + units) break;
       at += units;
     }
-    lds[4] = b;
-    lds[5] = at;
   }
-  __syncthreads();
+  const int owner = (int)__builtin_ctzll(__ballot(here));
   sh->first = first;
   sh->last = min(total, first + share);
   sh->per = share;
-  sh->b = lds[4];
-  sh->unit0 = lds[5];
+  sh->b = __builtin_amdgcn_readlane(b, owner);
+  sh->unit0 = __builtin_amdgcn_readlane(at, owner);
   return true;
 }
 
@@ -193,13 +209,6 @@ struct Tile {
                                       ? kPaWaveRows * kPitch : kPaHeads * kOutPitch * 4;
 };
 
-#ifndef OCC64
-#define OCC64 4
-#define OCC128 2
-#define OCC256 1
-#endif
-// Workgroups of a CU (wavefronts of a SIMD), by the registers that a width needs.
-constexpr int residents(int DP) { return DP <= 64 ? OCC64 : DP <= 128 ? OCC128 : OCC256; }
 
 template <class M, bool FP8, int DP, bool P16, bool FULL>
 __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(const KernelArgs A) {
@@ -208,7 +217,6 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
   const PagedAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[kPaWaves * L::kWaveLds];
   __shared__ float wave_m[kPaWaves][kPaHeads], wave_l[kPaWaves][kPaHeads];
-  __shared__ int share_lds[8];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -218,14 +226,19 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
 
   Share sh;
   int item_in_b = 0;
+  u32x4* const ends_here = (u32x4*)((char*)a.workspace + A.p.ends_at) + blockIdx.x;
   if (A.p.workgroups > 0) {
-    if (!find_share(A, &sh, share_lds)) return;
+    if (!find_share(A, &sh)) {
+      if (threadIdx.x == 0) *ends_here = u32x4{0, 0, 0, 0};
+      return;
+    }
   } else {
     sh.first = 0;
     sh.b = blockIdx.x / item_heads;
     item_in_b = blockIdx.x % item_heads;
   }
-  Span span = span_of(a.lens[sh.b], a.max_len, a.window);
+  const ConstInts lens = read_only(a.lens);
+  Span span = span_of(lens[sh.b], a.max_len, a.window);
   int unit_at;         // unit of the item that the segment begins with
   int left;            // units of the share that are left
   if (A.p.workgroups > 0) {
@@ -239,13 +252,20 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
   }
   int b = sh.b;
   int item_unit0 = A.p.workgroups > 0 ? sh.first - unit_at : 0;   // the item's first unit
+  if (A.p.workgroups > 0 && threadIdx.x == 0) {
+    // For the join: the item that other workgroups began and this one ends, if there is one.
+    const bool ends = unit_at > 0 && span.units - unit_at <= left;
+    const int begun = item_unit0 / sh.per;
+    *ends_here = u32x4{(uint32_t)(b * item_heads + item_in_b), (uint32_t)begun,
+                       ends ? (uint32_t)((int)blockIdx.x - begun + 1) : 0u, 0u};
+  }
 
   const int64_t slot_bytes = a.slot_stride * L::kElem, page_bytes = a.page_stride * L::kElem;
   while (left > 0) {
     const int units = min(left, span.units - unit_at);
     const int g = item_in_b / A.p.head_tiles, head0 = (item_in_b % A.p.head_tiles) * kPaHeads;
     const int heads = min(kPaHeads, a.G - head0);
-    const int32_t* const pages = a.table + (int64_t)b * a.table_stride;
+    const ConstInts pages = read_only(a.table + (int64_t)b * a.table_stride);
     const char* const kbase = (const char*)a.k_cache + (int64_t)g * a.head_stride * L::kElem;
     const char* const vbase = (const char*)a.v_cache + (int64_t)g * a.head_stride * L::kElem;
 
@@ -254,13 +274,14 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     // in two operands; the keys below are dealt out alike).
     V8 q[L::kSteps];
     {
-      const char* row = (const char*)a.q + ((int64_t)b * a.q_stride_b + (int64_t)(g * a.G + head0 + col) * a.q_stride_h) * 2;
+      // (a lane without a head or past the width reads the first values instead)
+      const int64_t head = (int64_t)(g * a.G + head0 + min(col, heads - 1)) * a.q_stride_h;
+      const char* const row = (const char*)a.q + ((int64_t)b * a.q_stride_b + head) * 2;
 #pragma unroll
       for (int i = 0; i < L::kSteps; ++i) {
         const int d = FP8 ? (i / 2) * 64 + quad * 16 + (i % 2) * 8 : i * 32 + quad * 8;
-        u32x4 x = {0, 0, 0, 0};
-        if (col < heads && d < a.D) x = *(const u32x4*)(row + d * 2);
-        q[i] = as_v8<M>(x);
+        const u32x4 x = *(const u32x4*)(row + (d < a.D ? d : 0) * 2);
+        q[i] = as_v8<M>(col < heads && d < a.D ? x : u32x4{0, 0, 0, 0});
       }
     }
     const float k_scale = a.k_scale != nullptr ? a.k_scale[g] : 1.0f;
@@ -274,33 +295,46 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     float m = kNegInf, l = 0.0f;
 
     u32x4 kreg[2][L::kKLoads], vreg[L::kVLoads];
-    // Of the tile that is loaded: which positions count (one page id per 16 positions where
-    // pages are multiples of 16 long, else one per lane).
-    int page0 = -1, page1 = -1;      // P16
-    int64_t row_at = 0;              // else: bytes from the cache's start to position lane % 32
-    bool row_ok = false;
-
     const int begin = span.start + unit_at * kPaUnit + wave * kPaWaveRows;
-    const int end = span.start + (unit_at + units) * kPaUnit;
+    const int end = min(span.start + (unit_at + units) * kPaUnit, span.len);   // no tile is wholly behind it
 
-    auto find_pages = [&](int pos0) {
+    // The table's entries of a tile, asked for a tile ahead of the loads that need them (one for
+    // each 16 positions where pages are multiples of 16 long, else one a lane: position lane % 32);
+    // -1 behind the length.  The last entry stands in for those that the table does not have.
+    const int last_entry = page_of(A, max(span.len - 1, 0));
+    int ids[2] = {-1, -1};
+    auto ask_pages = [&](int pos0) {
       if constexpr (P16) {
-        const int i0 = page_of(A, pos0), i1 = page_of(A, pos0 + 16);
-        page0 = pos0 < span.len ? pages[i0] : -1;
-        page1 = pos0 + 16 < span.len ? pages[i1] : -1;
-        if ((uint32_t)page0 >= (uint32_t)a.num_pages) page0 = -1;
-        if ((uint32_t)page1 >= (uint32_t)a.num_pages) page1 = -1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int id = pages[min(page_of(A, pos0 + 16 * t), last_entry)];
+          ids[t] = pos0 + 16 * t < span.len ? id : -1;
+        }
       } else {
         const int pos = pos0 + (lane & 31);
-        row_ok = pos >= span.lo && pos < span.len;
-        int page = 0, in_table = 0;
-        if (row_ok) {
-          in_table = page_of(A, pos);
-          page = pages[in_table];
-          row_ok = (uint32_t)page < (uint32_t)a.num_pages;
-          if (!row_ok) page = 0;
+        const int id = (a.table + (int64_t)b * a.table_stride)[min(page_of(A, pos), last_entry)];
+        ids[0] = pos >= span.lo && pos < span.len ? id : -1;
+      }
+    };
+    // Of the tile that is loaded: its pages (P16), or where the lane's position lies.
+    int page0 = -1, page1 = -1;
+    int64_t half_at[2] = {0, 0};     // bytes from the cache's start to positions 0 and 16 of the tile
+    int64_t row_at = 0;
+    bool row_ok = false;
+    auto take_pages = [&](int pos0) {
+      if constexpr (P16) {
+        page0 = (uint32_t)ids[0] < (uint32_t)a.num_pages ? ids[0] : -1;
+        page1 = (uint32_t)ids[1] < (uint32_t)a.num_pages ? ids[1] : -1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int pos = pos0 + 16 * t;
+          half_at[t] = (int64_t)max(t == 0 ? page0 : page1, 0) * page_bytes +
+                       (uint32_t)(pos - page_of(A, pos) * a.page_size) * (uint64_t)(uint32_t)slot_bytes;
         }
-        row_at = row_ok ? (int64_t)page * page_bytes + (int64_t)(pos - in_table * a.page_size) * slot_bytes : 0;
+      } else {
+        const int pos = pos0 + (lane & 31);
+        row_ok = (uint32_t)ids[0] < (uint32_t)a.num_pages;
+        row_at = row_ok ? (int64_t)ids[0] * page_bytes + (int64_t)(pos - page_of(A, pos) * a.page_size) * slot_bytes : 0;
       }
     };
     // Where a row of the loaded tile lies (generic pages), from the lane that looked it up.
@@ -321,43 +355,30 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     const int piece = lane % L::kPieces, sub = lane / L::kPieces;
     const uint32_t value_at = FULL ? piece * 16 : (piece * 16 < row_bytes ? piece * 16 : 0);
     const uint32_t key_lane = (uint32_t)col * (uint32_t)slot_bytes, value_lane = (uint32_t)sub * (uint32_t)slot_bytes + value_at;
-    auto half_tile = [&](int pos0, int page) -> int64_t {   // bytes to the row of position pos0
-      return (int64_t)max(page, 0) * page_bytes + (int64_t)(pos0 - page_of(A, pos0) * a.page_size) * slot_bytes;
-    };
-    auto load_k = [&](int pos0) {
+    auto load_k = [&] {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const char* row;
-        if constexpr (P16) row = kbase + half_tile(pos0 + 16 * t, t == 0 ? page0 : page1) + key_lane;
-        else row = kbase + row_from(16 * t + col);
+        const char* const row = P16 ? kbase + half_at[t] + key_lane : kbase + row_from(16 * t + col);
 #pragma unroll
         for (int i = 0; i < L::kKLoads; ++i) kreg[t][i] = key_piece(row, i);
       }
     };
-    auto load_v = [&](int pos0) {
-      if constexpr (P16) {
+    auto load_v = [&] {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const char* rows = vbase + half_tile(pos0 + 16 * t, t == 0 ? page0 : page1);
-#pragma unroll
-          for (int i = 0; i < L::kVLoads / 2; ++i)
-            vreg[t * (L::kVLoads / 2) + i] =
-                *(const u32x4*)(rows + (int64_t)(i * L::kRowsPerLoad) * slot_bytes + value_lane);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < L::kVLoads; ++i)
+      for (int i = 0; i < L::kVLoads; ++i) {
+        constexpr int kHalf = L::kVLoads / 2;
+        if constexpr (P16)
+          vreg[i] = *(const u32x4*)(vbase + (half_at[i / kHalf] + (int64_t)(i % kHalf * L::kRowsPerLoad) * slot_bytes) +
+                                    value_lane);
+        else
           vreg[i] = *(const u32x4*)(vbase + row_from(i * L::kRowsPerLoad + sub) + value_at);
       }
     };
 
-    if (begin < end) {
-      find_pages(begin);
-      load_k(begin);
-      load_v(begin);
-    }
-    for (int pos0 = begin; pos0 < end; pos0 += kPaUnit) {
-      const bool more = pos0 + kPaUnit < end;
+    // One tile; with MORE behind it, the next one's keys are asked for as soon as this one's have
+    // been multiplied, its values as soon as this one's are in LDS.
+    auto tile = [&](int pos0, auto more) {
+      constexpr bool MORE = decltype(more)::value;
       // which of the 8 positions of this lane count, and which value rows it loaded do
       bool whole;
       uint32_t rows;        // bit r: position pos0 + r counts
@@ -391,9 +412,10 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
           for (int i = 0; i < L::kKLoads; ++i) s[t] = M::mfma(as_v8<M>(kreg[t][i]), q[i], s[t]);
         }
       }
-      if (more) {
-        find_pages(pos0 + kPaUnit);
-        load_k(pos0 + kPaUnit);
+      if constexpr (MORE) {
+        take_pages(pos0 + kPaUnit);
+        load_k();
+        ask_pages(pos0 + 2 * kPaUnit);
       }
 
       // scores in powers of two
@@ -423,12 +445,6 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             if (!((rows >> (t * 16 + quad * 4 + r)) & 1u)) x[t * 4 + r] = kNegInf;
-      }
-      if (A.p.score_pitch > 0 && col < heads) {
-        float* to = (float*)((char*)a.workspace + A.p.scores_at) +
-                    ((int64_t)(b * a.Hkv + g) * a.G + head0 + col) * A.p.score_pitch + pos0 + quad * 4;
-        if (pos0 + quad * 4 < span.len) *(f32x4*)to = f32x4{x[0], x[1], x[2], x[3]};
-        if (pos0 + 16 + quad * 4 < span.len) *(f32x4*)(to + 16) = f32x4{x[4], x[5], x[6], x[7]};
       }
       float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
       top = over_column_max(top);
@@ -465,7 +481,16 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
           *(u32x4*)(my_lds + row * L::kPitch + ((piece ^ turn) * 16)) = vreg[i];
         }
       }
-      if (more) load_v(pos0 + kPaUnit);
+      // The scores, where the positions' weights are wanted: [16 positions][head][position], what a
+      // wavefront holds in one piece.  (A row for each head, 64 KB apart at 16384 positions, cost
+      // 20 % of the kernel's time.)
+      if (A.p.score_pitch > 0 && col < heads) {
+        float* const to = (float*)((char*)a.workspace + A.p.scores_at) + quad * 4 +
+                          (((int64_t)(b * a.Hkv + g) * A.p.score_pitch + pos0) * a.G + (head0 + col) * 16);
+        if (pos0 + quad * 4 < span.len) *(f32x4*)to = f32x4{x[0], x[1], x[2], x[3]};
+        if (pos0 + 16 + quad * 4 < span.len) *(f32x4*)(to + 16 * a.G) = f32x4{x[4], x[5], x[6], x[7]};
+      }
+      if constexpr (MORE) load_v();
       // (lanes read what other lanes of their wavefront wrote: LDS keeps the order, and so must the compiler)
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -478,30 +503,59 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         const int turn = L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 7 & (L::kPieces - 1) : 0;
         const int at = row * L::kPitch + (col & 1) * 8;
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) i32x2*)(my_lds + at + ((i ^ turn) * 16)));
-          const V8 v = fp8x8<M>((uint32_t)c[0], (uint32_t)c[1]);
-          acc[i] = M::mfma(v, hi.v, acc[i]);
-          acc[i] = M::mfma(v, lo.v, acc[i]);
+        for (int i0 = 0; i0 < DP / 16; i0 += kAhead) {
+          i32x2 c[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            if (i0 + i < DP / 16)
+              c[i] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                  (__attribute__((address_space(3))) i32x2*)(my_lds + at + (((i0 + i) ^ turn) * 16)));
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i < DP / 16) {
+              const V8 v = fp8x8<M>((uint32_t)c[i][0], (uint32_t)c[i][1]);
+              acc[i0 + i] = M::mfma(v, hi.v, acc[i0 + i]);
+              acc[i0 + i] = M::mfma(v, lo.v, acc[i0 + i]);
+            }
+          }
         }
       } else {
         const int row = quad * 4 + (col >> 2);
         const int turn = L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 3 : 0;
         const int at = row * L::kPitch + (col & 3) * 8;
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          union { i16x4 h[2]; V8 v; } c;
-          char* const from = my_lds + at + ((i ^ turn) * 32);
-          c.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)from);
-          c.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) i16x4*)(from + 16 * L::kPitch));
-          acc[i] = M::mfma(c.v, hi.v, acc[i]);
-          acc[i] = M::mfma(c.v, lo.v, acc[i]);
+        for (int i0 = 0; i0 < DP / 16; i0 += kAhead) {
+          union { i16x4 h[2]; V8 v; } c[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i < DP / 16) {
+              char* const from = my_lds + at + (((i0 + i) ^ turn) * 32);
+              c[i].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)from);
+              c[i].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) i16x4*)(from + 16 * L::kPitch));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i < DP / 16) {
+              acc[i0 + i] = M::mfma(c[i].v, hi.v, acc[i0 + i]);
+              acc[i0 + i] = M::mfma(c[i].v, lo.v, acc[i0 + i]);
+            }
+          }
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
+    };
+    if (begin < end) {
+      ask_pages(begin);
+      take_pages(begin);
+      load_k();
+      ask_pages(begin + kPaUnit);
+      load_v();
+      int pos0 = begin;
+      for (; pos0 + kPaUnit < end; pos0 += kPaUnit) tile(pos0, std::true_type{});
+      tile(pos0, std::false_type{});
     }
 
     // The four wavefronts' sums, joined in LDS.
@@ -519,10 +573,9 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     const int item = b * item_heads + item_in_b;
     const bool begins = unit_at == 0, ends = unit_at + units == span.units;
     const bool alone = begins && ends;
-    int64_t* const meta = (int64_t*)((char*)a.workspace + A.p.meta_at);
     if (A.p.workgroups > 0 && begins && threadIdx.x == 0) {
       const int count = (item_unit0 + span.units - 1) / sh.per - (int)blockIdx.x + 1;
-      meta[item] = ((int64_t)count << 32) | blockIdx.x;
+      ((int64_t*)((char*)a.workspace + A.p.meta_at))[item] = ((int64_t)count << 32) | blockIdx.x;
     }
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
     const int pairs = a.D / 4;
@@ -569,119 +622,214 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     if (left > 0 && ++item_in_b == item_heads) {
       item_in_b = 0;
       ++b;
-      span = span_of(a.lens[b], a.max_len, a.window);
+      span = span_of(lens[b], a.max_len, a.window);
     }
     if (left > 0) __syncthreads();   // (the sums are read before the next item's values come)
   }
 }
 
-// Reference and sum of a head over the partial results of its item, the sink included; every
-// lane of the wavefront gets them.  `first`: the workgroup whose share begins the item.
-__device__ __forceinline__ f32x2 joined_stats(const f32x2* ml, int first, int count, int h, float sink) {
+// The slot of partial result p of an item whose first share is workgroup `first`'s.
+__device__ __forceinline__ int slot_of(int first, int p) { return 2 * (first + p) + (p == 0 ? 1 : 0); }
+
+// Reference and sum of a head over the partial results of its item (`ml`: of slot 0), the sink
+// included; every lane of the wavefront gets them.  `first`: the workgroup whose share begins the item.
+__device__ __forceinline__ f32x2 joined_stats(const f32x2* ml, int first, int count, float sink) {
   const int lane = threadIdx.x & 63;
-  float m = sink;
-  for (int p = lane; p < count; p += 64) m = fmaxf(m, ml[(2 * (first + p) + (p == 0 ? 1 : 0)) * kPaHeads + h][0]);
+  f32x2 x = {kNegInf, 0.0f};
+  if (lane < count) x = ml[slot_of(first, lane) * kPaHeads];
+  float m = fmaxf(sink, x[0]);
+  for (int p = lane + 64; p < count; p += 64) m = fmaxf(m, ml[slot_of(first, p) * kPaHeads][0]);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
   const float ref = or_zero(m);
-  float l = lane == 0 ? exp2_fast(sink - ref) : 0.0f;
-  for (int p = lane; p < count; p += 64) {
-    const f32x2 x = ml[(2 * (first + p) + (p == 0 ? 1 : 0)) * kPaHeads + h];
-    l += x[1] * exp2_fast(x[0] - ref);
+  float l = (lane == 0 ? exp2_fast(sink - ref) : 0.0f) + x[1] * exp2_fast(x[0] - ref);
+  for (int p = lane + 64; p < count; p += 64) {
+    const f32x2 y = ml[slot_of(first, p) * kPaHeads];
+    l += y[1] * exp2_fast(y[0] - ref);
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
   return f32x2{ref, l};
 }
 
-// Joins the items that several workgroups had a share of (a workgroup per head: blocks below
-// `join_blocks`) and adds up the weights that the positions received (the other blocks: 1024
-// positions of a key/value head each).
-template <class M>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(const KernelArgs A, int padded, int join_blocks,
-                                                                   int chunks) {
+// Joins the items that several workgroups had a share of.  Where there are few items (SPLIT 4) a
+// block takes one head of an item, and its four wavefronts share the partial results; else a
+// block looks at the item that ends in workgroup blockIdx.x / groups' share (there is at most one
+// that others began) and takes four of its heads, a wavefront each: a block for every item would
+// find nothing to do more often than not.  A lane holds four values of the head; where the width
+// leaves lanes over, they take other partial results.
+// All latency: the partial results of a first round are asked for before the references are known.
+template <class M, int SPLIT>
+__device__ __forceinline__ void join_heads(const KernelArgs& A, int padded, int groups, f32x4 (*joined)[64]) {
   const PagedAttentionArgs& a = A.a;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t* const meta = (const int64_t*)((const char*)a.workspace + A.p.meta_at);
-  const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at);
-  const int Hq = a.Hkv * a.G;
-  __shared__ float o_lds[kPaWaves][256];
-  __shared__ f32x2 stats[64];
-  if ((int)blockIdx.x < join_blocks) {
-    const int b = blockIdx.x / Hq, hq = blockIdx.x % Hq;
-    const int g = hq / a.G, hg = hq % a.G, h = hg % kPaHeads;
-    const int64_t mt = meta[((int64_t)b * a.Hkv + g) * A.p.head_tiles + hg / kPaHeads];
-    const int first = (int)(uint32_t)mt, count = (int)(mt >> 32);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, turn = SPLIT > 1 ? wave : 0;
+  const int row = blockIdx.x / groups, group = blockIdx.x % groups;
+  int item, first, count;
+  if constexpr (SPLIT > 1) {
+    const int64_t mt = ((const int64_t*)((const char*)a.workspace + A.p.meta_at))[row];
+    item = row;
+    first = (int)(uint32_t)mt;
+    count = (int)(mt >> 32);
     if (count <= 1) return;
-    const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
-    const f32x2 st = joined_stats(ml, first, count, h, sink);
-    const float* const part = (const float*)((const char*)a.workspace + A.p.part_at) + (int64_t)h * padded;
-    f32x4 o = {0, 0, 0, 0};
-    // a wavefront takes every fourth partial result; a lane four of up to 256 values
-    if (lane * 4 < a.D) {
-#pragma unroll 4
-      for (int p = wave; p < count; p += kPaWaves) {
-        const int slot = 2 * (first + p) + (p == 0 ? 1 : 0);
-        const float f = exp2_fast(ml[slot * kPaHeads + h][0] - st[0]);
-        o += f * *(const f32x4*)(part + (int64_t)slot * kPaHeads * padded + lane * 4);
-      }
-      *(f32x4*)&o_lds[wave][lane * 4] = o;
+  } else {
+    const u32x4 ends = ((const u32x4*)((const char*)a.workspace + A.p.ends_at))[row];
+    item = (int)ends[0];
+    first = (int)ends[1];
+    count = (int)ends[2];
+    if (count == 0) return;
+  }
+  const int item_heads = a.Hkv * A.p.head_tiles;
+  const int b = item / item_heads, in_b = item % item_heads;
+  const int g = in_b / A.p.head_tiles, head0 = (in_b % A.p.head_tiles) * kPaHeads;
+  const int h = SPLIT > 1 ? group : group * 4 + wave, hq = g * a.G + head0 + h;
+  const bool there = h < min(kPaHeads, a.G - head0);
+  const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at) + h;
+  const int lanes = padded <= 64 ? 16 : padded <= 128 ? 32 : 64, at_once = 64 / lanes;   // lanes of a row
+  const int d = (lane & (lanes - 1)) * 4;
+  const float* const part = (const float*)((const char*)a.workspace + A.p.part_at) + (int64_t)h * padded + d;
+  const int64_t pitch = (int64_t)kPaHeads * padded;
+  f32x4 o = {0, 0, 0, 0};
+  f32x2 st = {0, 0};
+  if (there) {
+    const int p0 = turn * at_once + lane / lanes;
+    const bool mine = d < a.D;
+    f32x4 x = {0, 0, 0, 0};
+    if (mine && p0 < count) x = *(const f32x4*)(part + slot_of(first, p0) * pitch);
+    st = joined_stats(ml, first, count, a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf);
+    if (mine && p0 < count) {
+      o = exp2_fast(ml[slot_of(first, p0) * kPaHeads][0] - st[0]) * x;
+#pragma unroll 8
+      for (int p = p0 + SPLIT * at_once; p < count; p += SPLIT * at_once)
+        o += exp2_fast(ml[slot_of(first, p) * kPaHeads][0] - st[0]) * *(const f32x4*)(part + slot_of(first, p) * pitch);
     }
+    for (int across = lanes; across < 64; across <<= 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], across);
+  }
+  if constexpr (SPLIT > 1) {
+    joined[turn][lane] = o;
     __syncthreads();
+    if (turn > 0) return;
+#pragma unroll
+    for (int i = 1; i < SPLIT; ++i) o += joined[i][lane];
+  }
+  if (!there) return;
+  if (lane < lanes && d < a.D) {
     const float inv = (st[1] == 0.0f ? 0.0f : 1.0f / st[1]) * (a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
-    const int d = threadIdx.x;
-    if (d < a.D) {
-      const float sum = (o_lds[0][d] + o_lds[1][d]) + (o_lds[2][d] + o_lds[3][d]);
-      ((typename M::T*)a.out)[((int64_t)b * Hq + hq) * a.D + d] = (typename M::T)(sum * inv);
-    }
-    if (threadIdx.x == 0 && a.lse != nullptr)
-      a.lse[(int64_t)b * Hq + hq] = log_of_sum(st[0], st[1], a.sinks != nullptr ? a.sinks + hq : nullptr);
-    return;
-  }
-  const int block = blockIdx.x - join_blocks;
-  const int bg = block / chunks, b = bg / a.Hkv, g = bg % a.Hkv;
-  const Span span = span_of(a.lens[b], a.max_len, a.window);
-  const int at = span.start + (block % chunks) * kPaSumsChunk;
-  if (at >= span.len) return;
-  const int pos = at + threadIdx.x * 4;
-  const float* const scores = (const float*)((const char*)a.workspace + A.p.scores_at) +
-                              (int64_t)bg * a.G * A.p.score_pitch + pos;
-  float sum[4] = {0, 0, 0, 0};
-  for (int h0 = 0; h0 < a.G; h0 += 64) {
-    const int n = min(64, a.G - h0);
-    __syncthreads();
-    for (int i = wave; i < n; i += kPaWaves) {
-      const int hg = h0 + i, hq = g * a.G + hg;
-      const int64_t mt = A.p.workgroups > 0 ? meta[(int64_t)bg * A.p.head_tiles + hg / kPaHeads] : 0;
-      const int first = (int)(uint32_t)mt, count = (int)(mt >> 32);
-      f32x2 st;
-      if (count <= 1)
-        st = ((const f32x2*)((const char*)a.workspace + A.p.stats_at))[(int64_t)b * Hq + hq];
-      else
-        st = joined_stats(ml, first, count, hg % kPaHeads, a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf);
-      if (lane == 0) stats[i] = f32x2{st[0], st[1] == 0.0f ? 0.0f : 1.0f / st[1]};
-    }
-    __syncthreads();
-    if (pos < span.len) {
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const f32x4 x = *(const f32x4*)(scores + (int64_t)(h0 + i) * A.p.score_pitch);
-        const f32x2 st = stats[i];
+    union { typename M::T e[4]; u32x2 u; } r;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += exp2_fast(x[j] - st[0]) * st[1];
-      }
-    }
+    for (int j = 0; j < 4; ++j) r.e[j] = (typename M::T)(o[j] * inv);
+    *(u32x2*)((typename M::T*)a.out + ((int64_t)b * a.Hkv * a.G + hq) * a.D + d) = r.u;
   }
-  float* const to = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)g * a.sums_stride_h + pos;
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (pos + j >= span.lo && pos + j < span.len) to[j] += sum[j];
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[(int64_t)b * a.Hkv * a.G + hq] = log_of_sum(st[0], st[1], a.sinks != nullptr ? a.sinks + hq : nullptr);
 }
 
-int padded_width(int D, bool fp8) {
-  if (D <= 64) return 64;
-  if (D <= 96 && !fp8) return 96;
-  return D <= 128 ? 128 : D <= 192 ? 192 : 256;
+// Adds up the weights that the positions received: a workgroup for 1024 PER positions of a key/value
+// head, a thread for 4 PER.  The scores of the first heads and the sums are asked for before the
+// heads' references and sums are known, a wavefront for each head.  Bound by the scores, read once.
+constexpr int kSumHeads = kPaWaves;
+template <int PER>
+__device__ __forceinline__ void add_weights(const KernelArgs& A, int block, int chunks, f32x2* stats) {
+  const PagedAttentionArgs& a = A.a;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int bg = block / chunks, b = bg / a.Hkv, g = bg % a.Hkv, Hq = a.Hkv * a.G;
+  const Span span = span_of(read_only(a.lens)[b], a.max_len, a.window);
+  const int at = span.start + (block % chunks) * (1024 * PER);
+  if (at >= span.len) return;
+  const float* const scores = (const float*)((const char*)a.workspace + A.p.scores_at) +
+                              (int64_t)bg * A.p.score_pitch * a.G;
+  float* const to = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)g * a.sums_stride_h;
+  const int pos0 = at + threadIdx.x * 4;        // and 1024, 2048, 3072 behind it
+  // (16 bytes at a time where the sums' rows allow it and all four positions are seen)
+  const bool wide = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+  auto all_seen = [&](int pos) { return wide && pos >= span.lo && pos + 3 < span.len; };
+  float sum[PER][4];
+  f32x4 old[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int pos = pos0 + 1024 * k;
+    old[k] = f32x4{0, 0, 0, 0};
+    if (all_seen(pos)) old[k] = *(const f32x4*)(to + pos);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[k][j] = 0.0f;
+  }
+  for (int h0 = 0; h0 < a.G; h0 += kSumHeads) {
+    const int n = min(kSumHeads, a.G - h0);
+    f32x4 x[kSumHeads][PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int pos = min(pos0 + 1024 * k, (span.len - 1) & ~3);
+#pragma unroll
+      for (int i = 0; i < kSumHeads; ++i)
+        x[i][k] = *(const f32x4*)(scores + (int64_t)(pos & ~15) * a.G + (h0 + min(i, n - 1)) * 16 + (pos & 15));
+    }
+    if (h0 > 0) __syncthreads();
+    if (wave < n) {
+      const int hg = h0 + wave, hq = g * a.G + hg;
+      f32x2 st = ((const f32x2*)((const char*)a.workspace + A.p.stats_at))[(int64_t)b * Hq + hq];
+      if (A.p.workgroups > 0) {
+        const int64_t mt = ((const int64_t*)((const char*)a.workspace + A.p.meta_at))[(int64_t)bg * A.p.head_tiles + hg / kPaHeads];
+        const int first = (int)(uint32_t)mt, count = (int)(mt >> 32);
+        if (count > 1)
+          st = joined_stats((const f32x2*)((const char*)a.workspace + A.p.ml_at) + hg % kPaHeads, first, count,
+                            a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf);
+      }
+      if (lane == 0) stats[wave] = f32x2{st[0], st[1] == 0.0f ? 0.0f : 1.0f / st[1]};
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSumHeads; ++i) {
+      if (i < n) {
+        const f32x2 st = stats[i];
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sum[k][j] += exp2_fast(x[i][k][j] - st[0]) * st[1];
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int pos = pos0 + 1024 * k;
+    if (all_seen(pos)) {
+      *(f32x4*)(to + pos) = old[k] + f32x4{sum[k][0], sum[k][1], sum[k][2], sum[k][3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (pos + j >= span.lo && pos + j < span.len) to[pos + j] += sum[k][j];
+    }
+  }
+}
+
+// What is left to do behind the shares: blocks below `join_blocks` join, the others add up weights.
+template <class M, int SPLIT, int PER>
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const KernelArgs A, int padded, int groups,
+                                                                   int join_blocks, int chunks) {
+  __shared__ f32x4 lds[kPaWaves][64];
+  if ((int)blockIdx.x < join_blocks)
+    join_heads<M, SPLIT>(A, padded, groups, lds);
+  else
+    add_weights<PER>(A, blockIdx.x - join_blocks, chunks, (f32x2*)lds);
+}
+
+template <class M, int SPLIT>
+void launch_join(const KernelArgs& A, int padded, hipStream_t stream) {
+  const PagedAttentionArgs& a = A.a;
+  const int heads = std::min(a.G, kPaHeads), groups = SPLIT > 1 ? heads : (heads + 3) / 4;
+  const int join_blocks = A.p.workgroups > 0 ? (SPLIT > 1 ? A.p.items : A.p.workgroups) * groups : 0;
+  const int seen = a.sums == nullptr ? 0 : a.window > 0 && a.window + 16 < a.max_len ? a.window + 16 : a.max_len;
+  // (four times the positions a block where the card has blocks enough, for fewer latencies in a row)
+  const bool many = (int64_t)a.B * a.Hkv * ((seen + 1023) / 1024) > 2048;
+  const int chunks = many ? (seen + 4095) / 4096 : (seen + 1023) / 1024;
+  const int blocks = join_blocks + a.B * a.Hkv * chunks;
+  if (blocks == 0) return;
+  if (many)
+    hipLaunchKernelGGL((paged_attention_join_kernel<M, SPLIT, 4>), dim3(blocks), dim3(256), 0, stream, A, padded, groups,
+                       join_blocks, chunks);
+  else
+    hipLaunchKernelGGL((paged_attention_join_kernel<M, SPLIT, 1>), dim3(blocks), dim3(256), 0, stream, A, padded, groups,
+                       join_blocks, chunks);
 }
 
 template <class M, bool FP8, int DP>
@@ -708,36 +856,36 @@ void launch_kind(const KernelArgs& A, hipStream_t stream) {
     case 192: launch_width<M, FP8, 192>(A, stream); break;
     default: launch_width<M, FP8, 256>(A, stream); break;
   }
-  const int join_blocks = A.p.workgroups > 0 ? A.a.B * A.a.Hkv * A.a.G : 0;
-  const int seen = A.a.window > 0 && A.a.window + 16 < A.a.max_len ? A.a.window + 16 : A.a.max_len;
-  const int chunks = (seen + kPaSumsChunk - 1) / kPaSumsChunk;
-  const int blocks = join_blocks + (A.a.sums != nullptr ? A.a.B * A.a.Hkv * chunks : 0);
-  if (blocks > 0)
-    hipLaunchKernelGGL((paged_attention_join_kernel<M>), dim3(blocks), dim3(256), 0, stream, A, padded, join_blocks,
-                       chunks);
+  if (A.p.workgroups >= 16 * A.p.items)
+    launch_join<M, 4>(A, padded, stream);
+  else
+    launch_join<M, 1>(A, padded, stream);
 }
 
 }  // namespace
 
-PagedAttentionPlan paged_attention_plan(int B, int Hkv, int G, int D, int max_len, int window, bool counted) {
+PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window, bool counted) {
   PagedAttentionPlan p{};
   p.head_tiles = (G + kPaHeads - 1) / kPaHeads;
   p.items = B * Hkv * p.head_tiles;
   const int seen = window > 0 && window + 16 < max_len ? window + 16 : max_len;
   const int units = (seen + kPaUnit - 1) / kPaUnit;
   p.min_units = 2;
-  p.workgroups = units > 4 ? 256 * residents(D) : 0;
+  const bool fp8 = kind >= kKvFp8Bf16;
+  const int padded = padded_width(D, fp8);
+  p.workgroups = units > 4 ? 256 * residents(padded) : 0;
   size_t at = 0;
   auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   if (p.workgroups > 0) {
     const size_t slots = 2 * (size_t)p.workgroups;
+    p.ends_at = part((size_t)p.workgroups * 16);
     p.meta_at = part((size_t)p.items * 8);
     p.ml_at = part(slots * kPaHeads * 8);
-    p.part_at = part(slots * kPaHeads * 256 * 4);
+    p.part_at = part(slots * kPaHeads * padded * 4);
   }
   if (counted) {
     p.stats_at = part((size_t)B * Hkv * G * 8);
-    p.score_pitch = (max_len + 15) / 16 * 16;
+    p.score_pitch = (max_len + 15) / 16 * 16;   // positions
     p.scores_at = part((size_t)B * Hkv * G * p.score_pitch * 4);
   }
   p.bytes = at;
@@ -747,7 +895,7 @@ PagedAttentionPlan paged_attention_plan(int B, int Hkv, int G, int D, int max_le
 void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t stream) {
   KernelArgs A{};
   A.a = a;
-  A.p = paged_attention_plan(a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.sums != nullptr);
+  A.p = paged_attention_plan(kind, a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.sums != nullptr);
   A.by_page = fast_div(a.page_size);
   switch (kind) {
     case kKvBf16: launch_kind<Bf16, false>(A, stream); break;

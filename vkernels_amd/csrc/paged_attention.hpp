@@ -16,7 +16,6 @@ constexpr int kPaHeads = 16;       // query heads of a work item: the columns of
 constexpr int kPaWaveRows = 32;    // positions a wavefront takes at a time
 constexpr int kPaWaves = 4;
 constexpr int kPaUnit = kPaWaveRows * kPaWaves;  // positions a workgroup takes at a time
-constexpr int kPaSumsChunk = 1024; // positions of a workgroup that adds up the weights
 
 struct PagedAttentionArgs {
   const void* q;            // [B, Hkv * G, D], rows of D values 16-byte aligned
@@ -46,10 +45,10 @@ struct PagedAttentionPlan {
   int workgroups;           // workgroups that share the units evenly; 0: one for each item, whole
   int min_units;            // least share of a workgroup
   int score_pitch;          // positions a row of kept scores is long (0: none are kept)
-  size_t meta_at, stats_at, ml_at, part_at, scores_at, bytes;  // parts of the workspace
+  size_t ends_at, meta_at, stats_at, ml_at, part_at, scores_at, bytes;  // parts of the workspace
 };
 
-PagedAttentionPlan paged_attention_plan(int B, int Hkv, int G, int D, int max_len, int window, bool counted);
+PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window, bool counted);
 void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t stream);
 
 }  // namespace vk

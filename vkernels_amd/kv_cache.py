@@ -41,7 +41,7 @@ def _fn(name):
         lib = load_libvkernels_hip()
         argtypes, restype = {
             "vk_hip_kv_cache_append": ([_P] * 9 + [_I] * 9 + [_L] * 7 + [_P], _I),
-            "vk_hip_paged_attention_workspace_bytes": ([_I] * 7, _Z),
+            "vk_hip_paged_attention_workspace_bytes": ([_I] * 8, _Z),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
             "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 6, _Z),
             "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P, _Z, _P], _I),
@@ -191,7 +191,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
               weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.get_device() == device,
               "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
-    size = _fn("vk_hip_paged_attention_workspace_bytes")(B, Hkv, G, D, max_len, window, sums is not None)
+    size = _fn("vk_hip_paged_attention_workspace_bytes")(kind, B, Hkv, G, D, max_len, window, sums is not None)
     workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     qs = q.stride()
     status = _fn("vk_hip_paged_attention")(
