@@ -472,18 +472,24 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       // there may be anything), 32-byte pairs of pieces exchanged by the row so that the
       // transposed reads below spread over the banks.
       {
+        if (!whole) {
+#pragma unroll
+          for (int i = 0; i < L::kVLoads; ++i)
+            if (!((rows >> (i * L::kRowsPerLoad + sub)) & 1u)) vreg[i] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int i = 0; i < L::kVLoads; ++i) {
           const int row = i * L::kRowsPerLoad + sub;
-          if (!whole && !((rows >> row) & 1u)) vreg[i] = u32x4{0, 0, 0, 0};
           const int turn = FP8 ? (L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 7 & (L::kPieces - 1) : 0)
                                : 2 * (L::kPieces >= 16 ? row & 7 : L::kPieces == 8 ? (row >> 1) & 3 : 0);
           *(u32x4*)(my_lds + row * L::kPitch + ((piece ^ turn) * 16)) = vreg[i];
         }
       }
-      // The scores, where the positions' weights are wanted: [16 positions][head][position], what a
-      // wavefront holds in one piece.  (A row for each head, 64 KB apart at 16384 positions, cost
-      // 20 % of the kernel's time.)
+      // The scores, where the positions' weights are wanted: [16 positions][head][position], so that a
+      // wavefront's are one piece.  (75 MB of them beside 2.4 GB of keys and values cost 85 us of 500:
+      // the same stores dropped by a range check cost nothing, a quarter of them 36 us, one in eight
+      // tiles' 14 us, and neither their cache hints nor their place in the loop change it: it is the
+      // memory's price of writes among reads.)
       if (A.p.score_pitch > 0 && col < heads) {
         float* const to = (float*)((char*)a.workspace + A.p.scores_at) + quad * 4 +
                           (((int64_t)(b * a.Hkv + g) * A.p.score_pitch + pos0) * a.G + (head0 + col) * 16);
