@@ -736,7 +736,7 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
  * positions in order, -1 beyond the new length.  A shorter sequence keeps all it has
  * (its sums are copied).  The pages of a sequence that is cut have to be its own.
  * elem_bytes: 1 or 2, a value of the cache.  The workspace of
- * vk_hip_kv_cache_evict_workspace_bytes (4-byte aligned) is scratch of this call alone. */
+ * vk_hip_kv_cache_evict_workspace_bytes (16-byte aligned) is scratch of this call alone. */
 size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget);
 int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_table,
                           const int32_t* seq_lens, const float* weight_sums, float* sums_out,

@@ -179,15 +179,20 @@ struct SelectRow {
   template <class F>
   __device__ __forceinline__ void walk(float (&x)[kSelectLoads], bool again, F f) const {
     for (int j0 = from; j0 < to; j0 += 64 * kSelectLoads) {
-      if (!again || !resident) {
-#pragma unroll
-        for (int i = 0; i < kSelectLoads; ++i)
-          if (j0 + 64 * i < to) x[i] = sums[min(j0 + 64 * i + lane, to - 1)];
-      }
+      if (!again || !resident) load(x, j0);
 #pragma unroll
       for (int i = 0; i < kSelectLoads; ++i)
         if (j0 + 64 * i < to) f(j0 + 64 * i + lane, j0 + 64 * i + lane < to, x[i]);
     }
+  }
+  __device__ __forceinline__ void load(float (&x)[kSelectLoads], int j0) const {
+#pragma unroll
+    for (int i = 0; i < kSelectLoads; ++i)
+      if (j0 + 64 * i < to) x[i] = sums[min(j0 + 64 * i + lane, to - 1)];
+  }
+  // (ahead of other work, so that the first pass finds the sums there: it is then one `again`)
+  __device__ __forceinline__ void preload(float (&x)[kSelectLoads]) const {
+    if (resident) load(x, from);
   }
   __device__ __forceinline__ bool earns(int j, bool real) const { return real && j >= lo && j < hi; }
   __device__ __forceinline__ bool given(int j, bool real) const { return real && (j < lo || j >= hi); }
@@ -358,12 +363,13 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvict
 // digits of its part and leaves the counts in the workspace; the next launch adds the parts' counts
 // up and goes on from the digit found.  What a part keeps for certain follows from the counts as
 // well, so that the last launch knows where each part's positions begin.
+constexpr int kMostParts = 16;
 struct SplitRow {
   uint32_t* counts;   // [3][parts][kBins]
   uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] certain ones by those
 };
 __device__ __forceinline__ SplitRow split_row(const KvEvictArgs& a, int row) {
-  const int words = 3 * a.parts * kBins + 4 + 2 * a.parts;
+  const int words = 3 * a.parts * kBins + 4 + 2 * a.parts;   // (even: pairs of counts are read)
   uint32_t* const base = a.split + (int64_t)row * words;
   return SplitRow{base, base + 3 * a.parts * kBins};
 }
@@ -376,8 +382,12 @@ __device__ void split_digit(const KvEvictArgs& a, const SplitRow& s, int pass, i
   uint32_t c[2] = {0, 0}, mine[2] = {0, 0};
   if (2 * t < n) {
     const uint32_t* const from = s.counts + (int64_t)pass * a.parts * kBins + (n - 2 - 2 * t);
-    for (int p = 0; p < a.parts; ++p) {
-      const uint32_t high = from[p * kBins + 1], low = from[p * kBins];
+    uint64_t pair[kMostParts];      // both digits of a part, all parts' loads at once
+#pragma unroll
+    for (int p = 0; p < kMostParts; ++p) pair[p] = p < a.parts ? *(const uint64_t*)(from + p * kBins) : 0ull;
+#pragma unroll
+    for (int p = 0; p < kMostParts; ++p) {
+      const uint32_t high = (uint32_t)(pair[p] >> 32), low = (uint32_t)pair[p];
       c[0] += high;
       c[1] += low;
       if (p == part) {
@@ -423,10 +433,11 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const K
     need = s.state[1];
   }
   for (int i = t; i < kBinCopies * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
+  float x[kSelectLoads];
+  r.preload(x);
   if constexpr (PASS > 0) split_digit(a, s, PASS - 1, part, least, need, scan_lds, found);
   __syncthreads();
-  float x[kSelectLoads];
-  r.walk(x, false, [&](int j, bool real, float v) {
+  r.walk(x, true, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
     constexpr uint32_t same = PASS == 1 ? 21 : 10;
     if (r.earns(j, real) && (PASS == 0 || key >> same == least >> same))
@@ -450,18 +461,24 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   const SplitRow s = split_row(a, row);
   uint32_t least = 0, need = r.places;
   uint32_t before_sure = 0, before_equal = 0;      // kept in the parts before this one
+  float x[kSelectLoads];
+  r.preload(x);
   if (r.places > 0) {
     least = s.state[2];
     need = s.state[3];
     split_digit(a, s, 2, part, least, need, scan_lds, found);
     const uint32_t digit = least & 1023u;
     uint32_t sure = 0;
-    for (int p = 0; p < part; ++p) {
-      const uint32_t* const counts = s.counts + ((int64_t)2 * a.parts + p) * kBins;
-      if ((uint32_t)t > digit && t < 1024) sure += counts[t];
-      if (t == 0) sure += s.state[4 + p] + s.state[4 + a.parts + p];
-      before_equal += counts[digit];
+    const uint32_t* const counts = s.counts + (int64_t)2 * a.parts * kBins;
+#pragma unroll
+    for (int p = 0; p < kMostParts; ++p) {
+      if (p < part) {
+        before_equal += counts[p * kBins + digit];
+        const uint32_t n = counts[p * kBins + t];
+        sure += (uint32_t)t > digit ? n : 0u;
+      }
     }
+    if (t < part) sure += s.state[4 + t] + s.state[4 + a.parts + t];
     sure = wave_scan(sure);
     if ((t & 63) == 63) scan_lds[t >> 6] = sure;
     __syncthreads();
@@ -473,9 +490,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   const int begin = min(r.len, part * kSelectWaves * stretch);
   before_sure += (uint32_t)(min(begin, r.lo) + max(0, begin - r.hi));
 
-  float x[kSelectLoads];
   uint32_t sure = 0, equal = 0;
-  r.walk(x, false, [&](int j, bool real, float v) {
+  r.walk(x, true, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
     const bool middle = r.earns(j, real) && r.places > 0;
     sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key > least)));
@@ -485,13 +501,16 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   write_kept(r, x, least, need, before_sure + sure, before_equal + equal);
 }
 
-// The compaction.  A batch is 32 KB of rows that become neighbours: the keys or the values
+// The compaction.  A batch is 64 KB of rows that become neighbours: the keys or the values
 // of a head, kept[j] -> j for `rows` successive j.  A workgroup reads its batch into
 // registers, says so, and writes once every batch that reads what it overwrites has been
 // read.  kept[j] >= j grows with j, so those are earlier batches of the same list; the
 // workgroups of a list take its batches in the order in which they start, and say that
 // they have read without waiting for anything: every wait ends.
-constexpr int kMoveLoads = 8, kMoveThreads = 256;
+// Bound by the rows read and written (64 sequences of 8 heads of 128 to 2048 positions: 1.07 GB
+// in 214 us, 5.0 TB/s; a copy of that size reaches 5.2), past the caches: nothing is used twice.
+// Batches of 32 KB are 2 to 8 % behind, rows that stay in the caches 5 %.
+constexpr int kMoveLoads = 8, kMoveThreads = 512;
 constexpr int kMovePieces = kMoveLoads * kMoveThreads;    // of 16 bytes
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs a) {
   __shared__ uint32_t ticket_lds;
@@ -535,8 +554,8 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
     const bool there = (uint32_t)src_page[i] < (uint32_t)a.num_pages;
     moves[i] = moves[i] && there && (uint32_t)dst_page[i] < (uint32_t)a.num_pages;
     const int slot = src[i] - divided(src[i], a.by_page) * a.page_size;
-    x[i] = *(const u32x4*)(cache + (there ? (int64_t)src_page[i] * a.page_stride + (int64_t)slot * a.slot_stride : 0) +
-                           piece[i] * 16);
+    const int64_t at = there ? (int64_t)src_page[i] * a.page_stride + (int64_t)slot * a.slot_stride : 0;
+    x[i] = __builtin_nontemporal_load((const u32x4*)(cache + at + piece[i] * 16));
   }
   // The rows' sums go with the keys.
   const bool with_sums = which == 0;
@@ -566,8 +585,8 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
 #pragma unroll
   for (int i = 0; i < kMoveLoads; ++i) {
     const int slot = dst[i] - divided(dst[i], a.by_page) * a.page_size;
-    if (moves[i])
-      *(u32x4*)(cache + (int64_t)dst_page[i] * a.page_stride + (int64_t)slot * a.slot_stride + piece[i] * 16) = x[i];
+    const int64_t at = (int64_t)dst_page[i] * a.page_stride + (int64_t)slot * a.slot_stride;
+    if (moves[i]) __builtin_nontemporal_store(x[i], (u32x4*)(cache + at + piece[i] * 16));
   }
   if (with_sums) {
 #pragma unroll
@@ -605,7 +624,7 @@ int kv_evict_parts(int rows, int max_len) {
   // the launches of the split form cost more than they save.
   if (max_len <= 8192 || rows > 128) return 1;
   const int most = (max_len + 4095) / 4096;
-  return min(min(256 / rows, most), 16);
+  return min(min(256 / rows, most), kMostParts);
 }
 
 size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget) {

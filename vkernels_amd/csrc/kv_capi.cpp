@@ -179,7 +179,7 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
   if ((int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2 ||
       (int64_t)B * Hkv * vk::kv_evict_batches(budget, D * elem_bytes) > kInt32 / 2)
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many rows for one call");
-  if (workspace == nullptr || !aligned(workspace, 4) ||
+  if (workspace == nullptr || !aligned(workspace, 16) ||
       workspace_bytes < vk_hip_kv_cache_evict_workspace_bytes(elem_bytes, B, Hkv, D, max_len, budget))
     return refuse(VK_ERROR_INVALID_ARGUMENT, who, "a workspace of vk_hip_kv_cache_evict_workspace_bytes is needed");
   vk::KvEvictArgs a{};

@@ -15,6 +15,7 @@ The entry points are additive: the reference keeps its cache outside this path. 
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -55,6 +56,12 @@ def _fn(name):
     return fn
 
 
+@functools.lru_cache(maxsize=256)
+def _bytes(name, *sizes):
+    """The workspace of a call of these sizes (the library's answer follows them alone)."""
+    return _fn(name)(*sizes)
+
+
 def _failed(status, name):
     raise RuntimeError(f"{name} failed with status {status}: {last_error(load_libvkernels_hip())}")
 
@@ -68,12 +75,11 @@ def _need(ok, message):
 # call counts); the functions _explain_* say which part of it did not hold.
 
 def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
-    B = block_table.shape[0]
     return (len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is k_cache.dtype and strides[3] == 1 and
-            v_cache.stride() == strides and device >= 0 and v_cache.get_device() == device and
-            block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1 and
-            block_table.get_device() == device and seq_lens.dtype is torch.int32 and seq_lens.shape == (B,) and
-            seq_lens.is_contiguous() and seq_lens.get_device() == device and _device() == device)
+            v_cache.stride() == strides and v_cache.get_device() == device and block_table.dtype is torch.int32 and
+            block_table.get_device() == device and seq_lens.dtype is torch.int32 and
+            seq_lens.shape == block_table.shape[:1] and seq_lens.is_contiguous() and seq_lens.get_device() == device and
+            device >= 0 and _current_device() == device)
 
 
 def _explain_cache(k_cache, v_cache, block_table, seq_lens):
@@ -87,22 +93,25 @@ def _explain_cache(k_cache, v_cache, block_table, seq_lens):
           "seq_lens must be int32 [B], contiguous")
     devices = {t.get_device() for t in (k_cache, v_cache, block_table, seq_lens)}
     _need(len(devices) == 1 and devices != {-1}, "the cache, block_table and seq_lens must be on one device")
-    _need(devices == {_device()}, "the tensors' device must be the current device")
+    _need(devices == {_current_device()}, "the tensors' device must be the current device")
 
 
-def _device():
-    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -1
-
-
-def _stream(device):
-    """The raw current stream of the device."""
-    return torch._C._cuda_getCurrentRawStream(device)
+# The current device, and a device's current stream as the address that the library takes.
+_current_device = torch._C._cuda_getDevice
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _head_vector(t, n, name, device):
-    _need(t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == device,
-          f"{name} must be {n} contiguous float32 values on the cache's device")
+    if not (t.dtype is torch.float32 and t.numel() == n and t.is_contiguous() and t.get_device() == device):
+        raise ValueError(f"{name} must be {n} contiguous float32 values on the cache's device")
     return t.data_ptr()
+
+
+def _table(block_table):
+    """(B, W, elements from row to row)"""
+    (B, W), (stride, one) = block_table.shape, block_table.stride()
+    _need(one == 1, "block_table must be int32 [B, W] with contiguous rows")
+    return B, W, max(stride, W)
 
 
 def _rows(t):
@@ -127,7 +136,7 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
         _explain_cache(k_cache, v_cache, block_table, seq_lens)
     pages, Hkv, ps, D = shape
-    B, W = block_table.shape
+    B, W, table_stride = _table(block_table)
     tokens = k.shape[0]
     _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype,
           "k and v must be [tokens, Hkv, D] alike")
@@ -147,7 +156,7 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
         seq_lens.data_ptr(), query_start,
         None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
         None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device), kind, B, tokens, Hkv, D, pages, ps,
-        W, max(block_table.stride(0), W), ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2],
+        W, table_stride, ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2],
         _stream(device))
     if status:
         _failed(status, "vk_hip_kv_cache_append")
@@ -169,11 +178,11 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
         _explain_cache(k_cache, v_cache, block_table, seq_lens)
     pages, Hkv, ps, D = shape
-    B, W = block_table.shape
-    _need(q.dim() == 3 and q.get_device() == device, "q must be [B, Hq, D] on the cache's device")
-    Hq = q.shape[1]
+    B, W, table_stride = _table(block_table)
+    Hq = q.shape[1] if q.dim() == 3 else 0
     G = Hq // Hkv
-    _need(q.shape == (B, G * Hkv, D) and G > 0, "q must be [B, Hq, D] with Hq a multiple of the cache's heads")
+    _need(q.shape == (B, G * Hkv, D) and G > 0 and q.get_device() == device,
+          "q must be [B, Hq, D] on the cache's device with Hq a multiple of the cache's heads")
     kind = _KINDS.get((k_cache.dtype, q.dtype))
     _need(kind is not None, "the cache's type does not take queries of this type")
     if max_len is None:
@@ -184,15 +193,15 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     else:
         _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and out.get_device() == device,
               "out must be contiguous and like q")
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
         _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3 and weight_sums.shape[:2] == (B, Hkv) and
               weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.get_device() == device,
               "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
-    size = _fn("vk_hip_paged_attention_workspace_bytes")(kind, B, Hkv, G, D, max_len, window, sums is not None)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    size = _bytes("vk_hip_paged_attention_workspace_bytes", kind, B, Hkv, G, D, max_len, window, sums is not None)
+    workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     qs = q.stride()
     status = _fn("vk_hip_paged_attention")(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
@@ -200,7 +209,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
         None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device),
         out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind, B, Hkv, G, D, pages, ps, W,
-        max(block_table.stride(0), W), max_len, window, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
+        table_stride, max_len, window, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
         strides[0], strides[1], strides[2], sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size,
         _stream(device))
     if status:
@@ -223,7 +232,7 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
         _explain_cache(k_cache, v_cache, block_table, seq_lens)
     pages, Hkv, ps, D = shape
-    B, W = block_table.shape
+    B, W, table_stride = _table(block_table)
     if max_len is None:
         max_len = W * ps
     sums_out = weight_sums if sums_out is None else sums_out
@@ -234,13 +243,13 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     new_lens = torch.empty_like(seq_lens)
     kept = seq_lens.new_empty((B, Hkv, max(budget, 0)))
     elem = k_cache.element_size()
-    size = _fn("vk_hip_kv_cache_evict_workspace_bytes")(elem, B, Hkv, D, max_len, budget)
-    workspace = torch.empty(size, dtype=torch.uint8, device=k_cache.device)
+    size = _bytes("vk_hip_kv_cache_evict_workspace_bytes", elem, B, Hkv, D, max_len, budget)
+    workspace = seq_lens.new_empty((size,), dtype=torch.uint8)
     ss, so = weight_sums.stride(), sums_out.stride()
     status = _fn("vk_hip_kv_cache_evict")(
         k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), weight_sums.data_ptr(),
         sums_out.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), elem, B, Hkv, D, pages, ps, W,
-        max(block_table.stride(0), W), max_len, budget, keep_first, keep_last, strides[0], strides[1], strides[2],
+        table_stride, max_len, budget, keep_first, keep_last, strides[0], strides[1], strides[2],
         ss[0], ss[1], so[0], so[1], workspace.data_ptr(), size, _stream(device))
     if status:
         _failed(status, "vk_hip_kv_cache_evict")
