@@ -317,6 +317,29 @@ def test_append_from_slices_of_a_fused_projection(hip_lib):
     assert all(torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) for a, b in zip((s.k, s.v), want))
 
 
+def test_calls_without_sequences_or_tokens(hip_lib):
+    s = Setup([40, 3], 2, 4, 64, 16)
+    before = s.k.clone()
+    none = torch.zeros((0, 2, 64), dtype=BF16, device=dev())
+    kv.kv_cache_append(none, none, s.k, s.v, s.table[:0], s.lens[:0])
+    kv.kv_cache_append(none, none, s.k, s.v, s.table, s.lens, query_start=torch.zeros(3, dtype=torch.int32, device=dev()))
+    out, lse = kv.paged_attention(s.q[:0], s.k, s.v, s.table[:0], s.lens[:0], return_lse=True)
+    assert out.shape == (0, 8, 64) and lse.shape == (0, 8)
+    new_lens, kept = kv.kv_cache_evict(s.k, s.v, s.table[:0], s.lens[:0], torch.zeros((0, 2, 48), device=dev()), 8)
+    assert new_lens.shape == (0,) and kept.shape == (0, 2, 8)
+    assert torch.equal(s.k.view(torch.int16), before.view(torch.int16))
+
+
+def test_append_of_a_stretch_of_the_tokens(hip_lib):
+    """query_start that begins behind token 0 and ends before the last: the tokens outside go nowhere."""
+    s = Setup([40, 20, 9], 2, 1, 64, 16, seed=5)
+    rows = torch.randn((30, 2, 64), device=dev()).to(BF16)
+    starts = torch.tensor([6, 14, 14, 23], dtype=torch.int32, device=dev())
+    want = ref.append(s.k, s.v, rows, -rows, s.table, s.lens, starts.cpu(), None, None)
+    kv.kv_cache_append(rows, -rows, s.k, s.v, s.table, s.lens, query_start=starts)
+    assert all(torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) for a, b in zip((s.k, s.v), want))
+
+
 def test_append_many_sequences_of_few_tokens(hip_lib):
     """More sequences than the search's 64 candidates, many of them without a token."""
     g = torch.Generator().manual_seed(1)
@@ -402,6 +425,16 @@ def test_evict_many_rows(hip_lib, rows, longest):
     s = Setup(lens, 1, 1, 16, 16, seed=2)
     sums = torch.exp(3 * torch.randn((rows, 1, s.table.shape[1] * 16), device=dev()))
     _check_evict(s, sums, 150, 3, 40, in_place=True)
+
+
+@pytest.mark.parametrize("cache,D", [(FP8, 16), (FP8, 64), (BF16, 128)])
+def test_evict_in_many_batches_of_rows_that_share_lines(hip_lib, cache, D):
+    """Several batches of rows a head, which wait for each other, and heads whose rows lie in the same lines."""
+    s = Setup([12000, 9000, 8500], 4, 1, D, 24, cache=cache, layout="tokens", seed=D)
+    g = torch.Generator(device=dev()).manual_seed(D)
+    sums = torch.rand((3, 4, s.table.shape[1] * 24), device=dev(), generator=g)
+    sums[1, :, :3000] = 0.0                     # nearly all of the first rows go: every row moves far
+    _check_evict(s, sums, 8500, 3, 60, in_place=True)
 
 
 def test_evict_twice_in_place(hip_lib):

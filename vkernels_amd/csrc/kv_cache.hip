@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, in
   } else {
     seq = t;
   }
-  if (t >= a.tokens || seq >= a.B) return;
+  if (t >= a.tokens || seq >= a.B || (a.starts != nullptr && t < a.starts[seq])) return;
   const int rest = (int)(idx - (int64_t)t * per_token);
   const int which = rest / (a.Hkv * pieces), in_row = rest % (a.Hkv * pieces);
   const int h = in_row / pieces, d = (in_row % pieces) * values;
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
 // Bound by the rows read and written (64 sequences of 8 heads of 128 to 2048 positions: 1.07 GB
 // in 214 us, 5.0 TB/s; a copy of that size reaches 5.2), past the caches: nothing is used twice.
 // Batches of 32 KB are 2 to 8 % behind, rows that stay in the caches 5 %.
-constexpr int kMoveLoads = 8, kMoveThreads = 512;
+constexpr int kMoveLoads = 8, kMoveThreads = kKvMoveThreads;
 constexpr int kMovePieces = kMoveLoads * kMoveThreads;    // of 16 bytes
 __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs a) {
   __shared__ uint32_t ticket_lds;
