@@ -11,10 +11,11 @@ namespace vk {
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 // ---- append --------------------------------------------------------------------------------
 
-// The largest of 64-bit-scaled E4M3: what does not fit is stored as the largest finite code.
+// What does not fit into E4M3 is stored as its largest finite code.
 __device__ __forceinline__ float e4m3_range(float x) {
   // (comparisons that leave a NaN a NaN)
   x = x > 448.0f ? 448.0f : x;
@@ -28,21 +29,44 @@ __device__ __forceinline__ float f16_bits_to_f32(uint32_t bits, bool bf16) {
   return (float)c.h;
 }
 
-// A thread takes 8 values (16 bytes) of a key or value row, or 16 values of a row that is
-// stored in 8 bits.  Bytes bound: a row is read once and written once.
+// 8 values of a row as E4M3 codes.
+__device__ __forceinline__ u32x2 e4m3_codes(u32x4 x, float scale, bool bf16) {
+  u32x2 codes;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = x[2 * i + j / 2];
+      f[j] = e4m3_range(f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu, bf16) / scale);
+    }
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], c, true);
+    codes[i] = (uint32_t)c;
+  }
+  return codes;
+}
+
+// A thread takes the same 8 values (16 bytes) of a token's key and value in a head.  The rows are
+// asked for before their place is looked up: length, then page, then store are the latency that
+// a decode step's call consists of (4 us for 255 tokens); a prompt's is bound by the rows read
+// and written (8191 tokens of 8 heads of 128: 67 MB in 13.9 us, 4.8 TB/s; a thread for each key
+// or value, its row behind the look-up, took 17).
 template <bool FP8>
 __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, int bf16) {
-  const int values = FP8 ? 16 : 8;
-  const int pieces = a.D / values, per_token = 2 * a.Hkv * pieces;
-  const int64_t first = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63);
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (first >= (int64_t)a.tokens * per_token) return;
-  int seq = 0;
-  const int t = (int)(idx / per_token);
+  const int per_token = a.Hkv * a.pieces;
+  const int first = (int)(blockIdx.x * 256 + (threadIdx.x & ~63)), idx = (int)(blockIdx.x * 256 + threadIdx.x);
+  if (first >= a.tokens * per_token) return;
+  const int t = divided(idx, a.by_token), rest = idx - t * per_token;
+  const int h = divided(rest, a.by_pieces), d = (rest - h * a.pieces) * 8;
+  const int there = min(t, a.tokens - 1);
+  const u32x4 k = *(const u32x4*)((const char*)a.k + ((int64_t)there * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2);
+  const u32x4 v = *(const u32x4*)((const char*)a.v + ((int64_t)there * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
+  int seq = there;
   if (a.starts != nullptr) {
     // The sequence of the wavefront's first token, 64 candidates at a time; the other
     // lanes walk on from there.
-    const int lane = threadIdx.x & 63, t0 = (int)(first / per_token);
+    const int lane = threadIdx.x & 63, t0 = divided(first, a.by_token);
     int lo = 0, hi = a.B;           // the last i in [lo, hi) with starts[i] <= t0
     while (hi - lo > 1) {
       const int step = (hi - lo + 63) / 64;
@@ -53,46 +77,24 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, in
       lo += (n - 1) * step;
     }
     seq = lo;
-    if (t < a.tokens)
-      while (seq + 1 < a.B && a.starts[seq + 1] <= t) ++seq;
-  } else {
-    seq = t;
+    while (seq + 1 < a.B && a.starts[seq + 1] <= there) ++seq;
   }
   if (t >= a.tokens || seq >= a.B || (a.starts != nullptr && t < a.starts[seq])) return;
-  const int rest = (int)(idx - (int64_t)t * per_token);
-  const int which = rest / (a.Hkv * pieces), in_row = rest % (a.Hkv * pieces);
-  const int h = in_row / pieces, d = (in_row % pieces) * values;
-  const int pos = a.starts != nullptr ? a.lens[seq] - a.starts[seq + 1] + t : a.lens[seq] - 1;
-  if (pos < 0 || pos >= a.lens[seq]) return;
+  const int len = a.lens[seq];
+  const int pos = a.starts != nullptr ? len - a.starts[seq + 1] + t : len - 1;
+  if (pos < 0 || pos >= len) return;
   const int in_table = divided(pos, a.by_page);
   if (in_table >= a.table_width) return;
   const int page = a.table[(int64_t)seq * a.table_stride + in_table];
   if ((uint32_t)page >= (uint32_t)a.num_pages) return;
-  const char* src = (const char*)(which ? a.v : a.k) +
-                    ((int64_t)t * (which ? a.v_stride_t : a.k_stride_t) +
-                     (int64_t)h * (which ? a.v_stride_h : a.k_stride_h) + d) * 2;
   const int64_t to = (int64_t)page * a.page_stride + (int64_t)h * a.head_stride +
                      (int64_t)(pos - in_table * a.page_size) * a.slot_stride + d;
-  char* cache = (char*)(which ? a.v_cache : a.k_cache);
   if constexpr (!FP8) {
-    *(u32x4*)(cache + to * 2) = *(const u32x4*)src;
+    *(u32x4*)((char*)a.k_cache + to * 2) = k;
+    *(u32x4*)((char*)a.v_cache + to * 2) = v;
   } else {
-    const float scale = (which ? a.v_scale : a.k_scale)[h];
-    const u32x4 x[2] = {*(const u32x4*)src, *(const u32x4*)(src + 16)};
-    u32x4 codes;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float f[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t w = x[i / 2][(i % 2) * 2 + j / 2];
-        f[j] = e4m3_range(f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu, bf16 != 0) / scale);
-      }
-      int c = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-      c = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], c, true);
-      codes[i] = (uint32_t)c;
-    }
-    *(u32x4*)(cache + to) = codes;
+    *(u32x2*)((char*)a.k_cache + to) = e4m3_codes(k, a.k_scale[h], bf16 != 0);
+    *(u32x2*)((char*)a.v_cache + to) = e4m3_codes(v, a.v_scale[h], bf16 != 0);
   }
 }
 
@@ -603,9 +605,12 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
 
 void launch_kv_append(const KvAppendArgs& args, int kind, hipStream_t stream) {
   KvAppendArgs a = args;
-  a.by_page = fast_div(a.page_size);
   const bool fp8 = kind == kKvFp8Bf16 || kind == kKvFp8F16;
-  const int64_t items = (int64_t)a.tokens * 2 * a.Hkv * (a.D / (fp8 ? 16 : 8));
+  a.pieces = a.D / 8;
+  a.by_page = fast_div(a.page_size);
+  a.by_pieces = fast_div(a.pieces);
+  a.by_token = fast_div(a.Hkv * a.pieces);
+  const int64_t items = (int64_t)a.tokens * a.Hkv * a.pieces;
   const dim3 grid((unsigned)((items + 255) / 256)), block(256);
   const int bf16 = kind == kKvBf16 || kind == kKvFp8Bf16;
   if (fp8)

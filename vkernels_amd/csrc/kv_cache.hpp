@@ -23,7 +23,9 @@ struct KvAppendArgs {
   int64_t page_stride, head_stride, slot_stride;            // elements, of both caches
   int table_stride, table_width, num_pages, page_size;
   int B, tokens, Hkv, D;
-  FastDiv by_page;                                          // (set by the launcher)
+  // (set by the launcher)
+  int pieces;               // of a row: what a thread takes
+  FastDiv by_page, by_pieces, by_token;
 };
 void launch_kv_append(const KvAppendArgs& a, int kind, hipStream_t stream);
 

@@ -78,7 +78,7 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
   if (why == nullptr && elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr))
     why = "k_scale and v_scale are for 8-bit caches";
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  if ((int64_t)tokens * Hkv * D / 4 > kInt32) return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
+  if ((int64_t)tokens * Hkv > kInt32 / D) return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
   vk::KvAppendArgs a{};
   a.k = k; a.v = v; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
   a.starts = query_start; a.k_scale = k_scale; a.v_scale = v_scale;
