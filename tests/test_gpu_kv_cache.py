@@ -83,7 +83,7 @@ class Setup:
 
 # ---- attention ----------------------------------------------------------------------------------
 
-# one wavefront's tile is 32 positions, a workgroup's 128; calls that see more than 512 are shared out
+# one wavefront's tile is 32 positions, a workgroup's 128; calls that see more than 1024 are shared out
 LENGTHS = [0, 1, 15, 16, 17, 31, 33, 127, 128, 129, 300]
 
 
@@ -104,7 +104,7 @@ def test_head_layouts(hip_lib, Hkv, G, long):
 @pytest.mark.parametrize("ps", [1, 2, 3, 7, 8, 16, 17, 24, 32, 48, 64, 100, 256, 1000])
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
 def test_page_sizes_and_layouts(hip_lib, ps, layout):
-    Setup([ps, ps + 1, max(1, ps - 1), 3 * ps, 601], 2, 3, 64, ps, layout=layout, seed=ps).check(counted=True)
+    Setup([ps, ps + 1, max(1, ps - 1), 3 * ps, 1201], 2, 3, 64, ps, layout=layout, seed=ps).check(counted=True)
     Setup([200, 31, 77], 2, 3, 80, ps, layout=layout, seed=ps, cache=FP8).check(counted=True)
 
 
@@ -131,7 +131,7 @@ def test_many_sequences_share_the_workgroups(hip_lib):
     Setup(lens, 1, 2, 64, 16, seed=11).check(counted=True)
 
 
-@pytest.mark.parametrize("L", [513, 4096, 20000])
+@pytest.mark.parametrize("L", [513, 1024, 1025, 4096, 20000])
 def test_one_long_sequence(hip_lib, L):
     for peak in (0.3, 6.0):
         Setup([L], 2, 4, 128, 64, seed=L, peak=peak).check(counted=True, sinks=True)
@@ -150,7 +150,7 @@ def test_a_bound_above_the_lengths_changes_nothing_but_the_split(hip_lib):
 def test_pages_that_are_not_there(hip_lib):
     """Entries outside [0, pages) leave their positions out, whole sequences included."""
     for ps in (16, 12):
-        for lens in ([200, 200, 90, 200], [900, 700, 90, 40]):
+        for lens in ([200, 200, 90, 200], [1300, 700, 90, 40]):
             s = Setup(lens, 2, 4, 64, ps, seed=5)
             table = s.table.clone()
             table[0, 0] = -1
@@ -169,7 +169,7 @@ def test_scores_of_infinity_and_nan(hip_lib):
     """What is stored at positions that count is computed with as the definition says: a score of -inf
     gets no weight, a row of nothing else is 0, +inf or NaN make the row NaN; other rows are not
     touched."""
-    for n in (40, 700):
+    for n in (40, 1200):
         s = Setup([n, n, n, n], 1, 1, 64, 16, seed=9)
         s.q.zero_()
         s.q[:, :, 0] = 1.0
@@ -206,7 +206,7 @@ def test_large_scores_and_rising_maxima(hip_lib):
 
 
 def test_strided_queries_tables_and_sums(hip_lib):
-    s = Setup([100, 640, 3], 2, 4, 64, 16, seed=6)
+    s = Setup([100, 1140, 3], 2, 4, 64, 16, seed=6)
     want, want_lse, _ = s.check()
     fused = torch.randn((3, 8 + 4, 64), device=dev()).to(BF16)       # queries as part of a fused projection
     fused[:, :8] = s.q
