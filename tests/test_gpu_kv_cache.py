@@ -232,6 +232,22 @@ def test_strided_queries_tables_and_sums(hip_lib):
     assert kv.paged_attention(*s.args(), out=out) is out and torch.equal(out, want)
 
 
+def test_broadcast_tables_queries_and_rows(hip_lib):
+    """One row of the table for all sequences (a shared prompt), one query for all heads, one key for all heads."""
+    s = Setup([1500], 2, 4, 64, 16, seed=16)
+    table, lens = s.table.expand(3, -1), torch.tensor([1500, 0, 77], dtype=torch.int32, device=dev())
+    q = torch.randn((3, 1, 64), device=dev()).to(BF16)
+    want = kv.paged_attention(q.repeat(1, 8, 1), s.k, s.v, table.contiguous(), lens)
+    assert torch.equal(kv.paged_attention(q.expand(-1, 8, -1), s.k, s.v, table, lens), want)
+    few = Setup([40, 17, 3], 2, 1, 64, 16, seed=3)
+    row = torch.randn((3, 1, 64), device=dev()).to(BF16).expand(-1, 2, -1)
+    after = ref.append(few.k, few.v, row, -row, few.table, few.lens, None, None, None)
+    kv.kv_cache_append(row, -row, few.k, few.v, few.table, few.lens)
+    assert all(torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) for a, b in zip((few.k, few.v), after))
+    with pytest.raises(ValueError):      # sums that heads would share cannot be added to
+        kv.paged_attention(*s.args(), weight_sums=torch.zeros((1, 1, 1504), device=dev()).expand(-1, 2, -1))
+
+
 def test_results_do_not_depend_on_the_run(hip_lib):
     s = Setup([900, 30, 2222, 0, 511], 2, 8, 128, 16, seed=8)
     runs = []

@@ -26,7 +26,7 @@ EVICT = dict(k_cache=P, v_cache=P, block_table=P, seq_lens=P, weight_sums=P, sum
 CALLS = {"vk_hip_kv_cache_append": APPEND, "vk_hip_paged_attention": ATTEND, "vk_hip_kv_cache_evict": EVICT}
 
 CACHE = [dict(D=0), dict(D=24), dict(D=272), dict(D=-16), dict(Hkv=0), dict(num_pages=0), dict(page_size=0),
-         dict(table_width=0), dict(table_stride=3), dict(k_cache=None), dict(v_cache=None), dict(block_table=None),
+         dict(table_width=0), dict(table_stride=-1), dict(k_cache=None), dict(v_cache=None), dict(block_table=None),
          dict(seq_lens=None), dict(k_cache=P + 8), dict(v_cache=P + 2), dict(page_stride=2044), dict(head_stride=1028),
          dict(slot_stride=68), dict(slot_stride=-64), dict(slot_stride=1 << 27), dict(B=-1)]
 INVALID = {

@@ -30,7 +30,7 @@ const char* cache_refusal(const void* k_cache, const void* v_cache, const int32_
   if (Hkv <= 0) return "Hkv must be positive";
   if (D <= 0 || D % 16 != 0 || D > 256) return "D must be a multiple of 16 up to 256";
   if (num_pages <= 0 || page_size <= 0) return "num_pages and page_size must be positive";
-  if (table_width <= 0 || table_stride < table_width) return "block_table must have columns, table_stride of them at least";
+  if (table_width <= 0 || table_stride < 0) return "block_table must have columns and no negative table_stride";
   if (k_cache == nullptr || v_cache == nullptr || table == nullptr || lens == nullptr)
     return "k_cache/v_cache/block_table/seq_lens must not be null";
   if (!aligned(k_cache, 16) || !aligned(v_cache, 16) || page_stride * elem % 16 != 0 ||

@@ -33,6 +33,7 @@ _KINDS = {
     (torch.float8_e4m3fn, torch.float16): 3,
 }
 
+_INT32 = torch.int32
 _fns: dict = {}
 
 
@@ -74,12 +75,12 @@ def _need(ok, message):
 # The checks are one expression each on the path that is taken (a decode step is short: the host's work per
 # call counts); the functions _explain_* say which part of it did not hold.
 
-def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
-    return (len(shape) == 4 and v_cache.shape == shape and v_cache.dtype is k_cache.dtype and strides[3] == 1 and
-            v_cache.stride() == strides and v_cache.get_device() == device and block_table.dtype is torch.int32 and
-            block_table.get_device() == device and seq_lens.dtype is torch.int32 and
-            seq_lens.shape == block_table.shape[:1] and seq_lens.is_contiguous() and seq_lens.get_device() == device and
-            device >= 0 and _current_device() == device)
+def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device, table, table_strides):
+    return (v_cache.shape == shape and v_cache.stride() == strides and strides[3] == 1 and
+            v_cache.dtype is k_cache.dtype and block_table.dtype is _INT32 and seq_lens.dtype is _INT32 and
+            table_strides[1] == 1 and seq_lens.shape == table[:1] and seq_lens.is_contiguous() and
+            v_cache.get_device() == device and block_table.get_device() == device and
+            seq_lens.get_device() == device and device >= 0 and _current_device() == device)
 
 
 def _explain_cache(k_cache, v_cache, block_table, seq_lens):
@@ -107,11 +108,24 @@ def _head_vector(t, n, name, device):
     return t.data_ptr()
 
 
-def _table(block_table):
-    """(B, W, elements from row to row)"""
-    (B, W), (stride, one) = block_table.shape, block_table.stride()
-    _need(one == 1, "block_table must be int32 [B, W] with contiguous rows")
-    return B, W, max(stride, W)
+def _cache(k_cache, v_cache, block_table, seq_lens):
+    """Checks what every operator takes: (pages, Hkv, page_size, D), the cache's strides, its device, and
+    the table's (B, W) and elements from row to row."""
+    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
+    table, table_strides = block_table.shape, block_table.stride()
+    if len(shape) != 4 or len(table) != 2 or not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides,
+                                                           device, table, table_strides):
+        _explain_cache(k_cache, v_cache, block_table, seq_lens)
+    return shape, strides, device, table, table_strides[0] if table[0] > 1 else table[1]
+
+
+def _sums_ok(t, B, Hkv, positions, device):
+    """float32 [B, Hkv, positions or more], rows contiguous and each its own."""
+    if t.dim() != 3:
+        return False
+    (b, h, n), (sb, sh, one) = t.shape, t.stride()
+    return (t.dtype is torch.float32 and b == B and h == Hkv and n >= positions and one == 1 and
+            (sb > 0 or B <= 1) and (sh > 0 or Hkv == 1) and t.get_device() == device)
 
 
 def _rows(t):
@@ -132,11 +146,7 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     sequence (a sequence of length 0 takes none).  Positions whose page is outside [0, pages) are
     skipped.  An 8-bit cache holds the codes nearest to value / scale of the head (``k_scale``,
     ``v_scale`` [Hkv]), the largest finite code beyond +-448."""
-    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
-    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
-        _explain_cache(k_cache, v_cache, block_table, seq_lens)
-    pages, Hkv, ps, D = shape
-    B, W, table_stride = _table(block_table)
+    (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     tokens = k.shape[0]
     _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype,
           "k and v must be [tokens, Hkv, D] alike")
@@ -174,11 +184,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     float32: every position's weights, summed over the heads of the group, are added to it.
     Returns out [B, Hq, D], or (out, lse [B, Hq] float32).  A row that nothing is left of is 0, its
     lse -inf (its sink, where there is one)."""
-    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
-    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
-        _explain_cache(k_cache, v_cache, block_table, seq_lens)
-    pages, Hkv, ps, D = shape
-    B, W, table_stride = _table(block_table)
+    (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     Hq = q.shape[1] if q.dim() == 3 else 0
     G = Hq // Hkv
     _need(q.shape == (B, G * Hkv, D) and G > 0 and q.get_device() == device,
@@ -196,8 +202,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
-        _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3 and weight_sums.shape[:2] == (B, Hkv) and
-              weight_sums.shape[2] >= max_len and weight_sums.stride(2) == 1 and weight_sums.get_device() == device,
+        _need(_sums_ok(weight_sums, B, Hkv, max_len, device),
               "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
     size = _bytes("vk_hip_paged_attention_workspace_bytes", kind, B, Hkv, G, D, max_len, window, sums is not None)
@@ -228,17 +233,12 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     Returns (new_lens [B] int32, kept [B, Hkv, budget] int32: the old positions, -1 beyond the new
     length).  The pages of a sequence that is cut must be its own; those behind its new length are
     free afterwards.  Rows keep the position encoding they were stored with."""
-    shape, strides, device = k_cache.shape, k_cache.stride(), k_cache.get_device()
-    if not _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device):
-        _explain_cache(k_cache, v_cache, block_table, seq_lens)
-    pages, Hkv, ps, D = shape
-    B, W, table_stride = _table(block_table)
+    (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     if max_len is None:
         max_len = W * ps
     sums_out = weight_sums if sums_out is None else sums_out
     for name, t in (("weight_sums", weight_sums), ("sums_out", sums_out)):
-        _need(t.dtype is torch.float32 and t.dim() == 3 and t.shape[:2] == (B, Hkv) and t.shape[2] >= max_len and
-              t.stride(2) == 1 and t.get_device() == device,
+        _need(_sums_ok(t, B, Hkv, max_len, device),
               f"{name} must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
     new_lens = torch.empty_like(seq_lens)
     kept = seq_lens.new_empty((B, Hkv, max(budget, 0)))
