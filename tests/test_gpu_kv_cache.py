@@ -422,9 +422,11 @@ def test_evict_ties_zeros_and_odd_values(hip_lib):
 @pytest.mark.parametrize("budget,first,last", [(4097, 1, 64), (8999, 0, 0), (300, 100, 200), (9001, 9001, 0), (5, 0, 2)])
 @pytest.mark.parametrize("kind", ["close", "spread", "ties", "zero"])
 @pytest.mark.parametrize("in_place", [False, True])
-def test_evict_long(hip_lib, budget, first, last, kind, in_place):
-    """Rows that several workgroups share: keys that agree in their leading digits, that do not, few values."""
-    s = Setup([20000, 9000, 100, 8193], 1, 1, 16, 16, seed=2)
+@pytest.mark.parametrize("width", [None, 2100])
+def test_evict_long(hip_lib, budget, first, last, kind, in_place, width):
+    """Rows that a workgroup does not hold in registers, and (a table of more than 32768 positions) rows that
+    several workgroups share: keys that agree in their leading digits, that do not, few values."""
+    s = Setup([20000, 9000, 100, 8193], 1, 1, 16, 16, seed=2, width=width)
     g = torch.Generator(device=dev()).manual_seed(budget)
     sums = torch.rand((4, 1, s.table.shape[1] * 16), device=dev(), generator=g)
     sums = {"close": 1 + 2e-4 * sums, "spread": torch.exp(40 * sums - 20), "ties": (5 * sums).floor(),
@@ -432,7 +434,7 @@ def test_evict_long(hip_lib, budget, first, last, kind, in_place):
     _check_evict(s, sums, budget, first, last, in_place)
 
 
-@pytest.mark.parametrize("rows,longest", [(129, 9000), (40, 12288), (256, 40000)])
+@pytest.mark.parametrize("rows,longest", [(129, 9000), (40, 12288), (256, 40000), (128, 32769), (40, 32768)])
 def test_evict_many_rows(hip_lib, rows, longest):
     """A workgroup for each of many rows longer than it holds in registers, and the rule's edges."""
     g = torch.Generator().manual_seed(rows)

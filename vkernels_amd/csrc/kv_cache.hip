@@ -275,6 +275,8 @@ __device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, u
 // LDS, where the other two digits are found (the sums are walked again for those when there
 // are too many such keys).  The last pass writes the kept positions down: every wavefront
 // walks a stretch of its own, from the counts of the ones before it.
+// Bound by its barriers and dependent loads: 512 rows of 2304 sums (9 MB in and out) in 20 us,
+// 32 rows of 65536 in 66 us, a CU each, where the split form takes 34.
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvictArgs a) {
   __shared__ uint32_t bins[kBinCopies][kBins];
   __shared__ uint32_t listed[kSelectWaves][kListed];
@@ -625,9 +627,9 @@ int kv_evict_batches(int budget, int row_bytes) {
 }
 
 int kv_evict_parts(int rows, int max_len) {
-  // A workgroup walks a row of 8192 positions in 20 us; below that, and with a row for every CU,
-  // the launches of the split form cost more than they save.
-  if (max_len <= 8192 || rows > 128) return 1;
+  // One workgroup takes 10 us for a row of 2304 positions, 19 for 16384, 33 for 32768 and 66 for
+  // 65536, whatever their number up to 128; four launches 24 to 28, 28 to 32, 33 to 37 and 34.
+  if (max_len <= 32768 || rows > 128) return 1;
   const int most = (max_len + 4095) / 4096;
   return min(min(256 / rows, most), kMostParts);
 }

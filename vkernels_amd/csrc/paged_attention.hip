@@ -210,6 +210,22 @@ struct Tile {
 };
 
 
+// The attention itself.  A work item is 16 query heads on one key/value head of one sequence; a
+// workgroup has an even share of all items' units (128 positions) and walks through the items in
+// it, or one whole item where the call is short.  A wavefront takes 32 positions at a time, by itself:
+//   S = K q^T      (16 x 16 x 32, keys the first operand: a lane holds one head's scores of 8
+//                   positions, and running maximum, sum and rescaling stay in the lane),
+//   O^T += V^T P^T (the weights are in the lane that the second product wants them in; the
+//                   values go to LDS by rows and come back transposed, 4 x 16 at a time).
+// The four wavefronts' results meet in LDS at an item's end, several workgroups' in the joining
+// kernel.  The matrix cores run at 1 % of their rate and a CU issues some 170 vector instructions
+// a tile: the stream of keys and values bounds it.  One sequence of 131071 positions, 8 heads of
+// 128: 88 us for 537 MB, 6.1 TB/s (a kernel that only reads reaches 7.0); 255 sequences on an
+// 8-bit cache, 2.34 GB: 373 us, 6.3 TB/s; 64 sequences of 64-wide heads, the cache token by
+// token, 563 MB: 106 us, 5.3 TB/s (head by head 96 us).  5.6 us of each are start, length,
+// page, first tile and the way out.  Registers: with fewer than 256 a lane (three workgroups a
+// CU) a 128-wide head spills (131 us where two take 97), a 64-wide one gains nothing.
+// FULL: D is DP.  P16: pages are multiples of 16 positions, so that a page is the same for 16 rows.
 template <class M, bool FP8, int DP, bool P16, bool FULL>
 __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(const KernelArgs A) {
   typedef Tile<M, FP8, DP> L;
