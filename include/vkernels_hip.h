@@ -708,7 +708,8 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
  *   cut to max_len;  Z = sum_j e^{s_j} + e^{sinks[h]} (sinks [Hq] or NULL),
  *   out_h = v_scale[g] * sum_j e^{s_j} v_j / Z,  lse_h = log Z.
  * A row that nothing is left of, or whose every score is -inf, gives 0 and lse -inf (the
- * sink, where there is one).  weight_sums (or NULL): element [b][g][j] (strides in elements)
+ * sink, where there is one); a NaN, or a score of +inf, at a position that counts makes the
+ * row NaN, an infinite value its column of the result infinite or NaN.  weight_sums (or NULL): element [b][g][j] (strides in elements)
  * grows by the sum over the heads h of g of e^{s_j} / Z.  max_len: at least every length,
  * at most table_width * page_size; launches and workspace follow it, not the lengths.
  * The workspace (16-byte aligned) of vk_hip_paged_attention_workspace_bytes is scratch of

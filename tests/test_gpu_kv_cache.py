@@ -190,6 +190,18 @@ def test_scores_of_infinity_and_nan(hip_lib):
         assert torch.equal(out[0, 0], s.v[page[0, 2], 0, 1])
 
 
+@pytest.mark.parametrize("cache", [BF16, F16])
+def test_an_infinite_value_stays_in_its_column(hip_lib, cache):
+    for n in (40, 1200):
+        s = Setup([n, n], 1, 4, 64, 16, seed=10, cache=cache, q=cache)
+        want = kv.paged_attention(*s.args())
+        s.v[s.table[0, 1].long(), 0, 2, 9] = math.inf
+        got = kv.paged_attention(*s.args())
+        assert not bool(torch.isfinite(got[0, :, 9]).any())
+        got[0, :, 9] = want[0, :, 9]
+        assert torch.equal(got, want)
+
+
 def test_large_scores_and_rising_maxima(hip_lib):
     """The reference of the exponentials moves many times, in both directions of the scores' order."""
     for flip in (False, True):

@@ -52,6 +52,10 @@ OTHER = [
     ("vk_hip_paged_attention", dict(B=1 << 20, Hkv=32, table_width=1 << 20, table_stride=1 << 20, max_len=1 << 23),
      ve.VK_ERROR_OUT_OF_RANGE),
     ("vk_hip_paged_attention", dict(B=1 << 20, Hkv=16, G=1, max_len=100), ve.VK_ERROR_OUT_OF_RANGE),
+    ("vk_hip_paged_attention", dict(B=1, Hkv=1, G=1, table_width=1 << 28, table_stride=1 << 28, max_len=(1 << 31) - 64),
+     ve.VK_ERROR_OUT_OF_RANGE),
+    ("vk_hip_kv_cache_evict", dict(B=1, Hkv=1, table_width=1 << 28, table_stride=1 << 28, max_len=(1 << 31) - 64),
+     ve.VK_ERROR_OUT_OF_RANGE),
     ("vk_hip_kv_cache_evict", dict(B=1 << 17, Hkv=64, max_len=60), ve.VK_ERROR_OUT_OF_RANGE),
     ("vk_hip_kv_cache_evict", dict(elem_bytes=4), ve.VK_ERROR_UNSUPPORTED),
     ("vk_hip_kv_cache_evict", dict(B=1 << 26, Hkv=32), ve.VK_ERROR_OUT_OF_RANGE),

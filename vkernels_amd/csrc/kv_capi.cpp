@@ -15,6 +15,7 @@ namespace {
 
 constexpr int64_t kInt32 = 0x7FFFFFFFll;
 constexpr int64_t kThreads = 0xFFFFFFFFll;   // of a launch
+constexpr int64_t kPositions = kInt32 - (1 << 20);   // positions are ints, a tile or a stretch beyond the last one too
 
 int refuse(int code, const char* who, const char* why) {
   vk_set_last_error(code, (std::string(who) + ": " + why).c_str());
@@ -126,7 +127,7 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
   // (units of work are counted in 32 bits, and so are a launch's threads, 256 for each item or chunk)
   const int64_t rows = (int64_t)B * Hkv, items = rows * ((G + vk::kPaHeads - 1) / vk::kPaHeads);
-  if (rows > kInt32 / G || items > kThreads / 512 || items > kInt32 / (max_len / vk::kPaUnit + 3) / 2 ||
+  if (max_len > kPositions || rows > kInt32 / G || items > kThreads / 512 || items > kInt32 / (max_len / vk::kPaUnit + 3) / 2 ||
       rows > kThreads / 512 / (max_len / 4096 + 2))
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, heads and positions for one call");
   const vk::PagedAttentionPlan plan = vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, weight_sums != nullptr);
@@ -178,7 +179,7 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
     why = "sums_out in place has weight_sums' strides";
   if (why == nullptr && new_lens == seq_lens) why = "new_lens must not be seq_lens";
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  if ((int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2 ||
+  if (max_len > kPositions || (int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2 ||
       (int64_t)B * Hkv * vk::kv_evict_batches(budget, D * elem_bytes) > kThreads / 2 / vk::kKvMoveThreads)
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many rows for one call");
   if (workspace == nullptr || !aligned(workspace, 16) ||

@@ -209,7 +209,6 @@ struct Tile {
                                       ? kPaWaveRows * kPitch : kPaHeads * kOutPitch * 4;
 };
 
-
 // The attention itself.  A work item is 16 query heads on one key/value head of one sequence; a
 // workgroup has an even share of all items' units (128 positions) and walks through the items in
 // it, or one whole item where the call is short.  A wavefront takes 32 positions at a time, by itself:
