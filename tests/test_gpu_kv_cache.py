@@ -53,7 +53,7 @@ class Setup:
             caches = [c.transpose(1, 2).contiguous().transpose(1, 2) for c in caches]
         self.k, self.v = (c.to(dev()) for c in caches)
         if layout == "tokens":
-            assert self.k.stride(1) == D
+            assert self.k.stride(1) == D or 1 in (Hkv, ps)      # (a single head or position has any stride)
         self.q = (peak * torch.randn((self.B, Hkv * G, D), generator=g)).to(q).to(dev())
         self.sinks = torch.randn(Hkv * G, generator=g)
         self.scale = D ** -0.5
