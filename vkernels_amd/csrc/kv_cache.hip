@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvict
 constexpr int kMostParts = 16;
 struct SplitRow {
   uint32_t* counts;   // [3][parts][kBins]
-  uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] certain ones by those
+  uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] kept before a part by those
 };
 __device__ __forceinline__ SplitRow split_row(const KvEvictArgs& a, int row) {
   const int words = 3 * a.parts * kBins + 4 + 2 * a.parts;   // (even: pairs of counts are read)
@@ -378,12 +378,16 @@ __device__ __forceinline__ SplitRow split_row(const KvEvictArgs& a, int row) {
   return SplitRow{base, base + 3 * a.parts * kBins};
 }
 
-// Digit `pass` of the least key from the parts' counts; part 0 leaves what is known behind it, every
-// part what it keeps for certain by this digit.
-__device__ void split_digit(const KvEvictArgs& a, const SplitRow& s, int pass, int part, uint32_t& least, uint32_t& need,
-                            uint32_t* scan_lds, uint32_t* found) {
+// Digit `pass` of the least key from the parts' counts, and of the keys in the parts before this one
+// how many are above it by this digit, and how many share it.  Part 0 leaves what is known
+// behind digits 0 and 1, every part its own count above by them.
+struct PartsBefore {
+  uint32_t above, equal;
+};
+__device__ PartsBefore split_digit(const KvEvictArgs& a, const SplitRow& s, int pass, int part, uint32_t& least,
+                                   uint32_t& need, uint32_t (*lds)[kSelectWaves], uint32_t* found) {
   const int t = threadIdx.x, n = digit_values(pass);
-  uint32_t c[2] = {0, 0}, mine[2] = {0, 0};
+  uint32_t c[2] = {0, 0}, before[2] = {0, 0};
   if (2 * t < n) {
     const uint32_t* const from = s.counts + (int64_t)pass * a.parts * kBins + (n - 2 - 2 * t);
     uint64_t pair[kMostParts];      // both digits of a part, all parts' loads at once
@@ -394,39 +398,50 @@ __device__ void split_digit(const KvEvictArgs& a, const SplitRow& s, int pass, i
       const uint32_t high = (uint32_t)(pair[p] >> 32), low = (uint32_t)pair[p];
       c[0] += high;
       c[1] += low;
-      if (p == part) {
-        mine[0] = high;
-        mine[1] = low;
-      }
+      before[0] += p < part ? high : 0u;
+      before[1] += p < part ? low : 0u;
     }
   }
-  find_digit(c, n, need, scan_lds, found);
+  find_digit(c, n, need, lds[0], found);
   const uint32_t digit = found[0];
   least |= digit << digit_shift(pass);
   need = found[1];
-  uint32_t sure = 0;
+  uint32_t above = 0, equal = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (2 * t < n && (uint32_t)(n - 1 - 2 * t - i) > digit) sure += mine[i];
-  sure = wave_scan(sure);
-  if ((t & 63) == 63) scan_lds[t >> 6] = sure;
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t mine = (uint32_t)(n - 1 - 2 * t - i);
+    if (2 * t < n) {
+      above += mine > digit ? before[i] : 0u;
+      equal += mine == digit ? before[i] : 0u;
+    }
+  }
+  above = wave_scan(above);
+  equal = wave_scan(equal);
+  if ((t & 63) == 63) {
+    lds[0][t >> 6] = above;
+    lds[1][t >> 6] = equal;
+  }
   __syncthreads();
+  PartsBefore r = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kSelectWaves; ++w) {
+    r.above += lds[0][w];
+    r.equal += lds[1][w];
+  }
   if (t == 0 && pass < 2) {
-    uint32_t all = 0;
-    for (int w = 0; w < kSelectWaves; ++w) all += scan_lds[w];
-    s.state[4 + pass * a.parts + part] = all;
+    s.state[4 + pass * a.parts + part] = r.above;
     if (part == 0) {
       s.state[2 * pass] = least;
       s.state[2 * pass + 1] = need;
     }
   }
-  __syncthreads();
+  return r;
 }
 
 template <int PASS>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const KvEvictArgs a) {
   __shared__ uint32_t bins[kBinCopies][kBins];
-  __shared__ uint32_t scan_lds[kSelectWaves], found[2];
+  __shared__ uint32_t scan_lds[2][kSelectWaves], found[2];
   const int t = threadIdx.x, wave = t >> 6, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
   if (!select_row(a, row, part, a.parts, PASS == 0, &r) || r.places == 0) return;
@@ -458,8 +473,8 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const K
 }
 
 __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const KvEvictArgs a) {
-  __shared__ uint32_t scan_lds[kSelectWaves], counts_lds[2][kSelectWaves], found[2];
-  const int t = threadIdx.x, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  __shared__ uint32_t scan_lds[2][kSelectWaves], counts_lds[2][kSelectWaves], found[2];
+  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
   if (!select_row(a, row, part, a.parts, false, &r)) return;
   const SplitRow s = split_row(a, row);
@@ -470,24 +485,10 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   if (r.places > 0) {
     least = s.state[2];
     need = s.state[3];
-    split_digit(a, s, 2, part, least, need, scan_lds, found);
-    const uint32_t digit = least & 1023u;
-    uint32_t sure = 0;
-    const uint32_t* const counts = s.counts + (int64_t)2 * a.parts * kBins;
-#pragma unroll
-    for (int p = 0; p < kMostParts; ++p) {
-      if (p < part) {
-        before_equal += counts[p * kBins + digit];
-        const uint32_t n = counts[p * kBins + t];
-        sure += (uint32_t)t > digit ? n : 0u;
-      }
-    }
-    if (t < part) sure += s.state[4 + t] + s.state[4 + a.parts + t];
-    sure = wave_scan(sure);
-    if ((t & 63) == 63) scan_lds[t >> 6] = sure;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSelectWaves; ++w) before_sure += scan_lds[w];
+    before_sure = s.state[4 + part] + s.state[4 + a.parts + part];
+    const PartsBefore before = split_digit(a, s, 2, part, least, need, scan_lds, found);
+    before_sure += before.above;
+    before_equal = before.equal;
   }
   // (the ends before this part's stretch are kept as well)
   const int stretch = (r.len + 64 * a.parts * kSelectWaves - 1) / (64 * a.parts * kSelectWaves) * 64;
