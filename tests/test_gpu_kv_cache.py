@@ -446,7 +446,7 @@ def test_evict_long(hip_lib, budget, first, last, kind, in_place, width):
     _check_evict(s, sums, budget, first, last, in_place)
 
 
-@pytest.mark.parametrize("rows,longest", [(129, 9000), (40, 12288), (256, 40000), (128, 32769), (40, 32768)])
+@pytest.mark.parametrize("rows,longest", [(129, 9000), (40, 12288), (256, 40000), (65, 32769), (64, 32769), (40, 32768)])
 def test_evict_many_rows(hip_lib, rows, longest):
     """A workgroup for each of many rows longer than it holds in registers, and the rule's edges."""
     g = torch.Generator().manual_seed(rows)

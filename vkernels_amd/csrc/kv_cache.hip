@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, in
 
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
 constexpr int kBins = 2048, kBinCopies = 4;
-constexpr int kSelectLoads = 16;
+constexpr int kSelectLoads = 8;
 constexpr int kListed = 512;   // candidates of a wavefront that are kept in LDS
 
 // A sum as a number that orders as the sums do (NaN above all, -0 like 0).
@@ -275,8 +275,9 @@ __device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, u
 // LDS, where the other two digits are found (the sums are walked again for those when there
 // are too many such keys).  The last pass writes the kept positions down: every wavefront
 // walks a stretch of its own, from the counts of the ones before it.
-// Bound by its barriers and dependent loads: 512 rows of 2304 sums (9 MB in and out) in 20 us,
-// 32 rows of 65536 in 66 us, a CU each, where the split form takes 34.
+// Bound by its barriers and dependent loads: 512 rows of 2304 sums (9 MB in and out) in 15 us (21
+// with 16 sums a lane in registers, which leave a CU room for one workgroup); 32 rows of 65536 in 58 us,
+// a CU each, where the split form takes 32.
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvictArgs a) {
   __shared__ uint32_t bins[kBinCopies][kBins];
   __shared__ uint32_t listed[kSelectWaves][kListed];
@@ -628,9 +629,10 @@ int kv_evict_batches(int budget, int row_bytes) {
 }
 
 int kv_evict_parts(int rows, int max_len) {
-  // One workgroup takes 10 us for a row of 2304 positions, 19 for 16384, 33 for 32768 and 66 for
-  // 65536, whatever their number up to 128; four launches 24 to 28, 28 to 32, 33 to 37 and 34.
-  if (max_len <= 32768 || rows > 128) return 1;
+  // One workgroup takes 9 us for a row of 2304 positions, 20 for 16384, 33 for 32768 and 58 for 65536,
+  // whatever their number up to 192; the four launches 30, 31 and 39 us at 32768 and 33, 40 and 59 at
+  // 65536 for 32, 64 and 128 rows (and 25 and more below).
+  if (max_len <= 32768 || rows > 64) return 1;
   const int most = (max_len + 4095) / 4096;
   return min(min(256 / rows, most), kMostParts);
 }
