@@ -457,6 +457,19 @@ def test_evict_many_rows(hip_lib, rows, longest):
     _check_evict(s, sums, 150, 3, 40, in_place=True)
 
 
+@pytest.mark.parametrize("rows,longest,budget", [(1100, 8192, 511), (1100, 8208, 512), (600, 4800, 513), (600, 4816, 90), (5, 2048, 512), (5, 2064, 513)])
+@pytest.mark.parametrize("kind", ["spread", "close", "ties"])
+def test_evict_rows_of_a_small_workgroup(hip_lib, rows, longest, budget, kind):
+    """The edges of the rules on a row's workgroup: positions to rows, and bytes of a head's kept rows."""
+    g = torch.Generator().manual_seed(rows + longest)
+    lens = torch.randint(1, 900, (rows,), generator=g).tolist()
+    lens[0], lens[rows // 2], lens[-1] = longest, min(longest, 4100), longest - 7
+    s = Setup(lens, 1, 1, 16, 16, seed=2)
+    sums = torch.rand((rows, 1, s.table.shape[1] * 16), device=dev())
+    sums = {"close": 1 + 2e-4 * sums, "spread": torch.exp(40 * sums - 20), "ties": (5 * sums).floor()}[kind]
+    _check_evict(s, sums, budget, 3, 40, in_place=kind != "close")
+
+
 @pytest.mark.parametrize("cache,D", [(FP8, 16), (FP8, 64), (BF16, 128)])
 def test_evict_in_many_batches_of_rows_that_share_lines(hip_lib, cache, D):
     """Several batches of rows a head, which wait for each other, and heads whose rows lie in the same lines."""

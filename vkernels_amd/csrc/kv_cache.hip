@@ -4,6 +4,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "kv_cache.hpp"
 #include "paged_attention.hpp"
 
@@ -100,8 +102,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, in
 
 // ---- eviction ----------------------------------------------------------------------------------
 
-constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64;
-constexpr int kBins = 2048, kBinCopies = 4;
+// A row's workgroup: 16 wavefronts, or 4 for short and for many rows.  (The split form: 16.)
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kFewThreads = 256;
+constexpr int kBins = 2048;
+constexpr int bin_copies(int threads) { return threads / 256; }
 constexpr int kSelectLoads = 8;
 constexpr int kListed = 512;   // candidates of a wavefront that are kept in LDS
 
@@ -125,22 +129,27 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
   return x;
 }
 
-// The workgroup's threads hold the counts c of two digits each, from the largest digit down
-// (thread t those of digits n - 1 - 2 t and n - 2 - 2 t).  Finds the digit that the need-th
+// The workgroup's threads hold the counts c of N successive digits each, from the largest digit
+// down (thread t those of digits n - 1 - N t and below).  Finds the digit that the need-th
 // largest key has, found[0], and how many keys of it are still wanted, found[1].
-__device__ void find_digit(const uint32_t (&c)[2], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
+template <int THREADS, int N>
+__device__ void find_digit(const uint32_t (&c)[N], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
+  static_assert(N * THREADS == kBins, "a thread for every N digits");
   const int t = threadIdx.x, wave = t >> 6;
-  uint32_t above = wave_scan(c[0] + c[1]);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mine += c[i];
+  uint32_t above = wave_scan(mine);
   if ((t & 63) == 63) scan_lds[wave] = above;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w)
+  for (int w = 0; w < THREADS / 64; ++w)
     if (w < wave) above += scan_lds[w];
-  above -= c[0] + c[1];
+  above -= mine;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < N; ++i) {
     if (c[i] > 0 && above < need && above + c[i] >= need) {
-      found[0] = (uint32_t)(n - 1 - 2 * t - i);
+      found[0] = (uint32_t)(n - 1 - N * t - i);
       found[1] = need - above;
     }
     above += c[i];
@@ -149,15 +158,17 @@ __device__ void find_digit(const uint32_t (&c)[2], int n, uint32_t need, uint32_
 }
 
 // The same from histograms in LDS.
+template <int THREADS>
 __device__ void find_digit_lds(uint32_t (*bins)[kBins], int n, uint32_t need, uint32_t* scan_lds, uint32_t* found) {
-  uint32_t c[2] = {0, 0};
-  if (2 * (int)threadIdx.x < n) {
+  constexpr int N = kBins / THREADS;
+  uint32_t c[N] = {};
+  if (N * (int)threadIdx.x < n) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int k = 0; k < kBinCopies; ++k) c[i] += bins[k][n - 1 - 2 * threadIdx.x - i];
+      for (int k = 0; k < bin_copies(THREADS); ++k) c[i] += bins[k][n - 1 - N * threadIdx.x - i];
   }
-  find_digit(c, n, need, scan_lds, found);
+  find_digit<THREADS>(c, n, need, scan_lds, found);
 }
 
 // The digits, from the most significant one: their shifts, numbers of values and the bits above.
@@ -202,6 +213,7 @@ struct SelectRow {
 
 // What a row that is cut and one that is not have in common: true for the first.  `part` of
 // `parts` workgroups of the row, a stretch for each of their wavefronts.
+template <int THREADS>
 __device__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, bool first_pass, SelectRow* r) {
   const int t = threadIdx.x, wave = t >> 6, b = row / a.Hkv, h = row % a.Hkv;
   r->len = min(max(a.lens[b], 0), a.max_len);
@@ -211,22 +223,22 @@ __device__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, b
   if (first_pass && part == 0) {
     // What orders the workgroups of the compaction behind this, for the keys and the values: a
     // count of the batches taken, and a word for each batch that has been read.
-    for (int i = t; i < 2 * (1 + a.batches); i += kSelectThreads) a.order[(int64_t)row * 2 * (1 + a.batches) + i] = 0;
+    for (int i = t; i < 2 * (1 + a.batches); i += THREADS) a.order[(int64_t)row * 2 * (1 + a.batches) + i] = 0;
     if (h == 0 && t == 0) a.new_lens[b] = min(r->len, a.budget);
     if (r->len <= a.budget) {
       float* const out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
-      for (int j = t; j < a.budget; j += kSelectThreads) r->kept[j] = j < r->len ? j : -1;
+      for (int j = t; j < a.budget; j += THREADS) r->kept[j] = j < r->len ? j : -1;
       if (out != r->sums)
-        for (int j = t; j < r->len; j += kSelectThreads) out[j] = r->sums[j];
+        for (int j = t; j < r->len; j += THREADS) out[j] = r->sums[j];
     }
   }
   if (r->len <= a.budget) return false;
   r->lo = a.keep_first;
   r->hi = r->len - a.keep_last;
   r->places = (uint32_t)(a.budget - a.keep_first - a.keep_last);
-  const int waves = parts * kSelectWaves;
+  const int waves = parts * (THREADS / 64);
   const int stretch = (r->len + 64 * waves - 1) / (64 * waves) * 64;
-  r->from = min(r->len, (part * kSelectWaves + wave) * stretch);
+  r->from = min(r->len, (part * (THREADS / 64) + wave) * stretch);
   r->to = min(r->len, r->from + stretch);
   r->resident = stretch <= 64 * kSelectLoads;
   return true;
@@ -252,7 +264,8 @@ __device__ __forceinline__ void write_kept(const SelectRow& r, float (&x)[kSelec
 }
 
 // Sums over the workgroup's wavefronts before this one, of a pair of counts.
-__device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, uint32_t (*lds)[kSelectWaves]) {
+template <int WAVES>
+__device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, uint32_t (*lds)[WAVES]) {
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) {
     lds[0][wave] = sure;
@@ -261,7 +274,7 @@ __device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, u
   __syncthreads();
   sure = equal = 0;
 #pragma unroll
-  for (int w = 0; w < kSelectWaves; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (w < wave) {
       sure += lds[0][w];
       equal += lds[1][w];
@@ -278,18 +291,20 @@ __device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, u
 // Bound by its barriers and dependent loads: 512 rows of 2304 sums (9 MB in and out) in 15 us (21
 // with 16 sums a lane in registers, which leave a CU room for one workgroup); 32 rows of 65536 in 58 us,
 // a CU each, where the split form takes 32.
-__global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvictArgs a) {
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a) {
+  constexpr int kWaves = THREADS / 64, kBinCopies = bin_copies(THREADS);
   __shared__ uint32_t bins[kBinCopies][kBins];
-  __shared__ uint32_t listed[kSelectWaves][kListed];
-  __shared__ uint32_t scan_lds[kSelectWaves], counts_lds[2][kSelectWaves];
+  __shared__ uint32_t listed[kWaves][kListed];
+  __shared__ uint32_t scan_lds[kWaves], counts_lds[2][kWaves];
   __shared__ uint32_t found[2], too_many;
   const int t = threadIdx.x, wave = t >> 6;
   SelectRow r;
-  if (!select_row(a, blockIdx.x, 0, 1, true, &r)) return;
+  if (!select_row<THREADS>(a, blockIdx.x, 0, 1, true, &r)) return;
   float x[kSelectLoads];
   uint32_t least = 0, need = r.places;   // the least key that is kept; of its equals, the first `need` are
   auto clear_bins = [&] {
-    for (int i = t; i < kBinCopies * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
+    for (int i = t; i < kBinCopies * kBins; i += THREADS) (&bins[0][0])[i] = 0;
     __syncthreads();
   };
   auto count = [&](uint32_t digit) { atomicAdd(&bins[wave % kBinCopies][digit], 1u); };
@@ -300,7 +315,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvict
   if (t == 0) too_many = 0;
   __syncthreads();
   if (r.places > 0) {
-    find_digit_lds(bins, 2048, r.places, scan_lds, found);
+    find_digit_lds<THREADS>(bins, 2048, r.places, scan_lds, found);
     least = found[0] << 21;
     need = found[1];
   }
@@ -339,7 +354,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(const KvEvict
         });
       }
       __syncthreads();
-      find_digit_lds(bins, n, need, scan_lds, found);
+      find_digit_lds<THREADS>(bins, n, need, scan_lds, found);
       least |= found[0] << shift;
       need = found[1];
       __syncthreads();
@@ -403,7 +418,7 @@ __device__ PartsBefore split_digit(const KvEvictArgs& a, const SplitRow& s, int 
       before[1] += p < part ? low : 0u;
     }
   }
-  find_digit(c, n, need, lds[0], found);
+  find_digit<kSelectThreads>(c, n, need, lds[0], found);
   const uint32_t digit = found[0];
   least |= digit << digit_shift(pass);
   need = found[1];
@@ -441,11 +456,12 @@ __device__ PartsBefore split_digit(const KvEvictArgs& a, const SplitRow& s, int 
 
 template <int PASS>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const KvEvictArgs a) {
+  constexpr int kBinCopies = bin_copies(kSelectThreads);
   __shared__ uint32_t bins[kBinCopies][kBins];
   __shared__ uint32_t scan_lds[2][kSelectWaves], found[2];
   const int t = threadIdx.x, wave = t >> 6, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
-  if (!select_row(a, row, part, a.parts, PASS == 0, &r) || r.places == 0) return;
+  if (!select_row<kSelectThreads>(a, row, part, a.parts, PASS == 0, &r) || r.places == 0) return;
   const SplitRow s = split_row(a, row);
   uint32_t least = 0, need = r.places;
   if constexpr (PASS == 2) {
@@ -477,7 +493,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   __shared__ uint32_t scan_lds[2][kSelectWaves], counts_lds[2][kSelectWaves], found[2];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
-  if (!select_row(a, row, part, a.parts, false, &r)) return;
+  if (!select_row<kSelectThreads>(a, row, part, a.parts, false, &r)) return;
   const SplitRow s = split_row(a, row);
   uint32_t least = 0, need = r.places;
   uint32_t before_sure = 0, before_equal = 0;      // kept in the parts before this one
@@ -516,9 +532,9 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
 // Bound by the rows read and written (64 sequences of 8 heads of 128 to 2048 positions: 1.07 GB
 // in 214 us, 5.0 TB/s; a copy of that size reaches 5.2), past the caches: nothing is used twice.
 // Batches of 32 KB are 2 to 8 % behind, rows that stay in the caches 5 %.
-constexpr int kMoveLoads = 8, kMoveThreads = kKvMoveThreads;
-constexpr int kMovePieces = kMoveLoads * kMoveThreads;    // of 16 bytes
-__global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs a) {
+constexpr int kMoveLoads = 8;       // of 16 bytes a thread
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_move_kernel(const KvEvictArgs a) {
   __shared__ uint32_t ticket_lds;
   const int t = threadIdx.x;
   const int list = blockIdx.x % (2 * a.B * a.Hkv);
@@ -533,7 +549,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
   char* const cache = (char*)(which ? a.v_cache : a.k_cache) + (int64_t)h * a.head_stride;
   const int32_t* const kept = a.kept + (int64_t)bh * a.budget;
   const int32_t* const pages = a.table + (int64_t)b * a.table_stride;
-  const int pieces = a.row_bytes / 16, rows = kMovePieces / pieces;
+  const int pieces = a.row_bytes / 16, rows = (kMoveLoads * THREADS) / pieces;
   const int first = batch * rows, last = min(a.budget, first + rows);     // rows that are written
   // Three rounds of loads, each of them all at once: the old places, the pages, the rows.  (A lane
   // without a row, or with one that stays, reads a valid one and writes nothing.)
@@ -542,7 +558,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
   bool moves[kMoveLoads];
 #pragma unroll
   for (int i = 0; i < kMoveLoads; ++i) {
-    const int e = i * kMoveThreads + t, in_batch = divided(e, a.by_pieces);
+    const int e = i * THREADS + t, in_batch = divided(e, a.by_pieces);
     piece[i] = e - in_batch * pieces;
     dst[i] = min(first + in_batch, last - 1);
     moves[i] = in_batch < rows && first + in_batch < last;
@@ -567,11 +583,11 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
   const bool with_sums = which == 0;
   const float* const sums = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)h * a.sums_stride_h;
   float* const sums_out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
-  float sum[kMovePieces / kMoveThreads];
+  float sum[kMoveLoads];
   if (with_sums) {
 #pragma unroll
-    for (int i = 0; i < kMovePieces / kMoveThreads; ++i)
-      if (i * kMoveThreads < rows) sum[i] = sums[kept[min(first + i * kMoveThreads + t, last - 1)]];
+    for (int i = 0; i < kMoveLoads; ++i)
+      if (i * THREADS < rows) sum[i] = sums[kept[min(first + i * THREADS + t, last - 1)]];
   }
   // Every read of the batch has arrived: the rows are in registers, and nobody reads in this
   // kernel what another workgroup writes, so that the words need no cache to be written
@@ -582,7 +598,7 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
   // earlier batches with a source among the rows first .. last - 1 (and, before the sums behind the
   // last row are cleared, those with a source there)
   const bool clears = with_sums && batch == a.batches - 1;
-  for (int c = t; c < batch; c += kMoveThreads) {
+  for (int c = t; c < batch; c += THREADS) {
     const int c_last = kept[c * rows + rows - 1];
     if ((kept[c * rows] < last && c_last >= first) || (clears && c_last >= a.budget))
       while (__hip_atomic_load(read + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(2);
@@ -596,12 +612,12 @@ __global__ __launch_bounds__(kMoveThreads) void kv_move_kernel(const KvEvictArgs
   }
   if (with_sums) {
 #pragma unroll
-    for (int i = 0; i < kMovePieces / kMoveThreads; ++i) {
-      const int j = first + i * kMoveThreads + t;
-      if (i * kMoveThreads < rows && i * kMoveThreads + t < rows && j < last) sums_out[j] = sum[i];
+    for (int i = 0; i < kMoveLoads; ++i) {
+      const int j = first + i * THREADS + t;
+      if (i * THREADS < rows && i * THREADS + t < rows && j < last) sums_out[j] = sum[i];
     }
     if (clears)
-      for (int j = a.budget + t; j < len; j += kMoveThreads) sums_out[j] = 0.0f;
+      for (int j = a.budget + t; j < len; j += THREADS) sums_out[j] = 0.0f;
   }
 }
 
@@ -623,8 +639,14 @@ void launch_kv_append(const KvAppendArgs& args, int kind, hipStream_t stream) {
     hipLaunchKernelGGL((kv_append_kernel<false>), grid, block, 0, stream, a, bf16);
 }
 
+int kv_evict_move_threads(int budget, int row_bytes) {
+  // A head's rows that fit a batch of 16 KB need no larger workgroup: 13952 lists of 43 rows of 128
+  // bytes in 43 us (512 threads, with room for twelve times the rows: 124), 6848 of 41 in 27 (65).
+  return (int64_t)budget * row_bytes <= kMoveLoads * kKvMoveFewThreads * 16 ? kKvMoveFewThreads : kKvMoveThreads;
+}
+
 int kv_evict_batches(int budget, int row_bytes) {
-  const int rows = kMovePieces / (row_bytes / 16);
+  const int rows = kMoveLoads * kv_evict_move_threads(budget, row_bytes) / (row_bytes / 16);
   return (budget + rows - 1) / rows;
 }
 
@@ -635,6 +657,17 @@ int kv_evict_parts(int rows, int max_len) {
   if (max_len <= 32768 || rows > 64) return 1;
   const int most = (max_len + 4095) / 4096;
   return min(min(256 / rows, most), kMostParts);
+}
+
+// A row of 2048 sums is in the registers of 256 threads, which cost less to start and to bring to a
+// barrier, and more rows share a CU: 6976 rows of up to 64 sums in 27 us (1024 threads: 99), 3424 of
+// up to 927 in 22 (64), 1024 of up to 600 in 10 (20), 128 in 7.5 (8.2), 8 of 2000 in 10.2 (9.4).
+// Past that a few threads have to read a row again for each digit, which pays as long as other rows
+// hide it: 576 rows of up to 4000 in 17 (20), but of 8000 in 26 (23); 1024 of 5000 in 22 (28) and of
+// 9000 in 32 (40), but of 16000 in 60 (56); 256 of 2300 in 12.1 (10.8).
+static int select_threads(int rows, int max_len) {
+  return max_len <= kSelectLoads * kFewThreads || max_len <= std::min<int64_t>(8 * (int64_t)rows, kSelectLoads * kSelectThreads)
+             ? kFewThreads : kSelectThreads;
 }
 
 size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget) {
@@ -651,8 +684,10 @@ void launch_kv_evict(const KvEvictArgs& args, hipStream_t stream) {
   a.batches = kv_evict_batches(a.budget, a.row_bytes);
   a.parts = kv_evict_parts(rows, a.max_len);
   a.split = a.order + 2 * (size_t)rows * (1 + a.batches);
-  if (a.parts == 1) {
-    hipLaunchKernelGGL(kv_select_kernel, dim3(rows), dim3(kSelectThreads), 0, stream, a);
+  if (a.parts == 1 && select_threads(rows, a.max_len) == kFewThreads) {
+    hipLaunchKernelGGL((kv_select_kernel<kFewThreads>), dim3(rows), dim3(kFewThreads), 0, stream, a);
+  } else if (a.parts == 1) {
+    hipLaunchKernelGGL((kv_select_kernel<kSelectThreads>), dim3(rows), dim3(kSelectThreads), 0, stream, a);
   } else {
     const dim3 grid(rows * a.parts), block(kSelectThreads);
     hipLaunchKernelGGL((kv_select_digit_kernel<0>), grid, block, 0, stream, a);
@@ -660,7 +695,11 @@ void launch_kv_evict(const KvEvictArgs& args, hipStream_t stream) {
     hipLaunchKernelGGL((kv_select_digit_kernel<2>), grid, block, 0, stream, a);
     hipLaunchKernelGGL(kv_select_keep_kernel, grid, block, 0, stream, a);
   }
-  hipLaunchKernelGGL(kv_move_kernel, dim3(2 * rows * a.batches), dim3(kMoveThreads), 0, stream, a);
+  const dim3 batches(2 * rows * a.batches);
+  if (kv_evict_move_threads(a.budget, a.row_bytes) == kKvMoveThreads)
+    hipLaunchKernelGGL((kv_move_kernel<kKvMoveThreads>), batches, dim3(kKvMoveThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kv_move_kernel<kKvMoveFewThreads>), batches, dim3(kKvMoveFewThreads), 0, stream, a);
 }
 
 }  // namespace vk

@@ -50,7 +50,7 @@ struct KvEvictArgs {
   FastDiv by_page, by_pieces;
 };
 int kv_evict_batches(int budget, int row_bytes);   // of the keys (or values) of a head
-constexpr int kKvMoveThreads = 512;                // of a batch's workgroup
+constexpr int kKvMoveThreads = 512, kKvMoveFewThreads = 128;   // of a batch's workgroup
 size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget);
 void launch_kv_evict(const KvEvictArgs& a, hipStream_t stream);
 
