@@ -101,6 +101,14 @@ def test_head_layouts(hip_lib, Hkv, G, long):
     Setup(lens, Hkv, G, 64, 16, seed=Hkv * 100 + G).check(counted=True, sinks=True)
 
 
+@pytest.mark.parametrize("Hkv,G,D", [(1, 24, 64), (3, 40, 64), (1, 128, 128), (1, 250, 64), (1, 256, 192), (1, 260, 64), (2, 272, 16), (1, 273, 64)])
+@pytest.mark.parametrize("lens,window", [([9000], 0), ([1, 2500, 0, 3001, 17], 0), ([5000, 1300, 4999], 2000), ([40, 3, 1030], 1025)])
+def test_head_tiles_that_share_a_stream(hip_lib, Hkv, G, D, lens, window):
+    """Up to 16 tiles of heads each have workgroups of their own (a number that does not divide the grid
+    among them, and one tile more than that)."""
+    Setup(lens, Hkv, G, D, 16, seed=G + len(lens)).check(counted=True, sinks=True, window=window)
+
+
 @pytest.mark.parametrize("ps", [1, 2, 3, 7, 8, 16, 17, 24, 32, 48, 64, 100, 256, 1000])
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
 def test_page_sizes_and_layouts(hip_lib, ps, layout):

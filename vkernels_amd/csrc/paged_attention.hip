@@ -139,9 +139,10 @@ __device__ __forceinline__ int page_of(const KernelArgs& A, int pos) { return di
 
 // The units of all items in order (sequence, head item, unit), cut into equal shares.
 struct Share {
-  int first, last;   // units of this workgroup
+  int first, last;   // units of this workgroup, of those of its group
   int per;           // units of a share
   int b, unit0;      // the sequence that `first` lies in, and its first unit
+  int group, index;  // head tile (where those have workgroups of their own; else 0), workgroup of it
 };
 
 // Inclusive sum over the lanes of a wavefront up to this one.
@@ -163,7 +164,10 @@ __device__ __forceinline__ int lanes_up_to(int x) {
 __device__ __forceinline__ bool find_share(const KernelArgs& A, Share* sh) {
   const PagedAttentionArgs& a = A.a;
   const int lane = threadIdx.x & 63;
-  const int heads = a.Hkv * A.p.head_tiles;
+  const int heads = a.Hkv * (A.p.head_tiles / A.p.tile_groups);
+  sh->group = (int)blockIdx.x / A.p.group_workgroups;
+  sh->index = (int)blockIdx.x - sh->group * A.p.group_workgroups;
+  if (sh->group >= A.p.tile_groups) return false;   // (uniform over the workgroup, as below)
   const int per = (a.B + 63) / 64;
   int mine = 0;
   for (int i = 0; i < per; ++i) {
@@ -172,9 +176,9 @@ __device__ __forceinline__ bool find_share(const KernelArgs& A, Share* sh) {
   }
   const int scan = lanes_up_to(mine);
   const int total = __builtin_amdgcn_readlane(scan, 63) * heads;
-  const int share = max(A.p.min_units, (total + A.p.workgroups - 1) / A.p.workgroups);
-  const int first = (int)blockIdx.x * share;
-  if (first >= total) return false;   // (uniform over the workgroup)
+  const int share = max(A.p.min_units, (total + A.p.group_workgroups - 1) / A.p.group_workgroups);
+  const int first = sh->index * share;
+  if (first >= total) return false;
   int at = (scan - mine) * heads, b = lane * per;
   const bool here = first >= at && first < at + mine * heads;
   if (here && per > 1) {
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int item_heads = a.Hkv * A.p.head_tiles;
+  const int tiles = A.p.head_tiles / A.p.tile_groups, item_heads = a.Hkv * tiles;   // of a sequence, in the group
   char* const my_lds = lds + wave * L::kWaveLds;
 
   Share sh;
@@ -248,7 +252,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       return;
     }
   } else {
-    sh.first = 0;
+    sh.first = sh.group = 0;
     sh.b = blockIdx.x / item_heads;
     item_in_b = blockIdx.x % item_heads;
   }
@@ -267,18 +271,19 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
   }
   int b = sh.b;
   int item_unit0 = A.p.workgroups > 0 ? sh.first - unit_at : 0;   // the item's first unit
+  auto item_at = [&](int b, int in_b) { return (b * a.Hkv + in_b / tiles) * A.p.head_tiles + sh.group + in_b % tiles; };
   if (A.p.workgroups > 0 && threadIdx.x == 0) {
     // For the join: the item that other workgroups began and this one ends, if there is one.
     const bool ends = unit_at > 0 && span.units - unit_at <= left;
     const int begun = item_unit0 / sh.per;
-    *ends_here = u32x4{(uint32_t)(b * item_heads + item_in_b), (uint32_t)begun,
-                       ends ? (uint32_t)((int)blockIdx.x - begun + 1) : 0u, 0u};
+    *ends_here = u32x4{(uint32_t)item_at(b, item_in_b), (uint32_t)((int)blockIdx.x - sh.index + begun),
+                       ends ? (uint32_t)(sh.index - begun + 1) : 0u, 0u};
   }
 
   const int64_t slot_bytes = a.slot_stride * L::kElem, page_bytes = a.page_stride * L::kElem;
   while (left > 0) {
     const int units = min(left, span.units - unit_at);
-    const int g = item_in_b / A.p.head_tiles, head0 = (item_in_b % A.p.head_tiles) * kPaHeads;
+    const int g = item_in_b / tiles, head0 = (sh.group + item_in_b % tiles) * kPaHeads;
     const int heads = min(kPaHeads, a.G - head0);
     const ConstInts pages = read_only(a.table + (int64_t)b * a.table_stride);
     const char* const kbase = (const char*)a.k_cache + (int64_t)g * a.head_stride * L::kElem;
@@ -378,9 +383,10 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         for (int i = 0; i < L::kKLoads; ++i) kreg[t][i] = key_piece(row, i);
       }
     };
-    // (Values past the caches: nobody reads them again, and the keys' lines, which two loads share, then
+    // (Values past the caches: with up to 16 heads nobody reads them again, and the keys' lines, which two loads share, then
     // stay until the second: 97 -> 87 us for 131071 positions of 8 heads of 128.  Keys past the
-    // caches too cost a fifth at rows of 128 bytes.)
+    // caches too cost a fifth at rows of 128 bytes.  Of more heads' tiles the later ones would gain 5 to
+    // 10 % by values that stay, and lose as much where scores are kept.)
     auto load_v = [&] {
 #pragma unroll
       for (int i = 0; i < L::kVLoads; ++i) {
@@ -595,12 +601,11 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       for (int i = 0; i < DP / 16; ++i) *(f32x4*)(to + i * 16) = acc[i];
     }
     __syncthreads();
-    const int item = b * item_heads + item_in_b;
     const bool begins = unit_at == 0, ends = unit_at + units == span.units;
     const bool alone = begins && ends;
     if (A.p.workgroups > 0 && begins && threadIdx.x == 0) {
-      const int count = (item_unit0 + span.units - 1) / sh.per - (int)blockIdx.x + 1;
-      ((int64_t*)((char*)a.workspace + A.p.meta_at))[item] = ((int64_t)count << 32) | blockIdx.x;
+      const int count = (item_unit0 + span.units - 1) / sh.per - sh.index + 1;
+      ((int64_t*)((char*)a.workspace + A.p.meta_at))[item_at(b, item_in_b)] = ((int64_t)count << 32) | blockIdx.x;
     }
     const int slot = 2 * blockIdx.x + (begins ? 1 : 0);
     const int pairs = a.D / 4;
@@ -905,6 +910,14 @@ PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, 
   const bool fp8 = kind >= kKvFp8Bf16;
   const int padded = padded_width(D, fp8);
   p.workgroups = units > 8 ? 256 * residents(padded) : 0;
+  // More than 16 query heads a key/value head: every tile of 16 has an equal part of the workgroups and
+  // the same shares, and workgroups that read the same at about the same time sit on one XCD (8
+  // workgroups apart), so that the cache comes from memory about once.  Tiles as items one behind the
+  // other: 33 sequences of up to 14156 positions, 16 heads of 24: 393 us against 336 (1.08 GB; two tiles);
+  // one of 131071, 2 heads of 48: 63 / 50; 255 on an 8-bit cache, 1 head of 64: 180 / 148; only with kept
+  // scores, which go out twice as well, 998 / 1014.  Beyond 16 tiles a part would be a few workgroups.
+  p.tile_groups = p.workgroups > 0 && p.head_tiles <= 16 ? p.head_tiles : 1;
+  p.group_workgroups = p.tile_groups > 1 ? p.workgroups / p.tile_groups / 8 * 8 : p.workgroups;
   size_t at = 0;
   auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   if (p.workgroups > 0) {

@@ -43,6 +43,8 @@ struct PagedAttentionPlan {
   int head_tiles;           // work items of 16 query heads for each key/value head
   int items;                // B * Hkv * head_tiles
   int workgroups;           // workgroups that share the units evenly; 0: one for each item, whole
+  int tile_groups;          // head_tiles, where each tile's items have workgroups of their own; else 1
+  int group_workgroups;     // ... so many
   int min_units;            // least share of a workgroup
   int score_pitch;          // positions a row of kept scores is long (0: none are kept)
   size_t ends_at, meta_at, stats_at, ml_at, part_at, scores_at, bytes;  // parts of the workspace
