@@ -14,6 +14,7 @@
 
 #include "fast_div.hpp"
 #include "paged_attention.hpp"
+#include "paged_attention_layout.hpp"
 
 namespace vk {
 namespace {
@@ -123,11 +124,6 @@ __device__ __forceinline__ Span span_of(int len, int max_len, int window) {
 // Workgroups of a CU (wavefronts of a SIMD), by the registers that a width needs: the grid is as
 // many as the card holds at once.
 constexpr int residents(int DP) { return DP <= 128 ? 2 : 1; }
-int padded_width(int D, bool fp8) {
-  if (D <= 64) return 64;
-  if (D <= 96 && !fp8) return 96;
-  return D <= 128 ? 128 : D <= 192 ? 192 : 256;
-}
 
 struct KernelArgs {
   PagedAttentionArgs a;
@@ -201,12 +197,11 @@ template <class M, bool FP8, int DP>
 struct Tile {
   static constexpr int kElem = FP8 ? 1 : 2;
   static constexpr int kRowBytes = DP * kElem;
-  // 16-byte pieces of a value row, rounded up to a power of two: lanes that load a row
-  static constexpr int kPieces = kRowBytes <= 64 ? 4 : kRowBytes <= 128 ? 8 : kRowBytes <= 256 ? 16 : 32;
+  static constexpr int kPieces = pa_value_pieces(kRowBytes);   // lanes that load a value row
   static constexpr int kRowsPerLoad = 64 / kPieces;
   static constexpr int kVLoads = kPaWaveRows / kRowsPerLoad;
   static constexpr int kPitch = kPieces * 16;            // bytes of a row in LDS
-  static constexpr int kKLoads = kRowBytes / 64;         // 64 bytes of 16 rows each
+  static constexpr int kKLoads = pa_key_loads(kRowBytes);   // 64 bytes of 16 rows each
   static constexpr int kSteps = DP / 32;                 // MFMAs over the head's width
   static constexpr int kOutPitch = DP + 4;               // floats of a head's sums in LDS
   static constexpr int kWaveLds = kPaWaveRows * kPitch > kPaHeads * kOutPitch * 4
@@ -363,17 +358,16 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       const int hi = __shfl((int)(row_at >> 32), row);
       return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
     };
-    // A row of a width below DP: what lies behind its last value is read as zeros (keys) or not
-    // used (values); such lanes read the row's first bytes instead.
-    const int row_bytes = a.D * L::kElem;
+    // What lies behind a row's last value is taken as zeros (keys) or not used (values), and such lanes
+    // read the row's first bytes instead.
+    const int row_bytes = FULL ? L::kRowBytes : a.D * L::kElem;
     auto key_piece = [&](const char* row, int i) -> u32x4 {
-      if constexpr (FULL) return *(const u32x4*)(row + quad * 16 + i * 64);
-      const int at = quad * 16 + i * 64;
-      const u32x4 x = *(const u32x4*)(row + (at < row_bytes ? at : 0));
+      const int at = pa_key_at(quad, i);
+      const u32x4 x = *(const u32x4*)(row + pa_piece_at(at, row_bytes));
       return at < row_bytes ? x : u32x4{0, 0, 0, 0};
     };
     const int piece = lane % L::kPieces, sub = lane / L::kPieces;
-    const uint32_t value_at = FULL ? piece * 16 : (piece * 16 < row_bytes ? piece * 16 : 0);
+    const uint32_t value_at = pa_value_at(piece, row_bytes);
     const uint32_t key_lane = (uint32_t)col * (uint32_t)slot_bytes, value_lane = (uint32_t)sub * (uint32_t)slot_bytes + value_at;
     auto load_k = [&] {
 #pragma unroll
@@ -880,7 +874,7 @@ void launch_width(const KernelArgs& A, hipStream_t stream) {
 
 template <class M, bool FP8>
 void launch_kind(const KernelArgs& A, hipStream_t stream) {
-  const int padded = padded_width(A.a.D, FP8);
+  const int padded = pa_padded_width(A.a.D, FP8);
   switch (padded) {
     case 64: launch_width<M, FP8, 64>(A, stream); break;
     case 96: if constexpr (!FP8) launch_width<M, FP8, 96>(A, stream); break;
@@ -908,7 +902,7 @@ PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, 
   // Shares of less than 2 units would leave more partial results than they save time.
   p.min_units = 2;
   const bool fp8 = kind >= kKvFp8Bf16;
-  const int padded = padded_width(D, fp8);
+  const int padded = pa_padded_width(D, fp8);
   p.workgroups = units > 8 ? 256 * residents(padded) : 0;
   // More than 16 query heads a key/value head: every tile of 16 has an equal part of the workgroups and
   // the same shares, and workgroups that read the same at about the same time sit on one XCD (8
