@@ -98,3 +98,12 @@ def test_workspace_bytes(lib):
     assert 0 < plain < counted
     assert counted >= plain + 4 * 64 * 32 * 8192           # every score is kept
     assert size(0, 64, 8, 4, 128, 100, 0, 1) >= 4 * 64 * 32 * 100
+
+
+@pytest.mark.parametrize("window", [8192 - 16, 8192, 2 ** 31 - 17, 2 ** 31 - 16, 2 ** 31 - 1, -1, -2 ** 31])
+@pytest.mark.parametrize("counted", [0, 1])
+def test_a_window_beyond_the_lengths_is_planned_like_none(lib, window, counted):
+    """The largest integers are a usual way to say that there is no window."""
+    size = kv._fn("vk_hip_paged_attention_workspace_bytes")
+    for B, Hkv, G in ((64, 8, 4), (8, 8, 4), (1, 1, 40)):
+        assert size(0, B, Hkv, G, 128, 8192, window, counted) == size(0, B, Hkv, G, 128, 8192, 0, counted) > 0

@@ -133,6 +133,10 @@ struct KernelArgs {
 
 __device__ __forceinline__ int page_of(const KernelArgs& A, int pos) { return divided(pos, A.by_page); }
 
+// Positions from a span's start to its end, at most.  (Any window may be asked for: nothing is added to one
+// that reaches beyond max_len.)
+int most_seen(int max_len, int window) { return window > 0 && window < max_len - 16 ? window + 16 : max_len; }
+
 // The units of all items in order (sequence, head item, unit), cut into equal shares.
 struct Share {
   int first, last;   // units of this workgroup, of those of its group
@@ -844,7 +848,7 @@ void launch_join(const KernelArgs& A, int padded, hipStream_t stream) {
   const PagedAttentionArgs& a = A.a;
   const int heads = std::min(a.G, kPaHeads), groups = SPLIT > 1 ? heads : (heads + 3) / 4;
   const int join_blocks = A.p.workgroups > 0 ? (SPLIT > 1 ? A.p.items : A.p.workgroups) * groups : 0;
-  const int seen = a.sums == nullptr ? 0 : a.window > 0 && a.window + 16 < a.max_len ? a.window + 16 : a.max_len;
+  const int seen = a.sums == nullptr ? 0 : most_seen(a.max_len, a.window);
   // (four times the positions a block where the card has blocks enough, for fewer latencies in a row)
   const bool many = (int64_t)a.B * a.Hkv * ((seen + 1023) / 1024) > 2048;
   const int chunks = many ? (seen + 4095) / 4096 : (seen + 1023) / 1024;
@@ -894,7 +898,7 @@ PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, 
   PagedAttentionPlan p{};
   p.head_tiles = (G + kPaHeads - 1) / kPaHeads;
   p.items = B * Hkv * p.head_tiles;
-  const int seen = window > 0 && window + 16 < max_len ? window + 16 : max_len;
+  const int seen = most_seen(max_len, window);
   const int units = (seen + kPaUnit - 1) / kPaUnit;
   // Up to 8 units an item is one workgroup's and there is no second launch (64 heads on 8, 1000
   // positions: 1 sequence 10.0 us against 7.2 + 3.9, 8 sequences 11.0 / 8.6 + 4.0, 64 sequences
