@@ -5,7 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_kv_cache import BF16, Setup, dev
+import kv_reference as ref
+from test_gpu_kv_cache import BF16, F16, FP8, Setup, dev
 from vkernels_amd import kv_cache as kv
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +20,42 @@ def test_a_window_beyond_every_length(hip_lib, window, lens):
     out, lse, _ = s.check(window=window, counted=True, sinks=True)
     want, want_lse, _ = s.check(counted=True, sinks=True)
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (F16, F16), (FP8, BF16), (FP8, F16)])
+@pytest.mark.parametrize("n", [33, 40, 1200, 20000])
+@pytest.mark.parametrize("where", ["first", "last", "every 32"])
+def test_many_small_weights_beside_a_large_one(hip_lib, cache, q, n, where):
+    """One position takes nearly all the weight and has a value of zero (or of one), all others are `gap`
+    nats below it and alike: what they add up to is the result (or part of it), to the result's own
+    rounding.  Or every tile of 32 has such a position.
+
+    Scores are single products, exact.  A weight is off by 2^-24 of its exponent in powers of two (less
+    than 64) twice and by 2^-22 of the exponential, and bf16 keeps 2^-17 of it; a lane adds up fewer than
+    64 tiles one after the other; numerator and sum: below 2^-15 of the result in all, its rounding aside."""
+    s = Setup([n] * 6, 1, 1, 64, 16, cache=cache, q=q, seed=n)
+    at = {"first": [0], "last": [n - 1], "every 32": list(range(5, n, 32))}[where]
+    gaps = torch.tensor([8.0, 12.0, 16.0, 18.0, 20.0, 16.0])
+    s.q.zero_()
+    s.q[:, :, 0] = 1.0
+    if s.k_scale is not None:
+        s.k_scale, s.v_scale = torch.ones_like(s.k_scale), torch.ones_like(s.v_scale)
+    j = torch.arange(n, device=dev())
+    for b, gap in enumerate(gaps.tolist()):
+        rows, values = torch.zeros((n, 1, 64), device=dev()), torch.ones((n, 1, 64), device=dev())
+        rows[:, 0, 0] = -gap
+        rows[at] = 0.0
+        if b < 5:
+            values[:, 0, ::2] += torch.rand((n, 32), device=dev(), generator=torch.Generator(device=dev()).manual_seed(b))
+            values[at] = 0.0
+        page = s.table[b].long()[j // 16]
+        for c, x in ((s.k, rows), (s.v, values)):
+            if c.element_size() == 1:
+                c.view(torch.uint8)[page, :, j % 16] = x.to(c.dtype).view(torch.uint8)
+            else:
+                c[page, :, j % 16] = x.to(c.dtype)
+    out = kv.paged_attention(*s.args(), scale=1.0, k_scale=s.k_scale, v_scale=s.v_scale)
+    want = ref.attention(*s.args(), scale=1.0, k_scale=s.k_scale, v_scale=s.v_scale)[0]
+    unit, small = (2.0 ** -7, 2.0 ** -133) if q == BF16 else (2.0 ** -10, 2.0 ** -24)
+    off = (ref.host(out) - want).abs() - (unit / 2 + 2.0 ** -15) * want - small / 2
+    assert float(off.max()) <= 0, [float(x) for x in off.amax((1, 2))]
