@@ -1,0 +1,29 @@
+"""A decode layer goes on after a call that it refused as if that call had not been made: the steps behind it
+are checked against the definition on what the cache should hold."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_decode_layer import _layer
+
+pytestmark = pytest.mark.gpu
+
+
+def _steps(layer, normal, cfg, n):
+    hidden = normal(3, cfg.H)
+    for _ in range(n):
+        hidden = layer.step(hidden)
+        hidden = (hidden.float() / hidden.float().std(-1, keepdim=True)).to(torch.bfloat16)
+    assert sorted(layer.free + sum(layer.owned, [])) == list(range(24))
+
+
+@pytest.mark.parametrize("budget", [None, 40])
+def test_steps_after_the_pages_ran_out(hip_lib, budget):
+    layer, normal, cfg = _layer(budget, False)
+    layer.prefill(normal(40, 2, 64), normal(40, 2, 64), [17, 3, 20])
+    with pytest.raises(RuntimeError, match="no page left"):
+        layer.prefill(normal(360, 2, 64), normal(360, 2, 64), [120, 120, 120])
+    layer.prefill(normal(25, 2, 64), normal(25, 2, 64), [8, 0, 17])
+    _steps(layer, normal, cfg, 30)
+    assert layer.steps == 30 and (budget is not None or max(layer.lens) == 67)

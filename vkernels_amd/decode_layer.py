@@ -58,21 +58,30 @@ class DecodeLayer:
         self.sums = None if budget is None else torch.zeros((sequences, kv_heads, width * page_size), device=dev)
 
     def _grow(self, by):
-        """Room for `by` more positions in every sequence (host lists, one small copy to the device)."""
+        """Room for `by` more positions in every sequence (host lists, one small copy to the device).  Where
+        there is none, nothing has been taken when the call is refused."""
+        lens = [n + by[b] for b, n in enumerate(self.lens)]
+        need = [-(-n // self.page_size) for n in lens]
+        left = len(self.free)
+        for b, owned in enumerate(self.owned):
+            left -= max(0, need[b] - len(owned))
+            if left < 0 or need[b] > self.table.shape[1]:
+                raise RuntimeError("the cache has no page left for sequence %d" % b)
         rows, columns, pages = [], [], []
-        for b, n in enumerate(self.lens):
-            while len(self.owned[b]) * self.page_size < n + by[b]:
-                if not self.free or len(self.owned[b]) == self.table.shape[1]:
-                    raise RuntimeError("the cache has no page left for sequence %d" % b)
+        for b, owned in enumerate(self.owned):
+            while len(owned) < need[b]:
                 rows.append(b)
-                columns.append(len(self.owned[b]))
+                columns.append(len(owned))
                 pages.append(self.free.pop())
-                self.owned[b].append(pages[-1])
-            self.lens[b] = n + by[b]
+                owned.append(pages[-1])
         if pages:
             at = torch.tensor([rows, columns, pages], device=self.table.device)
             self.table[at[0], at[1]] = at[2].to(torch.int32)
-        self.lens_dev.copy_(torch.tensor(self.lens, dtype=torch.int32))
+        self._set_lens(lens)
+
+    def _set_lens(self, lens):
+        self.lens[:] = lens
+        self.lens_dev.copy_(torch.tensor(lens, dtype=torch.int32))
 
     def prefill(self, k, v, lengths):
         """Keys and values [tokens, Hkv, D] of the sequences' prompts, one behind the other."""
