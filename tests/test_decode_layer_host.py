@@ -49,3 +49,20 @@ def test_growth_takes_the_pages_that_are_needed():
         _consistent(layer, 10)
         assert [len(x) for x in layer.owned] == [-(-n // 4) for n in layer.lens]
     assert layer.lens == [24, 4, 8] and len(layer.free) == 1
+
+
+def test_lengths_of_a_refused_call_are_taken_back():
+    """Rows or queries that the cache's operators refuse (here: all of them, without a GPU)."""
+    layer = _layer()
+    layer._grow([3, 0, 1])
+    rows = torch.zeros((5, 1, 16))
+    with pytest.raises(ValueError):
+        layer.prefill(rows, rows, [2, 3, 0])
+    assert layer.lens == [3, 0, 1]
+    with pytest.raises(ValueError):
+        layer.attend(torch.zeros((3, 2, 16)), rows[:3], rows[:3])
+    assert layer.lens == [3, 0, 1]
+    _consistent(layer, 10)
+    layer._grow([1, 3, 0])
+    assert layer.lens == [4, 3, 1]
+    _consistent(layer, 10)

@@ -27,3 +27,16 @@ def test_steps_after_the_pages_ran_out(hip_lib, budget):
     layer.prefill(normal(25, 2, 64), normal(25, 2, 64), [8, 0, 17])
     _steps(layer, normal, cfg, 30)
     assert layer.steps == 30 and (budget is not None or max(layer.lens) == 67)
+
+
+@pytest.mark.parametrize("budget", [None, 40])
+def test_steps_after_refused_rows_and_queries(hip_lib, budget):
+    layer, normal, cfg = _layer(budget, False)
+    layer.prefill(normal(40, 2, 64), normal(40, 2, 64), [17, 3, 20])
+    with pytest.raises(ValueError):
+        layer.prefill(normal(30, 2, 64).half(), normal(30, 2, 64).half(), [10, 10, 10])
+    with pytest.raises(ValueError):
+        layer.attend(normal(3, 5, 64), normal(3, 2, 64), normal(3, 2, 64))
+    assert layer.lens == [17, 3, 20] == layer.lens_dev.tolist()
+    _steps(layer, normal, cfg, 30)
+    assert layer.steps == 30

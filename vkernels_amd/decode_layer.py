@@ -9,6 +9,8 @@ so that no step asks the device for them) and what every position has been given
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from .kv_cache import kv_cache_append, kv_cache_evict, paged_attention
@@ -79,22 +81,34 @@ class DecodeLayer:
             self.table[at[0], at[1]] = at[2].to(torch.int32)
         self._set_lens(lens)
 
+    @contextlib.contextmanager
+    def _grown(self, by):
+        """The sequences longer by `by` for calls that fill the new positions; where one of them is refused the
+        lengths are what they were (the pages taken stay with their sequences)."""
+        before = list(self.lens)
+        self._grow(by)
+        try:
+            yield
+        except Exception:
+            self._set_lens(before)
+            raise
+
     def _set_lens(self, lens):
         self.lens[:] = lens
         self.lens_dev.copy_(torch.tensor(lens, dtype=torch.int32))
 
     def prefill(self, k, v, lengths):
         """Keys and values [tokens, Hkv, D] of the sequences' prompts, one behind the other."""
-        self._grow(lengths)
         starts = torch.tensor([0, *lengths]).cumsum(0).to(torch.int32).to(k.device)
-        kv_cache_append(k, v, self.k_cache, self.v_cache, self.table, self.lens_dev, query_start=starts, **self.scales)
+        with self._grown(lengths):
+            kv_cache_append(k, v, self.k_cache, self.v_cache, self.table, self.lens_dev, query_start=starts, **self.scales)
 
     def attend(self, q, k, v):
         """Attention of one new token of every sequence: q [B, Hq, D], its k and v [B, Hkv, D]."""
-        self._grow([1] * len(self.lens))
-        kv_cache_append(k, v, self.k_cache, self.v_cache, self.table, self.lens_dev, **self.scales)
-        return paged_attention(q, self.k_cache, self.v_cache, self.table, self.lens_dev, max_len=max(self.lens),
-                               sinks=self.sinks, weight_sums=self.sums, **self.scales)
+        with self._grown([1] * len(self.lens)):
+            kv_cache_append(k, v, self.k_cache, self.v_cache, self.table, self.lens_dev, **self.scales)
+            return paged_attention(q, self.k_cache, self.v_cache, self.table, self.lens_dev, max_len=max(self.lens),
+                                   sinks=self.sinks, weight_sums=self.sums, **self.scales)
 
     def evict(self):
         """Cuts the sequences back to the budget when one has outgrown it; the old positions that were
