@@ -59,3 +59,36 @@ def test_many_small_weights_beside_a_large_one(hip_lib, cache, q, n, where):
     unit, small = (2.0 ** -7, 2.0 ** -133) if q == BF16 else (2.0 ** -10, 2.0 ** -24)
     off = (ref.host(out) - want).abs() - (unit / 2 + 2.0 ** -15) * want - small / 2
     assert float(off.max()) <= 0, [float(x) for x in off.amax((1, 2))]
+
+
+def test_sizes_beyond_32_bits_are_not_cut_to_them(hip_lib):
+    """max_len, budget and what is always kept are refused, windows of any size are none."""
+    s = Setup([200, 150], 2, 4, 64, 16, seed=23)
+    sums = torch.rand((2, 2, 208), device=dev())
+    before = [t.clone() for t in (s.k, s.v, sums)]
+    for n in (2 ** 31, 2 ** 32, 2 ** 32 + 100, -2 ** 32 + 100, 2 ** 63 - 1, 2 ** 64 + 100):
+        for call in (lambda: kv.paged_attention(*s.args(), max_len=n),
+                     lambda: kv.paged_attention(*s.args(), max_len=n, weight_sums=sums),
+                     lambda: kv.kv_cache_evict(*s.args()[1:], sums, 100, max_len=n),
+                     lambda: kv.kv_cache_evict(*s.args()[1:], sums, n),
+                     lambda: kv.kv_cache_evict(*s.args()[1:], sums, 100, keep_first=n),
+                     lambda: kv.kv_cache_evict(*s.args()[1:], sums, 100, keep_last=n)):
+            with pytest.raises(ValueError):
+                call()
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(before, (s.k, s.v, sums)))
+    want = kv.paged_attention(*s.args())
+    for window in (2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1, 2 ** 64 + 5, -2 ** 32 + 5, -1):
+        assert torch.equal(kv.paged_attention(*s.args(), window=window), want), window
+
+
+def test_a_table_of_more_positions_than_32_bits_count(hip_lib):
+    """Its default bound is refused (it would be cut to 0 positions), a bound that is given is taken."""
+    s = Setup([200, 150], 1, 4, 16, 128, seed=24)
+    wide = s.table[:, :1].expand(-1, 1).repeat(1, 1 << 24)
+    wide[:, :s.table.shape[1]] = s.table
+    want = kv.paged_attention(*s.args())
+    with pytest.raises(ValueError, match="max_len"):
+        kv.paged_attention(s.q, s.k, s.v, wide, s.lens)
+    assert torch.equal(kv.paged_attention(s.q, s.k, s.v, wide, s.lens, max_len=256), want)
+    with pytest.raises(ValueError, match="max_len"):
+        kv.kv_cache_evict(s.k, s.v, wide, s.lens, torch.rand((2, 1, 256), device=dev()), 100)

@@ -80,7 +80,8 @@ def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device, t
             v_cache.dtype is k_cache.dtype and block_table.dtype is _INT32 and seq_lens.dtype is _INT32 and
             table_strides[1] == 1 and seq_lens.shape == table[:1] and seq_lens.is_contiguous() and
             v_cache.get_device() == device and block_table.get_device() == device and
-            seq_lens.get_device() == device and device >= 0 and _current_device() == device)
+            seq_lens.get_device() == device and device >= 0 and _current_device() == device and
+            not (shape[0] | shape[1] | shape[2] | table[0] | table[1] | table_strides[0]) >> 31)
 
 
 def _explain_cache(k_cache, v_cache, block_table, seq_lens):
@@ -95,6 +96,16 @@ def _explain_cache(k_cache, v_cache, block_table, seq_lens):
     devices = {t.get_device() for t in (k_cache, v_cache, block_table, seq_lens)}
     _need(len(devices) == 1 and devices != {-1}, "the cache, block_table and seq_lens must be on one device")
     _need(devices == {_current_device()}, "the tensors' device must be the current device")
+    _need(not any(n >> 31 for n in (*k_cache.shape, *block_table.shape, block_table.stride(0))),
+          "the sizes of the cache and of block_table must be below 2^31")
+
+
+def _int32(**sizes):
+    """The library takes these in 32 bits, and ctypes would cut what does not fit."""
+    for name, n in sizes.items():
+        if not -0x80000000 <= n <= 0x7FFFFFFF:
+            raise ValueError(f"{name} must be within 32 bits, not {n}" +
+                             (" (its default is what the table holds)" if name == "max_len" else ""))
 
 
 # The current device, and a device's current stream as the address that the library takes.
@@ -148,7 +159,7 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     ``v_scale`` [Hkv]), the largest finite code beyond +-448."""
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     tokens = k.shape[0]
-    _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype,
+    _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype and tokens < 1 << 31,
           "k and v must be [tokens, Hkv, D] alike")
     _need(k.get_device() == device and v.get_device() == device, "k and v must be on the cache's device")
     kind = _KINDS.get((k_cache.dtype, k.dtype))
@@ -187,12 +198,15 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     Hq = q.shape[1] if q.dim() == 3 else 0
     G = Hq // Hkv
-    _need(q.shape == (B, G * Hkv, D) and G > 0 and q.get_device() == device,
+    _need(q.shape == (B, G * Hkv, D) and 0 < G < 1 << 31 and q.get_device() == device,
           "q must be [B, Hq, D] on the cache's device with Hq a multiple of the cache's heads")
     kind = _KINDS.get((k_cache.dtype, q.dtype))
     _need(kind is not None, "the cache's type does not take queries of this type")
     if max_len is None:
         max_len = W * ps
+    _int32(max_len=max_len)
+    if not 0 < window < max_len:      # (any other sees everything, however large it is)
+        window = 0
     q = _rows(q)
     if out is None:
         out = q.new_empty((B, Hq, D))
@@ -236,6 +250,7 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     if max_len is None:
         max_len = W * ps
+    _int32(max_len=max_len, budget=budget, keep_first=keep_first, keep_last=keep_last)
     sums_out = weight_sums if sums_out is None else sums_out
     for name, t in (("weight_sums", weight_sums), ("sums_out", sums_out)):
         _need(_sums_ok(t, B, Hkv, max_len, device),
