@@ -92,3 +92,27 @@ def test_a_table_of_more_positions_than_32_bits_count(hip_lib):
     assert torch.equal(kv.paged_attention(s.q, s.k, s.v, wide, s.lens, max_len=256), want)
     with pytest.raises(ValueError, match="max_len"):
         kv.kv_cache_evict(s.k, s.v, wide, s.lens, torch.rand((2, 1, 256), device=dev()), 100)
+
+
+@pytest.mark.parametrize("pitch", [(65, 65), (64, 67), (129, 64)])
+def test_rows_of_odd_strides_in_dimensions_of_size_one(hip_lib, pitch):
+    """One sequence and one head out of a buffer of an odd pitch: contiguous, and its strides are no multiple
+    of 16 bytes all the same."""
+    s = Setup([90], 1, 1, 64, 16, seed=25)
+    want = kv.paged_attention(*s.args())
+    s.q = torch.empty(200, dtype=BF16, device=dev()).as_strided((1, 1, 64), (*pitch, 1)).copy_(s.q)
+    assert s.q.is_contiguous() and s.q.data_ptr() % 16 == 0 and s.q.stride() == (*pitch, 1)
+    assert torch.equal(kv.paged_attention(*s.args()), want)
+    after = ref.append(s.k, s.v, s.q, -s.q, s.table, s.lens, None, None, None)
+    kv.kv_cache_append(s.q, (-s.q).as_strided((1, 1, 64), (*pitch, 1)), s.k, s.v, s.table, s.lens)
+    assert all(torch.equal(a.cpu().view(torch.int16), b.view(torch.int16)) for a, b in zip((s.k, s.v), after))
+
+
+def test_rows_of_one_head_out_of_an_odd_pitch(hip_lib):
+    """Several sequences of one head whose strides over the heads are odd, and one sequence of several heads
+    whose stride over the sequences is."""
+    for B, Hq, strides in ((3, 1, (128, 65)), (1, 4, (259, 64))):
+        s = Setup([90] * B, 1, Hq, 64, 16, seed=26)
+        want = kv.paged_attention(*s.args())
+        s.q = torch.empty(1000, dtype=BF16, device=dev()).as_strided((B, Hq, 64), (*strides, 1)).copy_(s.q)
+        assert torch.equal(kv.paged_attention(*s.args()), want)

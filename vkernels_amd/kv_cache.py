@@ -143,9 +143,8 @@ def _rows(t):
     """`t` [n, heads, D], or a copy of it where its rows do not start on 16 bytes."""
     s = t.stride()
     if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
+        # (not contiguous(): that is the tensor itself where an odd stride belongs to a dimension of size 1)
+        t = t.new_empty(t.shape).copy_(t)
     return t
 
 
