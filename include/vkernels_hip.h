@@ -729,13 +729,17 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
 /* Eviction: a sequence of more than `budget` positions (its length cut to max_len) keeps
  * its first keep_first and last keep_last positions and of the others the
  * budget - keep_first - keep_last with the largest weight_sums, in every key/value head by
- * itself (NaN counts as largest, ties go to the lowest position).  Their rows move, in
- * order, to positions 0 .. budget - 1 of the same pages, in place; rows beyond stay as
- * they are.  sums_out [B, Hkv, positions] gets the kept sums, and 0 from budget up to the
+ * itself (NaN counts as largest, ties go to the lowest position; positions without a page
+ * are never among them).  Their rows move, in order, to positions 0 .. budget - 1 of the
+ * same pages, in place; rows beyond stay as they are.
+ * sums_out [B, Hkv, positions] gets the kept sums, and 0 from budget up to the
  * old length; it is weight_sums itself (with its strides) or an array that does not
  * overlap it.  new_lens [B] = min(length, budget); kept [B, Hkv, budget] int32 the old
  * positions in order, -1 beyond the new length.  A shorter sequence keeps all it has
- * (its sums are copied).  The pages of a sequence that is cut have to be its own.
+ * (its sums are copied).  So does a longer one that has a position without a page among
+ * its first `budget` ones, which the kept rows go to, or its last keep_last: it is not
+ * cut, its new length is its length (cut to max_len), kept the positions 0 .. budget - 1.
+ * The pages of a sequence that is cut have to be its own.
  * elem_bytes: 1 or 2, a value of the cache.  The workspace of
  * vk_hip_kv_cache_evict_workspace_bytes (16-byte aligned) is scratch of this call alone. */
 size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget);

@@ -179,7 +179,10 @@ __device__ __forceinline__ constexpr int digit_values(int pass) { return pass ==
 // walks.
 struct SelectRow {
   int len, lo, hi;      // positions; those in [lo, hi) have to earn their place
-  uint32_t places;      // how many of them do (fewer than there are)
+  uint32_t places;      // how many of them do (fewer than there are, those without a page not counted)
+  const int32_t* pages;
+  int num_pages;
+  FastDiv by_page;
   const float* sums;
   int32_t* kept;
   int from, to;         // the wavefront's stretch
@@ -207,32 +210,30 @@ struct SelectRow {
   __device__ __forceinline__ void preload(float (&x)[kSelectLoads]) const {
     if (resident) load(x, from);
   }
-  __device__ __forceinline__ bool earns(int j, bool real) const { return real && j >= lo && j < hi; }
+  __device__ __forceinline__ bool has_page(int j) const {
+    return (uint32_t)pages[divided(j, by_page)] < (uint32_t)num_pages;
+  }
+  // (HOLES: there are positions without a page, which are never kept.  Rows that have none, all but a few, take
+  // code of their own, without the look-ups in each pass.)
+  template <bool HOLES>
+  __device__ __forceinline__ bool earns(int j, bool real) const {
+    return real && j >= lo && j < hi && (!HOLES || has_page(j));
+  }
   __device__ __forceinline__ bool given(int j, bool real) const { return real && (j < lo || j >= hi); }
 };
 
-// What a row that is cut and one that is not have in common: true for the first.  `part` of
-// `parts` workgroups of the row, a stretch for each of their wavefronts.
+// Row and stretch of `part` of `parts` workgroups of a row, a stretch for each of their wavefronts; whether
+// it is longer than the budget.
 template <int THREADS>
-__device__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, bool first_pass, SelectRow* r) {
+__device__ __forceinline__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, SelectRow* r) {
   const int t = threadIdx.x, wave = t >> 6, b = row / a.Hkv, h = row % a.Hkv;
   r->len = min(max(a.lens[b], 0), a.max_len);
   r->sums = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)h * a.sums_stride_h;
   r->kept = a.kept + (int64_t)row * a.budget;
+  r->pages = a.table + (int64_t)b * a.table_stride;
+  r->num_pages = a.num_pages;
+  r->by_page = a.by_page;
   r->lane = t & 63;
-  if (first_pass && part == 0) {
-    // What orders the workgroups of the compaction behind this, for the keys and the values: a
-    // count of the batches taken, and a word for each batch that has been read.
-    for (int i = t; i < 2 * (1 + a.batches); i += THREADS) a.order[(int64_t)row * 2 * (1 + a.batches) + i] = 0;
-    if (h == 0 && t == 0) a.new_lens[b] = min(r->len, a.budget);
-    if (r->len <= a.budget) {
-      float* const out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
-      for (int j = t; j < a.budget; j += THREADS) r->kept[j] = j < r->len ? j : -1;
-      if (out != r->sums)
-        for (int j = t; j < r->len; j += THREADS) out[j] = r->sums[j];
-    }
-  }
-  if (r->len <= a.budget) return false;
   r->lo = a.keep_first;
   r->hi = r->len - a.keep_last;
   r->places = (uint32_t)(a.budget - a.keep_first - a.keep_last);
@@ -241,17 +242,63 @@ __device__ bool select_row(const KvEvictArgs& a, int row, int part, int parts, b
   r->from = min(r->len, (part * (THREADS / 64) + wave) * stretch);
   r->to = min(r->len, r->from + stretch);
   r->resident = stretch <= 64 * kSelectLoads;
-  return true;
+  return r->len > a.budget;
+}
+
+// Positions [from, to) of the row without a page, as a wavefront finds them: are there any, and is one of them
+// the new place of a kept position or kept itself (such a row is not cut).  Each wavefront looks through the
+// pages of its stretch: 1 us of the 15 that 512 rows of 2304 sums take, 0.7 of 27 for 6976 rows of up to 64.
+constexpr uint32_t kHole = 1, kHoleInTheWay = 2;
+__device__ __forceinline__ uint32_t find_holes(const KvEvictArgs& a, const SelectRow& r, int from, int to) {
+  const int last = to > from ? divided(to - 1, r.by_page) : -1;
+  uint32_t mine = 0;
+#pragma unroll 4
+  for (int i = divided(from, r.by_page) + r.lane; i <= last; i += 64) {
+    if ((uint32_t)r.pages[i] >= (uint32_t)r.num_pages) {
+      const int first = i * a.page_size, behind = (int)min((int64_t)first + a.page_size, (int64_t)r.len);
+      mine |= first < a.budget || behind > r.hi ? kHole | kHoleInTheWay : kHole;
+    }
+  }
+  return (__any(mine & kHole) ? kHole : 0u) | (__any(mine & kHoleInTheWay) ? kHoleInTheWay : 0u);
+}
+// The wavefronts' findings, left in LDS in front of a barrier.
+template <int WAVES>
+__device__ __forceinline__ uint32_t all_holes(const uint32_t* holes_lds) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) all |= holes_lds[w];
+  return __builtin_amdgcn_readfirstlane(all);
+}
+
+// What the first launch leaves for the compaction besides the kept positions: the new length of a row that
+// is cut, and the order of its workgroups (for the keys and the values a count of the batches taken, and a
+// word for each batch that has been read).
+template <int THREADS>
+__device__ __forceinline__ void open_row(const KvEvictArgs& a, int row, const SelectRow& r) {
+  const int t = threadIdx.x, b = row / a.Hkv, h = row % a.Hkv;
+  for (int i = t; i < 2 * (1 + a.batches); i += THREADS) a.order[(int64_t)row * 2 * (1 + a.batches) + i] = 0;
+  if (h == 0 && t == 0) a.new_lens[b] = min(r.len, a.budget);
+}
+// All there is of a row that is not cut.
+template <int THREADS>
+__device__ void leave_row(const KvEvictArgs& a, int row, const SelectRow& r) {
+  const int t = threadIdx.x, b = row / a.Hkv, h = row % a.Hkv;
+  if (h == 0 && t == 0) a.new_lens[b] = r.len;
+  float* const out = a.sums_out + (int64_t)b * a.out_stride_b + (int64_t)h * a.out_stride_h;
+  for (int j = t; j < a.budget; j += THREADS) r.kept[j] = j < r.len ? j : -1;
+  if (out != r.sums)
+    for (int j = t; j < r.len; j += THREADS) out[j] = r.sums[j];
 }
 
 // The last pass: the wavefront's kept positions, behind the `certain` and `ties` ones before its stretch;
 // of the keys equal to `least` the first `need` of the row are kept.
+template <bool HOLES>
 __device__ __forceinline__ void write_kept(const SelectRow& r, float (&x)[kSelectLoads], uint32_t least, uint32_t need,
                                            uint32_t certain, uint32_t ties) {
   const uint64_t below = (1ull << r.lane) - 1;
   r.walk(x, true, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
-    const bool middle = r.earns(j, real) && r.places > 0;
+    const bool middle = r.earns<HOLES>(j, real) && r.places > 0;
     const bool sure = r.given(j, real) || (middle && key > least), tied = middle && key == least;
     const uint64_t all_sure = __ballot(sure), all_tied = __ballot(tied);
     const uint32_t before = ties + (uint32_t)__popcll(all_tied & below);
@@ -291,33 +338,34 @@ __device__ __forceinline__ void counts_before(uint32_t& sure, uint32_t& equal, u
 // Bound by its barriers and dependent loads: 512 rows of 2304 sums (9 MB in and out) in 15 us (21
 // with 16 sums a lane in registers, which leave a CU room for one workgroup); 32 rows of 65536 in 58 us,
 // a CU each, where the split form takes 32.
+// (Pointers to arrays of their own: as members of one struct in LDS these cost 9 us for 6976 rows of up to 64
+// positions.)
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a) {
-  constexpr int kWaves = THREADS / 64, kBinCopies = bin_copies(THREADS);
-  __shared__ uint32_t bins[kBinCopies][kBins];
-  __shared__ uint32_t listed[kWaves][kListed];
-  __shared__ uint32_t scan_lds[kWaves], counts_lds[2][kWaves];
-  __shared__ uint32_t found[2], too_many;
+struct SelectLds {
+  uint32_t (*bins)[kBins];
+  uint32_t (*listed)[kListed];
+  uint32_t *scan, (*counts)[THREADS / 64], *found, *too_many;
+};
+
+template <int THREADS, bool HOLES>
+__device__ void select_kept(const SelectRow& r, float (&x)[kSelectLoads], const SelectLds<THREADS> lds) {
+  constexpr int kBinCopies = bin_copies(THREADS);
   const int t = threadIdx.x, wave = t >> 6;
-  SelectRow r;
-  if (!select_row<THREADS>(a, blockIdx.x, 0, 1, true, &r)) return;
-  float x[kSelectLoads];
   uint32_t least = 0, need = r.places;   // the least key that is kept; of its equals, the first `need` are
   auto clear_bins = [&] {
-    for (int i = t; i < kBinCopies * kBins; i += THREADS) (&bins[0][0])[i] = 0;
+    for (int i = t; i < kBinCopies * kBins; i += THREADS) (&lds.bins[0][0])[i] = 0;
     __syncthreads();
   };
-  auto count = [&](uint32_t digit) { atomicAdd(&bins[wave % kBinCopies][digit], 1u); };
-  clear_bins();
+  auto count = [&](uint32_t digit) { atomicAdd(&lds.bins[wave % kBinCopies][digit], 1u); };
   r.walk(x, false, [&](int j, bool real, float v) {
-    if (r.earns(j, real)) count(order_key(v) >> 21);
+    if (r.template earns<HOLES>(j, real)) count(order_key(v) >> 21);
   });
-  if (t == 0) too_many = 0;
+  if (t == 0) *lds.too_many = 0;
   __syncthreads();
   if (r.places > 0) {
-    find_digit_lds<THREADS>(bins, 2048, r.places, scan_lds, found);
-    least = found[0] << 21;
-    need = found[1];
+    find_digit_lds<THREADS>(lds.bins, 2048, r.places, lds.scan, lds.found);
+    least = lds.found[0] << 21;
+    need = lds.found[1];
   }
 
   // what this wavefront's stretch keeps for certain, and its candidates
@@ -325,18 +373,18 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a)
   const uint64_t below = (1ull << r.lane) - 1;
   r.walk(x, true, [&](int j, bool real, float v) {
     const uint32_t key = order_key(v);
-    const bool middle = r.earns(j, real) && r.places > 0;
+    const bool middle = r.template earns<HOLES>(j, real) && r.places > 0;
     sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key >> 21 > least >> 21)));
     const bool candidate = middle && key >> 21 == least >> 21;
     const uint64_t all = __ballot(candidate);
     const uint32_t at = n_listed + (uint32_t)__popcll(all & below);
-    if (candidate && at < kListed) listed[wave][at] = key;
+    if (candidate && at < kListed) lds.listed[wave][at] = key;
     n_listed += (uint32_t)__popcll(all);
   });
   if (r.places > 0) {
-    if (r.lane == 0 && n_listed > kListed) too_many = 1;
+    if (r.lane == 0 && n_listed > kListed) *lds.too_many = 1;
     __syncthreads();
-    const bool again = too_many != 0;
+    const bool again = *lds.too_many != 0;
 #pragma unroll 1
     for (int pass = 1; pass < 3; ++pass) {
       const int shift = digit_shift(pass), n = digit_values(pass);
@@ -344,39 +392,68 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a)
       clear_bins();
       if (!again) {
         for (uint32_t i = r.lane; i < n_listed; i += 64) {
-          const uint32_t key = listed[wave][i];
+          const uint32_t key = lds.listed[wave][i];
           if (key >> same == least >> same) count((key >> shift) & (n - 1));
         }
       } else {
         r.walk(x, true, [&](int j, bool real, float v) {
           const uint32_t key = order_key(v);
-          if (r.earns(j, real) && key >> same == least >> same) count((key >> shift) & (n - 1));
+          if (r.template earns<HOLES>(j, real) && key >> same == least >> same) count((key >> shift) & (n - 1));
         });
       }
       __syncthreads();
-      find_digit_lds<THREADS>(bins, n, need, scan_lds, found);
-      least |= found[0] << shift;
-      need = found[1];
+      find_digit_lds<THREADS>(lds.bins, n, need, lds.scan, lds.found);
+      least |= lds.found[0] << shift;
+      need = lds.found[1];
       __syncthreads();
     }
     if (!again) {
       for (uint32_t i0 = 0; i0 < n_listed; i0 += 64) {
         const bool real = i0 + r.lane < n_listed;
-        const uint32_t key = real ? listed[wave][i0 + r.lane] : 0u;
+        const uint32_t key = real ? lds.listed[wave][i0 + r.lane] : 0u;
         sure += (uint32_t)__popcll(__ballot(real && key > least));
         equal += (uint32_t)__popcll(__ballot(real && key == least));
       }
     } else {
       r.walk(x, true, [&](int j, bool real, float v) {
-        const bool middle = r.earns(j, real);
+        const bool middle = r.template earns<HOLES>(j, real);
         const uint32_t key = order_key(v);
         sure += (uint32_t)__popcll(__ballot(middle && key > least && key >> 21 == least >> 21));
         equal += (uint32_t)__popcll(__ballot(middle && key == least));
       });
     }
   }
-  counts_before(sure, equal, counts_lds);
-  write_kept(r, x, least, need, sure, equal);
+  counts_before(sure, equal, lds.counts);
+  write_kept<HOLES>(r, x, least, need, sure, equal);
+}
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a) {
+  __shared__ uint32_t bins[bin_copies(THREADS)][kBins];
+  __shared__ uint32_t listed[THREADS / 64][kListed];
+  __shared__ uint32_t scan_lds[THREADS / 64], counts_lds[2][THREADS / 64], holes_lds[THREADS / 64];
+  __shared__ uint32_t found[2], too_many;
+  const SelectLds<THREADS> lds = {bins, listed, scan_lds, counts_lds, found, &too_many};
+  const int t = threadIdx.x, wave = t >> 6;
+  SelectRow r;
+  const bool longer = select_row<THREADS>(a, blockIdx.x, 0, 1, &r);
+  open_row<THREADS>(a, blockIdx.x, r);
+  if (!longer) {
+    leave_row<THREADS>(a, blockIdx.x, r);
+    return;
+  }
+  float x[kSelectLoads];
+  const uint32_t mine = find_holes(a, r, r.from, r.to);
+  if (r.lane == 0) holes_lds[wave] = mine;
+  for (int i = t; i < bin_copies(THREADS) * kBins; i += THREADS) (&bins[0][0])[i] = 0;
+  __syncthreads();
+  const uint32_t holes = all_holes<THREADS / 64>(holes_lds);
+  if (holes == 0)
+    select_kept<THREADS, false>(r, x, lds);
+  else if (holes & kHoleInTheWay)
+    leave_row<THREADS>(a, blockIdx.x, r);
+  else
+    select_kept<THREADS, true>(r, x, lds);
 }
 
 // Few long rows: `parts` workgroups for each, a launch for each digit.  A workgroup counts the
@@ -384,12 +461,15 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(const KvEvictArgs a)
 // up and goes on from the digit found.  What a part keeps for certain follows from the counts as
 // well, so that the last launch knows where each part's positions begin.
 constexpr int kMostParts = 16;
+// (even: pairs of counts are read)
+__host__ __device__ constexpr int kv_split_words(int parts) { return 3 * parts * kBins + 4 + 3 * parts + (parts & 1); }
 struct SplitRow {
   uint32_t* counts;   // [3][parts][kBins]
-  uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] kept before a part by those
+  uint32_t* state;    // least, need behind digit 0 and behind digit 1; [2][parts] kept before a part by those;
+                      // [parts] the parts' positions without a page
 };
 __device__ __forceinline__ SplitRow split_row(const KvEvictArgs& a, int row) {
-  const int words = 3 * a.parts * kBins + 4 + 2 * a.parts;   // (even: pairs of counts are read)
+  const int words = kv_split_words(a.parts);
   uint32_t* const base = a.split + (int64_t)row * words;
   return SplitRow{base, base + 3 * a.parts * kBins};
 }
@@ -454,14 +534,38 @@ __device__ PartsBefore split_digit(const KvEvictArgs& a, const SplitRow& s, int 
   return r;
 }
 
+// All parts' positions without a page, behind the first launch.
+__device__ __forceinline__ uint32_t split_holes(const KvEvictArgs& a, const SplitRow& s) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int p = 0; p < kMostParts; ++p) all |= p < a.parts ? s.state[4 + 2 * a.parts + p] : 0u;
+  return __builtin_amdgcn_readfirstlane(all);
+}
+
+// The digits of the part's keys that agree with `least` so far.
+template <int PASS, bool HOLES>
+__device__ __forceinline__ void count_digits(const SelectRow& r, float (&x)[kSelectLoads], uint32_t least, uint32_t* bins) {
+  r.walk(x, true, [&](int j, bool real, float v) {
+    const uint32_t key = order_key(v);
+    constexpr uint32_t same = PASS == 1 ? 21 : 10;
+    if (r.template earns<HOLES>(j, real) && (PASS == 0 || key >> same == least >> same))
+      atomicAdd(bins + ((key >> digit_shift(PASS)) & (digit_values(PASS) - 1)), 1u);
+  });
+}
+
 template <int PASS>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const KvEvictArgs a) {
   constexpr int kBinCopies = bin_copies(kSelectThreads);
   __shared__ uint32_t bins[kBinCopies][kBins];
-  __shared__ uint32_t scan_lds[2][kSelectWaves], found[2];
+  __shared__ uint32_t scan_lds[2][kSelectWaves], found[2], holes_lds[kSelectWaves];
   const int t = threadIdx.x, wave = t >> 6, row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
-  if (!select_row<kSelectThreads>(a, row, part, a.parts, PASS == 0, &r) || r.places == 0) return;
+  const bool longer = select_row<kSelectThreads>(a, row, part, a.parts, &r);
+  if (PASS == 0 && part == 0) {
+    open_row<kSelectThreads>(a, row, r);
+    if (!longer) leave_row<kSelectThreads>(a, row, r);
+  }
+  if (!longer) return;
   const SplitRow s = split_row(a, row);
   uint32_t least = 0, need = r.places;
   if constexpr (PASS == 2) {
@@ -471,14 +575,29 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const K
   for (int i = t; i < kBinCopies * kBins; i += kSelectThreads) (&bins[0][0])[i] = 0;
   float x[kSelectLoads];
   r.preload(x);
-  if constexpr (PASS > 0) split_digit(a, s, PASS - 1, part, least, need, scan_lds, found);
-  __syncthreads();
-  r.walk(x, true, [&](int j, bool real, float v) {
-    const uint32_t key = order_key(v);
-    constexpr uint32_t same = PASS == 1 ? 21 : 10;
-    if (r.earns(j, real) && (PASS == 0 || key >> same == least >> same))
-      atomicAdd(&bins[wave % kBinCopies][(key >> digit_shift(PASS)) & (digit_values(PASS) - 1)], 1u);
-  });
+  uint32_t holes;      // (of this part; behind the first launch of the row)
+  if constexpr (PASS == 0) {
+    const uint32_t mine = find_holes(a, r, r.from, r.to);
+    if (r.lane == 0) holes_lds[wave] = mine;
+    __syncthreads();
+    holes = all_holes<kSelectWaves>(holes_lds);
+    if (t == 0) s.state[4 + 2 * a.parts + part] = holes;
+    if (r.places == 0) return;
+  } else {
+    holes = split_holes(a, s);
+    if (holes & kHoleInTheWay) {
+      if (PASS == 1 && part == 0) leave_row<kSelectThreads>(a, row, r);
+      return;
+    }
+    if (r.places == 0) return;
+    split_digit(a, s, PASS - 1, part, least, need, scan_lds, found);
+    __syncthreads();
+  }
+  uint32_t* const mine = bins[wave % kBinCopies];
+  if (holes == 0)
+    count_digits<PASS, false>(r, x, least, mine);
+  else
+    count_digits<PASS, true>(r, x, least, mine);
   __syncthreads();
   uint32_t* const to = s.counts + ((int64_t)PASS * a.parts + part) * kBins;
   for (int i = t; i < digit_values(PASS); i += kSelectThreads) {
@@ -489,16 +608,32 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_digit_kernel(const K
   }
 }
 
+template <bool HOLES>
+__device__ __forceinline__ void keep_part(const SelectRow& r, float (&x)[kSelectLoads], uint32_t least, uint32_t need,
+                                          uint32_t before_sure, uint32_t before_equal, uint32_t (*counts_lds)[kSelectWaves]) {
+  uint32_t sure = 0, equal = 0;
+  r.walk(x, true, [&](int j, bool real, float v) {
+    const uint32_t key = order_key(v);
+    const bool middle = r.template earns<HOLES>(j, real) && r.places > 0;
+    sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key > least)));
+    equal += (uint32_t)__popcll(__ballot(middle && key == least));
+  });
+  counts_before(sure, equal, counts_lds);
+  write_kept<HOLES>(r, x, least, need, before_sure + sure, before_equal + equal);
+}
+
 __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const KvEvictArgs a) {
   __shared__ uint32_t scan_lds[2][kSelectWaves], counts_lds[2][kSelectWaves], found[2];
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   SelectRow r;
-  if (!select_row<kSelectThreads>(a, row, part, a.parts, false, &r)) return;
+  if (!select_row<kSelectThreads>(a, row, part, a.parts, &r)) return;
   const SplitRow s = split_row(a, row);
   uint32_t least = 0, need = r.places;
   uint32_t before_sure = 0, before_equal = 0;      // kept in the parts before this one
   float x[kSelectLoads];
   r.preload(x);
+  const uint32_t holes = split_holes(a, s);
+  if (holes & kHoleInTheWay) return;
   if (r.places > 0) {
     least = s.state[2];
     need = s.state[3];
@@ -511,16 +646,10 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_keep_kernel(const Kv
   const int stretch = (r.len + 64 * a.parts * kSelectWaves - 1) / (64 * a.parts * kSelectWaves) * 64;
   const int begin = min(r.len, part * kSelectWaves * stretch);
   before_sure += (uint32_t)(min(begin, r.lo) + max(0, begin - r.hi));
-
-  uint32_t sure = 0, equal = 0;
-  r.walk(x, true, [&](int j, bool real, float v) {
-    const uint32_t key = order_key(v);
-    const bool middle = r.earns(j, real) && r.places > 0;
-    sure += (uint32_t)__popcll(__ballot(r.given(j, real) || (middle && key > least)));
-    equal += (uint32_t)__popcll(__ballot(middle && key == least));
-  });
-  counts_before(sure, equal, counts_lds);
-  write_kept(r, x, least, need, before_sure + sure, before_equal + equal);
+  if (holes == 0)
+    keep_part<false>(r, x, least, need, before_sure, before_equal, counts_lds);
+  else
+    keep_part<true>(r, x, least, need, before_sure, before_equal, counts_lds);
 }
 
 // The compaction.  A batch is 64 KB of rows that become neighbours: the keys or the values
@@ -540,7 +669,8 @@ __global__ __launch_bounds__(THREADS) void kv_move_kernel(const KvEvictArgs a) {
   const int list = blockIdx.x % (2 * a.B * a.Hkv);
   const int which = list & 1, bh = list >> 1, b = bh / a.Hkv, h = bh % a.Hkv;
   const int len = min(max(a.lens[b], 0), a.max_len);
-  if (len <= a.budget) return;
+  const int new_len = a.new_lens[b];
+  if (len <= a.budget || new_len != a.budget) return;     // (not cut)
   uint32_t* const taken = a.order + (int64_t)list * (1 + a.batches);
   uint32_t* const read = taken + 1;
   if (t == 0) ticket_lds = __hip_atomic_fetch_add(taken, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -673,7 +803,7 @@ static int select_threads(int rows, int max_len) {
 size_t kv_evict_workspace_bytes(int rows, int row_bytes, int max_len, int budget) {
   const size_t order = 2 * (size_t)rows * (1 + kv_evict_batches(budget, row_bytes));
   const int parts = kv_evict_parts(rows, max_len);
-  return 4 * (order + (parts > 1 ? (size_t)rows * (3 * parts * kBins + 4 + 2 * parts) : 0));
+  return 4 * (order + (parts > 1 ? (size_t)rows * kv_split_words(parts) : 0));
 }
 
 void launch_kv_evict(const KvEvictArgs& args, hipStream_t stream) {

@@ -245,7 +245,9 @@ def kv_cache_evict(k_cache, v_cache, block_table, seq_lens, weight_sums, budget,
     along, with zeros from the budget up to the old length: in place, or to ``sums_out``.
     Returns (new_lens [B] int32, kept [B, Hkv, budget] int32: the old positions, -1 beyond the new
     length).  The pages of a sequence that is cut must be its own; those behind its new length are
-    free afterwards.  Rows keep the position encoding they were stored with."""
+    free afterwards.  Rows keep the position encoding they were stored with.  Positions without a page
+    are not kept; a sequence that has one among its first ``budget`` positions or its last ``keep_last``
+    is left as it is, with its old length in new_lens and 0 .. budget - 1 in kept."""
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     if max_len is None:
         max_len = W * ps
