@@ -703,7 +703,8 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
 
 /* Attention of one new token of every sequence over its cache: q [B, Hq, D] (strides in
  * elements), out [B, Hq, D] contiguous, lse [B, Hq] fp32 or NULL.
- *   s_j = scale * k_scale[g] * q_h . k_j, then softcap * tanh(s_j / softcap) if softcap > 0,
+ *   s_j = scale * k_scale[g] * q_h . k_j, then softcap * tanh(s_j / softcap) if softcap > 0
+ *   (2^100 and beyond, infinity included: no cap),
  *   over the positions j in [max(0, L - window), L) (window <= 0: from 0), L = seq_lens[b]
  *   cut to max_len;  Z = sum_j e^{s_j} + e^{sinks[h]} (sinks [Hq] or NULL),
  *   out_h = v_scale[g] * sum_j e^{s_j} v_j / Z,  lse_h = log Z.

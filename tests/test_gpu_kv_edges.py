@@ -116,3 +116,24 @@ def test_rows_of_one_head_out_of_an_odd_pitch(hip_lib):
         want = kv.paged_attention(*s.args())
         s.q = torch.empty(1000, dtype=BF16, device=dev()).as_strided((B, Hq, 64), (*strides, 1)).copy_(s.q)
         assert torch.equal(kv.paged_attention(*s.args()), want)
+
+
+@pytest.mark.parametrize("cache,q", [(BF16, BF16), (FP8, F16)])
+def test_caps_of_any_size(hip_lib, cache, q):
+    """Infinity and caps that no score comes near change nothing; under the least caps all scores are alike."""
+    s = Setup([60, 1200], 2, 4, 64, 16, cache=cache, q=q, seed=27)
+    scales = dict(k_scale=s.k_scale, v_scale=s.v_scale)
+    want = kv.paged_attention(*s.args(), **scales)
+    for softcap in (float("inf"), 1e300, 3.4e38, 2.5e38, 1e38, 2.0 ** 100):
+        assert torch.equal(kv.paged_attention(*s.args(), softcap=softcap, **scales), want), softcap
+    # the two ways to a score differ by 2^-20 of it at most, scores here are below 32: 2^-15 of a weight, and
+    # the result's last place (8 or 11 bits) once for either
+    size = kv.paged_attention(s.q, s.k, (s.v.float().abs()).to(cache), s.table, s.lens, **scales).float()
+    unit = 2.0 ** -7 if q == BF16 else 2.0 ** -10
+    for softcap in (1e29, 1e20, 1e9):
+        got = kv.paged_attention(*s.args(), softcap=softcap, **scales)
+        assert float(((got.float() - want.float()).abs() - 2 * (unit + 2.0 ** -15) * size).max()) <= 0, softcap
+    zero = torch.zeros_like(s.q)
+    want = kv.paged_attention(zero, *s.args()[1:], **scales)
+    for softcap in (1e-44, 1e-38, 1e-30, 1e-20):
+        assert torch.equal(kv.paged_attention(*s.args(), softcap=softcap, **scales), want), softcap

@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -143,7 +144,9 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   a.sums_stride_b = sums_stride_b; a.sums_stride_h = sums_stride_h;
   a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
   a.B = B; a.Hkv = Hkv; a.G = G; a.D = D; a.max_len = max_len; a.window = window;
-  a.scale = scale; a.softcap = softcap;
+  // (Caps that no score comes near, infinity among them, are none, and below the other bound all scores are alike:
+  // the kernel's factors 1 / cap and cap then stay within 32-bit floats.)
+  a.scale = scale; a.softcap = softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f;
   const hipError_t before = hipPeekAtLastError();
   vk::launch_paged_attention(a, kind, static_cast<hipStream_t>(stream));
   return launched(who, before);
