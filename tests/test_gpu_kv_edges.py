@@ -137,3 +137,23 @@ def test_caps_of_any_size(hip_lib, cache, q):
     want = kv.paged_attention(zero, *s.args()[1:], **scales)
     for softcap in (1e-44, 1e-38, 1e-30, 1e-20):
         assert torch.equal(kv.paged_attention(*s.args(), softcap=softcap, **scales), want), softcap
+
+
+@pytest.mark.parametrize("which", ["q", "sinks", "k_cache"])
+def test_a_backward_pass_is_an_error(hip_lib, which):
+    """The results are those of inference, and what would be a gradient of nothing raises."""
+    s = Setup([60, 1200], 2, 4, 64, 16, seed=28)
+    want, want_lse = kv.paged_attention(*s.args(), sinks=s.sinks, return_lse=True)
+    assert not want.requires_grad and not want_lse.requires_grad
+    {"q": s.q, "sinks": s.sinks, "k_cache": s.k}[which].requires_grad_()
+    out, lse = kv.paged_attention(*s.args(), sinks=s.sinks, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    for result in (out, lse, kv.paged_attention(*s.args(), sinks=s.sinks)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            result.float().sum().backward()
+    mine = torch.empty_like(want)
+    assert kv.paged_attention(*s.args(), sinks=s.sinks, out=mine) is mine and torch.equal(mine, want)
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            out = kv.paged_attention(*s.args(), sinks=s.sinks)
+            assert not out.requires_grad and torch.equal(out, want)

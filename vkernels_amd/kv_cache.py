@@ -9,6 +9,9 @@ call is enqueued on the current stream of the tensors' device, with no host sync
 writes besides its arguments comes from torch's allocator, so calls on several streams do not share
 scratch and a call can be captured in a graph.
 
+These are operators of inference: no gradient passes through the cache, and a backward pass that comes to
+``paged_attention`` raises an error.
+
 The entry points are additive: the reference keeps its cache outside this path.  Everything runs in
 ``libvkernels_hip.so``; there is no fallback.
 """
@@ -148,6 +151,19 @@ def _rows(t):
     return t
 
 
+class _NoBackward(torch.autograd.Function):
+    """The results as they are; a backward pass that reaches them is an error instead of a gradient lost."""
+
+    @staticmethod
+    def forward(ctx, out, lse, *inputs):
+        return (out.view_as(out), None if lse is None else lse.view_as(lse))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("paged_attention has no backward pass: it is an operator of inference "
+                           "(call it under torch.no_grad(), or detach what requires a gradient)")
+
+
 def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_start=None, k_scale=None, v_scale=None):
     """New tokens' keys and values [tokens, Hkv, D] into the pages.
 
@@ -206,7 +222,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     _int32(max_len=max_len)
     if not 0 < window < max_len:      # (any other sees everything, however large it is)
         window = 0
-    q = _rows(q)
+    q, own_out = _rows(q), out is not None
     if out is None:
         out = q.new_empty((B, Hq, D))
     else:
@@ -232,6 +248,10 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         _stream(device))
     if status:
         _failed(status, "vk_hip_paged_attention")
+    if torch.is_grad_enabled() and not own_out:
+        inputs = [t for t in (q, k_cache, v_cache, sinks) if t is not None and t.requires_grad]
+        if inputs:
+            out, lse = _NoBackward.apply(out, lse, *inputs)
     return (out, lse) if return_lse else out
 
 
