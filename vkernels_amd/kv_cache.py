@@ -84,7 +84,7 @@ def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device, t
             table_strides[1] == 1 and seq_lens.shape == table[:1] and seq_lens.is_contiguous() and
             v_cache.get_device() == device and block_table.get_device() == device and
             seq_lens.get_device() == device and device >= 0 and _current_device() == device and
-            not (shape[0] | shape[1] | shape[2] | table[0] | table[1] | table_strides[0]) >> 31)
+            (shape[0] | shape[1] | shape[2] | table[0] | table[1] | table_strides[0]) <= 0x7FFFFFFF)
 
 
 def _explain_cache(k_cache, v_cache, block_table, seq_lens):
@@ -213,15 +213,17 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     Hq = q.shape[1] if q.dim() == 3 else 0
     G = Hq // Hkv
-    _need(q.shape == (B, G * Hkv, D) and 0 < G < 1 << 31 and q.get_device() == device,
-          "q must be [B, Hq, D] on the cache's device with Hq a multiple of the cache's heads")
+    if not (q.shape == (B, G * Hkv, D) and 0 < G <= 0x7FFFFFFF and q.get_device() == device):
+        raise ValueError("q must be [B, Hq, D] on the cache's device with Hq a multiple of the cache's heads")
     kind = _KINDS.get((k_cache.dtype, q.dtype))
-    _need(kind is not None, "the cache's type does not take queries of this type")
+    if kind is None:
+        raise ValueError("the cache's type does not take queries of this type")
     if max_len is None:
         max_len = W * ps
-    _int32(max_len=max_len)
     if not 0 < window < max_len:      # (any other sees everything, however large it is)
         window = 0
+    if not 0 <= max_len <= 0x7FFFFFFF:
+        _int32(max_len=max_len)
     q, own_out = _rows(q), out is not None
     if out is None:
         out = q.new_empty((B, Hq, D))
@@ -231,8 +233,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
-        _need(_sums_ok(weight_sums, B, Hkv, max_len, device),
-              "weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
+        if not _sums_ok(weight_sums, B, Hkv, max_len, device):
+            raise ValueError("weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
     size = _bytes("vk_hip_paged_attention_workspace_bytes", kind, B, Hkv, G, D, max_len, window, sums is not None)
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
@@ -248,10 +250,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         _stream(device))
     if status:
         _failed(status, "vk_hip_paged_attention")
-    if torch.is_grad_enabled() and not own_out:
-        inputs = [t for t in (q, k_cache, v_cache, sinks) if t is not None and t.requires_grad]
-        if inputs:
-            out, lse = _NoBackward.apply(out, lse, *inputs)
+    if ((q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
+         sinks is not None and sinks.requires_grad) and torch.is_grad_enabled() and not own_out):
+        out, lse = _NoBackward.apply(out, lse, q, k_cache, v_cache, sinks)
     return (out, lse) if return_lse else out
 
 
