@@ -107,3 +107,20 @@ def test_a_window_beyond_the_lengths_is_planned_like_none(lib, window, counted):
     size = kv._fn("vk_hip_paged_attention_workspace_bytes")
     for B, Hkv, G in ((64, 8, 4), (8, 8, 4), (1, 1, 40)):
         assert size(0, B, Hkv, G, 128, 8192, window, counted) == size(0, B, Hkv, G, 128, 8192, 0, counted) > 0
+
+
+@pytest.mark.parametrize("name,change", [
+    *((name, change) for name in ("vk_hip_kv_cache_append", "vk_hip_kv_cache_evict")
+      for change in (dict(page_stride=0), dict(head_stride=0), dict(slot_stride=0))),
+    ("vk_hip_paged_attention", dict(weight_sums=P, sums_stride_b=0, sums_stride_h=6400)),
+    ("vk_hip_paged_attention", dict(weight_sums=P, sums_stride_b=12800, sums_stride_h=0)),
+    ("vk_hip_kv_cache_evict", dict(out_stride_b=0, sums_out=3 * P)),
+    ("vk_hip_kv_cache_evict", dict(out_stride_h=0, sums_out=3 * P))])
+def test_what_is_written_to_must_not_be_broadcast(lib, name, change):
+    """Pages, heads, positions or sums that share their memory would be written by several workgroups at once."""
+    lib.vk_set_last_error(0, b"")
+    args = dict(CALLS[name], **change)
+    if name == "vk_hip_kv_cache_evict":
+        args["sums_out"] = 3 * P
+    assert kv._fn(name)(*args.values()) == ve.VK_ERROR_INVALID_ARGUMENT
+    assert "broadcast" in ve.last_error(lib)

@@ -43,6 +43,17 @@ const char* cache_refusal(const void* k_cache, const void* v_cache, const int32_
   return nullptr;
 }
 
+// What is written to holds every element once.
+const char* broadcast_refusal(int Hkv, int num_pages, int page_size, int64_t page_stride, int64_t head_stride,
+                              int64_t slot_stride) {
+  if ((page_stride == 0 && num_pages > 1) || (head_stride == 0 && Hkv > 1) || (slot_stride == 0 && page_size > 1))
+    return "a cache that is written to must not be broadcast";
+  return nullptr;
+}
+bool broadcast_sums(int B, int Hkv, int64_t stride_b, int64_t stride_h) {
+  return (stride_b == 0 && B > 1) || (stride_h == 0 && Hkv > 1);
+}
+
 int launched(const char* who, hipError_t before) {
   const hipError_t err = hipPeekAtLastError();
   if (err == hipSuccess || before != hipSuccess) return VK_OK;
@@ -71,6 +82,7 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
   if (tokens == 0 || B == 0) return VK_OK;
   const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
                                   table_width, table_stride, page_stride, head_stride, slot_stride);
+  if (why == nullptr) why = broadcast_refusal(Hkv, num_pages, page_size, page_stride, head_stride, slot_stride);
   if (why == nullptr && (k == nullptr || v == nullptr)) why = "k/v must not be null";
   if (why == nullptr && (!aligned(k, 16) || !aligned(v, 16) || k_stride_t % 8 != 0 || k_stride_h % 8 != 0 ||
                          v_stride_t % 8 != 0 || v_stride_h % 8 != 0))
@@ -120,6 +132,8 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
     why = "rows of q and out must start on 16 bytes";
   if (why == nullptr && (max_len < 0 || max_len > (int64_t)table_width * page_size))
     why = "max_len must be within the table's positions";
+  if (why == nullptr && weight_sums != nullptr && broadcast_sums(B, Hkv, sums_stride_b, sums_stride_h))
+    why = "weight_sums must not be broadcast";
   if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
   if (why == nullptr && elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr))
     why = "k_scale and v_scale are for 8-bit caches";
@@ -172,6 +186,7 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
   if (B == 0) return VK_OK;
   const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_bytes, Hkv, D, num_pages, page_size,
                                   table_width, table_stride, page_stride, head_stride, slot_stride);
+  if (why == nullptr) why = broadcast_refusal(Hkv, num_pages, page_size, page_stride, head_stride, slot_stride);
   if (why == nullptr && (weight_sums == nullptr || sums_out == nullptr || new_lens == nullptr || kept == nullptr))
     why = "weight_sums/sums_out/new_lens/kept must not be null";
   if (why == nullptr && (max_len < 0 || max_len > (int64_t)table_width * page_size))
@@ -180,6 +195,7 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
     why = "budget must be positive, keep_first and keep_last not negative and their sum within budget";
   if (why == nullptr && sums_out == weight_sums && (out_stride_b != sums_stride_b || out_stride_h != sums_stride_h))
     why = "sums_out in place has weight_sums' strides";
+  if (why == nullptr && broadcast_sums(B, Hkv, out_stride_b, out_stride_h)) why = "sums_out must not be broadcast";
   if (why == nullptr && new_lens == seq_lens) why = "new_lens must not be seq_lens";
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
   if (max_len > kPositions || (int64_t)B * Hkv > kInt32 / 2 || (int64_t)budget * D * elem_bytes / 16 > kInt32 / 2 ||
