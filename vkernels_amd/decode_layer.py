@@ -5,7 +5,9 @@ attention over it, eviction when the cache is over its budget, and the MoE layer
 
 runs it on synthetic weights of one of the benchmark configurations' widths.  What a serving program
 keeps is kept here as well: the pages and their free list, the block table, the lengths (on the host,
-so that no step asks the device for them) and what every position has been given so far.
+so that no step reads them back) and what every position has been given so far.  The lengths and new
+pages go to the device by small copies from ordinary host memory, for which the host waits in every step: a
+step cannot be captured in a graph (the operators by themselves can).
 """
 from __future__ import annotations
 
@@ -62,20 +64,24 @@ class DecodeLayer:
     def _grow(self, by):
         """Room for `by` more positions in every sequence (host lists, one small copy to the device).  Where
         there is none, nothing has been taken when the call is refused."""
-        lens = [n + by[b] for b, n in enumerate(self.lens)]
-        need = [-(-n // self.page_size) for n in lens]
-        left = len(self.free)
-        for b, owned in enumerate(self.owned):
-            left -= max(0, need[b] - len(owned))
-            if left < 0 or need[b] > self.table.shape[1]:
-                raise RuntimeError("the cache has no page left for sequence %d" % b)
+        lens, grow, left = [], [], len(self.free)
+        for b, n in enumerate(self.lens):
+            n += by[b]
+            lens.append(n)
+            have = len(self.owned[b])
+            if n > have * self.page_size:
+                more = -(-n // self.page_size) - have
+                left -= more
+                if left < 0 or have + more > self.table.shape[1]:
+                    raise RuntimeError("the cache has no page left for sequence %d" % b)
+                grow.append((b, more))
         rows, columns, pages = [], [], []
-        for b, owned in enumerate(self.owned):
-            while len(owned) < need[b]:
+        for b, more in grow:
+            for _ in range(more):
                 rows.append(b)
-                columns.append(len(owned))
+                columns.append(len(self.owned[b]))
                 pages.append(self.free.pop())
-                owned.append(pages[-1])
+                self.owned[b].append(pages[-1])
         if pages:
             at = torch.tensor([rows, columns, pages], device=self.table.device)
             self.table[at[0], at[1]] = at[2].to(torch.int32)
