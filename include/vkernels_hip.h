@@ -712,7 +712,8 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
  * sink, where there is one); a NaN, or a score of +inf, at a position that counts makes the
  * row NaN, an infinite value its column of the result infinite or NaN.  weight_sums (or NULL): element [b][g][j] (strides in elements)
  * grows by the sum over the heads h of g of e^{s_j} / Z.  max_len: at least every length,
- * at most table_width * page_size; launches and workspace follow it, not the lengths.
+ * at most table_width * page_size; launches and workspace follow it, not the lengths (with
+ * weight_sums the workspace holds every score: 4 * B * Hq * max_len bytes and a little more).
  * The workspace (16-byte aligned) of vk_hip_paged_attention_workspace_bytes is scratch of
  * this call alone; 0 bytes: none is needed.  Deterministic: no atomics. */
 size_t vk_hip_paged_attention_workspace_bytes(int kind, int B, int Hkv, int G, int D, int max_len, int window,

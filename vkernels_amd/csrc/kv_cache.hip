@@ -53,7 +53,8 @@ __device__ __forceinline__ u32x2 e4m3_codes(u32x4 x, float scale, bool bf16) {
 // asked for before their place is looked up: length, then page, then store are the latency that
 // a decode step's call consists of (4 us for 255 tokens); a prompt's is bound by the rows read
 // and written (8191 tokens of 8 heads of 128: 67 MB in 13.9 us, 4.8 TB/s; a thread for each key
-// or value, its row behind the look-up, took 17).
+// or value, its row behind the look-up, took 17).  Into an 8-bit cache these tokens take 15.7 us (50 MB):
+// 16 IEEE divisions a thread, and stores of half the width.
 template <bool FP8>
 __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, int bf16) {
   const int per_token = a.Hkv * a.pieces;
@@ -791,7 +792,7 @@ int kv_evict_parts(int rows, int max_len) {
 
 // A row of 2048 sums is in the registers of 256 threads, which cost less to start and to bring to a
 // barrier, and more rows share a CU: 6976 rows of up to 64 sums in 27 us (1024 threads: 99), 3424 of
-// up to 927 in 22 (64), 1024 of up to 600 in 10 (20), 128 in 7.5 (8.2), 8 of 2000 in 10.2 (9.4).
+// up to 927 in 23 (64), 1024 of up to 600 in 10 (20), 128 in 7.9 (8.2), 8 of 2000 in 10.1 (9.4).
 // Past that a few threads have to read a row again for each digit, which pays as long as other rows
 // hide it: 576 rows of up to 4000 in 17 (20), but of 8000 in 26 (23); 1024 of 5000 in 22 (28) and of
 // 9000 in 32 (40), but of 16000 in 60 (56); 256 of 2300 in 12.1 (10.8).

@@ -453,7 +453,8 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           // c tanh(y / c) = c (1 - 2 / (1 + e^{2 y / c})), and y (1 - z^2 / 3 + 2 z^4 / 15) with
-          // z = y / c below 0.1, where the first form cancels
+          // z = y / c below 0.1, where the first form cancels.  Hardware exponential and reciprocal
+          // leave less than 2^-20 of the cap.
           const float z2 = x[i] * cap_in;                       // 2 y / c, in powers of two
           const float big = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + exp2_fast(z2));
           const float z = z2 * (0.5f * kLn2), zz = z * z;

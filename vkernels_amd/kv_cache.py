@@ -207,7 +207,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     c tanh(s / c); ``sinks`` [Hq] float32 are scores whose value is zero.  ``max_len`` bounds every
     length (default: what the table holds; a longer sequence is cut to it): the launch and its
     workspace follow it, so a tight bound is worth giving.  ``weight_sums`` [B, Hkv, positions]
-    float32: every position's weights, summed over the heads of the group, are added to it.
+    float32: every position's weights, summed over the heads of the group, are added to it; the call's
+    scratch is then 4 B Hq max_len bytes, whatever the lengths are.
     Returns out [B, Hq, D], or (out, lse [B, Hq] float32).  A row that nothing is left of is 0, its
     lse -inf (its sink, where there is one)."""
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
