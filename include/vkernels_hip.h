@@ -754,6 +754,31 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
                           int64_t sums_stride_h, int64_t out_stride_b, int64_t out_stride_h, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* ---- Queries and keys in front of the cache (additive) --------------------------------
+ *
+ * RMS norm of every head of q [T, Hq, D] and k [T, Hkv, D] and the rotation of its first
+ * `turned` values by the token's position, in one pass:
+ *   y = x * w / sqrt(mean(x^2) + eps)    (norm != 0; w the weight [D], or 1 where it is NULL),
+ *   (a, b) -> (a cos - b sin, b cos + a sin), cos and sin of positions[axis(i)][t] * inv_freq[i]
+ *   times `factor`, for i < turned / 2, with (a, b) values i and i + turned / 2 of y, or
+ *   2 i and 2 i + 1 (pairs != 0);  values from `turned` on stay y.
+ * inv_freq [turned / 2] fp32; positions [axes, T] int32 (any values; axes axis_stride
+ * elements apart).  With several axes (up to 4) the first sections[0] frequencies belong to
+ * axis 0, the next sections[1] to axis 1 and so on; `sections` is HOST memory, axes numbers
+ * that add up to turned / 2 (NULL for one axis).  The angle is a product in 64 bits and
+ * exact to 2^-24 of a turn; everything else is 32 bits, rounded once.
+ * kind VK_HIP_KV_BF16 or VK_HIP_KV_F16: q, k, the results and, with weights_f32 == 0, the
+ * weights; weights_f32 != 0: weights in fp32.  Strides in elements.  q_out and k_out may be q
+ * and k themselves, with their strides; otherwise they overlap neither.  D a multiple of 16 up to 256, turned a
+ * multiple of 8 up to D, rows and weights start on 16 bytes. */
+int vk_hip_qk_norm_rope(const void* q, const void* k, const int32_t* positions, const float* inv_freq,
+                        const void* q_weight, const void* k_weight, void* q_out, void* k_out, int kind,
+                        int weights_f32, int T, int Hq, int Hkv, int D, int turned, int pairs, int axes,
+                        const int32_t* sections, int norm, float eps, float factor, int64_t q_stride_t,
+                        int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, int64_t q_out_stride_t,
+                        int64_t q_out_stride_h, int64_t k_out_stride_t, int64_t k_out_stride_h,
+                        int64_t axis_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@
 
 #include "kv_cache.hpp"
 #include "paged_attention.hpp"
+#include "qk_norm_rope.hpp"
 
 namespace {
 
@@ -216,6 +217,68 @@ int vk_hip_kv_cache_evict(void* k_cache, void* v_cache, const int32_t* block_tab
   a.order = static_cast<uint32_t*>(workspace);
   const hipError_t before = hipPeekAtLastError();
   vk::launch_kv_evict(a, static_cast<hipStream_t>(stream));
+  return launched(who, before);
+}
+
+int vk_hip_qk_norm_rope(const void* q, const void* k, const int32_t* positions, const float* inv_freq,
+                        const void* q_weight, const void* k_weight, void* q_out, void* k_out, int kind,
+                        int weights_f32, int T, int Hq, int Hkv, int D, int turned, int pairs, int axes,
+                        const int32_t* sections, int norm, float eps, float factor, int64_t q_stride_t,
+                        int64_t q_stride_h, int64_t k_stride_t, int64_t k_stride_h, int64_t q_out_stride_t,
+                        int64_t q_out_stride_h, int64_t k_out_stride_t, int64_t k_out_stride_h,
+                        int64_t axis_stride, void* stream) {
+  const char* const who = "vk_hip_qk_norm_rope";
+  if (kind != VK_HIP_KV_BF16 && kind != VK_HIP_KV_F16)
+    return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be VK_HIP_KV_BF16 or VK_HIP_KV_F16");
+  if (T < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "T must not be negative");
+  if (T == 0) return VK_OK;
+  const char* why = nullptr;
+  if (Hq <= 0 || Hkv <= 0) why = "Hq and Hkv must be positive";
+  if (why == nullptr && (D <= 0 || D % 16 != 0 || D > 256)) why = "D must be a multiple of 16 up to 256";
+  if (why == nullptr && (turned <= 0 || turned % 8 != 0 || turned > D))
+    why = "the values that are rotated must be a multiple of 8 up to D";
+  if (why == nullptr && (axes <= 0 || axes > vk::kRopeAxes)) why = "there are 1 to 4 axes";
+  if (why == nullptr && axes > 1 && sections == nullptr) why = "several axes need sections";
+  if (why == nullptr && (q == nullptr || k == nullptr || q_out == nullptr || k_out == nullptr || positions == nullptr ||
+                         inv_freq == nullptr))
+    why = "q/k/q_out/k_out/positions/inv_freq must not be null";
+  if (why == nullptr && !norm && (q_weight != nullptr || k_weight != nullptr)) why = "weights belong to the norm";
+  if (why == nullptr && norm && !(eps >= 0.0f)) why = "eps must not be negative";
+  if (why == nullptr && (!aligned(q_weight, 16) || !aligned(k_weight, 16))) why = "weights must start on 16 bytes";
+  if (why == nullptr && (!aligned(q, 16) || !aligned(k, 16) || !aligned(q_out, 16) || !aligned(k_out, 16) ||
+                         (q_stride_t | q_stride_h | k_stride_t | k_stride_h | q_out_stride_t | q_out_stride_h |
+                          k_out_stride_t | k_out_stride_h) % 8 != 0))
+    why = "rows of q, k and the results must start on 16 bytes";
+  if (why == nullptr && (q_stride_t < 0 || q_stride_h < 0 || k_stride_t < 0 || k_stride_h < 0 || axis_stride < 0))
+    why = "strides must not be negative";
+  // (results hold every value once)
+  auto rows_overlap = [T, D](int heads, int64_t by_t, int64_t by_h) {
+    return (T > 1 && by_t < D) || (heads > 1 && by_h < D);
+  };
+  if (why == nullptr && (rows_overlap(Hq, q_out_stride_t, q_out_stride_h) || rows_overlap(Hkv, k_out_stride_t, k_out_stride_h)))
+    why = "rows of the results must not overlap";
+  vk::QkNormRopeArgs a{};
+  a.section_end[0] = turned / 2;
+  int64_t all = 0;
+  for (int i = 0; why == nullptr && axes > 1 && i < axes; ++i) {
+    if (sections[i] < 0) why = "sections must not be negative";
+    all += sections[i];
+    a.section_end[i] = (int)(all < turned ? all : turned);
+  }
+  if (why == nullptr && axes > 1 && all != turned / 2) why = "sections must add up to half the values that are rotated";
+  if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
+  if (T > kThreads / 256 || Hq > kInt32 / 2 || Hkv > kInt32 / 2 - 4096)
+    return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many tokens or heads for one call");
+  a.q = q; a.k = k; a.q_out = q_out; a.k_out = k_out; a.q_weight = q_weight; a.k_weight = k_weight;
+  a.positions = positions; a.inv_freq = inv_freq;
+  a.q_stride_t = q_stride_t; a.q_stride_h = q_stride_h; a.k_stride_t = k_stride_t; a.k_stride_h = k_stride_h;
+  a.qo_stride_t = q_out_stride_t; a.qo_stride_h = q_out_stride_h;
+  a.ko_stride_t = k_out_stride_t; a.ko_stride_h = k_out_stride_h;
+  a.axis_stride = axis_stride;
+  a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.turned = turned; a.axes = axes;
+  a.eps = eps; a.factor = factor; a.norm = norm != 0; a.weights_f32 = weights_f32 != 0;
+  const hipError_t before = hipPeekAtLastError();
+  vk::launch_qk_norm_rope(a, kind == VK_HIP_KV_BF16, pairs != 0, static_cast<hipStream_t>(stream));
   return launched(who, before);
 }
 

@@ -1,0 +1,129 @@
+"""Queries and keys in front of the key-value cache: the RMS norm of every head and the rotation by the
+token's position, in one pass over them.
+
+The call is enqueued on the current stream of the tensors' device, without host synchronisation, and can be
+captured in a graph.  It is an operator of inference: a backward pass that comes to it raises an error.
+
+The entry point is additive: the reference leaves queries and keys to its caller.  Everything runs in
+``libvkernels_hip.so``; there is no fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .kv_cache import _current_device, _failed, _need, _rows, _stream
+from .vllm_experts import load_libvkernels_hip
+
+__all__ = ["qk_norm_rope"]
+
+_KINDS = {torch.bfloat16: 0, torch.float16: 1}
+_fn_cache: list = []
+
+
+def _fn():
+    if not _fn_cache:
+        fn = getattr(load_libvkernels_hip(), "vk_hip_qk_norm_rope", None)
+        if fn is None:
+            raise RuntimeError("vk_hip_qk_norm_rope not found in libvkernels_hip.so")
+        P, I, L, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+        fn.argtypes, fn.restype = [P] * 8 + [I] * 9 + [P, I, F, F] + [L] * 9 + [P], I
+        _fn_cache.append(fn)
+    return _fn_cache[0]
+
+
+class _NoBackward(torch.autograd.Function):
+    """The results as they are; a backward pass that reaches them is an error instead of a gradient lost."""
+
+    @staticmethod
+    def forward(ctx, q, k, *inputs):
+        return q.view_as(q), k.view_as(k)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("qk_norm_rope has no backward pass: it is an operator of inference "
+                           "(call it under torch.no_grad(), or detach what requires a gradient)")
+
+
+def _weight(w, D, kind, device, name):
+    if not (w.shape == (D,) and w.dtype is kind and w.get_device() == device and (D == 1 or w.stride(0) == 1)):
+        raise ValueError(f"{name} must be [D] contiguous on q's device, and both weights in float32 or in q's type")
+    return w if w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+
+
+def _check_out(out, like, name):
+    s = out.stride()
+    _need(out.shape == like.shape and out.dtype is like.dtype and out.get_device() == like.get_device() and s[2] == 1 and
+          s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0,
+          f"the result for {name} must be like {name}, with rows that start on 16 bytes")
+
+
+def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps=1e-6, sections=None, pairs=False,
+                 factor=1.0, out=None):
+    """Queries [T, Hq, D] and keys [T, Hkv, D] with every head normed and rotated by its token's position.
+
+    A head x becomes x * weight / sqrt(mean(x^2) + eps) (``q_weight``, ``k_weight`` [D] in q's type or both
+    float32, None: 1; ``eps`` None: no norm).  Of the result the first 2 R values, R the number of ``inv_freq``
+    (float32), are turned in pairs by the angles position * inv_freq[i], cosine and sine times ``factor``:
+    value i with value i + R, or with ``pairs`` 2 i with 2 i + 1.  The others stay.
+    ``positions`` [T] int32, or [axes, T] (time, height, width, ...; up to 4) with ``sections``: so many of
+    the frequencies, in order, turn by each axis.
+    Returns (q, k), new ones, or ``out`` (a pair of tensors, which may be q and k themselves).  q and k may be
+    views of one tensor of any strides with D contiguous."""
+    device = q.get_device()
+    _need(q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2],
+          "q and k must be [T, Hq, D] and [T, Hkv, D]")
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    kind = _KINDS.get(q.dtype)
+    _need(kind is not None and k.dtype is q.dtype, "q and k must both be bfloat16 or float16")
+    _need(device >= 0 and device == _current_device() and k.get_device() == device and
+          positions.get_device() == device and inv_freq.get_device() == device,
+          "the tensors must be on the current device")
+    _need(T < 1 << 31 and Hq < 1 << 31 and Hkv < 1 << 31 and Hq > 0 and Hkv > 0 and D > 0,
+          "q and k must have heads, and sizes below 2^31")
+    _need(inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
+          inv_freq.shape[0] <= D // 2, "inv_freq must be up to D / 2 contiguous float32 values")
+    R = inv_freq.shape[0]
+    if sections is None:
+        _need(positions.shape == (T,), "positions must be [T], or [axes, T] with sections")
+        axes, axis_stride, c_sections = 1, 0, None
+    else:
+        axes = len(sections)
+        _need(1 <= axes <= 4 and positions.shape == (axes, T), "positions must be [axes, T] with a section for each of up to 4 axes")
+        _need(all(0 <= n <= R for n in sections) and sum(sections) == R, "sections must add up to the number of inv_freq")
+        axis_stride, c_sections = positions.stride(0), (ctypes.c_int32 * axes)(*sections)
+    _need(positions.dtype is torch.int32 and (T <= 1 or positions.stride(-1) == 1),
+          "positions must be int32 with contiguous rows")
+    weights_f32 = 0
+    if eps is None:
+        _need(q_weight is None and k_weight is None, "weights belong to the norm, which eps=None leaves out")
+    elif q_weight is not None or k_weight is not None:
+        of = (q_weight if q_weight is not None else k_weight).dtype
+        weights_f32 = int(of is torch.float32)
+        of = torch.float32 if weights_f32 else q.dtype
+        q_weight = None if q_weight is None else _weight(q_weight, D, of, device, "q_weight")
+        k_weight = None if k_weight is None else _weight(k_weight, D, of, device, "k_weight")
+    wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
+        w is not None and w.requires_grad for w in (q_weight, k_weight)))
+    if out is None:
+        q_out, k_out = q.new_empty((T, Hq, D)), k.new_empty((T, Hkv, D))
+    else:
+        q_out, k_out = out
+        _check_out(q_out, q, "q")
+        _check_out(k_out, k, "k")
+    inputs = q, k
+    q, k = _rows(q), _rows(k)
+    qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    status = _fn()(
+        q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+        q_out.data_ptr(), k_out.data_ptr(), kind, weights_f32, T, Hq, Hkv, D, 2 * R, pairs, axes,
+        c_sections, eps is not None, 0.0 if eps is None else eps, factor, qs[0], qs[1], ks[0], ks[1], qo[0], qo[1],
+        ko[0], ko[1], axis_stride, _stream(device))
+    if status:
+        _failed(status, "vk_hip_qk_norm_rope")
+    if wants_grad and out is None:
+        q_out, k_out = _NoBackward.apply(q_out, k_out, *inputs, q_weight, k_weight)
+    return q_out, k_out
