@@ -701,6 +701,39 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
                            int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
                            int64_t head_stride, int64_t slot_stride, void* stream);
 
+/* The same for an 8-bit cache with a scale for each block of positions and head, which this call
+ * writes: k_scale, v_scale [num_pages, Hkv, scale_blocks] fp32 contiguous, a block page_size / scale_blocks
+ * positions of a page (scale_blocks divides page_size; 1: a scale for each page, page_size: for each position;
+ * 0: the call above).  Of every block that new rows go to, in every head and for keys and values by
+ * themselves,
+ *   s = max over the new rows' values of |x| / 448, and the block's old scale where the block has positions
+ *       in front of the new ones, if that is larger;
+ * the new codes are those nearest to x / s, and where s has grown the codes c in front of them become
+ * those nearest to c * (s_old / s) (each a quotient or product in fp32).  A block that begins with a new
+ * row takes nothing from what it held.  Infinite values and NaN do not count for s: they become the largest
+ * finite codes and NaN.  A block of zeros has scale 0.  The pages that are written to must not be shared. */
+int vk_hip_kv_cache_append_ex(const void* k, const void* v, void* k_cache, void* v_cache,
+                              const int32_t* block_table, const int32_t* seq_lens,
+                              const int32_t* query_start, float* k_scale, float* v_scale, int scale_blocks,
+                              int kind, int B, int tokens, int Hkv, int D, int num_pages, int page_size,
+                              int table_width, int table_stride, int64_t k_stride_t, int64_t k_stride_h,
+                              int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
+                              int64_t head_stride, int64_t slot_stride, void* stream);
+
+/* Positions of a cache as rows: k, v [tokens, Hkv, D] in the query type (strides in elements) get the last
+ * query_start[b + 1] - query_start[b] positions of every sequence, in the rows that vk_hip_kv_cache_append
+ * would take them from (NULL: the last position of every sequence, tokens == B), 8-bit codes times their
+ * scale (k_scale, v_scale [Hkv], or with scale_blocks > 0 [num_pages, Hkv, scale_blocks]), rounded once.
+ * Positions in front of the sequence or of an entry that is no page are rows of zeros; rows that belong to no sequence become zeros
+ * with clear_rest != 0 and else stay as they are. */
+int vk_hip_kv_cache_read(const void* k_cache, const void* v_cache, const int32_t* block_table,
+                         const int32_t* seq_lens, const int32_t* query_start, const float* k_scale,
+                         const float* v_scale, int scale_blocks, void* k, void* v, int kind, int B, int tokens,
+                         int Hkv, int D, int num_pages, int page_size, int table_width, int table_stride,
+                         int clear_rest, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                         int64_t v_stride_h, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                         void* stream);
+
 /* Attention of one new token of every sequence over its cache: q [B, Hq, D] (strides in
  * elements), out [B, Hq, D] contiguous, lse [B, Hq] fp32 or NULL.
  *   s_j = scale * k_scale[g] * q_h . k_j, then softcap * tanh(s_j / softcap) if softcap > 0

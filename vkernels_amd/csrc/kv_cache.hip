@@ -7,47 +7,16 @@
 #include <algorithm>
 
 #include "kv_cache.hpp"
+#include "kv_rows.hpp"
 #include "paged_attention.hpp"
 
 namespace vk {
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef kv_u32x4 u32x4;
+typedef kv_u32x2 u32x2;
 
 // ---- append --------------------------------------------------------------------------------
-
-// What does not fit into E4M3 is stored as its largest finite code.
-__device__ __forceinline__ float e4m3_range(float x) {
-  // (comparisons that leave a NaN a NaN)
-  x = x > 448.0f ? 448.0f : x;
-  return x < -448.0f ? -448.0f : x;
-}
-
-__device__ __forceinline__ float f16_bits_to_f32(uint32_t bits, bool bf16) {
-  if (bf16) return __uint_as_float(bits << 16);
-  union { uint16_t u; _Float16 h; } c;
-  c.u = (uint16_t)bits;
-  return (float)c.h;
-}
-
-// 8 values of a row as E4M3 codes.
-__device__ __forceinline__ u32x2 e4m3_codes(u32x4 x, float scale, bool bf16) {
-  u32x2 codes;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    float f[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t w = x[2 * i + j / 2];
-      f[j] = e4m3_range(f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu, bf16) / scale);
-    }
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
-    c = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], c, true);
-    codes[i] = (uint32_t)c;
-  }
-  return codes;
-}
 
 // A thread takes the same 8 values (16 bytes) of a token's key and value in a head.  The rows are
 // asked for before their place is looked up: length, then page, then store are the latency that
@@ -67,19 +36,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppendArgs a, in
   const u32x4 v = *(const u32x4*)((const char*)a.v + ((int64_t)there * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
   int seq = there;
   if (a.starts != nullptr) {
-    // The sequence of the wavefront's first token, 64 candidates at a time; the other
-    // lanes walk on from there.
-    const int lane = threadIdx.x & 63, t0 = divided(first, a.by_token);
-    int lo = 0, hi = a.B;           // the last i in [lo, hi) with starts[i] <= t0
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 63) / 64;
-      const int i = lo + lane * step;
-      const uint64_t below = __ballot(i < hi && a.starts[i] <= t0);
-      const int n = max(1, (int)__popcll(below));
-      hi = min(hi, lo + n * step);
-      lo += (n - 1) * step;
-    }
-    seq = lo;
+    // The sequence of the wavefront's first token; the other lanes walk on from there.
+    const int t0 = divided(first, a.by_token);
+    seq = last_not_above(a.B, t0, [&](int i) { return a.starts[i]; });
     while (seq + 1 < a.B && a.starts[seq + 1] <= there) ++seq;
   }
   if (t >= a.tokens || seq >= a.B || (a.starts != nullptr && t < a.starts[seq])) return;

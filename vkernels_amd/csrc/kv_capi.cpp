@@ -9,6 +9,7 @@
 #include <cstdint>
 #include <string>
 
+#include "kv_blocks.hpp"
 #include "kv_cache.hpp"
 #include "paged_attention.hpp"
 #include "qk_norm_rope.hpp"
@@ -64,6 +65,63 @@ int launched(const char* who, hipError_t before) {
 bool known_kind(int kind) { return kind >= VK_HIP_KV_BF16 && kind <= VK_HIP_KV_FP8_F16; }
 int elem_of(int kind) { return kind >= VK_HIP_KV_FP8_BF16 ? 1 : 2; }
 
+const char* rows_refusal(const void* k, const void* v, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                         int64_t v_stride_h) {
+  if (!aligned(k, 16) || !aligned(v, 16) || k_stride_t % 8 != 0 || k_stride_h % 8 != 0 || v_stride_t % 8 != 0 ||
+      v_stride_h % 8 != 0)
+    return "rows of k and v must start on 16 bytes";
+  return nullptr;
+}
+
+const char* scales_refusal(int kind, const float* k_scale, const float* v_scale, int scale_blocks, int page_size) {
+  if (elem_of(kind) == 1 && (k_scale == nullptr || v_scale == nullptr)) return "an 8-bit cache needs k_scale and v_scale";
+  if (elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr)) return "k_scale and v_scale are for 8-bit caches";
+  if (scale_blocks < 0 || (scale_blocks > 0 && (elem_of(kind) == 2 || page_size % scale_blocks != 0)))
+    return "blocks with a scale of their own are equal parts of an 8-bit cache's pages";
+  return nullptr;
+}
+
+// New rows into the cache: with scale_blocks > 0 their scales are the call's own.
+int append(const char* who, const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* block_table,
+           const int32_t* seq_lens, const int32_t* query_start, float* k_scale, float* v_scale, int scale_blocks, int kind,
+           int B, int tokens, int Hkv, int D, int num_pages, int page_size, int table_width, int table_stride,
+           int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
+           int64_t head_stride, int64_t slot_stride, void* stream) {
+  if (!known_kind(kind)) return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be one of VK_HIP_KV_*");
+  if (B < 0 || tokens < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B and tokens must not be negative");
+  if (query_start == nullptr && tokens != B)
+    return refuse(VK_ERROR_INVALID_ARGUMENT, who, "without query_start there is one token for each sequence");
+  if (tokens == 0 || B == 0) return VK_OK;
+  const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
+                                  table_width, table_stride, page_stride, head_stride, slot_stride);
+  if (why == nullptr) why = broadcast_refusal(Hkv, num_pages, page_size, page_stride, head_stride, slot_stride);
+  if (why == nullptr && (k == nullptr || v == nullptr)) why = "k/v must not be null";
+  if (why == nullptr) why = rows_refusal(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h);
+  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
+  if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
+  if ((int64_t)tokens * Hkv > kInt32 / D) return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
+  vk::KvAppendArgs a{};
+  a.k = k; a.v = v; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
+  a.starts = query_start; a.k_scale = k_scale; a.v_scale = v_scale;
+  a.k_stride_t = k_stride_t; a.k_stride_h = k_stride_h; a.v_stride_t = v_stride_t; a.v_stride_h = v_stride_h;
+  a.page_stride = page_stride; a.head_stride = head_stride; a.slot_stride = slot_stride;
+  a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
+  a.B = B; a.tokens = tokens; a.Hkv = Hkv; a.D = D;
+  if (scale_blocks > 0) {
+    vk::KvQuantiseArgs A{};
+    A.a = a;
+    A.k_scale = k_scale; A.v_scale = v_scale; A.blocks = scale_blocks; A.block = page_size / scale_blocks;
+    if (vk::kv_quantise_slots(B, tokens, A.block, query_start != nullptr) > kThreads / 128 / 2 / Hkv)
+      return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
+    const hipError_t before = hipPeekAtLastError();
+    vk::launch_kv_quantise(A, kind == VK_HIP_KV_FP8_BF16, static_cast<hipStream_t>(stream));
+    return launched(who, before);
+  }
+  const hipError_t before = hipPeekAtLastError();
+  vk::launch_kv_append(a, kind, static_cast<hipStream_t>(stream));
+  return launched(who, before);
+}
+
 }  // namespace
 
 extern "C" {
@@ -75,34 +133,58 @@ int vk_hip_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_
                            int table_width, int table_stride, int64_t k_stride_t, int64_t k_stride_h,
                            int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
                            int64_t head_stride, int64_t slot_stride, void* stream) {
-  const char* const who = "vk_hip_kv_cache_append";
+  return append("vk_hip_kv_cache_append", k, v, k_cache, v_cache, block_table, seq_lens, query_start, const_cast<float*>(k_scale),
+                const_cast<float*>(v_scale), 0, kind, B, tokens, Hkv, D, num_pages, page_size, table_width, table_stride,
+                k_stride_t, k_stride_h, v_stride_t, v_stride_h, page_stride, head_stride, slot_stride, stream);
+}
+
+int vk_hip_kv_cache_append_ex(const void* k, const void* v, void* k_cache, void* v_cache,
+                              const int32_t* block_table, const int32_t* seq_lens,
+                              const int32_t* query_start, float* k_scale, float* v_scale, int scale_blocks,
+                              int kind, int B, int tokens, int Hkv, int D, int num_pages, int page_size,
+                              int table_width, int table_stride, int64_t k_stride_t, int64_t k_stride_h,
+                              int64_t v_stride_t, int64_t v_stride_h, int64_t page_stride,
+                              int64_t head_stride, int64_t slot_stride, void* stream) {
+  return append("vk_hip_kv_cache_append_ex", k, v, k_cache, v_cache, block_table, seq_lens, query_start, k_scale, v_scale,
+                scale_blocks, kind, B, tokens, Hkv, D, num_pages, page_size, table_width, table_stride, k_stride_t, k_stride_h,
+                v_stride_t, v_stride_h, page_stride, head_stride, slot_stride, stream);
+}
+
+int vk_hip_kv_cache_read(const void* k_cache, const void* v_cache, const int32_t* block_table,
+                         const int32_t* seq_lens, const int32_t* query_start, const float* k_scale,
+                         const float* v_scale, int scale_blocks, void* k, void* v, int kind, int B, int tokens,
+                         int Hkv, int D, int num_pages, int page_size, int table_width, int table_stride,
+                         int clear_rest, int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_t,
+                         int64_t v_stride_h, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                         void* stream) {
+  const char* const who = "vk_hip_kv_cache_read";
   if (!known_kind(kind)) return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be one of VK_HIP_KV_*");
   if (B < 0 || tokens < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B and tokens must not be negative");
   if (query_start == nullptr && tokens != B)
     return refuse(VK_ERROR_INVALID_ARGUMENT, who, "without query_start there is one token for each sequence");
-  if (tokens == 0 || B == 0) return VK_OK;
+  if (tokens == 0) return VK_OK;
+  if (B == 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "rows need a sequence to be read from");
   const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
                                   table_width, table_stride, page_stride, head_stride, slot_stride);
-  if (why == nullptr) why = broadcast_refusal(Hkv, num_pages, page_size, page_stride, head_stride, slot_stride);
   if (why == nullptr && (k == nullptr || v == nullptr)) why = "k/v must not be null";
-  if (why == nullptr && (!aligned(k, 16) || !aligned(v, 16) || k_stride_t % 8 != 0 || k_stride_h % 8 != 0 ||
-                         v_stride_t % 8 != 0 || v_stride_h % 8 != 0))
-    why = "rows of k and v must start on 16 bytes";
-  if (why == nullptr && elem_of(kind) == 1 && (k_scale == nullptr || v_scale == nullptr))
-    why = "an 8-bit cache needs k_scale and v_scale";
-  if (why == nullptr && elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr))
-    why = "k_scale and v_scale are for 8-bit caches";
+  if (why == nullptr) why = rows_refusal(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h);
+  auto overlap = [tokens, Hkv, D](int64_t by_t, int64_t by_h) {
+    return by_t < 0 || by_h < 0 || (tokens > 1 && by_t < D) || (Hkv > 1 && by_h < D);
+  };
+  if (why == nullptr && (overlap(k_stride_t, k_stride_h) || overlap(v_stride_t, v_stride_h))) why = "rows of k and v must not overlap";
+  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
   if ((int64_t)tokens * Hkv > kInt32 / D) return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
-  vk::KvAppendArgs a{};
-  a.k = k; a.v = v; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
-  a.starts = query_start; a.k_scale = k_scale; a.v_scale = v_scale;
+  vk::KvReadArgs a{};
+  a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens; a.starts = query_start;
+  a.k_scale = k_scale; a.v_scale = v_scale; a.k = k; a.v = v;
   a.k_stride_t = k_stride_t; a.k_stride_h = k_stride_h; a.v_stride_t = v_stride_t; a.v_stride_h = v_stride_h;
   a.page_stride = page_stride; a.head_stride = head_stride; a.slot_stride = slot_stride;
   a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
-  a.B = B; a.tokens = tokens; a.Hkv = Hkv; a.D = D;
+  a.blocks = scale_blocks; a.block = scale_blocks > 0 ? page_size / scale_blocks : 0;
+  a.B = B; a.tokens = tokens; a.Hkv = Hkv; a.D = D; a.clear_rest = clear_rest != 0;
   const hipError_t before = hipPeekAtLastError();
-  vk::launch_kv_append(a, kind, static_cast<hipStream_t>(stream));
+  vk::launch_kv_read(a, kind, static_cast<hipStream_t>(stream));
   return launched(who, before);
 }
 
@@ -136,10 +218,7 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
   if (why == nullptr && weight_sums != nullptr && broadcast_sums(B, Hkv, sums_stride_b, sums_stride_h))
     why = "weight_sums must not be broadcast";
   if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
-  if (why == nullptr && elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr))
-    why = "k_scale and v_scale are for 8-bit caches";
-  if (why == nullptr && elem_of(kind) == 1 && (k_scale == nullptr || v_scale == nullptr))
-    why = "an 8-bit cache needs k_scale and v_scale";
+  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, 0, page_size);
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
   // (units of work are counted in 32 bits, and so are a launch's threads, 256 for each item or chunk)
   const int64_t rows = (int64_t)B * Hkv, items = rows * ((G + vk::kPaHeads - 1) / vk::kPaHeads);

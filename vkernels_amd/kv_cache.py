@@ -24,7 +24,7 @@ import torch
 
 from .vllm_experts import last_error, load_libvkernels_hip
 
-__all__ = ["kv_cache_append", "kv_cache_evict", "paged_attention"]
+__all__ = ["kv_cache_append", "kv_cache_evict", "kv_cache_read", "paged_attention"]
 
 _P, _I, _L, _F, _Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -46,6 +46,8 @@ def _fn(name):
         lib = load_libvkernels_hip()
         argtypes, restype = {
             "vk_hip_kv_cache_append": ([_P] * 9 + [_I] * 9 + [_L] * 7 + [_P], _I),
+            "vk_hip_kv_cache_append_ex": ([_P] * 9 + [_I] * 10 + [_L] * 7 + [_P], _I),
+            "vk_hip_kv_cache_read": ([_P] * 7 + [_I] + [_P] * 2 + [_I] * 10 + [_L] * 7 + [_P], _I),
             "vk_hip_paged_attention_workspace_bytes": ([_I] * 8, _Z),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
             "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 6, _Z),
@@ -122,6 +124,27 @@ def _head_vector(t, n, name, device):
     return t.data_ptr()
 
 
+def _scales(k_scale, v_scale, pages, Hkv, page_size, device):
+    """Addresses of the scales of an 8-bit cache and how many a page has for each head: 0 where there is one
+    for the head alone, [Hkv], else [pages, Hkv, blocks]."""
+    if k_scale is None or v_scale is None or k_scale.dim() != 3:
+        return (None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
+                None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device), 0)
+    blocks = k_scale.shape[2]
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if not (t.shape == (pages, Hkv, blocks) and blocks and page_size % blocks == 0 and t.dtype is torch.float32 and
+                t.is_contiguous() and t.get_device() == device):
+            raise ValueError(f"{name} must be contiguous float32 [Hkv], or [pages, Hkv, blocks] with blocks that "
+                             "divide a page, on the cache's device, both alike")
+    return k_scale.data_ptr(), v_scale.data_ptr(), blocks
+
+
+def _query_start(t, B, device):
+    _need(t.dtype is torch.int32 and t.numel() == B + 1 and t.is_contiguous() and t.get_device() == device,
+          "query_start must be int32 [B + 1] on the cache's device")
+    return t.data_ptr()
+
+
 def _cache(k_cache, v_cache, block_table, seq_lens):
     """Checks what every operator takes: (pages, Hkv, page_size, D), the cache's strides, its device, and
     the table's (B, W) and elements from row to row."""
@@ -171,7 +194,13 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     query_start[b] .. query_start[b + 1] - 1 and go to its last positions; None: one token for each
     sequence (a sequence of length 0 takes none).  Positions whose page is outside [0, pages) are
     skipped.  An 8-bit cache holds the codes nearest to value / scale of the head (``k_scale``,
-    ``v_scale`` [Hkv]), the largest finite code beyond +-448."""
+    ``v_scale`` [Hkv]), the largest finite code beyond +-448.
+
+    With ``k_scale``, ``v_scale`` [pages, Hkv, blocks] an 8-bit cache has a scale for each head and block of
+    page_size / blocks positions, and this call finds it: the block's largest magnitude / 448, of the new
+    rows and of the positions already in front of them, whose codes are rounded again where the scale grows
+    (a block that begins with a new row takes nothing from what it held).  Infinite values and NaN do not
+    count for it."""
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     tokens = k.shape[0]
     _need(k.shape == (tokens, Hkv, D) and v.shape == k.shape and v.dtype is k.dtype and tokens < 1 << 31,
@@ -180,22 +209,62 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
     kind = _KINDS.get((k_cache.dtype, k.dtype))
     _need(kind is not None, "the cache's type does not take rows of this type")
     if query_start is not None:
-        _need(query_start.dtype is torch.int32 and query_start.numel() == B + 1 and query_start.is_contiguous() and
-              query_start.get_device() == device, "query_start must be int32 [B + 1] on the cache's device")
-        query_start = query_start.data_ptr()
+        query_start = _query_start(query_start, B, device)
     else:
         _need(tokens == B, "without query_start there is one token for each sequence")
     k, v = _rows(k), _rows(v)
     ks, vs = k.stride(), v.stride()
-    status = _fn("vk_hip_kv_cache_append")(
+    k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
+    name, more = ("vk_hip_kv_cache_append_ex", (blocks,)) if blocks else ("vk_hip_kv_cache_append", ())
+    status = _fn(name)(
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-        seq_lens.data_ptr(), query_start,
-        None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
-        None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device), kind, B, tokens, Hkv, D, pages, ps,
+        seq_lens.data_ptr(), query_start, k_scale, v_scale, *more, kind, B, tokens, Hkv, D, pages, ps,
         W, table_stride, ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2],
         _stream(device))
     if status:
-        _failed(status, "vk_hip_kv_cache_append")
+        _failed(status, name)
+
+
+def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, tokens=None, k_scale=None, v_scale=None,
+                  dtype=None, out=None):
+    """Cached positions as rows: (k, v), each [tokens, Hkv, D].
+
+    ``query_start`` [B + 1] int32: rows query_start[b] .. query_start[b + 1] - 1 are the last so many positions of
+    sequence b, where ``kv_cache_append`` would have taken them from; ``tokens`` is how many rows there are.
+    None: the last position of every sequence.  A 16-bit cache's rows come in its type; of an 8-bit one codes
+    times scale ([Hkv] or [pages, Hkv, blocks]) in ``dtype``, bfloat16 (the default) or float16.
+    Positions in front of the sequence and those of an entry that is no page are rows of zeros.  Rows that belong to no sequence
+    are zeros in new tensors, and left as they are in ``out`` (a pair of tensors with rows that start on 16
+    bytes)."""
+    (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
+    if query_start is not None:
+        _need(tokens is not None and 0 <= tokens < 1 << 31, "query_start needs tokens, the number of rows")
+        query_start = _query_start(query_start, B, device)
+    else:
+        _need(tokens is None or tokens == B, "without query_start there is one token for each sequence")
+        tokens = B
+    if dtype is None:
+        dtype = torch.bfloat16 if k_cache.dtype is torch.float8_e4m3fn else k_cache.dtype
+    kind = _KINDS.get((k_cache.dtype, dtype))
+    _need(kind is not None, "the cache's type does not give rows of this type")
+    if out is None:
+        k, v = (k_cache.new_empty((tokens, Hkv, D), dtype=dtype) for _ in range(2))
+    else:
+        k, v = out
+        for t in (k, v):
+            s = t.stride()
+            _need(t.shape == (tokens, Hkv, D) and t.dtype is dtype and t.get_device() == device and s[2] == 1 and
+                  s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0,
+                  "out must be two [tokens, Hkv, D] on the cache's device with rows that start on 16 bytes")
+    ks, vs = k.stride(), v.stride()
+    k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
+    status = _fn("vk_hip_kv_cache_read")(
+        k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), query_start, k_scale, v_scale,
+        blocks, k.data_ptr(), v.data_ptr(), kind, B, tokens, Hkv, D, pages, ps, W, table_stride, out is None,
+        ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2], _stream(device))
+    if status:
+        _failed(status, "vk_hip_kv_cache_read")
+    return k, v
 
 
 def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, softcap=0.0,
