@@ -761,6 +761,22 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
                            int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* The same with two more choices.  keep_first > 0 together with a window: the sequence's first
+ * keep_first positions are seen as well, j < keep_first or j >= L - window (without a window all are).
+ * scale_blocks > 0: an 8-bit cache with scales [num_pages, Hkv, scale_blocks] as vk_hip_kv_cache_append_ex
+ * writes them, so that k_scale and v_scale above are those of position j's block. */
+size_t vk_hip_paged_attention_workspace_bytes_ex(int kind, int B, int Hkv, int G, int D, int max_len, int window,
+                                                 int keep_first, int counted);
+int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_table, const int32_t* seq_lens, const float* sinks,
+                              const float* k_scale, const float* v_scale, int scale_blocks, void* out, float* lse,
+                              float* weight_sums, int kind, int B, int Hkv, int G, int D, int num_pages,
+                              int page_size, int table_width, int table_stride, int max_len, int window,
+                              int keep_first, float scale, float softcap, int64_t q_stride_b, int64_t q_stride_h,
+                              int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                              int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* Eviction: a sequence of more than `budget` positions (its length cut to max_len) keeps
  * its first keep_first and last keep_last positions and of the others the
  * budget - keep_first - keep_last with the largest weight_sums, in every key/value head by

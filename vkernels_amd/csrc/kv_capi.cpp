@@ -122,6 +122,57 @@ int append(const char* who, const void* k, const void* v, void* k_cache, void* v
   return launched(who, before);
 }
 
+// Attention of one new token of every sequence.
+int attend(const char* who, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+           const int32_t* seq_lens, const float* sinks, const float* k_scale, const float* v_scale, int scale_blocks,
+           void* out, float* lse, float* weight_sums, int kind, int B, int Hkv, int G, int D, int num_pages, int page_size,
+           int table_width, int table_stride, int max_len, int window, int keep_first, float scale, float softcap,
+           int64_t q_stride_b, int64_t q_stride_h, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+           int64_t sums_stride_b, int64_t sums_stride_h, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!known_kind(kind)) return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be one of VK_HIP_KV_*");
+  if (B < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B must not be negative");
+  if (B == 0) return VK_OK;
+  const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
+                                  table_width, table_stride, page_stride, head_stride, slot_stride);
+  if (why == nullptr && G <= 0) why = "G must be positive";
+  if (why == nullptr && (q == nullptr || out == nullptr)) why = "q/out must not be null";
+  if (why == nullptr && (!aligned(q, 16) || !aligned(out, 16) || q_stride_b % 8 != 0 || q_stride_h % 8 != 0))
+    why = "rows of q and out must start on 16 bytes";
+  if (why == nullptr && (max_len < 0 || max_len > (int64_t)table_width * page_size))
+    why = "max_len must be within the table's positions";
+  if (why == nullptr && weight_sums != nullptr && broadcast_sums(B, Hkv, sums_stride_b, sums_stride_h))
+    why = "weight_sums must not be broadcast";
+  if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
+  if (why == nullptr && keep_first < 0) why = "keep_first must not be negative";
+  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
+  if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
+  // (units of work are counted in 32 bits, and so are a launch's threads, 256 for each item or chunk)
+  const int64_t rows = (int64_t)B * Hkv, items = rows * ((G + vk::kPaHeads - 1) / vk::kPaHeads);
+  if (max_len > kPositions || rows > kInt32 / G || items > kThreads / 512 || items > kInt32 / (max_len / vk::kPaUnit + 3) / 2 ||
+      rows > kThreads / 512 / (max_len / 4096 + 2))
+    return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, heads and positions for one call");
+  const vk::PagedAttentionPlan plan = vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, keep_first, weight_sums != nullptr);
+  if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
+    return refuse(VK_ERROR_INVALID_ARGUMENT, who,
+                  "a workspace of vk_hip_paged_attention_workspace_bytes (16-byte aligned) is needed");
+  vk::PagedAttentionArgs a{};
+  a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
+  a.sinks = sinks; a.k_scale = k_scale; a.v_scale = v_scale; a.out = out; a.lse = lse; a.sums = weight_sums;
+  a.workspace = workspace;
+  a.q_stride_b = q_stride_b; a.q_stride_h = q_stride_h;
+  a.page_stride = page_stride; a.head_stride = head_stride; a.slot_stride = slot_stride;
+  a.sums_stride_b = sums_stride_b; a.sums_stride_h = sums_stride_h;
+  a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
+  a.B = B; a.Hkv = Hkv; a.G = G; a.D = D; a.max_len = max_len; a.window = window;
+  a.keep_first = window > 0 ? keep_first : 0; a.scale_blocks = scale_blocks;
+  // (Caps that no score comes near, infinity among them, are none, and below the other bound all scores are alike:
+  // the kernel's factors 1 / cap and cap then stay within 32-bit floats.)
+  a.scale = scale; a.softcap = softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f;
+  const hipError_t before = hipPeekAtLastError();
+  vk::launch_paged_attention(a, kind, static_cast<hipStream_t>(stream));
+  return launched(who, before);
+}
+
 }  // namespace
 
 extern "C" {
@@ -190,8 +241,13 @@ int vk_hip_kv_cache_read(const void* k_cache, const void* v_cache, const int32_t
 
 size_t vk_hip_paged_attention_workspace_bytes(int kind, int B, int Hkv, int G, int D, int max_len, int window,
                                               int counted) {
-  if (!known_kind(kind) || B <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0) return 0;
-  return vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, counted != 0).bytes;
+  return vk_hip_paged_attention_workspace_bytes_ex(kind, B, Hkv, G, D, max_len, window, 0, counted);
+}
+
+size_t vk_hip_paged_attention_workspace_bytes_ex(int kind, int B, int Hkv, int G, int D, int max_len, int window,
+                                                 int keep_first, int counted) {
+  if (!known_kind(kind) || B <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0 || keep_first < 0) return 0;
+  return vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, keep_first, counted != 0).bytes;
 }
 
 int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cache,
@@ -203,47 +259,25 @@ int vk_hip_paged_attention(const void* q, const void* k_cache, const void* v_cac
                            int64_t page_stride, int64_t head_stride, int64_t slot_stride,
                            int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
                            size_t workspace_bytes, void* stream) {
-  const char* const who = "vk_hip_paged_attention";
-  if (!known_kind(kind)) return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be one of VK_HIP_KV_*");
-  if (B < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B must not be negative");
-  if (B == 0) return VK_OK;
-  const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
-                                  table_width, table_stride, page_stride, head_stride, slot_stride);
-  if (why == nullptr && G <= 0) why = "G must be positive";
-  if (why == nullptr && (q == nullptr || out == nullptr)) why = "q/out must not be null";
-  if (why == nullptr && (!aligned(q, 16) || !aligned(out, 16) || q_stride_b % 8 != 0 || q_stride_h % 8 != 0))
-    why = "rows of q and out must start on 16 bytes";
-  if (why == nullptr && (max_len < 0 || max_len > (int64_t)table_width * page_size))
-    why = "max_len must be within the table's positions";
-  if (why == nullptr && weight_sums != nullptr && broadcast_sums(B, Hkv, sums_stride_b, sums_stride_h))
-    why = "weight_sums must not be broadcast";
-  if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
-  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, 0, page_size);
-  if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  // (units of work are counted in 32 bits, and so are a launch's threads, 256 for each item or chunk)
-  const int64_t rows = (int64_t)B * Hkv, items = rows * ((G + vk::kPaHeads - 1) / vk::kPaHeads);
-  if (max_len > kPositions || rows > kInt32 / G || items > kThreads / 512 || items > kInt32 / (max_len / vk::kPaUnit + 3) / 2 ||
-      rows > kThreads / 512 / (max_len / 4096 + 2))
-    return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, heads and positions for one call");
-  const vk::PagedAttentionPlan plan = vk::paged_attention_plan(kind, B, Hkv, G, D, max_len, window, weight_sums != nullptr);
-  if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
-    return refuse(VK_ERROR_INVALID_ARGUMENT, who,
-                  "a workspace of vk_hip_paged_attention_workspace_bytes (16-byte aligned) is needed");
-  vk::PagedAttentionArgs a{};
-  a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens;
-  a.sinks = sinks; a.k_scale = k_scale; a.v_scale = v_scale; a.out = out; a.lse = lse; a.sums = weight_sums;
-  a.workspace = workspace;
-  a.q_stride_b = q_stride_b; a.q_stride_h = q_stride_h;
-  a.page_stride = page_stride; a.head_stride = head_stride; a.slot_stride = slot_stride;
-  a.sums_stride_b = sums_stride_b; a.sums_stride_h = sums_stride_h;
-  a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
-  a.B = B; a.Hkv = Hkv; a.G = G; a.D = D; a.max_len = max_len; a.window = window;
-  // (Caps that no score comes near, infinity among them, are none, and below the other bound all scores are alike:
-  // the kernel's factors 1 / cap and cap then stay within 32-bit floats.)
-  a.scale = scale; a.softcap = softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f;
-  const hipError_t before = hipPeekAtLastError();
-  vk::launch_paged_attention(a, kind, static_cast<hipStream_t>(stream));
-  return launched(who, before);
+  return attend("vk_hip_paged_attention", q, k_cache, v_cache, block_table, seq_lens, sinks, k_scale, v_scale, 0, out, lse,
+                weight_sums, kind, B, Hkv, G, D, num_pages, page_size, table_width, table_stride, max_len, window, 0, scale,
+                softcap, q_stride_b, q_stride_h, page_stride, head_stride, slot_stride, sums_stride_b, sums_stride_h,
+                workspace, workspace_bytes, stream);
+}
+
+int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_cache,
+                              const int32_t* block_table, const int32_t* seq_lens, const float* sinks,
+                              const float* k_scale, const float* v_scale, int scale_blocks, void* out, float* lse,
+                              float* weight_sums, int kind, int B, int Hkv, int G, int D, int num_pages,
+                              int page_size, int table_width, int table_stride, int max_len, int window,
+                              int keep_first, float scale, float softcap, int64_t q_stride_b, int64_t q_stride_h,
+                              int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                              int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return attend("vk_hip_paged_attention_ex", q, k_cache, v_cache, block_table, seq_lens, sinks, k_scale, v_scale, scale_blocks,
+                out, lse, weight_sums, kind, B, Hkv, G, D, num_pages, page_size, table_width, table_stride, max_len, window,
+                keep_first, scale, softcap, q_stride_b, q_stride_h, page_stride, head_stride, slot_stride, sums_stride_b,
+                sums_stride_h, workspace, workspace_bytes, stream);
 }
 
 size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget) {

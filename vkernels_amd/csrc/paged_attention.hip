@@ -108,18 +108,26 @@ __device__ __forceinline__ float or_zero(float m) { return m == kNegInf ? 0.0f :
 typedef const __attribute__((address_space(4))) int32_t* ConstInts;
 __device__ __forceinline__ ConstInts read_only(const int32_t* p) { return (ConstInts)(uintptr_t)p; }
 
-// What a work item (16 heads of one sequence) sees of its cache.
+// What a work item (16 heads of one sequence) sees of its cache: positions [lo, len) and, in front of a window,
+// [0, first).  It walks along a line of `walk` places, the first `split` of them the positions at the beginning,
+// the others positions `shift` further on (where the two parts meet or nearly do, all positions are
+// walked, those between hidden).
 struct Span {
-  int start;   // first position, rounded down to 16
-  int lo, len; // positions [lo, len)
-  int units;   // of kPaUnit positions from `start`; at least one
+  int lo, len, first;
+  int split, shift, walk;
+  int units;   // of kPaUnit places; at least one
+  __device__ __forceinline__ int position(int place) const { return place < split ? place : place + shift; }
 };
-__device__ __forceinline__ Span span_of(int len, int max_len, int window) {
+__device__ __forceinline__ Span span_of(int len, const PagedAttentionArgs& a) {
   Span s;
-  s.len = min(max(len, 0), max_len);
-  s.lo = window > 0 ? max(0, s.len - window) : 0;
-  s.start = s.lo & ~15;
-  s.units = max(1, (s.len - s.start + kPaUnit - 1) / kPaUnit);
+  s.len = min(max(len, 0), a.max_len);
+  s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
+  s.first = min(a.keep_first, s.lo);
+  s.split = (s.first + kPaUnit - 1) & ~(kPaUnit - 1);   // a whole number of units
+  s.shift = (s.lo & ~15) - s.split;
+  if (s.shift <= 0 && s.first > 0) s.split = s.shift = 0;
+  s.walk = s.len - s.shift;
+  s.units = max(1, (s.walk + kPaUnit - 1) / kPaUnit);
   return s;
 }
 
@@ -131,13 +139,18 @@ struct KernelArgs {
   PagedAttentionArgs a;
   PagedAttentionPlan p;
   FastDiv by_page;       // position / page_size
+  FastDiv by_block;      // slot of a page / positions with one scale
 };
 
 __device__ __forceinline__ int page_of(const KernelArgs& A, int pos) { return divided(pos, A.by_page); }
 
-// Positions from a span's start to its end, at most.  (Any window may be asked for: nothing is added to one
-// that reaches beyond max_len.)
-int most_seen(int max_len, int window) { return window > 0 && window < max_len - 16 ? window + 16 : max_len; }
+// Places of a span, at most.  (Any window may be asked for: nothing is added in 32 bits to one that reaches
+// beyond max_len.)
+int most_seen(int max_len, int window, int keep_first) {
+  if (window <= 0) return max_len;
+  const int64_t split = ((int64_t)std::min(keep_first, max_len) + kPaUnit - 1) / kPaUnit * kPaUnit;
+  return (int)std::min<int64_t>(max_len, (int64_t)window + 16 + split);
+}
 
 // The units of all items in order (sequence, head item, unit), cut into equal shares.
 struct Share {
@@ -174,7 +187,7 @@ __device__ __forceinline__ bool find_share(const KernelArgs& A, Share* sh) {
   int mine = 0;
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
-    if (b < a.B) mine += span_of(a.lens[b], a.max_len, a.window).units;
+    if (b < a.B) mine += span_of(a.lens[b], a).units;
   }
   const int scan = lanes_up_to(mine);
   const int total = __builtin_amdgcn_readlane(scan, 63) * heads;
@@ -185,7 +198,7 @@ __device__ __forceinline__ bool find_share(const KernelArgs& A, Share* sh) {
   const bool here = first >= at && first < at + mine * heads;
   if (here && per > 1) {
     for (;; ++b) {
-      const int units = span_of(a.lens[b], a.max_len, a.window).units * heads;
+      const int units = span_of(a.lens[b], a).units * heads;
       if (first < at + units) break;
       at += units;
     }
@@ -230,12 +243,18 @@ struct Tile {
 // page, first tile and the way out.  Registers: with fewer than 256 a lane (three workgroups a
 // CU) a 128-wide head spills (131 us where two take 97), a 64-wide one gains nothing.
 // FULL: D is DP.  P16: pages are multiples of 16 positions, so that a page is the same for 16 rows.
-template <class M, bool FP8, int DP, bool P16, bool FULL>
+// SCALES: an 8-bit cache's blocks of positions have scales of their own.  A lane loads the scale of one
+// position's keys or values with the tile; scores are multiplied by the keys', the weights by the values'
+// before they become 16-bit terms (in bf16 whatever the queries' type: codes are exact in it, and a weight
+// times a scale needs its range).
+template <class M, bool FP8, int DP, bool P16, bool FULL, bool SCALES>
 __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(const KernelArgs A) {
   typedef Tile<M, FP8, DP> L;
   typedef typename M::V8 V8;
+  typedef std::conditional_t<SCALES, Bf16, M> W;      // what weights and values are multiplied in
   const PagedAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[kPaWaves * L::kWaveLds];
+  __shared__ __attribute__((aligned(16))) float scale_lds[SCALES ? kPaWaves : 1][2 * kPaWaveRows];
   __shared__ float wave_m[kPaWaves][kPaHeads], wave_l[kPaWaves][kPaHeads];
 
   const int lane = threadIdx.x & 63;
@@ -258,7 +277,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     item_in_b = blockIdx.x % item_heads;
   }
   const ConstInts lens = read_only(a.lens);
-  Span span = span_of(lens[sh.b], a.max_len, a.window);
+  Span span = span_of(lens[sh.b], a);
   int unit_at;         // unit of the item that the segment begins with
   int left;            // units of the share that are left
   if (A.p.workgroups > 0) {
@@ -305,7 +324,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         q[i] = as_v8<M>(col < heads && d < a.D ? x : u32x4{0, 0, 0, 0});
       }
     }
-    const float k_scale = a.k_scale != nullptr ? a.k_scale[g] : 1.0f;
+    const float k_scale = !SCALES && a.k_scale != nullptr ? a.k_scale[g] : 1.0f;
     const float to_log2 = a.scale * k_scale * kLog2e;
     const float cap_in = a.softcap > 0.0f ? 2.0f * a.scale * k_scale * kLog2e / a.softcap : 0.0f;
     const float cap_out = a.softcap * kLog2e;
@@ -316,8 +335,8 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     float m = kNegInf, l = 0.0f;
 
     u32x4 kreg[2][L::kKLoads], vreg[L::kVLoads];
-    const int begin = span.start + unit_at * kPaUnit + wave * kPaWaveRows;
-    const int end = min(span.start + (unit_at + units) * kPaUnit, span.len);   // no tile is wholly behind it
+    const int begin = unit_at * kPaUnit + wave * kPaWaveRows;        // places
+    const int end = min((unit_at + units) * kPaUnit, span.walk);   // no tile is wholly behind it
 
     // The table's entries of a tile, asked for a tile ahead of the loads that need them (one for
     // each 16 positions where pages are multiples of 16 long, else one a lane: position lane % 32);
@@ -334,7 +353,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       } else {
         const int pos = pos0 + (lane & 31);
         const int id = (a.table + (int64_t)b * a.table_stride)[min(page_of(A, pos), last_entry)];
-        ids[0] = pos >= span.lo && pos < span.len ? id : -1;
+        ids[0] = (pos >= span.lo || pos < span.first) && pos < span.len ? id : -1;
       }
     };
     // Of the tile that is loaded: its pages (P16), or where the lane's position lies.
@@ -342,6 +361,14 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     int64_t half_at[2] = {0, 0};     // bytes from the cache's start to positions 0 and 16 of the tile
     int64_t row_at = 0;
     bool row_ok = false;
+    // The scale of position lane % 32 of the tile that is loaded: of its keys, or in the upper lanes of its values
+    // (1 where the position does not count: what is stored there may be anything).
+    float scale_of_row = 1.0f;
+    const float* const scales = lane < 32 ? a.k_scale : a.v_scale;
+    auto load_scale = [&](int page, int slot, bool there) {
+      const int64_t at = ((int64_t)page * a.Hkv + g) * a.scale_blocks + divided(slot, A.by_block);
+      scale_of_row = there ? scales[at] : 1.0f;
+    };
     auto take_pages = [&](int pos0) {
       if constexpr (P16) {
         page0 = (uint32_t)ids[0] < (uint32_t)a.num_pages ? ids[0] : -1;
@@ -352,10 +379,15 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
           half_at[t] = (int64_t)max(t == 0 ? page0 : page1, 0) * page_bytes +
                        (uint32_t)(pos - page_of(A, pos) * a.page_size) * (uint64_t)(uint32_t)slot_bytes;
         }
+        if constexpr (SCALES) {
+          const int half = lane & 16, pos = pos0 + half, page = half ? page1 : page0;
+          load_scale(page, pos - page_of(A, pos) * a.page_size + col, page >= 0 && pos + col < span.len);
+        }
       } else {
         const int pos = pos0 + (lane & 31);
         row_ok = (uint32_t)ids[0] < (uint32_t)a.num_pages;
         row_at = row_ok ? (int64_t)ids[0] * page_bytes + (int64_t)(pos - page_of(A, pos) * a.page_size) * slot_bytes : 0;
+        if constexpr (SCALES) load_scale(ids[0], pos - page_of(A, pos) * a.page_size, row_ok);
       }
     };
     // Where a row of the loaded tile lies (generic pages), from the lane that looked it up.
@@ -402,20 +434,22 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
 
     // One tile; with MORE behind it, the next one's keys are asked for as soon as this one's have
     // been multiplied, its values as soon as this one's are in LDS.
-    auto tile = [&](int pos0, auto more) {
+    auto tile = [&](int place, auto more) {
       constexpr bool MORE = decltype(more)::value;
+      const int pos0 = span.position(place);
+      if constexpr (SCALES) scale_lds[wave][lane] = scale_of_row;
       // which of the 8 positions of this lane count, and which value rows it loaded do
       bool whole;
       uint32_t rows;        // bit r: position pos0 + r counts
       if constexpr (P16) {
-        whole = pos0 >= span.lo && pos0 + 32 <= span.len && page0 >= 0 && page1 >= 0;
+        whole = (pos0 >= span.lo || pos0 + 32 <= span.first) && pos0 + 32 <= span.len && page0 >= 0 && page1 >= 0;
         rows = 0xFFFFFFFFu;
         if (!whole) {
           if (page0 < 0) rows &= 0xFFFF0000u;
           if (page1 < 0) rows &= 0x0000FFFFu;
-          const int n = span.len - pos0, skip = span.lo - pos0;
+          const int n = span.len - pos0, skip = span.lo - pos0, kept = span.first - pos0;
           if (n < 32) rows &= n <= 0 ? 0u : (1u << n) - 1u;
-          if (skip > 0) rows &= skip >= 32 ? 0u : ~0u << skip;
+          if (skip > 0) rows &= (skip >= 32 ? 0u : ~0u << skip) | (kept <= 0 ? 0u : kept >= 32 ? ~0u : (1u << kept) - 1u);
         }
       } else {
         rows = (uint32_t)__ballot(row_ok);
@@ -438,9 +472,9 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         }
       }
       if constexpr (MORE) {
-        take_pages(pos0 + kPaUnit);
+        take_pages(span.position(place + kPaUnit));
         load_k();
-        ask_pages(pos0 + 2 * kPaUnit);
+        ask_pages(span.position(place + 2 * kPaUnit));
       }
 
       // scores in powers of two
@@ -449,6 +483,18 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[t * 4 + r] = s[t][r];
+      f32x4 value_scale[2];
+      if constexpr (SCALES) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const f32x4 key_scale = *(const f32x4*)&scale_lds[wave][t * 16 + quad * 4];
+          value_scale[t] = *(const f32x4*)&scale_lds[wave][kPaWaveRows + t * 16 + quad * 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[t * 4 + r] *= key_scale[r];
+        }
+      }
       if (a.softcap > 0.0f) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -487,24 +533,25 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       // 2^-24, so that many positions far below one of large weight would be lost: there a tile's weights
       // are taken relative to its own maximum, as 2^15 of it, and what they sum to is brought to the
       // reference in 32 bits (131071 positions of 8 heads of 128: 94.3 us with and 94.2 without).
-      const float ref = M::kTileScale ? or_zero(top) - 15.0f : or_zero(m);
+      const float ref = W::kTileScale ? or_zero(top) - 15.0f : or_zero(m);
       const float to_ref = top == kNegInf ? 0.0f : exp2_fast(ref - m);
       float sum = 0.0f;
-      union { typename M::T e[8]; V8 v; } hi, lo;
+      union { typename W::T e[8]; typename W::V8 v; } hi, lo;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p = exp2_fast(x[i] - ref);
-        if constexpr (M::kTileScale) sum += p; else l += p;
-        hi.e[i] = (typename M::T)p;
-        lo.e[i] = (typename M::T)(p - (float)hi.e[i]);
+        float p = exp2_fast(x[i] - ref);
+        if constexpr (W::kTileScale) sum += p; else l += p;
+        if constexpr (SCALES) p *= value_scale[i / 4][i % 4];
+        hi.e[i] = (typename W::T)p;
+        lo.e[i] = (typename W::T)(p - (float)hi.e[i]);
       }
-      if constexpr (M::kTileScale) l += sum * to_ref;
-      auto add_values = [&](f32x4& sums, V8 v) {
-        if constexpr (M::kTileScale) {
-          sums += to_ref * M::mfma(v, lo.v, M::mfma(v, hi.v, f32x4{0, 0, 0, 0}));
+      if constexpr (W::kTileScale) l += sum * to_ref;
+      auto add_values = [&](f32x4& sums, typename W::V8 v) {
+        if constexpr (W::kTileScale) {
+          sums += to_ref * W::mfma(v, lo.v, W::mfma(v, hi.v, f32x4{0, 0, 0, 0}));
         } else {
-          sums = M::mfma(v, hi.v, sums);
-          sums = M::mfma(v, lo.v, sums);
+          sums = W::mfma(v, hi.v, sums);
+          sums = W::mfma(v, lo.v, sums);
         }
       };
 
@@ -559,7 +606,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) {
             if (i0 + i < DP / 16) {
-              add_values(acc[i0 + i], fp8x8<M>((uint32_t)c[i][0], (uint32_t)c[i][1]));
+              add_values(acc[i0 + i], fp8x8<W>((uint32_t)c[i][0], (uint32_t)c[i][1]));
             }
           }
         }
@@ -569,7 +616,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         const int at = row * L::kPitch + (col & 3) * 8;
 #pragma unroll
         for (int i0 = 0; i0 < DP / 16; i0 += kAhead) {
-          union { i16x4 h[2]; V8 v; } c[kAhead];
+          union { i16x4 h[2]; typename W::V8 v; } c[kAhead];
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) {
             if (i0 + i < DP / 16) {
@@ -591,14 +638,14 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
       __builtin_amdgcn_wave_barrier();
     };
     if (begin < end) {
-      ask_pages(begin);
-      take_pages(begin);
+      ask_pages(span.position(begin));
+      take_pages(span.position(begin));
       load_k();
-      ask_pages(begin + kPaUnit);
+      ask_pages(span.position(begin + kPaUnit));
       load_v();
-      int pos0 = begin;
-      for (; pos0 + kPaUnit < end; pos0 += kPaUnit) tile(pos0, std::true_type{});
-      tile(pos0, std::false_type{});
+      int place = begin;
+      for (; place + kPaUnit < end; place += kPaUnit) tile(place, std::true_type{});
+      tile(place, std::false_type{});
     }
 
     // The four wavefronts' sums, joined in LDS.
@@ -640,7 +687,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
         o += f * *(const f32x4*)((float*)(lds + w * L::kWaveLds) + h * L::kOutPitch + d);
       }
       if (alone) {
-        const float inv = (ll == 0.0f ? 0.0f : 1.0f / ll) * (a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
+        const float inv = (ll == 0.0f ? 0.0f : 1.0f / ll) * (!SCALES && a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
         typename M::T* to = (typename M::T*)a.out + ((int64_t)b * a.Hkv * a.G + hq) * a.D + d;
         union { typename M::T e[4]; u32x2 u; } r;
 #pragma unroll
@@ -664,7 +711,7 @@ __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(con
     if (left > 0 && ++item_in_b == item_heads) {
       item_in_b = 0;
       ++b;
-      span = span_of(lens[b], a.max_len, a.window);
+      span = span_of(lens[b], a);
     }
     if (left > 0) __syncthreads();   // (the sums are read before the next item's values come)
   }
@@ -757,7 +804,8 @@ __device__ __forceinline__ void join_heads(const KernelArgs& A, int padded, int 
   }
   if (!there) return;
   if (lane < lanes && d < a.D) {
-    const float inv = (st[1] == 0.0f ? 0.0f : 1.0f / st[1]) * (a.v_scale != nullptr ? a.v_scale[g] : 1.0f);
+    const float inv = (st[1] == 0.0f ? 0.0f : 1.0f / st[1]) *
+                      (a.v_scale != nullptr && a.scale_blocks == 0 ? a.v_scale[g] : 1.0f);
     union { typename M::T e[4]; u32x2 u; } r;
 #pragma unroll
     for (int j = 0; j < 4; ++j) r.e[j] = (typename M::T)(o[j] * inv);
@@ -778,21 +826,21 @@ __device__ __forceinline__ void add_weights(const KernelArgs& A, int block, int 
   const PagedAttentionArgs& a = A.a;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int bg = block / chunks, b = bg / a.Hkv, g = bg % a.Hkv, Hq = a.Hkv * a.G;
-  const Span span = span_of(read_only(a.lens)[b], a.max_len, a.window);
-  const int at = span.start + (block % chunks) * (1024 * PER);
-  if (at >= span.len) return;
+  const Span span = span_of(read_only(a.lens)[b], a);
+  const int at = (block % chunks) * (1024 * PER);       // places
+  if (at >= span.walk) return;
   const float* const scores = (const float*)((const char*)a.workspace + A.p.scores_at) +
                               (int64_t)bg * A.p.score_pitch * a.G;
   float* const to = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)g * a.sums_stride_h;
-  const int pos0 = at + threadIdx.x * 4;        // and 1024, 2048, 3072 behind it
+  const int place0 = at + threadIdx.x * 4;        // and 1024, 2048, 3072 behind it
   // (16 bytes at a time where the sums' rows allow it and all four positions are seen)
   const bool wide = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
-  auto all_seen = [&](int pos) { return wide && pos >= span.lo && pos + 3 < span.len; };
+  auto all_seen = [&](int pos) { return wide && (pos >= span.lo || pos + 3 < span.first) && pos + 3 < span.len; };
   float sum[PER][4];
   f32x4 old[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int pos = pos0 + 1024 * k;
+    const int pos = span.position(place0 + 1024 * k);
     old[k] = f32x4{0, 0, 0, 0};
     if (all_seen(pos)) old[k] = *(const f32x4*)(to + pos);
 #pragma unroll
@@ -803,7 +851,7 @@ __device__ __forceinline__ void add_weights(const KernelArgs& A, int block, int 
     f32x4 x[kSumHeads][PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int pos = min(pos0 + 1024 * k, (span.len - 1) & ~3);
+      const int pos = min(span.position(place0 + 1024 * k), (span.len - 1) & ~3);
 #pragma unroll
       for (int i = 0; i < kSumHeads; ++i)
         x[i][k] = *(const f32x4*)(scores + (int64_t)(pos & ~15) * a.G + (h0 + min(i, n - 1)) * 16 + (pos & 15));
@@ -835,13 +883,13 @@ __device__ __forceinline__ void add_weights(const KernelArgs& A, int block, int 
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int pos = pos0 + 1024 * k;
+    const int pos = span.position(place0 + 1024 * k);
     if (all_seen(pos)) {
       *(f32x4*)(to + pos) = old[k] + f32x4{sum[k][0], sum[k][1], sum[k][2], sum[k][3]};
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (pos + j >= span.lo && pos + j < span.len) to[pos + j] += sum[k][j];
+        if ((pos + j >= span.lo || pos + j < span.first) && pos + j < span.len) to[pos + j] += sum[k][j];
     }
   }
 }
@@ -862,7 +910,7 @@ void launch_join(const KernelArgs& A, int padded, hipStream_t stream) {
   const PagedAttentionArgs& a = A.a;
   const int heads = std::min(a.G, kPaHeads), groups = SPLIT > 1 ? heads : (heads + 3) / 4;
   const int join_blocks = A.p.workgroups > 0 ? (SPLIT > 1 ? A.p.items : A.p.workgroups) * groups : 0;
-  const int seen = a.sums == nullptr ? 0 : most_seen(a.max_len, a.window);
+  const int seen = a.sums == nullptr ? 0 : most_seen(a.max_len, a.window, a.keep_first);
   // (four times the positions a block where the card has blocks enough, for fewer latencies in a row)
   const bool many = (int64_t)a.B * a.Hkv * ((seen + 1023) / 1024) > 2048;
   const int chunks = many ? (seen + 4095) / 4096 : (seen + 1023) / 1024;
@@ -876,29 +924,29 @@ void launch_join(const KernelArgs& A, int padded, hipStream_t stream) {
                        join_blocks, chunks);
 }
 
-template <class M, bool FP8, int DP>
+template <class M, bool FP8, int DP, bool SCALES>
 void launch_width(const KernelArgs& A, hipStream_t stream) {
   const dim3 grid(A.p.workgroups > 0 ? A.p.workgroups : A.p.items), block(256);
   const bool aligned_pages = A.a.page_size % 16 == 0, full = A.a.D == DP;
   if (aligned_pages && full)
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, true>), grid, block, 0, stream, A);
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, true, SCALES>), grid, block, 0, stream, A);
   else if (aligned_pages)
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, false>), grid, block, 0, stream, A);
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, true, false, SCALES>), grid, block, 0, stream, A);
   else if (full)
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, true>), grid, block, 0, stream, A);
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, true, SCALES>), grid, block, 0, stream, A);
   else
-    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, false>), grid, block, 0, stream, A);
+    hipLaunchKernelGGL((paged_attention_kernel<M, FP8, DP, false, false, SCALES>), grid, block, 0, stream, A);
 }
 
-template <class M, bool FP8>
+template <class M, bool FP8, bool SCALES>
 void launch_kind(const KernelArgs& A, hipStream_t stream) {
   const int padded = pa_padded_width(A.a.D, FP8);
   switch (padded) {
-    case 64: launch_width<M, FP8, 64>(A, stream); break;
-    case 96: if constexpr (!FP8) launch_width<M, FP8, 96>(A, stream); break;
-    case 128: launch_width<M, FP8, 128>(A, stream); break;
-    case 192: launch_width<M, FP8, 192>(A, stream); break;
-    default: launch_width<M, FP8, 256>(A, stream); break;
+    case 64: launch_width<M, FP8, 64, SCALES>(A, stream); break;
+    case 96: if constexpr (!FP8) launch_width<M, FP8, 96, SCALES>(A, stream); break;
+    case 128: launch_width<M, FP8, 128, SCALES>(A, stream); break;
+    case 192: launch_width<M, FP8, 192, SCALES>(A, stream); break;
+    default: launch_width<M, FP8, 256, SCALES>(A, stream); break;
   }
   if (A.p.workgroups >= 16 * A.p.items)
     launch_join<M, 4>(A, padded, stream);
@@ -908,11 +956,12 @@ void launch_kind(const KernelArgs& A, hipStream_t stream) {
 
 }  // namespace
 
-PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window, bool counted) {
+PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window,
+                                        int keep_first, bool counted) {
   PagedAttentionPlan p{};
   p.head_tiles = (G + kPaHeads - 1) / kPaHeads;
   p.items = B * Hkv * p.head_tiles;
-  const int seen = most_seen(max_len, window);
+  const int seen = most_seen(max_len, window, keep_first);
   const int units = (seen + kPaUnit - 1) / kPaUnit;
   // Up to 8 units an item is one workgroup's and there is no second launch (64 heads on 8, 1000
   // positions: 1 sequence 10.0 us against 7.2 + 3.9, 8 sequences 11.0 / 8.6 + 4.0, 64 sequences
@@ -951,13 +1000,19 @@ PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, 
 void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t stream) {
   KernelArgs A{};
   A.a = a;
-  A.p = paged_attention_plan(kind, a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.sums != nullptr);
+  A.p = paged_attention_plan(kind, a.B, a.Hkv, a.G, a.D, a.max_len, a.window, a.keep_first, a.sums != nullptr);
   A.by_page = fast_div(a.page_size);
+  A.by_block = fast_div(a.scale_blocks > 0 ? a.page_size / a.scale_blocks : 1);
+  const bool scales = a.scale_blocks > 0;
   switch (kind) {
-    case kKvBf16: launch_kind<Bf16, false>(A, stream); break;
-    case kKvF16: launch_kind<F16, false>(A, stream); break;
-    case kKvFp8Bf16: launch_kind<Bf16, true>(A, stream); break;
-    default: launch_kind<F16, true>(A, stream); break;
+    case kKvBf16: launch_kind<Bf16, false, false>(A, stream); break;
+    case kKvF16: launch_kind<F16, false, false>(A, stream); break;
+    case kKvFp8Bf16:
+      if (scales) launch_kind<Bf16, true, true>(A, stream); else launch_kind<Bf16, true, false>(A, stream);
+      break;
+    default:
+      if (scales) launch_kind<F16, true, true>(A, stream); else launch_kind<F16, true, false>(A, stream);
+      break;
   }
 }
 

@@ -24,7 +24,7 @@ struct PagedAttentionArgs {
   const int32_t* table;     // [B, table_stride]: the page of every page_size positions
   const int32_t* lens;      // [B]
   const float* sinks;       // [Hkv * G] or null
-  const float* k_scale;     // [Hkv] or null
+  const float* k_scale;     // [Hkv] or null; with scale_blocks [pages, Hkv, scale_blocks]
   const float* v_scale;
   void* out;                // [B, Hkv * G, D]
   float* lse;               // [B, Hkv * G] or null
@@ -35,6 +35,8 @@ struct PagedAttentionArgs {
   int64_t sums_stride_b, sums_stride_h;                 // elements
   int table_stride, table_width, num_pages, page_size;
   int B, Hkv, G, D, max_len, window;
+  int keep_first;           // of a window: positions at the sequence's beginning that stay visible
+  int scale_blocks;         // blocks of a page that have a scale of their own (0: one for each head)
   float scale, softcap;
 };
 
@@ -50,7 +52,8 @@ struct PagedAttentionPlan {
   size_t ends_at, meta_at, stats_at, ml_at, part_at, scores_at, bytes;  // parts of the workspace
 };
 
-PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window, bool counted);
+PagedAttentionPlan paged_attention_plan(int kind, int B, int Hkv, int G, int D, int max_len, int window, int keep_first,
+                                        bool counted);
 void launch_paged_attention(const PagedAttentionArgs& a, int kind, hipStream_t stream);
 
 }  // namespace vk

@@ -49,6 +49,8 @@ def _fn(name):
             "vk_hip_kv_cache_append_ex": ([_P] * 9 + [_I] * 10 + [_L] * 7 + [_P], _I),
             "vk_hip_kv_cache_read": ([_P] * 7 + [_I] + [_P] * 2 + [_I] * 10 + [_L] * 7 + [_P], _I),
             "vk_hip_paged_attention_workspace_bytes": ([_I] * 8, _Z),
+            "vk_hip_paged_attention_workspace_bytes_ex": ([_I] * 9, _Z),
+            "vk_hip_paged_attention_ex": ([_P] * 8 + [_I] + [_P] * 3 + [_I] * 12 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
             "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 6, _Z),
             "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P, _Z, _P], _I),
@@ -267,13 +269,14 @@ def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, 
     return k, v
 
 
-def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, softcap=0.0,
-                    sinks=None, k_scale=None, v_scale=None, weight_sums=None, return_lse=False, out=None):
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, keep_first=0,
+                    softcap=0.0, sinks=None, k_scale=None, v_scale=None, weight_sums=None, return_lse=False, out=None):
     """Attention of one new token of every sequence, q [B, Hq, D], over its cached positions.
 
     Query heads G g .. G g + G - 1 read key/value head g (G = Hq / Hkv).  ``scale`` defaults to
-    D ** -0.5; ``window`` > 0 leaves the last so many positions; ``softcap`` c > 0 bounds the scores by
-    c tanh(s / c); ``sinks`` [Hq] float32 are scores whose value is zero.  ``max_len`` bounds every
+    D ** -0.5; ``window`` > 0 leaves the last so many positions and the first ``keep_first``; ``softcap`` c > 0
+    bounds the scores by c tanh(s / c); ``sinks`` [Hq] float32 are scores whose value is zero.  The scales of an
+    8-bit cache are [Hkv], or [pages, Hkv, blocks] as ``kv_cache_append`` has written them.  ``max_len`` bounds every
     length (default: what the table holds; a longer sequence is cut to it): the launch and its
     workspace follow it, so a tight bound is worth giving.  ``weight_sums`` [B, Hkv, positions]
     float32: every position's weights, summed over the heads of the group, are added to it; the call's
@@ -292,6 +295,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         max_len = W * ps
     if not 0 < window < max_len:      # (any other sees everything, however large it is)
         window = 0
+    if keep_first:
+        _need(keep_first > 0, "keep_first must not be negative")
+        keep_first = min(keep_first, max_len) if window else 0
     if not 0 <= max_len <= 0x7FFFFFFF:
         _int32(max_len=max_len)
     q, own_out = _rows(q), out is not None
@@ -306,20 +312,20 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         if not _sums_ok(weight_sums, B, Hkv, max_len, device):
             raise ValueError("weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
-    size = _bytes("vk_hip_paged_attention_workspace_bytes", kind, B, Hkv, G, D, max_len, window, sums is not None)
+    k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
+    size = _bytes("vk_hip_paged_attention_workspace_bytes_ex", kind, B, Hkv, G, D, max_len, window, keep_first,
+                  sums is not None)
     workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
     qs = q.stride()
-    status = _fn("vk_hip_paged_attention")(
+    status = _fn("vk_hip_paged_attention_ex")(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        None if sinks is None else _head_vector(sinks, Hq, "sinks", device),
-        None if k_scale is None else _head_vector(k_scale, Hkv, "k_scale", device),
-        None if v_scale is None else _head_vector(v_scale, Hkv, "v_scale", device),
+        None if sinks is None else _head_vector(sinks, Hq, "sinks", device), k_scale, v_scale, blocks,
         out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind, B, Hkv, G, D, pages, ps, W,
-        table_stride, max_len, window, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
+        table_stride, max_len, window, keep_first, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
         strides[0], strides[1], strides[2], sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size,
         _stream(device))
     if status:
-        _failed(status, "vk_hip_paged_attention")
+        _failed(status, "vk_hip_paged_attention_ex")
     if ((q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
          sinks is not None and sinks.requires_grad) and torch.is_grad_enabled() and not own_out):
         out, lse = _NoBackward.apply(out, lse, q, k_cache, v_cache, sinks)
