@@ -777,6 +777,26 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
                               int64_t sums_stride_b, int64_t sums_stride_h, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* Attention of several new tokens of every sequence over its cache, which holds them already: q, out
+ * [tokens, Hq, D], lse [tokens, Hq], the tokens of sequence b rows query_start[b] .. query_start[b + 1] - 1
+ * (query_start [B + 1] int32, from 0 on and not falling) and its last positions: with n of them and L as
+ * above, token i is at p = L - n + i and sees positions j <= p, with a window those with j > p - window or
+ * j < keep_first.  Scores, cap, sinks, scales, results and rows that see nothing as above; what is stored at a position
+ * that a token does not see has no part in its row, NaN and infinities included.  Weights enter the product with
+ * the values in 16 bits (bf16 with an 8-bit cache), rounded once.  Rows that belong to no sequence become 0 (lse
+ * -inf) with clear_rest != 0 and else stay as they are.  The workspace is scratch of this call alone; 0 bytes: none is
+ * needed.  Deterministic: no atomics on floating-point data. */
+size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,
+                                                     int keep_first);
+int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void* v_cache,
+                                  const int32_t* block_table, const int32_t* seq_lens, const int32_t* query_start,
+                                  const float* sinks, const float* k_scale, const float* v_scale, int scale_blocks,
+                                  void* out, float* lse, int kind, int B, int tokens, int Hkv, int G, int D,
+                                  int num_pages, int page_size, int table_width, int table_stride, int max_len,
+                                  int window, int keep_first, int clear_rest, float scale, float softcap,
+                                  int64_t q_stride_t, int64_t q_stride_h, int64_t page_stride, int64_t head_stride,
+                                  int64_t slot_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Eviction: a sequence of more than `budget` positions (its length cut to max_len) keeps
  * its first keep_first and last keep_last positions and of the others the
  * budget - keep_first - keep_last with the largest weight_sums, in every key/value head by

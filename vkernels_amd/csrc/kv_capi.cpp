@@ -12,6 +12,7 @@
 #include "kv_blocks.hpp"
 #include "kv_cache.hpp"
 #include "paged_attention.hpp"
+#include "prompt_attention.hpp"
 #include "qk_norm_rope.hpp"
 
 namespace {
@@ -122,6 +123,17 @@ int append(const char* who, const void* k, const void* v, void* k_cache, void* v
   return launched(who, before);
 }
 
+// Caps that no score comes near, infinity among them, are none, and below the other bound all scores are alike:
+// the kernels' factors 1 / cap and cap then stay within 32-bit floats.
+float cap_of(float softcap) { return softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f; }
+
+// Rows and slots are counted in 32 bits, and so are a launch's threads (with up to 1024 workgroups more, or 32 for a
+// tile's join).
+bool prompt_fits(int B, int tokens, int Hkv, int G) {
+  if (tokens > kInt32 / 4 / G || B > kInt32 / 4) return false;
+  return vk::prompt_attention_slots(B, tokens, G) <= kThreads / 256 / 64 / Hkv;
+}
+
 // Attention of one new token of every sequence.
 int attend(const char* who, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
            const int32_t* seq_lens, const float* sinks, const float* k_scale, const float* v_scale, int scale_blocks,
@@ -165,9 +177,7 @@ int attend(const char* who, const void* q, const void* k_cache, const void* v_ca
   a.table_stride = table_stride; a.table_width = table_width; a.num_pages = num_pages; a.page_size = page_size;
   a.B = B; a.Hkv = Hkv; a.G = G; a.D = D; a.max_len = max_len; a.window = window;
   a.keep_first = window > 0 ? keep_first : 0; a.scale_blocks = scale_blocks;
-  // (Caps that no score comes near, infinity among them, are none, and below the other bound all scores are alike:
-  // the kernel's factors 1 / cap and cap then stay within 32-bit floats.)
-  a.scale = scale; a.softcap = softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f;
+  a.scale = scale; a.softcap = cap_of(softcap);
   const hipError_t before = hipPeekAtLastError();
   vk::launch_paged_attention(a, kind, static_cast<hipStream_t>(stream));
   return launched(who, before);
@@ -278,6 +288,58 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
                 out, lse, weight_sums, kind, B, Hkv, G, D, num_pages, page_size, table_width, table_stride, max_len, window,
                 keep_first, scale, softcap, q_stride_b, q_stride_h, page_stride, head_stride, slot_stride, sums_stride_b,
                 sums_stride_h, workspace, workspace_bytes, stream);
+}
+
+size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,
+                                                     int keep_first) {
+  if (B <= 0 || tokens <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0 || keep_first < 0) return 0;
+  if (!prompt_fits(B, tokens, Hkv, G)) return 0;
+  return vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, window > 0 ? keep_first : 0).bytes;
+}
+
+int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void* v_cache,
+                                  const int32_t* block_table, const int32_t* seq_lens, const int32_t* query_start,
+                                  const float* sinks, const float* k_scale, const float* v_scale, int scale_blocks,
+                                  void* out, float* lse, int kind, int B, int tokens, int Hkv, int G, int D,
+                                  int num_pages, int page_size, int table_width, int table_stride, int max_len,
+                                  int window, int keep_first, int clear_rest, float scale, float softcap,
+                                  int64_t q_stride_t, int64_t q_stride_h, int64_t page_stride, int64_t head_stride,
+                                  int64_t slot_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* const who = "vk_hip_paged_attention_prompt";
+  if (!known_kind(kind)) return refuse(VK_ERROR_UNSUPPORTED, who, "kind must be one of VK_HIP_KV_*");
+  if (B < 0 || tokens < 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "B and tokens must not be negative");
+  if (tokens == 0) return VK_OK;
+  if (B == 0) return refuse(VK_ERROR_INVALID_ARGUMENT, who, "tokens need a sequence");
+  const char* why = cache_refusal(k_cache, v_cache, block_table, seq_lens, elem_of(kind), Hkv, D, num_pages, page_size,
+                                  table_width, table_stride, page_stride, head_stride, slot_stride);
+  if (why == nullptr && G <= 0) why = "G must be positive";
+  if (why == nullptr && (q == nullptr || out == nullptr || query_start == nullptr)) why = "q/out/query_start must not be null";
+  if (why == nullptr && (!aligned(q, 16) || !aligned(out, 16) || q_stride_t % 8 != 0 || q_stride_h % 8 != 0))
+    why = "rows of q and out must start on 16 bytes";
+  if (why == nullptr && (max_len < 0 || max_len > (int64_t)table_width * page_size))
+    why = "max_len must be within the table's positions";
+  if (why == nullptr && keep_first < 0) why = "keep_first must not be negative";
+  if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
+  if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
+  if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
+  if (max_len > kPositions || !prompt_fits(B, tokens, Hkv, G))
+    return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, tokens, heads and positions for one call");
+  keep_first = window > 0 ? keep_first : 0;
+  const vk::PromptAttentionPlan plan = vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, keep_first);
+  if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
+    return refuse(VK_ERROR_INVALID_ARGUMENT, who,
+                  "a workspace of vk_hip_paged_attention_prompt_workspace_bytes (16-byte aligned) is needed");
+  vk::PromptAttentionArgs a{};
+  a.q = q; a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens; a.starts = query_start;
+  a.sinks = sinks; a.k_scale = k_scale; a.v_scale = v_scale; a.out = out; a.lse = lse; a.workspace = workspace;
+  a.q_stride_t = q_stride_t; a.q_stride_h = q_stride_h;
+  a.page_stride = page_stride; a.head_stride = head_stride; a.slot_stride = slot_stride;
+  a.table_stride = table_stride; a.num_pages = num_pages; a.page_size = page_size; a.scale_blocks = scale_blocks;
+  a.B = B; a.tokens = tokens; a.Hkv = Hkv; a.G = G; a.D = D; a.max_len = max_len; a.window = window; a.keep_first = keep_first;
+  a.scale = scale; a.softcap = cap_of(softcap); a.clear_rest = clear_rest != 0;
+  const hipError_t before = hipPeekAtLastError();
+  vk::launch_prompt_attention(a, kind, static_cast<hipStream_t>(stream));
+  return launched(who, before);
 }
 
 size_t vk_hip_kv_cache_evict_workspace_bytes(int elem_bytes, int B, int Hkv, int D, int max_len, int budget) {

@@ -52,6 +52,8 @@ def _fn(name):
             "vk_hip_paged_attention_workspace_bytes_ex": ([_I] * 9, _Z),
             "vk_hip_paged_attention_ex": ([_P] * 8 + [_I] + [_P] * 3 + [_I] * 12 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
             "vk_hip_paged_attention": ([_P] * 11 + [_I] * 11 + [_F, _F] + [_L] * 7 + [_P, _Z, _P], _I),
+            "vk_hip_paged_attention_prompt_workspace_bytes": ([_I] * 8, _Z),
+            "vk_hip_paged_attention_prompt": ([_P] * 9 + [_I] + [_P] * 2 + [_I] * 14 + [_F, _F] + [_L] * 5 + [_P, _Z, _P], _I),
             "vk_hip_kv_cache_evict_workspace_bytes": ([_I] * 6, _Z),
             "vk_hip_kv_cache_evict": ([_P] * 8 + [_I] * 12 + [_L] * 7 + [_P, _Z, _P], _I),
         }[name]
@@ -269,9 +271,9 @@ def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, 
     return k, v
 
 
-def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None, scale=None, window=0, keep_first=0,
-                    softcap=0.0, sinks=None, k_scale=None, v_scale=None, weight_sums=None, return_lse=False, out=None):
-    """Attention of one new token of every sequence, q [B, Hq, D], over its cached positions.
+def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=None, max_len=None, scale=None, window=0,
+                    keep_first=0, softcap=0.0, sinks=None, k_scale=None, v_scale=None, weight_sums=None, return_lse=False, out=None):
+    """Attention of one new token of every sequence, q [B, Hq, D], over its cached positions, or of several.
 
     Query heads G g .. G g + G - 1 read key/value head g (G = Hq / Hkv).  ``scale`` defaults to
     D ** -0.5; ``window`` > 0 leaves the last so many positions and the first ``keep_first``; ``softcap`` c > 0
@@ -282,12 +284,20 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
     float32: every position's weights, summed over the heads of the group, are added to it; the call's
     scratch is then 4 B Hq max_len bytes, whatever the lengths are.
     Returns out [B, Hq, D], or (out, lse [B, Hq] float32).  A row that nothing is left of is 0, its
-    lse -inf (its sink, where there is one)."""
+    lse -inf (its sink, where there is one).
+
+    With ``query_start`` [B + 1] int32 q is [tokens, Hq, D], rows query_start[b] .. query_start[b + 1] - 1 the last
+    tokens of sequence b, whose keys and values are in the cache already (``kv_cache_append`` takes them by the
+    same query_start): each sees the positions up to its own, the window and ``keep_first`` counted from
+    there.  Rows that belong to no sequence are 0 with an lse of -inf, and left as they are in ``out``.
+    There are no ``weight_sums`` then."""
     (pages, Hkv, ps, D), strides, device, (B, W), table_stride = _cache(k_cache, v_cache, block_table, seq_lens)
     Hq = q.shape[1] if q.dim() == 3 else 0
     G = Hq // Hkv
-    if not (q.shape == (B, G * Hkv, D) and 0 < G <= 0x7FFFFFFF and q.get_device() == device):
-        raise ValueError("q must be [B, Hq, D] on the cache's device with Hq a multiple of the cache's heads")
+    rows = B if query_start is None else q.shape[0]
+    if not (q.shape == (rows, G * Hkv, D) and 0 < G <= 0x7FFFFFFF and rows <= 0x7FFFFFFF and q.get_device() == device):
+        raise ValueError("q must be [B, Hq, D] (with query_start [tokens, Hq, D]) on the cache's device with Hq a "
+                         "multiple of the cache's heads")
     kind = _KINDS.get((k_cache.dtype, q.dtype))
     if kind is None:
         raise ValueError("the cache's type does not take queries of this type")
@@ -302,30 +312,43 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, max_len=None,
         _int32(max_len=max_len)
     q, own_out = _rows(q), out is not None
     if out is None:
-        out = q.new_empty((B, Hq, D))
+        out = q.new_empty((rows, Hq, D))
     else:
         _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and out.get_device() == device,
               "out must be contiguous and like q")
-    lse = q.new_empty((B, Hq), dtype=torch.float32) if return_lse else None
+    lse = q.new_empty((rows, Hq), dtype=torch.float32) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
         if not _sums_ok(weight_sums, B, Hkv, max_len, device):
             raise ValueError("weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
     k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
-    size = _bytes("vk_hip_paged_attention_workspace_bytes_ex", kind, B, Hkv, G, D, max_len, window, keep_first,
-                  sums is not None)
-    workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
-    qs = q.stride()
-    status = _fn("vk_hip_paged_attention_ex")(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        None if sinks is None else _head_vector(sinks, Hq, "sinks", device), k_scale, v_scale, blocks,
-        out.data_ptr(), None if lse is None else lse.data_ptr(), sums, kind, B, Hkv, G, D, pages, ps, W,
-        table_stride, max_len, window, keep_first, D ** -0.5 if scale is None else scale, softcap, qs[0], qs[1],
-        strides[0], strides[1], strides[2], sums_b, sums_h, None if workspace is None else workspace.data_ptr(), size,
-        _stream(device))
+    sink_at = None if sinks is None else _head_vector(sinks, Hq, "sinks", device)
+    lse_at = None if lse is None else lse.data_ptr()
+    qs, scale = q.stride(), D ** -0.5 if scale is None else scale
+    if query_start is None:
+        size = _bytes("vk_hip_paged_attention_workspace_bytes_ex", kind, B, Hkv, G, D, max_len, window, keep_first,
+                      sums is not None)
+        workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
+        name, status = "vk_hip_paged_attention_ex", _fn("vk_hip_paged_attention_ex")(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), sink_at,
+            k_scale, v_scale, blocks, out.data_ptr(), lse_at, sums, kind, B, Hkv, G, D, pages, ps, W, table_stride,
+            max_len, window, keep_first, scale, softcap, qs[0], qs[1], strides[0], strides[1], strides[2], sums_b,
+            sums_h, None if workspace is None else workspace.data_ptr(), size, _stream(device))
+    else:
+        _need(sums is None, "there are no weight_sums with query_start")
+        if lse is not None and own_out:
+            lse.fill_(float("-inf"))
+        size = _bytes("vk_hip_paged_attention_prompt_workspace_bytes", B, rows, Hkv, G, D, max_len, window, keep_first)
+        workspace = q.new_empty((size,), dtype=torch.uint8) if size else None
+        name, status = "vk_hip_paged_attention_prompt", _fn("vk_hip_paged_attention_prompt")(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            _query_start(query_start, B, device), sink_at, k_scale, v_scale, blocks, out.data_ptr(), lse_at, kind, B, rows,
+            Hkv, G, D, pages, ps, W, table_stride, max_len, window, keep_first, not own_out, scale, softcap, qs[0],
+            qs[1], strides[0], strides[1], strides[2], None if workspace is None else workspace.data_ptr(), size,
+            _stream(device))
     if status:
-        _failed(status, "vk_hip_paged_attention_ex")
+        _failed(status, name)
     if ((q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
          sinks is not None and sinks.requires_grad) and torch.is_grad_enabled() and not own_out):
         out, lse = _NoBackward.apply(out, lse, q, k_cache, v_cache, sinks)
