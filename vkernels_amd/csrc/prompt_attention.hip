@@ -112,6 +112,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const PromptAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[L::kLds];
   __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? 2 : 1][kWaves][2][kPromptKeys];
+  __shared__ int64_t row_lds[kWaves][kPromptKeys];
   __shared__ uint32_t any_bad;      // values that are no finite numbers have been left out
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
@@ -205,22 +206,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   float ks = 1.0f, vs = 1.0f;
   uint64_t loaded = 0;         // which positions of the loaded tile there are
   auto fetch = [&](int tile, int ids) {
-    const int pos0 = walk.position(tile * kPromptKeys);
+    // A lane works out where its position's rows lie, for the wavefront's lanes that load them.
+    const int pos = walk.position(tile * kPromptKeys) + lane, slot = pos - divided(pos, A.by_page) * a.page_size;
     loaded = __ballot(ids >= 0);
-#pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) {
-      const int r = piece_row + i * L::kPass, pos = pos0 + r;
-      const int id = max(__shfl(ids, r), 0);
-      const int64_t at = (int64_t)id * page_bytes + (int64_t)(pos - divided(pos, A.by_page) * a.page_size) * slot_bytes + piece_at;
-      kreg[i] = *(const Piece*)(kbase + at);
-      vreg[i] = *(const Piece*)(vbase + at);
-    }
+    row_lds[wave][lane] = max(ids, 0) * page_bytes + (uint32_t)slot * (uint64_t)(uint32_t)slot_bytes;
     if constexpr (FP8) {
-      const int pos = pos0 + lane, slot = pos - divided(pos, A.by_page) * a.page_size;
       const int64_t at = a.scale_blocks == 0 ? t.head
                                              : ((int64_t)max(ids, 0) * a.Hkv + t.head) * a.scale_blocks + divided(slot, A.by_block);
       ks = ids >= 0 ? a.k_scale[at] * a.scale : 0.0f;
       vs = ids >= 0 ? a.v_scale[at] : 0.0f;
+    }
+    // (lanes read what other lanes of their wavefront wrote: LDS keeps the order, and so must the compiler)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    int64_t at[L::kLoads];
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) at[i] = row_lds[wave][piece_row + i * L::kPass] + piece_at;
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) {
+      kreg[i] = *(const Piece*)(kbase + at[i]);
+      vreg[i] = *(const Piece*)(vbase + at[i]);
     }
   };
   // Does any row of the workgroup not see all of a tile?
@@ -250,15 +255,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       }
       if (!((loaded >> r) & 1)) v = u32x4{0, 0, 0, 0};
       if (look) {
-        bool bad = false;
+        // (an exponent of ones carries into the half's sign)
+        constexpr uint32_t kExponents = std::is_same_v<W, F16> ? 0x7C007C00u : 0x7F807F80u;
+        constexpr uint32_t kOnes = std::is_same_v<W, F16> ? 0x04000400u : 0x00800080u;
+        uint32_t all = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (!finite<W>(e & 1 ? v[e / 2] >> 16 : v[e / 2])) {
-            bad = true;
-            v[e / 2] &= e & 1 ? 0xFFFFu : 0xFFFF0000u;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
+          v[e] &= ~((bad >> 15) * 0xFFFFu);
+          all |= bad;
         }
-        if (bad && has_piece) any_bad = 1;
+        if (all != 0 && has_piece) any_bad = 1;
       }
       if (has_piece) {
         *(u32x4*)(to + r * L::kKeyPitch + piece * 16) = k;
@@ -339,15 +346,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         }
         const bool whole = these == ~0ull && pos0 + kPromptKeys - 1 <= wave_lo &&
                            (a.window <= 0 || pos0 > low_of(wave_hi) || pos0 + kPromptKeys <= a.keep_first);
-        uint32_t hidden = 0;
+        uint64_t sees = ~0ull;      // the positions of the tile that this lane's row sees
         if (!whole) {
+          auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+          sees = below(place + 1 - pos0) & (~below(low + 1 - pos0) | below(a.keep_first - pos0)) & these;
+          const uint64_t mine = sees >> (half * 4);
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const int r = j / 16 * 32 + j % 16 / 4 * 8 + half * 4 + j % 4, pos = pos0 + r;
-            if (!(pos <= place && (pos > low || pos < a.keep_first) && ((these >> r) & 1))) {
-              x[j] = kNegInf;
-              hidden |= 1u << j;
-            }
+            const int r = j / 16 * 32 + j % 16 / 4 * 8 + j % 4;
+            if (!((mine >> r) & 1)) x[j] = kNegInf;
           }
         }
         float top = x[0];
@@ -371,6 +378,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         // rounding); their sum is of those in 32.
         union { typename W::T e[32]; typename W::V8 v[4]; } p;
         auto weigh = [&](auto all) {
+          const uint64_t mine = sees >> (half * 4);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -380,7 +388,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
               const float w = exp2_fast(__builtin_fmaf(x[j + i], c, -ref));
               l += w;
               // (a scale that is not seen may be anything)
-              const float scaled = FP8 ? decltype(all)::value || !((hidden >> (j + i)) & 1) ? w * f[i] : 0.0f : w;
+              const float scaled = FP8 ? decltype(all)::value || ((mine >> (j / 16 * 32 + j % 16 / 4 * 8 + i)) & 1) ? w * f[i] : 0.0f : w;
               p.e[j + i] = (typename W::T)scaled;
             }
           }
@@ -403,38 +411,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       }
       __syncthreads();
     }
-    if (any_bad) {
-      // What was left out, at the positions that a row sees (whatever its weight: an infinity stays one, or
-      // becomes NaN).
-      for (int tile = tile_begin; tile < tile_end; ++tile) {
-        const int pos0 = walk.position(tile * kPromptKeys);
-        if (!partial(pos0)) continue;
-        const uint64_t these = __ballot(ask(tile) >= 0);
-        for (int r = 0; r < kPromptKeys; ++r) {
-          const int pos = pos0 + r, entry = divided(pos, A.by_page);
-          if (!((these >> r) & 1)) continue;
-          const bool sees = pos <= place && (pos > low || pos < a.keep_first);
-          const char* const from = vbase + (int64_t)table[entry] * page_bytes + (int64_t)(pos - entry * a.page_size) * slot_bytes;
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int d = i * 32 + j / 4 * 8 + half * 4 + j % 4;
-              union { uint16_t u; typename W::T t; } v;
-              v.u = 0;
-              if (d < a.D) {
-                if constexpr (FP8)
-                  v.t = fp8x8<W>(((const uint8_t*)from)[d], 0)[0];
-                else
-                  v.u = ((const uint16_t*)from)[d];
-              }
-              if (sees && !finite<W>(v.u)) acc[i][j] += (float)v.t;
-            }
-          }
+  }
+
+  // What was left out is added to the row's sums in memory (the values that this lane has written): values at positions
+  // that the row sees, whatever their weight.  An infinity stays one, or becomes NaN.
+  auto add_bad = [&](auto* sums) {
+#pragma unroll 1
+    for (int tile = tile_begin; tile < tile_end; ++tile) {
+      const int pos0 = walk.position(tile * kPromptKeys);
+      if (!partial(pos0)) continue;
+#pragma unroll 1
+      for (int pos = pos0; pos < min(pos0 + kPromptKeys, hi); ++pos) {
+        const int entry = divided(pos, A.by_page), id = table[entry];
+        if (!(pos <= place && (pos > low || pos < a.keep_first)) || (uint32_t)id >= (uint32_t)a.num_pages) continue;
+        const char* const from = vbase + (int64_t)id * page_bytes + (int64_t)(pos - entry * a.page_size) * slot_bytes;
+#pragma unroll 1
+        for (int d = half * 4; d < a.D; d += d % 4 == 3 ? 5 : 1) {
+          union { uint16_t u; typename W::T t; } v;
+          if constexpr (FP8)
+            v.t = fp8x8<W>(((const uint8_t*)from)[d], 0)[0];
+          else
+            v.u = ((const uint16_t*)from)[d];
+          if (!finite<W>(v.u)) sums[d] = (std::remove_reference_t<decltype(*sums)>)((float)sums[d] + (float)v.t);
         }
       }
     }
-  }
+  };
 
   // The sums of a row: this lane's positions and those of the lane 32 on.
   {
@@ -453,6 +455,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *(f32x4*)(part + i * 32 + j * 8) = f32x4{acc[i][j * 4], acc[i][j * 4 + 1], acc[i][j * 4 + 2], acc[i][j * 4 + 3]};
+    if (any_bad && tile_begin < tile_end) add_bad(part - half * 4);
     return;
   }
   if (!valid) return;
@@ -475,6 +478,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       if (i * 32 + j * 8 + half * 4 < a.D) *(u32x2*)(to + (i * 32 + j * 8) * 2) = r.u;
     }
   }
+  if (any_bad && tile_begin < tile_end) add_bad((typename M::T*)a.out + out_row * a.D);
 }
 
 // Joins the parts of tiles whose positions several workgroups shared: a lane holds 4 values of a row.
