@@ -77,20 +77,31 @@ __device__ __forceinline__ Walk walk_of(int lo, int hi, int keep_first) {
   return w;
 }
 
-template <bool FP8, int DP>
+template <int DP>
 struct Layout {
-  static constexpr int kPieces = DP / 8;                       // of a row: 8 values
-  static constexpr int kLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // threads that load a row
-  static constexpr int kPass = 256 / kLanes;                   // rows that the workgroup loads at once
+  static constexpr int kLanes = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // threads that load a row: 8 values each
+  static constexpr int kWaveLoad = 64 / kLanes;                // rows that a wavefront loads at once
+  static constexpr int kPass = kWaves * kWaveLoad;             // ... and the workgroup
   static constexpr int kLoads = kPromptKeys / kPass;
-  // Keys: 16 bytes behind each row, so that 16 rows' pieces lie in different banks.  Values: rows of a power of two
-  // pieces, pairs of them exchanged by the row for the transposed reads.
-  static constexpr int kKeyPitch = DP * 2 + 16, kValuePitch = kLanes * 16;
-  static constexpr int kKeyBytes = kPromptKeys * kKeyPitch, kValueBytes = kPromptKeys * kValuePitch;
-  static constexpr int kBuffer = kKeyBytes + kValueBytes;
-  static constexpr int kLds = 2 * kBuffer;
-  static __device__ __forceinline__ int turn(int row) { return DP <= 64 ? (row >> 1) & 3 : row & 7; }
+  static constexpr int kPitch = kLanes * 16;                   // bytes of a row in LDS
+  static constexpr int kTile = kPromptKeys * kPitch;
+  static constexpr int kLds = 4 * kTile;                       // two buffers for keys, two for values
+  // Where in its row a piece of 16 bytes lies: exchanged by the row, so that 16 rows' pieces (keys) and 8 rows' pairs
+  // of pieces (values, for the transposed reads) spread over the banks.  Each is its own inverse.
+  static __device__ __forceinline__ int key_turn(int row) { return DP <= 64 ? (row >> 1) & 7 : row & 15; }
+  static __device__ __forceinline__ int value_turn(int row) { return DP <= 64 ? (row >> 1) & 3 : row & 7; }
+  static __device__ __forceinline__ int key_piece(int slot, int row) { return slot ^ key_turn(row); }
+  static __device__ __forceinline__ int value_piece(int slot, int row) { return slot ^ (value_turn(row) * 2); }
 };
+
+// 16 bytes a lane from `from` to LDS, at `to` (uniform) + 16 lane.  Not waited for.
+__device__ __forceinline__ void dma16(const char* from, char* to) {
+  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)to;
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                   :
+                   : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(from)
+                   : "memory");
+}
 
 // Is a 16-bit value (in the lower half of x) a finite number?
 template <class W>
@@ -103,16 +114,18 @@ __device__ __forceinline__ bool finite(uint32_t x) {
 // rows as columns: a lane holds half of one row's scores, so that maximum, sum and rescaling stay in the lane and its
 // neighbour 32 lanes on, and its weights are where the second product wants them, in the order of positions in
 // which the values are read from LDS (transposed, 4 x 16 at a time).
-// Keys and values of 64 positions go to LDS through registers, a tile ahead, in two buffers.
+// Keys and values of 64 positions go to LDS without a register between (8-bit ones through registers, where they
+// become 16-bit ones), a tile ahead, in two buffers each.  A wavefront takes 32 positions at a time and works out
+// the scores of the next 32 beside the weights of these, so that the matrix instructions run under the exponentials: the
+// tiles of keys are 32 positions on from those of values, and both are done with when a tile ends.
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(const KernelArgs A) {
-  typedef Layout<FP8, DP> L;
+  typedef Layout<DP> L;
   typedef std::conditional_t<FP8, Bf16, M> W;      // what weights and values are multiplied in
-  typedef std::conditional_t<FP8, u32x2, u32x4> Piece;
   const PromptAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[L::kLds];
-  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? 2 : 1][kWaves][2][kPromptKeys];
-  __shared__ int64_t row_lds[kWaves][kPromptKeys];
+  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][2][2 * kPromptKeys];   // as well
+  __shared__ int64_t row_lds[kWaves][2 * kPromptKeys];      // by the place mod 128
   __shared__ uint32_t any_bad;      // values that are no finite numbers have been left out
 
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
@@ -177,239 +190,357 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   // (fp16 weights end at 2^-24: they are kept 2^7 above the reference, so that with the slack they reach 2^15)
   constexpr float kLift = std::is_same_v<W, F16> ? 7.0f : 0.0f;
 
-  // What lies behind a row's last value is zeros, once for all.
-  if (a.D < DP) {
-    const int empty = L::kPieces - a.D / 8;
-    for (int i = tid; i < 2 * kPromptKeys * empty; i += 256) {
-      const int buf = i / (kPromptKeys * empty), r = i / empty % kPromptKeys;
-      *(u32x4*)(lds + buf * L::kBuffer + r * L::kKeyPitch + (a.D / 8 + i % empty) * 16) = u32x4{0, 0, 0, 0};
-    }
-  }
-
   const int32_t* const table = a.table + (int64_t)t.b * a.table_stride;
   const int last_entry = divided(max(hi - 1, 0), A.by_page);
   constexpr int kElem = FP8 ? 1 : 2;
   const char* const kbase = (const char*)a.k_cache + (int64_t)t.head * a.head_stride * kElem;
   const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
   const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
-  const int piece = tid % L::kLanes, piece_row = tid / L::kLanes;
-  const bool has_piece = piece * 8 < a.D;
-  const int piece_at = has_piece ? piece * 8 * kElem : 0;
+  const int slot = tid % L::kLanes, slot_row = tid / L::kLanes;    // what this thread loads of a row, and of which rows
+  auto lds_keys = [&](int tile) { return lds + (tile & 1) * L::kTile; };
+  auto lds_values = [&](int tile) { return lds + (2 + (tile & 1)) * L::kTile; };
+  // What lies behind a key's last value is zeros, once for all.
+  if (a.D < DP) {
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) {
+      const int r = slot_row + i * L::kPass;
+      if (L::key_piece(slot, r) * 8 >= a.D) {
+        *(u32x4*)(lds_keys(0) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+        *(u32x4*)(lds_keys(1) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
 
-  // The page of position lane of a tile, asked for a tile ahead; -1 where there is none.
+  // The table's entry for a place of a tile of keys (which begin half a tile behind the tile's beginning), a lane each,
+  // asked for a tile ahead.
   auto ask = [&](int tile) {
-    const int pos = walk.position(tile * kPromptKeys) + lane;
-    const int id = table[min(divided(pos, A.by_page), last_entry)];
-    return pos < hi && (uint32_t)id < (uint32_t)a.num_pages ? id : -1;
+    const int pos = walk.position(max(tile * kPromptKeys + kPromptKeys / 2 + lane, 0));
+    return table[min(divided(pos, A.by_page), last_entry)];
   };
-  Piece kreg[L::kLoads], vreg[L::kLoads];
+  u32x2 kreg[L::kLoads], vreg[L::kLoads];      // (8-bit caches)
   float ks = 1.0f, vs = 1.0f;
-  uint64_t loaded = 0;         // which positions of the loaded tile there are
-  auto fetch = [&](int tile, int ids) {
-    // A lane works out where its position's rows lie, for the wavefront's lanes that load them.
-    const int pos = walk.position(tile * kPromptKeys) + lane, slot = pos - divided(pos, A.by_page) * a.page_size;
-    loaded = __ballot(ids >= 0);
-    row_lds[wave][lane] = max(ids, 0) * page_bytes + (uint32_t)slot * (uint64_t)(uint32_t)slot_bytes;
+  // A lane works out where its place's rows lie, for the wavefront's lanes that load them; which of the places there are.
+  auto find_rows = [&](int tile, int entry) -> uint64_t {
+    const int at_place = tile * kPromptKeys + kPromptKeys / 2 + lane, pos = walk.position(max(at_place, 0));
+    const int ids = at_place >= 0 && pos < hi && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
+    const int in_page = pos - divided(pos, A.by_page) * a.page_size;
+    row_lds[wave][at_place & (2 * kPromptKeys - 1)] = max(ids, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
     if constexpr (FP8) {
       const int64_t at = a.scale_blocks == 0 ? t.head
-                                             : ((int64_t)max(ids, 0) * a.Hkv + t.head) * a.scale_blocks + divided(slot, A.by_block);
+                                             : ((int64_t)max(ids, 0) * a.Hkv + t.head) * a.scale_blocks + divided(in_page, A.by_block);
       ks = ids >= 0 ? a.k_scale[at] * a.scale : 0.0f;
       vs = ids >= 0 ? a.v_scale[at] : 0.0f;
     }
     // (lanes read what other lanes of their wavefront wrote: LDS keeps the order, and so must the compiler)
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    int64_t at[L::kLoads];
-#pragma unroll
-    for (int i = 0; i < L::kLoads; ++i) at[i] = row_lds[wave][piece_row + i * L::kPass] + piece_at;
+    return __ballot(ids >= 0);
+  };
+  auto load = [&](int tile, const char* base, bool values, u32x2* regs) {
+    char* const to = values ? lds_values(tile) : lds_keys(tile);
+    const int place0 = tile * kPromptKeys + (values ? 0 : kPromptKeys / 2);
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
-      kreg[i] = *(const Piece*)(kbase + at[i]);
-      vreg[i] = *(const Piece*)(vbase + at[i]);
+      const int r = slot_row + i * L::kPass, piece = values ? L::value_piece(slot, r) : L::key_piece(slot, r);
+      const char* const from = base + row_lds[wave][(place0 + r) & (2 * kPromptKeys - 1)];
+      if constexpr (FP8) {
+        regs[i] = *(const u32x2*)(from + (piece * 8 < a.D ? piece * 8 : 0));
+      } else {
+        if (piece * 8 < a.D) dma16(from + piece * 16, to + (i * L::kPass + wave * L::kWaveLoad) * L::kPitch);
+      }
     }
   };
+  auto load_keys = [&](int tile) { load(tile, kbase, false, kreg); };
+  auto load_values = [&](int tile) { load(tile, vbase, true, vreg); };
   // Does any row of the workgroup not see all of a tile?
   auto partial = [&](int pos0) {
     return pos0 + kPromptKeys - 1 > tile_lo ||
            (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kPromptKeys > a.keep_first);
   };
-  // The loaded tile to LDS: positions that there are not as zeros.  Where some rows do not see all of it, so are values
-  // that are no finite numbers: a weight of 0 times them would not be 0 (they are added in the end).
-  auto put = [&](int buf, int tile) {
-    char* const to = lds + buf * L::kBuffer;
+  // Values as the product may have them: positions that there are not as zeros, and where some rows do not see all of
+  // the tile, values that are no finite numbers as well: a weight of 0 times them would not be 0 (they are added in
+  // the end).
+  auto clean = [&](u32x4 v, bool there, bool look) {
+    if (!there) v = u32x4{0, 0, 0, 0};
+    if (look) {
+      // (an exponent of ones carries into the half's sign)
+      constexpr uint32_t kExponents = std::is_same_v<W, F16> ? 0x7C007C00u : 0x7F807F80u;
+      constexpr uint32_t kOnes = std::is_same_v<W, F16> ? 0x04000400u : 0x00800080u;
+      uint32_t all = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
+        v[e] &= ~((bad >> 15) * 0xFFFFu);
+        all |= bad;
+      }
+      if (all != 0) any_bad = 1;
+    }
+    return v;
+  };
+  // 8-bit keys and values out of the registers, and their scales.
+  auto put_keys = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) {
+      const int r = slot_row + i * L::kPass;
+      union { typename M::V8 v; u32x4 u; } k;
+      k.v = fp8x8<M>(kreg[i][0], kreg[i][1]);
+      if (L::key_piece(slot, r) * 8 < a.D) *(u32x4*)(lds_keys(tile) + r * L::kPitch + slot * 16) = k.u;
+    }
+    const int at = (tile * kPromptKeys + kPromptKeys / 2 + lane) & (2 * kPromptKeys - 1);
+    scale_lds[wave][0][at] = ks;
+    scale_lds[wave][1][at] = vs;
+  };
+  auto put_values = [&](int tile, uint64_t there) {
     const bool look = partial(walk.position(tile * kPromptKeys));
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
-      const int r = piece_row + i * L::kPass;
-      u32x4 k, v;
-      if constexpr (FP8) {
-        union { typename M::V8 v; u32x4 u; } kc;
-        union { typename W::V8 v; u32x4 u; } vc;
-        kc.v = fp8x8<M>(kreg[i][0], kreg[i][1]);
-        vc.v = fp8x8<W>(vreg[i][0], vreg[i][1]);
-        k = kc.u;
-        v = vc.u;
-      } else {
-        k = kreg[i];
-        v = vreg[i];
-      }
-      if (!((loaded >> r) & 1)) v = u32x4{0, 0, 0, 0};
-      if (look) {
-        // (an exponent of ones carries into the half's sign)
-        constexpr uint32_t kExponents = std::is_same_v<W, F16> ? 0x7C007C00u : 0x7F807F80u;
-        constexpr uint32_t kOnes = std::is_same_v<W, F16> ? 0x04000400u : 0x00800080u;
-        uint32_t all = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
-          v[e] &= ~((bad >> 15) * 0xFFFFu);
-          all |= bad;
-        }
-        if (all != 0 && has_piece) any_bad = 1;
-      }
-      if (has_piece) {
-        *(u32x4*)(to + r * L::kKeyPitch + piece * 16) = k;
-        *(u32x4*)(to + L::kKeyBytes + r * L::kValuePitch + ((piece >> 1) ^ L::turn(r)) * 32 + (piece & 1) * 16) = v;
-      }
+      const int r = slot_row + i * L::kPass;
+      union { typename W::V8 v; u32x4 u; } v;
+      v.v = fp8x8<W>(vreg[i][0], vreg[i][1]);
+      if (L::value_piece(slot, r) * 8 < a.D)
+        *(u32x4*)(lds_values(tile) + r * L::kPitch + slot * 16) = clean(v.u, (there >> r) & 1, look);
     }
-    if constexpr (FP8) {
-      scale_lds[buf][wave][0][lane] = ks;
-      scale_lds[buf][wave][1][lane] = vs;
+  };
+  // 16-bit values that are in LDS already.
+  auto clean_values = [&](int tile, uint64_t there, bool look) {
+#pragma unroll
+    for (int i = 0; i < L::kLoads; ++i) {
+      const int r = slot_row + i * L::kPass;
+      u32x4* const at = (u32x4*)(lds_values(tile) + r * L::kPitch + slot * 16);
+      if (L::value_piece(slot, r) * 8 < a.D) *at = clean(*at, (there >> r) & 1, look);
+    }
+  };
+  auto landed = [&] {
+    if constexpr (!FP8) __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+
+  // Hidden from every row of the wavefront: behind the last one's place, or in front of the first one's window.
+  constexpr int kSub = kPromptKeys / 2;
+  auto hidden = [&](int sub) {
+    const int pos0 = walk.position(sub * kSub);
+    return pos0 > wave_hi || (pos0 + kSub - 1 <= wave_low && pos0 >= a.keep_first) || wave_first >= t.rows;
+  };
+  const int key_at = n * L::kPitch + (half ^ L::key_turn(n)) * 16;
+  // Scores of 32 positions: sub - 1 of its tile of keys.
+  auto read_keys = [&](int sub, int i) {
+    const char* const keys = lds_keys((sub - 1) >> 1) + ((sub - 1) & 1) * kSub * L::kPitch;
+    return as_v8<M>(*(const u32x4*)(keys + (key_at ^ (i * 32))));
+  };
+  f32x16 zero;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) zero[j] = 0.0f;
+  auto score = [&](int sub, f32x16& s) {
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) s = M::mfma(read_keys(sub, i), q[i], i == 0 ? zero : s);
+  };
+  const int quarter = (lane >> 4) & 1, l16 = lane & 15;
+  const int value_row = half * 4 + (l16 >> 2), value_turn = L::value_turn(value_row);
+  const int value_at = value_row * L::kPitch + (l16 & 3) * 8;
+  // Positions 16 j .. 16 j + 15 of a sub, 32 of the head's values; and all of those times their weights.
+  auto read_values = [&](int sub, int j, int i) {
+    const char* const column = lds_values(sub >> 1) + ((sub & 1) * kSub + j * 16) * L::kPitch + value_at +
+                               ((i * 2 + quarter) ^ value_turn) * 32;
+    union { i16x4 h[2]; typename W::V8 v; } v;
+    v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
+    v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * L::kPitch));
+    return v.v;
+  };
+  auto add_values = [&](int sub, int j, typename W::V8 p) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] = W::mfma(read_values(sub, j, i), p, acc[i]);
+  };
+  // The largest of a row's scores (both halves').
+  auto over_halves = [](float top) {
+    const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+  };
+  auto largest = [&](const f32x16& x) {
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+    return over_halves(top);
+  };
+  auto raise = [&](float top) {
+    if (__any(top > m + kSlack)) {
+      // (a row by itself: what it gives does not depend on the rows beside it)
+      const float m_new = top > m + kSlack ? top : m;
+      const float fix = exp2_fast(m - or_zero(m_new));
+      m = m_new;
+      l *= fix;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= fix;
     }
   };
 
-  const int quarter = (lane >> 4) & 1, l16 = lane & 15;
-  const int value_row = half * 4 + (l16 >> 2), value_turn = L::turn(value_row);
-  uint64_t there = 0;
+  // The same where every row of the workgroup sees all of the sub and the scores need nothing but their factor: one
+  // stretch of code in a fixed order, reads from LDS three operands ahead and the exponentials (then the next
+  // scores' maximum) between the matrix instructions.  `top`: the largest scores, of the next sub afterwards.
+  auto attend_whole = [&](int sub, const f32x16& x, f32x16& next, float& top) {
+    constexpr int kSteps = DP / 16, kAhead = 3;
+    raise(top * to_log2);
+    const float ref = or_zero(m) - kLift;
+    union { typename W::T e[16]; typename W::V8 v[2]; } p;
+    typename M::V8 k[kSteps];
+    typename W::V8 v[kSteps];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) k[i] = read_keys(sub + 1, i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      next = M::mfma(k[i], q[i], i == 0 ? zero : next);
+      if (i + kAhead < kSteps)
+        k[i + kAhead] = read_keys(sub + 1, i + kAhead);
+      else
+        v[i + kAhead - kSteps] = read_values(sub, (i + kAhead - kSteps) / (DP / 32), (i + kAhead - kSteps) % (DP / 32));
+#pragma unroll
+      for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) {
+        const float w = exp2_fast(__builtin_fmaf(x[j], to_log2, -ref));
+        l += w;
+        p.e[j] = (typename W::T)w;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float most[2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      acc[i % (DP / 32)] = W::mfma(v[i], p.v[i / (DP / 32)], acc[i % (DP / 32)]);
+      if (i + kAhead < kSteps) v[i + kAhead] = read_values(sub, (i + kAhead) / (DP / 32), (i + kAhead) % (DP / 32));
+#pragma unroll
+      for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    top = over_halves(fmaxf(most[0], most[1]));
+  };
+
+  // Positions of a sub, whose scores are in `x`, and the scores of the next one (skip_next: not those).
+  auto attend = [&](int sub, uint32_t there, f32x16& x, f32x16& next, bool skip_next) {
+    const int pos0 = walk.position(sub * kSub);
+    const bool whole = there == ~0u && pos0 + kSub - 1 <= wave_lo &&
+                       (a.window <= 0 || pos0 > low_of(wave_hi) || pos0 + kSub <= a.keep_first);
+    if (!skip_next) score(sub + 1, next);
+    if (hidden(sub)) return;
+    // Scores in powers of two, unless they are taken there with the reference.
+    float c = to_log2;
+    const int scales = sub * kSub & (2 * kPromptKeys - 1);
+    if (!plain) {
+      c = 1.0f;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const f32x4 f = *(const f32x4*)&scale_lds[wave][0][scales + j * 2 + half * 4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
+        }
+      }
+      if (a.softcap > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = capped(x[j] * cap_in, cap_out);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] *= to_log2;
+      }
+    }
+    uint32_t sees = ~0u;      // the positions that this lane's row sees
+    if (!whole) {
+      auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+      sees = below(place + 1 - pos0) & (~below(low + 1 - pos0) | below(a.keep_first - pos0)) & there;
+      sees >>= half * 4;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
+      }
+    }
+    raise(largest(x) * c);
+    const float ref = or_zero(m) - kLift;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      union { typename W::T e[8]; typename W::V8 v; } p;
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (FP8) f = *(const f32x4*)&scale_lds[wave][1][scales + (g * 8 + i) * 2 + half * 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = g * 8 + i + e;
+          const float w = exp2_fast(__builtin_fmaf(x[j], c, -ref));
+          l += w;
+          // (a scale that is not seen may be anything)
+          p.e[i + e] = (typename W::T)(!FP8 ? w : whole || ((sees >> (j / 4 * 8 + j % 4)) & 1) ? w * f[e] : 0.0f);
+        }
+      }
+      add_values(sub, g, p.v);
+    }
+  };
+
   if (tid == 0) any_bad = 0;
   if (tile_begin < tile_end) {
-    fetch(tile_begin, ask(tile_begin));
-    int ids = ask(tile_begin + 1);
-    __syncthreads();
-    put(0, tile_begin);
-    there = loaded;
-    if (tile_begin + 1 < tile_end) {
-      fetch(tile_begin + 1, ids);
-      ids = ask(tile_begin + 2);
+    // Which of a tile's positions there are: its second half and the next tile's first come with its keys.
+    uint64_t there = find_rows(tile_begin - 1, ask(tile_begin - 1));
+    load_keys(tile_begin - 1);
+    if constexpr (FP8) {
+      __syncthreads();      // (the zeros behind the keys)
+      put_keys(tile_begin - 1);
     }
-    __syncthreads();
-    for (int tile = tile_begin; tile < tile_end; ++tile) {
-      const int buf = (tile - tile_begin) & 1;
-      const char* const keys = lds + buf * L::kBuffer;
-      const int pos0 = walk.position(tile * kPromptKeys);
-      // Hidden from every row of the wavefront: behind the last one's place, or in front of the first one's window.
-      const bool skip = pos0 > wave_hi || (pos0 + kPromptKeys - 1 <= wave_low && pos0 >= a.keep_first) || wave_first >= t.rows;
-      float x[32];
-      if (!skip) {
-        f32x16 s[2];
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) s[kt][j] = 0.0f;
-          const char* const from = keys + (kt * 32 + n) * L::kKeyPitch + half * 16;
-#pragma unroll
-          for (int i = 0; i < DP / 16; ++i) s[kt] = M::mfma(as_v8<M>(*(const u32x4*)(from + i * 32)), q[i], s[kt]);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) x[kt * 16 + j] = s[kt][j];
-        }
-      }
-      const bool more = tile + 1 < tile_end;
-      const uint64_t these = there;
-      if (more) {
-        put(buf ^ 1, tile + 1);
-        there = loaded;
-        if (tile + 2 < tile_end) {
-          fetch(tile + 2, ids);
-          ids = ask(tile + 3);
-        }
-      }
-      if (!skip) {
-        // Scores in powers of two, unless they are taken there with the reference.
-        float c = to_log2;
-        if (!plain) {
-          c = 1.0f;
-          if constexpr (FP8) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-              const f32x4 f = *(const f32x4*)&scale_lds[buf][wave][0][j / 16 * 32 + j % 16 / 4 * 8 + half * 4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
-            }
-          }
-          if (a.softcap > 0.0f) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = capped(x[j] * cap_in, cap_out);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] *= to_log2;
-          }
-        }
-        const bool whole = these == ~0ull && pos0 + kPromptKeys - 1 <= wave_lo &&
-                           (a.window <= 0 || pos0 > low_of(wave_hi) || pos0 + kPromptKeys <= a.keep_first);
-        uint64_t sees = ~0ull;      // the positions of the tile that this lane's row sees
-        if (!whole) {
-          auto below = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
-          sees = below(place + 1 - pos0) & (~below(low + 1 - pos0) | below(a.keep_first - pos0)) & these;
-          const uint64_t mine = sees >> (half * 4);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const int r = j / 16 * 32 + j % 16 / 4 * 8 + j % 4;
-            if (!((mine >> r) & 1)) x[j] = kNegInf;
-          }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int j = 1; j < 32; ++j) top = fmaxf(top, x[j]);
-        const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c;
-        if (__any(top > m + kSlack)) {
-          // (a row by itself: what it gives does not depend on the rows beside it)
-          const float m_new = top > m + kSlack ? top : m;
-          const float fix = exp2_fast(m - or_zero(m_new));
-          m = m_new;
-          l *= fix;
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[i][j] *= fix;
-        }
-        const float ref = or_zero(m) - kLift;
-        // Weights of 16 bits (half a step of their type is what the result is off by from each, as from its own
-        // rounding); their sum is of those in 32.
-        union { typename W::T e[32]; typename W::V8 v[4]; } p;
-        auto weigh = [&](auto all) {
-          const uint64_t mine = sees >> (half * 4);
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
-            if constexpr (FP8) f = *(const f32x4*)&scale_lds[buf][wave][1][j / 16 * 32 + j % 16 / 4 * 8 + half * 4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float w = exp2_fast(__builtin_fmaf(x[j + i], c, -ref));
-              l += w;
-              // (a scale that is not seen may be anything)
-              const float scaled = FP8 ? decltype(all)::value || ((mine >> (j / 16 * 32 + j % 16 / 4 * 8 + i)) & 1) ? w * f[i] : 0.0f : w;
-              p.e[j + i] = (typename W::T)scaled;
-            }
-          }
-        };
-        if (!FP8 || whole) weigh(std::true_type{}); else weigh(std::false_type{});
-        const char* const values = keys + L::kKeyBytes + value_row * L::kValuePitch + (l16 & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-          const char* const column = values + ((i * 2 + quarter) ^ value_turn) * 32;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            union { i16x4 h[2]; typename W::V8 v; } v;
-            v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4*)(column + j * 16 * L::kValuePitch));
-            v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) i16x4*)(column + (j * 16 + 8) * L::kValuePitch));
-            acc[i] = W::mfma(v.v, p.v[j], acc[i]);
-          }
-        }
-      }
+    uint32_t first = (uint32_t)(there >> 32);
+    there = find_rows(tile_begin, ask(tile_begin));
+    load_keys(tile_begin);
+    load_values(tile_begin);
+    int ids = ask(tile_begin + 1);
+    landed();             // (any_bad as well)
+    if constexpr (FP8) {
+      put_keys(tile_begin);
+      put_values(tile_begin, there << 32 | first);
       __syncthreads();
+    }
+    f32x16 even, odd;
+    if (!hidden(2 * tile_begin)) score(2 * tile_begin, even);
+    __syncthreads();
+    uint64_t these = there << 32 | first;
+    // The next tile's keys and values are on their way while this one's are multiplied.
+    auto ahead = [&](int tile) {
+      first = (uint32_t)(there >> 32);
+      if (tile + 1 < tile_end) {
+        there = find_rows(tile + 1, ids);
+        load_keys(tile + 1);
+        load_values(tile + 1);
+        ids = ask(tile + 2);
+      }
+    };
+    for (int tile = tile_begin; tile < tile_end;) {
+      // (heads of more than 128 do not have the registers)
+      if constexpr (!FP8 && DP <= 128) {
+        if (plain) {
+          float top = largest(even);
+          for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
+            ahead(tile);
+            attend_whole(2 * tile, even, odd, top);
+            attend_whole(2 * tile + 1, odd, even, top);
+            landed();
+            these = there << 32 | first;
+          }
+        }
+      }
+      ahead(tile);
+      const bool more = tile + 1 < tile_end;
+      if constexpr (!FP8) {
+        const bool look = partial(walk.position(tile * kPromptKeys));
+        if (look || these != ~0ull) {
+          clean_values(tile, these, look);
+          __syncthreads();
+        }
+      }
+      attend(2 * tile, (uint32_t)these, even, odd, hidden(2 * tile + 1));
+      attend(2 * tile + 1, (uint32_t)(these >> 32), odd, even, !more || hidden(2 * tile + 2));
+      if constexpr (FP8) {
+        if (more) {
+          put_keys(tile + 1);
+          put_values(tile + 1, there << 32 | first);
+        }
+      }
+      landed();
+      these = there << 32 | first;
+      ++tile;
     }
   }
 
