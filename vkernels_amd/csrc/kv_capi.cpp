@@ -127,11 +127,11 @@ int append(const char* who, const void* k, const void* v, void* k_cache, void* v
 // the kernels' factors 1 / cap and cap then stay within 32-bit floats.
 float cap_of(float softcap) { return softcap >= 0x1p100f ? 0.0f : softcap > 0.0f ? std::fmax(softcap, 0x1p-100f) : 0.0f; }
 
-// Rows and slots are counted in 32 bits, and so are a launch's threads (with up to 1024 workgroups more, or 32 for a
-// tile's join).
-bool prompt_fits(int B, int tokens, int Hkv, int G) {
+// Rows and slots are counted in 32 bits, and so are a launch's threads.  (Where tiles are shared there are few: at most
+// 4096 workgroups and one for every head more.)
+bool prompt_fits(int B, int tokens, int Hkv, int G, int D) {
   if (tokens > kInt32 / 4 / G || B > kInt32 / 4) return false;
-  return vk::prompt_attention_slots(B, tokens, G) <= kThreads / 256 / 64 / Hkv;
+  return vk::prompt_attention_slots(B, tokens, G, D) <= kThreads / 512 / Hkv;
 }
 
 // Attention of one new token of every sequence.
@@ -293,7 +293,7 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
 size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,
                                                      int keep_first) {
   if (B <= 0 || tokens <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0 || keep_first < 0) return 0;
-  if (!prompt_fits(B, tokens, Hkv, G)) return 0;
+  if (!prompt_fits(B, tokens, Hkv, G, D)) return 0;
   return vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, window > 0 ? keep_first : 0).bytes;
 }
 
@@ -322,7 +322,7 @@ int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void
   if (why == nullptr && !(softcap >= 0.0f)) why = "softcap must not be negative";
   if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  if (max_len > kPositions || !prompt_fits(B, tokens, Hkv, G))
+  if (max_len > kPositions || !prompt_fits(B, tokens, Hkv, G, D))
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, tokens, heads and positions for one call");
   keep_first = window > 0 ? keep_first : 0;
   const vk::PromptAttentionPlan plan = vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, keep_first);

@@ -49,15 +49,29 @@ __device__ __forceinline__ bool find_tile(const KernelArgs& A, int block, Tile* 
   t->split = rest - from_end * A.p.splits;
   t->slot = A.p.slots - 1 - from_end;
   auto start = [&](int i) { return min(max(a.starts[i], 0), a.tokens); };
-  // The tiles of sequence b begin at start rows / 128 + b: it has at most as many as lie up to the next one's.
-  auto base = [&](int i) { return start(i) * a.G / kPromptRows + i; };
+  // The tiles (of R rows) of sequence b begin at start rows / R + b: it has at most as many as lie up to the next one's.
+  auto base = [&](int i) { return (start(i) * a.G >> A.p.row_shift) + i; };
   t->b = __builtin_amdgcn_readfirstlane(last_not_above(a.B + 1, t->slot, base));
   const int k = t->slot - base(t->b);
   t->s0 = start(t->b);
   t->tokens = (t->b < a.B ? max(start(t->b + 1), t->s0) : a.tokens) - t->s0;
-  t->first = k * kPromptRows;
+  t->first = k << A.p.row_shift;
   t->rows = t->tokens * a.G;
   return k >= 0 && t->first < t->rows;
+}
+
+// Rows that belong to no sequence.
+__device__ __forceinline__ void clear_rows(const KernelArgs& A, const Tile& t) {
+  const PromptAttentionArgs& a = A.a;
+  if (!a.clear_rest || t.split > 0) return;
+  const int pieces = a.D / 8;
+  for (int i = threadIdx.x; i < pieces << A.p.row_shift; i += 256) {
+    const int r = t.first + i / pieces, tok = divided(r, A.by_group);
+    if (r >= t.rows) break;
+    const int64_t row = ((int64_t)(t.s0 + tok) * a.Hkv + t.head) * a.G + (r - tok * a.G);
+    *(u32x4*)((char*)a.out + (row * a.D + i % pieces * 8) * 2) = u32x4{0, 0, 0, 0};
+    if (i % pieces == 0 && a.lse != nullptr) a.lse[row] = kNegInf;
+  }
 }
 
 // The positions a tile sees, as a line of places: the first `split` of them the positions at the beginning, the
@@ -94,9 +108,12 @@ struct Layout {
   static __device__ __forceinline__ int value_piece(int slot, int row) { return slot ^ (value_turn(row) * 2); }
 };
 
+typedef __attribute__((address_space(3))) char* Lds;
+typedef __attribute__((address_space(3))) u32x4* LdsPiece;
+
 // 16 bytes a lane from `from` to LDS, at `to` (uniform) + 16 lane.  Not waited for.
-__device__ __forceinline__ void dma16(const char* from, char* to) {
-  const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)to;
+__device__ __forceinline__ void dma16(const char* from, Lds to) {
+  const uint32_t at = (uint32_t)(uintptr_t)to;
   __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                    :
                    : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(from)
@@ -109,6 +126,35 @@ __device__ __forceinline__ bool finite(uint32_t x) {
   constexpr uint32_t kExponent = std::is_same_v<W, F16> ? 0x7C00u : 0x7F80u;
   return (x & kExponent) != kExponent;
 }
+
+// Zeros for what is no finite number among 8 values; whether there was one.  (An exponent of ones carries into
+// the half's sign.)
+template <class W>
+__device__ __forceinline__ bool drop_others(u32x4& v) {
+  constexpr uint32_t kExponents = std::is_same_v<W, F16> ? 0x7C007C00u : 0x7F807F80u;
+  constexpr uint32_t kOnes = std::is_same_v<W, F16> ? 0x04000400u : 0x00800080u;
+  uint32_t all = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
+    v[e] &= ~((bad >> 15) * 0xFFFFu);
+    all |= bad;
+  }
+  return all != 0;
+}
+
+// The larger (the sum) of a value here and 32 lanes on.
+__device__ __forceinline__ float over_halves_max(float x) {
+  const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float over_halves_sum(float x) {
+  const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
+// Bits below n of 32.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 // S^T = K q^T and O^T += V^T P^T, both 32 x 32 x 16 with the keys (the head's width) as rows and a wavefront's 32
 // rows as columns: a lane holds half of one row's scores, so that maximum, sum and rescaling stay in the lane and its
@@ -134,16 +180,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   if (!find_tile(A, blockIdx.x, &t)) return;
   const int Hq = a.Hkv * a.G;
   if (t.b == a.B) {
-    // Rows that belong to no sequence.
-    if (!a.clear_rest || t.split > 0) return;
-    const int pieces = a.D / 8;
-    for (int i = tid; i < kPromptRows * pieces; i += 256) {
-      const int r = t.first + i / pieces, tok = divided(r, A.by_group);
-      if (r >= t.rows) break;
-      const int64_t row = (int64_t)(t.s0 + tok) * Hq + t.head * a.G + (r - tok * a.G);
-      *(u32x4*)((char*)a.out + (row * a.D + i % pieces * 8) * 2) = u32x4{0, 0, 0, 0};
-      if (i % pieces == 0 && a.lse != nullptr) a.lse[row] = kNegInf;
-    }
+    clear_rows(A, t);
     return;
   }
 
@@ -197,16 +234,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
   const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
   const int slot = tid % L::kLanes, slot_row = tid / L::kLanes;    // what this thread loads of a row, and of which rows
-  auto lds_keys = [&](int tile) { return lds + (tile & 1) * L::kTile; };
-  auto lds_values = [&](int tile) { return lds + (2 + (tile & 1)) * L::kTile; };
+  auto lds_keys = [&](int tile) { return (Lds)&lds[0] + (tile & 1) * L::kTile; };
+  auto lds_values = [&](int tile) { return (Lds)&lds[0] + (2 + (tile & 1)) * L::kTile; };
   // What lies behind a key's last value is zeros, once for all.
   if (a.D < DP) {
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
       const int r = slot_row + i * L::kPass;
       if (L::key_piece(slot, r) * 8 >= a.D) {
-        *(u32x4*)(lds_keys(0) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
-        *(u32x4*)(lds_keys(1) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+        *(LdsPiece)(lds_keys(0) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+        *(LdsPiece)(lds_keys(1) + r * L::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -237,7 +274,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     return __ballot(ids >= 0);
   };
   auto load = [&](int tile, const char* base, bool values, u32x2* regs) {
-    char* const to = values ? lds_values(tile) : lds_keys(tile);
+    const Lds to = values ? lds_values(tile) : lds_keys(tile);
     const int place0 = tile * kPromptKeys + (values ? 0 : kPromptKeys / 2);
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
@@ -262,19 +299,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   // the end).
   auto clean = [&](u32x4 v, bool there, bool look) {
     if (!there) v = u32x4{0, 0, 0, 0};
-    if (look) {
-      // (an exponent of ones carries into the half's sign)
-      constexpr uint32_t kExponents = std::is_same_v<W, F16> ? 0x7C007C00u : 0x7F807F80u;
-      constexpr uint32_t kOnes = std::is_same_v<W, F16> ? 0x04000400u : 0x00800080u;
-      uint32_t all = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
-        v[e] &= ~((bad >> 15) * 0xFFFFu);
-        all |= bad;
-      }
-      if (all != 0) any_bad = 1;
-    }
+    if (look && drop_others<W>(v)) any_bad = 1;
     return v;
   };
   // 8-bit keys and values out of the registers, and their scales.
@@ -284,7 +309,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       const int r = slot_row + i * L::kPass;
       union { typename M::V8 v; u32x4 u; } k;
       k.v = fp8x8<M>(kreg[i][0], kreg[i][1]);
-      if (L::key_piece(slot, r) * 8 < a.D) *(u32x4*)(lds_keys(tile) + r * L::kPitch + slot * 16) = k.u;
+      if (L::key_piece(slot, r) * 8 < a.D) *(LdsPiece)(lds_keys(tile) + r * L::kPitch + slot * 16) = k.u;
     }
     const int at = (tile * kPromptKeys + kPromptKeys / 2 + lane) & (2 * kPromptKeys - 1);
     scale_lds[wave][0][at] = ks;
@@ -298,7 +323,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       union { typename W::V8 v; u32x4 u; } v;
       v.v = fp8x8<W>(vreg[i][0], vreg[i][1]);
       if (L::value_piece(slot, r) * 8 < a.D)
-        *(u32x4*)(lds_values(tile) + r * L::kPitch + slot * 16) = clean(v.u, (there >> r) & 1, look);
+        *(LdsPiece)(lds_values(tile) + r * L::kPitch + slot * 16) = clean(v.u, (there >> r) & 1, look);
     }
   };
   // 16-bit values that are in LDS already.
@@ -306,7 +331,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
     for (int i = 0; i < L::kLoads; ++i) {
       const int r = slot_row + i * L::kPass;
-      u32x4* const at = (u32x4*)(lds_values(tile) + r * L::kPitch + slot * 16);
+      const LdsPiece at = (LdsPiece)(lds_values(tile) + r * L::kPitch + slot * 16);
       if (L::value_piece(slot, r) * 8 < a.D) *at = clean(*at, (there >> r) & 1, look);
     }
   };
@@ -324,8 +349,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const int key_at = n * L::kPitch + (half ^ L::key_turn(n)) * 16;
   // Scores of 32 positions: sub - 1 of its tile of keys.
   auto read_keys = [&](int sub, int i) {
-    const char* const keys = lds_keys((sub - 1) >> 1) + ((sub - 1) & 1) * kSub * L::kPitch;
-    return as_v8<M>(*(const u32x4*)(keys + (key_at ^ (i * 32))));
+    const Lds keys = lds_keys((sub - 1) >> 1) + ((sub - 1) & 1) * kSub * L::kPitch;
+    return as_v8<M>(*(LdsPiece)(keys + (key_at ^ (i * 32))));
   };
   f32x16 zero;
 #pragma unroll
@@ -339,7 +364,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const int value_at = value_row * L::kPitch + (l16 & 3) * 8;
   // Positions 16 j .. 16 j + 15 of a sub, 32 of the head's values; and all of those times their weights.
   auto read_values = [&](int sub, int j, int i) {
-    const char* const column = lds_values(sub >> 1) + ((sub & 1) * kSub + j * 16) * L::kPitch + value_at +
+    const Lds column = lds_values(sub >> 1) + ((sub & 1) * kSub + j * 16) * L::kPitch + value_at +
                                ((i * 2 + quarter) ^ value_turn) * 32;
     union { i16x4 h[2]; typename W::V8 v; } v;
     v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
@@ -351,15 +376,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     for (int i = 0; i < DP / 32; ++i) acc[i] = W::mfma(read_values(sub, j, i), p, acc[i]);
   };
   // The largest of a row's scores (both halves').
-  auto over_halves = [](float top) {
-    const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-  };
   auto largest = [&](const f32x16& x) {
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-    return over_halves(top);
+    return over_halves_max(top);
   };
   auto raise = [&](float top) {
     if (__any(top > m + kSlack)) {
@@ -410,7 +431,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    top = over_halves(fmaxf(most[0], most[1]));
+    top = over_halves_max(fmaxf(most[0], most[1]));
   };
 
   // Positions of a sub, whose scores are in `x`, and the scores of the next one (skip_next: not those).
@@ -443,8 +464,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     }
     uint32_t sees = ~0u;      // the positions that this lane's row sees
     if (!whole) {
-      auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
-      sees = below(place + 1 - pos0) & (~below(low + 1 - pos0) | below(a.keep_first - pos0)) & there;
+      sees = bits_below(place + 1 - pos0) & (~bits_below(low + 1 - pos0) | bits_below(a.keep_first - pos0)) & there;
       sees >>= half * 4;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -569,11 +589,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     }
   };
 
-  // The sums of a row: this lane's positions and those of the lane 32 on.
-  {
-    const u32x2 both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-    l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-  }
+  l = over_halves_sum(l);
   const float ref = or_zero(m) - kLift;        // l and the sums are relative to 2^ref
   if (A.p.splits > 1) {
     const int64_t slot = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
@@ -612,6 +628,300 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   if (any_bad && tile_begin < tile_end) add_bad((typename M::T*)a.out + out_row * a.D);
 }
 
+// The same for tiles of 32 rows: every wavefront has all of the rows and takes every fourth 32 positions, by itself.  Keys
+// come as the product's operands straight from the cache, values by way of the wavefront's own part of LDS; the
+// next ones are asked for as soon as these have been taken.  The wavefronts' results meet in LDS at the end, one
+// after the other.  Bound by the keys' and values' stream.
+template <class M, bool FP8, int DP>
+__global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const KernelArgs A) {
+  typedef Layout<DP> L;
+  typedef std::conditional_t<FP8, Bf16, M> W;
+  typedef std::conditional_t<FP8, u32x2, u32x4> Piece;
+  constexpr int kSub = 32, kKeyLoads = FP8 ? DP / 32 : DP / 16, kValueLoads = kSub / L::kWaveLoad, kSumPitch = DP + 4;
+  const PromptAttentionArgs& a = A.a;
+  __shared__ __attribute__((aligned(16))) char lds[kWaves][kSub * L::kPitch];
+  __shared__ __attribute__((aligned(16))) float sums[kPromptFewRows][kSumPitch];
+  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][2 * kSub];
+  __shared__ int64_t row_lds[kWaves][kSub];
+  __shared__ f32x2 ml_lds[kWaves][kPromptFewRows];
+
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Tile t;
+  if (!find_tile(A, blockIdx.x, &t)) return;
+  if (t.b == a.B) {
+    clear_rows(A, t);
+    return;
+  }
+  const int len = min(max(a.lens[t.b], 0), a.max_len), before = len - t.tokens;
+  const int row = min(t.first + n, t.rows - 1), tok = divided(row, A.by_group), g = row - tok * a.G;
+  const int place = before + tok;
+  const int tile_lo = before + divided(t.first, A.by_group);
+  const int tile_hi = before + divided(min(t.first + kPromptFewRows, t.rows) - 1, A.by_group);
+  auto low_of = [&](int place) { return a.window > 0 ? max(place, a.window - 1) - a.window : -1; };
+  const int low = low_of(place), hi = tile_hi + 1;
+  const Walk walk = walk_of(low_of(tile_lo) + 1, hi, a.keep_first);
+  const int subs = hi <= 0 ? 0 : (hi - walk.shift + kSub - 1) / kSub;
+  const int share = (subs + A.p.splits * kWaves - 1) / (A.p.splits * kWaves) * kWaves;
+  const int sub_begin = t.split * share, sub_end = min(subs, sub_begin + share);
+
+  // Queries, dealt out as the keys are: of 16 values the 8 at 8 half, of an 8-bit cache's 32 the 16 at 16 half in two
+  // operands.
+  typename M::V8 q[DP / 16];
+  {
+    const char* const from = (const char*)a.q + ((int64_t)(t.s0 + tok) * a.q_stride_t + (int64_t)(t.head * a.G + g) * a.q_stride_h) * 2;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      const int d = FP8 ? i / 2 * 32 + half * 16 + i % 2 * 8 : i * 16 + half * 8;
+      const u32x4 x = *(const u32x4*)(from + (d < a.D ? d : 0) * 2);
+      q[i] = as_v8<M>(d < a.D ? x : u32x4{0, 0, 0, 0});
+    }
+  }
+  const float to_log2 = (FP8 ? 1.0f : a.scale) * kLog2e;      // (8-bit keys: with the positions' scales)
+  const float cap_in = a.softcap > 0.0f ? 2.0f * to_log2 / a.softcap : 0.0f, cap_out = a.softcap * kLog2e;
+  constexpr float kLift = std::is_same_v<W, F16> ? 7.0f : 0.0f;
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+  float m = kNegInf, l = 0.0f;
+  bool bad = false;             // this lane has left values out that are no finite numbers
+
+  const int32_t* const table = a.table + (int64_t)t.b * a.table_stride;
+  const int last_entry = divided(max(hi - 1, 0), A.by_page);
+  constexpr int kElem = FP8 ? 1 : 2;
+  const char* const kbase = (const char*)a.k_cache + (int64_t)t.head * a.head_stride * kElem;
+  const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
+  const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
+  const int slot = lane % L::kLanes, slot_row = lane / L::kLanes;
+
+  auto ask = [&](int sub) { return table[min(divided(walk.position(sub * kSub) + n, A.by_page), last_entry)]; };
+  auto partial = [&](int pos0) {
+    return pos0 + kSub - 1 > tile_lo || (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kSub > a.keep_first);
+  };
+  u32x4 kreg[kKeyLoads];
+  Piece vreg[kValueLoads];
+  float scale_of = 0.0f;        // of position n's key, in the upper half its value
+  uint32_t loaded = 0;          // which positions of the loaded sub there are
+  auto fetch = [&](int sub, int entry) {
+    const int pos = walk.position(sub * kSub) + n, in_page = pos - divided(pos, A.by_page) * a.page_size;
+    const int id = pos < hi && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
+    const int64_t at = max(id, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
+    loaded = (uint32_t)__ballot(id >= 0);
+    if (half == 0) row_lds[wave][n] = at;
+#pragma unroll
+    for (int i = 0; i < kKeyLoads; ++i) {
+      const int d = FP8 ? i * 32 + half * 16 : i * 16 + half * 8;
+      const u32x4 x = *(const u32x4*)(kbase + at + (d < a.D ? d * kElem : 0));
+      kreg[i] = d < a.D ? x : u32x4{0, 0, 0, 0};
+    }
+    if constexpr (FP8) {
+      const int64_t s = a.scale_blocks == 0 ? t.head
+                                            : ((int64_t)max(id, 0) * a.Hkv + t.head) * a.scale_blocks + divided(in_page, A.by_block);
+      scale_of = id < 0 ? 0.0f : half == 0 ? a.k_scale[s] * a.scale : a.v_scale[s];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kValueLoads; ++i) {
+      const int r = slot_row + i * L::kWaveLoad, piece = L::value_piece(slot, r);
+      vreg[i] = *(const Piece*)(vbase + row_lds[wave][r] + (piece * 8 < a.D ? piece * 8 * kElem : 0));
+    }
+  };
+
+  const int quarter = (lane >> 4) & 1, l16 = lane & 15;
+  const int value_row = half * 4 + (l16 >> 2), value_turn = L::value_turn(value_row);
+  const Lds values = (Lds)&lds[wave][0] + value_row * L::kPitch + (l16 & 3) * 8;
+  int entry = 0;
+  if (sub_begin + wave < sub_end) {
+    fetch(sub_begin + wave, ask(sub_begin + wave));
+    entry = ask(sub_begin + wave + kWaves);
+  }
+  for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
+    const int pos0 = walk.position(sub * kSub);
+    const uint32_t there = loaded;
+    f32x16 x;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kKeyLoads; ++i) {
+      if constexpr (FP8) {
+        x = M::mfma(fp8x8<M>(kreg[i][0], kreg[i][1]), q[2 * i], x);
+        x = M::mfma(fp8x8<M>(kreg[i][2], kreg[i][3]), q[2 * i + 1], x);
+      } else {
+        x = M::mfma(as_v8<M>(kreg[i]), q[i], x);
+      }
+    }
+    const bool look = partial(pos0);
+#pragma unroll
+    for (int i = 0; i < kValueLoads; ++i) {
+      const int r = slot_row + i * L::kWaveLoad;
+      u32x4 v;
+      if constexpr (FP8) {
+        union { typename W::V8 v; u32x4 u; } c;
+        c.v = fp8x8<W>(vreg[i][0], vreg[i][1]);
+        v = c.u;
+      } else {
+        v = vreg[i];
+      }
+      if (!((there >> r) & 1)) v = u32x4{0, 0, 0, 0};
+      if (look && drop_others<W>(v)) bad = true;
+      *(u32x4*)(lds[wave] + r * L::kPitch + slot * 16) = v;
+    }
+    if constexpr (FP8) scale_lds[wave][lane] = scale_of;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (sub + kWaves < sub_end) {
+      fetch(sub + kWaves, entry);
+      entry = ask(sub + 2 * kWaves);
+    }
+
+    if constexpr (FP8) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const f32x4 f = *(const f32x4*)&scale_lds[wave][j * 2 + half * 4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
+      }
+    }
+    if (a.softcap > 0.0f) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = capped(x[j] * cap_in, cap_out);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] *= to_log2;
+    }
+    uint32_t sees = ~0u;
+    if (look || there != ~0u) {
+      sees = bits_below(place + 1 - pos0) & (~bits_below(low + 1 - pos0) | bits_below(a.keep_first - pos0)) & there;
+      sees >>= half * 4;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
+    }
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+    top = over_halves_max(top);
+    if (__any(top > m + kSlack)) {
+      const float m_new = top > m + kSlack ? top : m;
+      const float fix = exp2_fast(m - or_zero(m_new));
+      m = m_new;
+      l *= fix;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= fix;
+    }
+    const float ref = or_zero(m) - kLift;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      union { typename W::T e[8]; typename W::V8 v; } p;
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (FP8) f = *(const f32x4*)&scale_lds[wave][kSub + (j * 8 + i) * 2 + half * 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = j * 8 + i + e;
+          const float w = exp2_fast(x[at] - ref);
+          l += w;
+          // (a scale that is not seen may be anything)
+          p.e[i + e] = (typename W::T)(!FP8 ? w : ((sees >> (at / 4 * 8 + at % 4)) & 1) ? w * f[e] : 0.0f);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const Lds column = values + j * 16 * L::kPitch + ((i * 2 + quarter) ^ value_turn) * 32;
+        union { i16x4 h[2]; typename W::V8 v; } v;
+        v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
+        v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * L::kPitch));
+        acc[i] = W::mfma(v.v, p.v, acc[i]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+
+  // The four wavefronts' sums, relative to 2^ref each.
+  l = over_halves_sum(l);
+  const float ref = l == 0.0f ? kNegInf : or_zero(m) - kLift;
+  if (half == 0) ml_lds[wave][n] = f32x2{ref, l};
+  __syncthreads();
+  auto joined = [&](int r) {
+    float top = kNegInf, all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml_lds[w][r][0]);
+    const float at = or_zero(top);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += ml_lds[w][r][1] * (ml_lds[w][r][1] == 0.0f ? 0.0f : exp2_fast(ml_lds[w][r][0] - at));
+    return f32x2{all == 0.0f ? kNegInf : at, all};
+  };
+  const float f = l == 0.0f ? 0.0f : exp2_fast(ref - or_zero(joined(n)[0]));
+  bad = __any(bad);
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4* const to = (f32x4*)&sums[n][i * 32 + j * 8 + half * 4];
+          f32x4 x = {acc[i][j * 4], acc[i][j * 4 + 1], acc[i][j * 4 + 2], acc[i][j * 4 + 3]};
+          x *= f;
+          *to = w == 0 ? x : *to + x;
+        }
+      }
+      if (bad) {
+        // What was left out, at the positions that a row sees (whatever its weight: an infinity stays one, or becomes NaN).
+#pragma unroll 1
+        for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
+          const int pos0 = walk.position(sub * kSub);
+          if (!partial(pos0)) continue;
+#pragma unroll 1
+          for (int pos = pos0; pos < min(pos0 + kSub, hi); ++pos) {
+            const int in_table = divided(pos, A.by_page), id = table[in_table];
+            if (!(pos <= place && (pos > low || pos < a.keep_first)) || (uint32_t)id >= (uint32_t)a.num_pages) continue;
+            const char* const from = vbase + (int64_t)id * page_bytes + (int64_t)(pos - in_table * a.page_size) * slot_bytes;
+#pragma unroll 1
+            for (int d = half * 4; d < a.D; d += d % 4 == 3 ? 5 : 1) {
+              union { uint16_t u; typename W::T t; } v;
+              if constexpr (FP8)
+                v.t = fp8x8<W>(((const uint8_t*)from)[d], 0)[0];
+              else
+                v.u = ((const uint16_t*)from)[d];
+              if (!finite<W>(v.u)) sums[n][d] += (float)v.t;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  const int quads = a.D / 4;
+  const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
+  for (int i = tid; i < kPromptFewRows * quads; i += 256) {
+    const int r = i / quads, d = (i - r * quads) * 4, my_row = t.first + r;
+    if (my_row >= t.rows) break;
+    const f32x2 st = joined(r);
+    const f32x4 x = *(const f32x4*)&sums[r][d];
+    if (A.p.splits > 1) {
+      if (d == 0) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + r] = st;
+      *(f32x4*)((float*)((char*)a.workspace + A.p.part_at) + (part * kPromptFewRows + r) * DP + d) = x;
+    } else {
+      const int my_tok = divided(my_row, A.by_group), hq = t.head * a.G + (my_row - my_tok * a.G);
+      const int64_t out_row = (int64_t)(t.s0 + my_tok) * a.Hkv * a.G + hq;
+      const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
+      const float top = or_zero(fmaxf(st[0], sink)), fix = st[1] == 0.0f ? 0.0f : exp2_fast(st[0] - top);
+      const float total = st[1] * fix + exp2_fast(sink - top), inv = total == 0.0f ? 0.0f : fix / total;
+      union { typename M::T e[4]; u32x2 u; } o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o.e[e] = (typename M::T)(x[e] * inv);
+      *(u32x2*)((char*)a.out + (out_row * a.D + d) * 2) = o.u;
+      if (d == 0 && a.lse != nullptr) a.lse[out_row] = log_of_sum(top, total, a.sinks != nullptr ? a.sinks + hq : nullptr);
+    }
+  }
+}
+
 // Joins the parts of tiles whose positions several workgroups shared: a lane holds 4 values of a row.
 template <class M>
 __global__ __launch_bounds__(256) void prompt_attention_join_kernel(const KernelArgs A, int padded, int per_tile) {
@@ -623,24 +933,25 @@ __global__ __launch_bounds__(256) void prompt_attention_join_kernel(const Kernel
   one.by_splits = FastDiv{0, -1};
   if (!find_tile(one, rest, &t) || t.b == a.B) return;
   const int lanes = padded <= 64 ? 16 : padded <= 128 ? 32 : 64;      // of a row
+  const int rows = 1 << A.p.row_shift;
   const int at = part * (256 / lanes) + threadIdx.x / lanes, d = threadIdx.x % lanes * 4, row = t.first + at;
-  if (at >= kPromptRows || row >= t.rows || d >= a.D) return;
+  if (at >= rows || row >= t.rows || d >= a.D) return;
   const int tok = divided(row, A.by_group), hq = t.head * a.G + (row - tok * a.G);
   const int64_t slot = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits;
-  const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at) + slot * kPromptRows + at;
-  const float* const parts = (const float*)((const char*)a.workspace + A.p.part_at) + (slot * kPromptRows + at) * padded + d;
+  const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at) + slot * rows + at;
+  const float* const parts = (const float*)((const char*)a.workspace + A.p.part_at) + (slot * rows + at) * padded + d;
   const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
   float top = sink;
-  for (int s = 0; s < A.p.splits; ++s) top = fmaxf(top, ml[s * kPromptRows][0]);
+  for (int s = 0; s < A.p.splits; ++s) top = fmaxf(top, ml[s * rows][0]);
   top = or_zero(top);
   float total = exp2_fast(sink - top);
   f32x4 o = {0, 0, 0, 0};
   for (int s = 0; s < A.p.splits; ++s) {
-    const f32x2 x = ml[s * kPromptRows];
+    const f32x2 x = ml[s * rows];
     if (x[1] == 0.0f) continue;          // (a part that saw nothing has left no sums)
     const float f = exp2_fast(x[0] - top);
     total += x[1] * f;
-    o += f * *(const f32x4*)(parts + (int64_t)s * kPromptRows * padded);
+    o += f * *(const f32x4*)(parts + (int64_t)s * rows * padded);
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   const int64_t out_row = (int64_t)(t.s0 + tok) * a.Hkv * a.G + hq;
@@ -656,9 +967,15 @@ int padded_width(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 
 template <class M, bool FP8, int DP>
 void launch_width(const KernelArgs& A, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)A.p.slots * A.a.Hkv * A.p.splits)), block(256);
-  hipLaunchKernelGGL((prompt_attention_kernel<M, FP8, DP>), grid, block, 0, stream, A);
+  const int rows = 1 << A.p.row_shift;
+  bool few = false;
+  if constexpr (DP <= kPromptFewWidth) {
+    few = rows == kPromptFewRows;
+    if (few) hipLaunchKernelGGL((prompt_attention_few_kernel<M, FP8, DP>), grid, block, 0, stream, A);
+  }
+  if (!few) hipLaunchKernelGGL((prompt_attention_kernel<M, FP8, DP>), grid, block, 0, stream, A);
   if (A.p.splits > 1) {
-    const int per_tile = kPromptRows / (256 / (DP <= 64 ? 16 : DP <= 128 ? 32 : 64));
+    const int per_tile = rows / (256 / (DP <= 64 ? 16 : DP <= 128 ? 32 : 64));
     hipLaunchKernelGGL((prompt_attention_join_kernel<M>), dim3((unsigned)((int64_t)A.p.slots * A.a.Hkv * per_tile)), block, 0,
                        stream, A, DP, per_tile);
   }
@@ -677,23 +994,33 @@ void launch_kind(const KernelArgs& A, hipStream_t stream) {
 
 }  // namespace
 
-int64_t prompt_attention_slots(int B, int tokens, int G) { return (int64_t)tokens * G / kPromptRows + B + 1; }
+// Tiles of 32 rows where the sequences have no more on average.  (Wider heads do not have the registers.)
+static int row_shift_of(int B, int tokens, int G, int D) {
+  return D <= kPromptFewWidth && (int64_t)tokens * G <= (int64_t)kPromptFewRows * B ? 5 : 7;
+}
+
+int64_t prompt_attention_slots(int B, int tokens, int G, int D) {
+  return ((int64_t)tokens * G >> row_shift_of(B, tokens, G, D)) + B + 1;
+}
 
 PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first) {
   PromptAttentionPlan p{};
-  p.slots = (int)prompt_attention_slots(B, tokens, G);
+  p.row_shift = row_shift_of(B, tokens, G, D);
+  p.slots = (int)prompt_attention_slots(B, tokens, G, D);
+  const int rows = 1 << p.row_shift;
   // Where there are fewer tiles than the card holds workgroups, several share the positions of each.
-  const int64_t tiles = ((int64_t)tokens * G / kPromptRows + std::min(B, tokens)) * Hkv;
+  const int64_t tiles = (p.slots - 1) * (int64_t)Hkv;
   int64_t seen = max_len;
-  if (window > 0) seen = std::min<int64_t>(max_len, (int64_t)window + kPromptRows + 16 + std::min(keep_first, max_len) + kPromptKeys);
+  if (window > 0) seen = std::min<int64_t>(max_len, (int64_t)window + rows + 16 + std::min(keep_first, max_len) + kPromptKeys);
   const int64_t most = std::max<int64_t>(1, seen / (4 * kPromptKeys));
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, 1024 / std::max<int64_t>(1, tiles)));
+  const int64_t wanted = rows == kPromptFewRows ? 2048 : 1024;
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, wanted / tiles));
   size_t at = 0;
   auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   if (p.splits > 1) {
-    const size_t rows = (size_t)p.slots * Hkv * p.splits * kPromptRows;
-    p.ml_at = part(rows * 8);
-    p.part_at = part(rows * padded_width(D) * 4);
+    const size_t all = (size_t)p.slots * Hkv * p.splits * rows;
+    p.ml_at = part(all * 8);
+    p.part_at = part(all * padded_width(D) * 4);
   }
   p.bytes = at;
   return p;

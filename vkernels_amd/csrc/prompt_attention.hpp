@@ -11,6 +11,8 @@ namespace vk {
 
 constexpr int kPromptRows = 128;   // of a workgroup: a row is a query head of a token, the G heads of a key/value
                                    // head and a token one behind the other
+constexpr int kPromptFewRows = 32; // ... where sequences have few rows: the wavefronts share the positions instead
+constexpr int kPromptFewWidth = 128;   // ... and heads of no more values
 constexpr int kPromptKeys = 64;    // positions a workgroup takes at a time
 
 struct PromptAttentionArgs {
@@ -35,12 +37,12 @@ struct PromptAttentionArgs {
 };
 
 struct PromptAttentionPlan {
+  int row_shift;            // a tile has 2^row_shift rows
   int slots;                // places for the tiles of all sequences, and of the rows behind them
   int splits;               // workgroups that share a tile's positions; more than 1: joined by a second launch
   size_t ml_at, part_at, bytes;   // parts of the workspace
 };
-// Slots are counted in 32 bits: -1 where they do not fit.
-int64_t prompt_attention_slots(int B, int tokens, int G);
+int64_t prompt_attention_slots(int B, int tokens, int G, int D);
 PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first);
 void launch_prompt_attention(const PromptAttentionArgs& a, int kind, hipStream_t stream);
 
