@@ -110,6 +110,7 @@ struct Layout {
 
 typedef __attribute__((address_space(3))) char* Lds;
 typedef __attribute__((address_space(3))) u32x4* LdsPiece;
+typedef __attribute__((address_space(3))) u32x2* LdsCodes;
 
 // 16 bytes a lane from `from` to LDS, at `to` (uniform) + 16 lane.  Not waited for.
 __device__ __forceinline__ void dma16(const char* from, Lds to) {
@@ -138,6 +139,18 @@ __device__ __forceinline__ bool drop_others(u32x4& v) {
   for (int e = 0; e < 4; ++e) {
     const uint32_t bad = ((v[e] & kExponents) + kOnes) & 0x80008000u;
     v[e] &= ~((bad >> 15) * 0xFFFFu);
+    all |= bad;
+  }
+  return all != 0;
+}
+
+// The same among 16 E4M3 codes: 0x7F and 0xFF.
+__device__ __forceinline__ bool drop_codes(u32x4& v) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t bad = ((v[e] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    v[e] &= ~((bad >> 7) * 0xFFu);
     all |= bad;
   }
   return all != 0;
@@ -199,8 +212,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const int low = low_of(place), wave_low = low_of(wave_lo);
   const int hi = tile_hi + 1;
   const Walk walk = walk_of(low_of(tile_lo) + 1, hi, a.keep_first);
-  const int share = (walk.tiles + A.p.splits - 1) / A.p.splits;
-  const int tile_begin = t.split * share, tile_end = min(walk.tiles, tile_begin + share);
+  const int tile_begin = t.split * A.p.share, tile_end = min(walk.tiles, tile_begin + A.p.share);
 
   // Queries: the second operand of the first product.
   typename M::V8 q[DP / 16];
@@ -628,19 +640,39 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   if (any_bad && tile_begin < tile_end) add_bad((typename M::T*)a.out + out_row * a.D);
 }
 
+// A wavefront's 32 positions in LDS: rows as they are in the cache, pieces of 16 bytes exchanged by the row (each exchange
+// its own inverse) so that 16 rows' pieces spread over the banks.
+template <bool FP8, int DP>
+struct FewLayout {
+  typedef Layout<DP> L;
+  static constexpr int kPitch = FP8 ? L::kPitch / 2 : L::kPitch, kLanes = kPitch / 16;
+  static constexpr int kRows = 64 / kLanes, kLoads = 32 / kRows;      // rows that a load takes; loads
+  static __device__ __forceinline__ int code_turn(int row) { return kLanes == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int key_piece(int slot, int row) {
+    return FP8 ? slot ^ code_turn(row) : L::key_piece(slot, row);
+  }
+  static __device__ __forceinline__ int value_piece(int slot, int row) {
+    return FP8 ? slot ^ code_turn(row) : L::value_piece(slot, row);
+  }
+  static __device__ __forceinline__ int value_pair(int pair, int row) { return pair ^ L::value_turn(row); }
+};
+
 // The same for tiles of 32 rows: every wavefront has all of the rows and takes every fourth 32 positions, by itself.  Keys
-// come as the product's operands straight from the cache, values by way of the wavefront's own part of LDS; the
-// next ones are asked for as soon as these have been taken.  The wavefronts' results meet in LDS at the end, one
+// and values go to the wavefront's own part of LDS as they are (8-bit codes become 16-bit values as they are read from
+// there), the next ones on their way while these are multiplied.  The wavefronts' results meet in LDS at the end, one
 // after the other.  Bound by the keys' and values' stream.
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const KernelArgs A) {
-  typedef Layout<DP> L;
   typedef std::conditional_t<FP8, Bf16, M> W;
-  typedef std::conditional_t<FP8, u32x2, u32x4> Piece;
-  constexpr int kSub = 32, kKeyLoads = FP8 ? DP / 32 : DP / 16, kValueLoads = kSub / L::kWaveLoad, kSumPitch = DP + 4;
+  typedef FewLayout<FP8, DP> F;
+  constexpr int kSub = 32, kSumPitch = DP + 4;
   const PromptAttentionArgs& a = A.a;
-  __shared__ __attribute__((aligned(16))) char lds[kWaves][kSub * L::kPitch];
-  __shared__ __attribute__((aligned(16))) float sums[kPromptFewRows][kSumPitch];
+  union Shared {
+    char tiles[kWaves][2][2][kSub * F::kPitch];   // two buffers of keys and values
+    float sums[kPromptFewRows][kSumPitch];        // (when all are done with those)
+  };
+  __shared__ __attribute__((aligned(16))) Shared lds;
+  auto& sums = lds.sums;
   __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][2 * kSub];
   __shared__ int64_t row_lds[kWaves][kSub];
   __shared__ f32x2 ml_lds[kWaves][kPromptFewRows];
@@ -662,17 +694,20 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
   const int low = low_of(place), hi = tile_hi + 1;
   const Walk walk = walk_of(low_of(tile_lo) + 1, hi, a.keep_first);
   const int subs = hi <= 0 ? 0 : (hi - walk.shift + kSub - 1) / kSub;
-  const int share = (subs + A.p.splits * kWaves - 1) / (A.p.splits * kWaves) * kWaves;
-  const int sub_begin = t.split * share, sub_end = min(subs, sub_begin + share);
+  const int sub_begin = t.split * A.p.share * 2, sub_end = min(subs, sub_begin + A.p.share * 2);
+  if (sub_begin >= sub_end && A.p.splits > 1) {
+    // (a shorter sequence's)
+    const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
+    if (tid < kPromptFewRows) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + tid] = f32x2{kNegInf, 0.0f};
+    return;
+  }
 
-  // Queries, dealt out as the keys are: of 16 values the 8 at 8 half, of an 8-bit cache's 32 the 16 at 16 half in two
-  // operands.
   typename M::V8 q[DP / 16];
   {
     const char* const from = (const char*)a.q + ((int64_t)(t.s0 + tok) * a.q_stride_t + (int64_t)(t.head * a.G + g) * a.q_stride_h) * 2;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-      const int d = FP8 ? i / 2 * 32 + half * 16 + i % 2 * 8 : i * 16 + half * 8;
+      const int d = i * 16 + half * 8;
       const u32x4 x = *(const u32x4*)(from + (d < a.D ? d : 0) * 2);
       q[i] = as_v8<M>(d < a.D ? x : u32x4{0, 0, 0, 0});
     }
@@ -694,28 +729,32 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
   const char* const kbase = (const char*)a.k_cache + (int64_t)t.head * a.head_stride * kElem;
   const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
   const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
-  const int slot = lane % L::kLanes, slot_row = lane / L::kLanes;
+  const int slot = lane % F::kLanes, slot_row = lane / F::kLanes, row_bytes = a.D * kElem;
+  auto lds_keys = [&](int buf) { return (Lds)&lds.tiles[wave][buf][0][0]; };
+  auto lds_values = [&](int buf) { return (Lds)&lds.tiles[wave][buf][1][0]; };
+  // What lies behind a key's last value is zeros, once for all.
+  if (a.D < DP) {
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) {
+      const int r = slot_row + i * F::kRows;
+      if (F::key_piece(slot, r) * 16 >= row_bytes) {
+        *(LdsPiece)(lds_keys(0) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+        *(LdsPiece)(lds_keys(1) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
 
   auto ask = [&](int sub) { return table[min(divided(walk.position(sub * kSub) + n, A.by_page), last_entry)]; };
   auto partial = [&](int pos0) {
     return pos0 + kSub - 1 > tile_lo || (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kSub > a.keep_first);
   };
-  u32x4 kreg[kKeyLoads];
-  Piece vreg[kValueLoads];
   float scale_of = 0.0f;        // of position n's key, in the upper half its value
   uint32_t loaded = 0;          // which positions of the loaded sub there are
-  auto fetch = [&](int sub, int entry) {
+  auto fetch = [&](int sub, int entry, int buf) {
     const int pos = walk.position(sub * kSub) + n, in_page = pos - divided(pos, A.by_page) * a.page_size;
     const int id = pos < hi && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
-    const int64_t at = max(id, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
     loaded = (uint32_t)__ballot(id >= 0);
-    if (half == 0) row_lds[wave][n] = at;
-#pragma unroll
-    for (int i = 0; i < kKeyLoads; ++i) {
-      const int d = FP8 ? i * 32 + half * 16 : i * 16 + half * 8;
-      const u32x4 x = *(const u32x4*)(kbase + at + (d < a.D ? d * kElem : 0));
-      kreg[i] = d < a.D ? x : u32x4{0, 0, 0, 0};
-    }
+    if (half == 0) row_lds[wave][n] = max(id, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
     if constexpr (FP8) {
       const int64_t s = a.scale_blocks == 0 ? t.head
                                             : ((int64_t)max(id, 0) * a.Hkv + t.head) * a.scale_blocks + divided(in_page, A.by_block);
@@ -723,58 +762,67 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    int64_t at[F::kLoads];
 #pragma unroll
-    for (int i = 0; i < kValueLoads; ++i) {
-      const int r = slot_row + i * L::kWaveLoad, piece = L::value_piece(slot, r);
-      vreg[i] = *(const Piece*)(vbase + row_lds[wave][r] + (piece * 8 < a.D ? piece * 8 * kElem : 0));
+    for (int i = 0; i < F::kLoads; ++i) at[i] = row_lds[wave][slot_row + i * F::kRows];
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) {
+      const int piece = F::key_piece(slot, slot_row + i * F::kRows) * 16;
+      if (piece < row_bytes) dma16(kbase + at[i] + piece, lds_keys(buf) + i * F::kRows * F::kPitch);
+    }
+#pragma unroll
+    for (int i = 0; i < F::kLoads; ++i) {
+      const int piece = F::value_piece(slot, slot_row + i * F::kRows) * 16;
+      if (piece < row_bytes) dma16(vbase + at[i] + piece, lds_values(buf) + i * F::kRows * F::kPitch);
     }
   };
 
   const int quarter = (lane >> 4) & 1, l16 = lane & 15;
-  const int value_row = half * 4 + (l16 >> 2), value_turn = L::value_turn(value_row);
-  const Lds values = (Lds)&lds[wave][0] + value_row * L::kPitch + (l16 & 3) * 8;
+  // (8-bit values are read 8 x 16 at a time, 16-bit ones 4 x 16)
+  const int value_row = FP8 ? half * 4 + (l16 >> 1) + (l16 >= 8 ? 4 : 0) : half * 4 + (l16 >> 2);
+  const int value_at = value_row * F::kPitch + (FP8 ? l16 & 1 : l16 & 3) * 8, key_row = n * F::kPitch;
   int entry = 0;
   if (sub_begin + wave < sub_end) {
-    fetch(sub_begin + wave, ask(sub_begin + wave));
+    fetch(sub_begin + wave, ask(sub_begin + wave), 0);
     entry = ask(sub_begin + wave + kWaves);
   }
+  int buf = 0;
   for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
     const int pos0 = walk.position(sub * kSub);
     const uint32_t there = loaded;
+    const bool look = partial(pos0);
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (FP8) scale_lds[wave][lane] = scale_of;
+    if (sub + kWaves < sub_end) {
+      fetch(sub + kWaves, entry, buf ^ 1);
+      entry = ask(sub + 2 * kWaves);
+    }
+    const Lds keys = lds_keys(buf), values = lds_values(buf);
+    buf ^= 1;
+    if (look || there != ~0u) {
+      // Values as the product may have them.
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) {
+        const int r = slot_row + i * F::kRows;
+        const LdsPiece at = (LdsPiece)(values + r * F::kPitch + slot * 16);
+        u32x4 v = *at;
+        if (look && (FP8 ? drop_codes(v) : drop_others<W>(v)) && F::value_piece(slot, r) * 16 < row_bytes) bad = true;
+        *at = (there >> r) & 1 ? v : u32x4{0, 0, 0, 0};
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     f32x16 x;
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kKeyLoads; ++i) {
+    for (int i = 0; i < DP / 16; ++i) {
       if constexpr (FP8) {
-        x = M::mfma(fp8x8<M>(kreg[i][0], kreg[i][1]), q[2 * i], x);
-        x = M::mfma(fp8x8<M>(kreg[i][2], kreg[i][3]), q[2 * i + 1], x);
+        const u32x2 c = *(LdsCodes)(keys + key_row + F::key_piece(i, n) * 16 + half * 8);
+        x = M::mfma(fp8x8<M>(c[0], c[1]), q[i], x);
       } else {
-        x = M::mfma(as_v8<M>(kreg[i]), q[i], x);
+        x = M::mfma(as_v8<M>(*(LdsPiece)(keys + key_row + F::key_piece(i * 2 + half, n) * 16)), q[i], x);
       }
-    }
-    const bool look = partial(pos0);
-#pragma unroll
-    for (int i = 0; i < kValueLoads; ++i) {
-      const int r = slot_row + i * L::kWaveLoad;
-      u32x4 v;
-      if constexpr (FP8) {
-        union { typename W::V8 v; u32x4 u; } c;
-        c.v = fp8x8<W>(vreg[i][0], vreg[i][1]);
-        v = c.u;
-      } else {
-        v = vreg[i];
-      }
-      if (!((there >> r) & 1)) v = u32x4{0, 0, 0, 0};
-      if (look && drop_others<W>(v)) bad = true;
-      *(u32x4*)(lds[wave] + r * L::kPitch + slot * 16) = v;
-    }
-    if constexpr (FP8) scale_lds[wave][lane] = scale_of;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    if (sub + kWaves < sub_end) {
-      fetch(sub + kWaves, entry);
-      entry = ask(sub + 2 * kWaves);
     }
 
     if constexpr (FP8) {
@@ -831,11 +879,19 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
       }
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
-        const Lds column = values + j * 16 * L::kPitch + ((i * 2 + quarter) ^ value_turn) * 32;
-        union { i16x4 h[2]; typename W::V8 v; } v;
-        v.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
-        v.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * L::kPitch));
-        acc[i] = W::mfma(v.v, p.v, acc[i]);
+        typename W::V8 v;
+        if constexpr (FP8) {
+          const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(
+              values + j * 16 * F::kPitch + value_at + F::value_piece(i * 2 + quarter, value_row) * 16));
+          v = fp8x8<W>((uint32_t)c[0], (uint32_t)c[1]);
+        } else {
+          const Lds column = values + j * 16 * F::kPitch + value_at + F::value_pair(i * 2 + quarter, value_row) * 32;
+          union { i16x4 h[2]; typename W::V8 v; } both;
+          both.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
+          both.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * F::kPitch));
+          v = both.v;
+        }
+        acc[i] = W::mfma(v, p.v, acc[i]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -1012,9 +1068,15 @@ PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int
   const int64_t tiles = (p.slots - 1) * (int64_t)Hkv;
   int64_t seen = max_len;
   if (window > 0) seen = std::min<int64_t>(max_len, (int64_t)window + rows + 16 + std::min(keep_first, max_len) + kPromptKeys);
-  const int64_t most = std::max<int64_t>(1, seen / (4 * kPromptKeys));
-  const int64_t wanted = rows == kPromptFewRows ? 2048 : 1024;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, wanted / tiles));
+  // Shares of one size, so that all workgroups that have one work equally long (those behind a shorter sequence's end
+  // have none): shares by the sequence's own length took 108 us for 5 tokens over 1024 to 8192 positions of 32 sequences,
+  // the workgroups of the longest ones ending last.
+  const int64_t keys = std::max<int64_t>(1, (seen + kPromptKeys - 1) / kPromptKeys);
+  const int64_t wanted = rows == kPromptFewRows ? 4096 : 1024;
+  const int64_t splits = std::max<int64_t>(1, std::min(keys / 4, wanted / tiles));
+  p.share = (int)((keys + splits - 1) / splits);
+  if (rows == kPromptFewRows) p.share = (p.share + 1) / 2 * 2;      // (two for each wavefront of two subs)
+  p.splits = (int)((keys + p.share - 1) / p.share);
   size_t at = 0;
   auto part = [&at](size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
   if (p.splits > 1) {

@@ -40,6 +40,7 @@ struct PromptAttentionPlan {
   int row_shift;            // a tile has 2^row_shift rows
   int slots;                // places for the tiles of all sequences, and of the rows behind them
   int splits;               // workgroups that share a tile's positions; more than 1: joined by a second launch
+  int share;                // kPromptKeys positions that each of them takes at most
   size_t ml_at, part_at, bytes;   // parts of the workspace
 };
 int64_t prompt_attention_slots(int B, int tokens, int G, int D);
