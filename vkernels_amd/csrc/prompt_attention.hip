@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     }
   }
   const float k_scale = FP8 ? 1.0f : a.scale;      // (8-bit keys: with the positions' scales)
-  const bool plain = !FP8 && !(a.softcap > 0.0f) && a.scale > 0.0f;
+  const bool plain = !(a.softcap > 0.0f) && (FP8 || a.scale > 0.0f);
   const float to_log2 = k_scale * kLog2e;
   const float cap_in = a.softcap > 0.0f ? 2.0f * k_scale * kLog2e / a.softcap : 0.0f, cap_out = a.softcap * kLog2e;
 
@@ -367,9 +367,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   f32x16 zero;
 #pragma unroll
   for (int j = 0; j < 16; ++j) zero[j] = 0.0f;
+  // The scales of the keys (values) that four of a lane's scores belong to.
+  auto scales_of = [&](int sub, int values, int j) {
+    return *(const f32x4*)&scale_lds[wave][values][(sub * kSub & (2 * kPromptKeys - 1)) + j * 2 + half * 4];
+  };
   auto score = [&](int sub, f32x16& s) {
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) s = M::mfma(read_keys(sub, i), q[i], i == 0 ? zero : s);
+    if constexpr (FP8) {
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const f32x4 f = scales_of(sub, 0, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[j + i] *= f[i];
+      }
+    }
   };
   const int quarter = (lane >> 4) & 1, l16 = lane & 15;
   const int value_row = half * 4 + (l16 >> 2), value_turn = L::value_turn(value_row);
@@ -416,6 +428,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     union { typename W::T e[16]; typename W::V8 v[2]; } p;
     typename M::V8 k[kSteps];
     typename W::V8 v[kSteps];
+    f32x4 f;                     // (8-bit caches: scales)
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) k[i] = read_keys(sub + 1, i);
     __builtin_amdgcn_sched_barrier(0);
@@ -430,7 +443,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) {
         const float w = exp2_fast(__builtin_fmaf(x[j], to_log2, -ref));
         l += w;
-        p.e[j] = (typename W::T)w;
+        if constexpr (FP8) {
+          if (j % 4 == 0) f = scales_of(sub, 1, j);
+          p.e[j] = (typename W::T)(w * f[j % 4]);
+        } else {
+          p.e[j] = (typename W::T)w;
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -440,7 +458,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       acc[i % (DP / 32)] = W::mfma(v[i], p.v[i / (DP / 32)], acc[i % (DP / 32)]);
       if (i + kAhead < kSteps) v[i + kAhead] = read_values(sub, (i + kAhead) / (DP / 32), (i + kAhead) % (DP / 32));
 #pragma unroll
-      for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
+      for (int j = 16 * i / kSteps; j < 16 * (i + 1) / kSteps; ++j) {
+        if constexpr (FP8) {
+          if (j % 4 == 0) f = scales_of(sub + 1, 0, j);
+          next[j] *= f[j % 4];
+        }
+        most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     top = over_halves_max(fmaxf(most[0], most[1]));
@@ -455,17 +479,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     if (hidden(sub)) return;
     // Scores in powers of two, unless they are taken there with the reference.
     float c = to_log2;
-    const int scales = sub * kSub & (2 * kPromptKeys - 1);
     if (!plain) {
       c = 1.0f;
-      if constexpr (FP8) {
-#pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-          const f32x4 f = *(const f32x4*)&scale_lds[wave][0][scales + j * 2 + half * 4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
-        }
-      }
       if (a.softcap > 0.0f) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = capped(x[j] * cap_in, cap_out);
@@ -491,7 +506,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
         f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (FP8) f = *(const f32x4*)&scale_lds[wave][1][scales + (g * 8 + i) * 2 + half * 4];
+        if constexpr (FP8) f = scales_of(sub, 1, g * 8 + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = g * 8 + i + e;
@@ -541,13 +556,17 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     };
     for (int tile = tile_begin; tile < tile_end;) {
       // (heads of more than 128 do not have the registers)
-      if constexpr (!FP8 && DP <= 128) {
+      if constexpr (DP <= 128) {
         if (plain) {
           float top = largest(even);
           for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
             ahead(tile);
             attend_whole(2 * tile, even, odd, top);
             attend_whole(2 * tile + 1, odd, even, top);
+            if constexpr (FP8) {
+              put_keys(tile + 1);
+              put_values(tile + 1, there << 32 | first);
+            }
             landed();
             these = there << 32 | first;
           }
@@ -647,6 +666,10 @@ struct FewLayout {
   typedef Layout<DP> L;
   static constexpr int kPitch = FP8 ? L::kPitch / 2 : L::kPitch, kLanes = kPitch / 16;
   static constexpr int kRows = 64 / kLanes, kLoads = 32 / kRows;      // rows that a load takes; loads
+  // Straight to LDS, in two buffers, where two workgroups of those fit a CU; else by way of registers and one buffer
+  // (32 sequences of up to 8192, 8 heads of 128 in bf16: 163 us with one workgroup a CU, 138 so).
+  static constexpr bool kDirect = FP8 || DP <= 64;
+  static constexpr int kBuffers = kDirect ? 2 : 1;
   static __device__ __forceinline__ int code_turn(int row) { return kLanes == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
   static __device__ __forceinline__ int key_piece(int slot, int row) {
     return FP8 ? slot ^ code_turn(row) : L::key_piece(slot, row);
@@ -668,7 +691,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
   constexpr int kSub = 32, kSumPitch = DP + 4;
   const PromptAttentionArgs& a = A.a;
   union Shared {
-    char tiles[kWaves][2][2][kSub * F::kPitch];   // two buffers of keys and values
+    char tiles[kWaves][F::kBuffers][2][kSub * F::kPitch];   // keys and values
     float sums[kPromptFewRows][kSumPitch];        // (when all are done with those)
   };
   __shared__ __attribute__((aligned(16))) Shared lds;
@@ -738,8 +761,8 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
     for (int i = 0; i < F::kLoads; ++i) {
       const int r = slot_row + i * F::kRows;
       if (F::key_piece(slot, r) * 16 >= row_bytes) {
-        *(LdsPiece)(lds_keys(0) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
-        *(LdsPiece)(lds_keys(1) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < F::kBuffers; ++b) *(LdsPiece)(lds_keys(b) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
       }
     }
   }
@@ -748,6 +771,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
   auto partial = [&](int pos0) {
     return pos0 + kSub - 1 > tile_lo || (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kSub > a.keep_first);
   };
+  u32x4 kreg[F::kLoads], vreg[F::kLoads];      // (those that do not go straight to LDS)
   float scale_of = 0.0f;        // of position n's key, in the upper half its value
   uint32_t loaded = 0;          // which positions of the loaded sub there are
   auto fetch = [&](int sub, int entry, int buf) {
@@ -768,12 +792,18 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
 #pragma unroll
     for (int i = 0; i < F::kLoads; ++i) {
       const int piece = F::key_piece(slot, slot_row + i * F::kRows) * 16;
-      if (piece < row_bytes) dma16(kbase + at[i] + piece, lds_keys(buf) + i * F::kRows * F::kPitch);
+      if constexpr (!F::kDirect)
+        kreg[i] = *(const u32x4*)(kbase + at[i] + (piece < row_bytes ? piece : 0));
+      else if (piece < row_bytes)
+        dma16(kbase + at[i] + piece, lds_keys(buf) + i * F::kRows * F::kPitch);
     }
 #pragma unroll
     for (int i = 0; i < F::kLoads; ++i) {
       const int piece = F::value_piece(slot, slot_row + i * F::kRows) * 16;
-      if (piece < row_bytes) dma16(vbase + at[i] + piece, lds_values(buf) + i * F::kRows * F::kPitch);
+      if constexpr (!F::kDirect)
+        vreg[i] = *(const u32x4*)(vbase + at[i] + (piece < row_bytes ? piece : 0));
+      else if (piece < row_bytes)
+        dma16(vbase + at[i] + piece, lds_values(buf) + i * F::kRows * F::kPitch);
     }
   };
 
@@ -791,14 +821,23 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
     const int pos0 = walk.position(sub * kSub);
     const uint32_t there = loaded;
     const bool look = partial(pos0);
-    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const Lds keys = lds_keys(buf), values = lds_values(buf);
+    buf ^= F::kBuffers - 1;
+    if constexpr (F::kDirect) {
+      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) {
+        const int r = slot_row + i * F::kRows;
+        if (F::key_piece(slot, r) * 16 < row_bytes) *(LdsPiece)(keys + r * F::kPitch + slot * 16) = kreg[i];
+        *(LdsPiece)(values + r * F::kPitch + slot * 16) = vreg[i];
+      }
+    }
     if constexpr (FP8) scale_lds[wave][lane] = scale_of;
     if (sub + kWaves < sub_end) {
-      fetch(sub + kWaves, entry, buf ^ 1);
+      fetch(sub + kWaves, entry, buf);
       entry = ask(sub + 2 * kWaves);
     }
-    const Lds keys = lds_keys(buf), values = lds_values(buf);
-    buf ^= 1;
     if (look || there != ~0u) {
       // Values as the product may have them.
 #pragma unroll
@@ -978,44 +1017,68 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
   }
 }
 
-// Joins the parts of tiles whose positions several workgroups shared: a lane holds 4 values of a row.
+// Joins the parts of tiles whose positions several workgroups shared: a lane holds 4 values of a row.  Where there are many
+// parts, all of a workgroup's lanes have the same row and share them (`groups` of lanes); else each has a row.
 template <class M>
-__global__ __launch_bounds__(256) void prompt_attention_join_kernel(const KernelArgs A, int padded, int per_tile) {
+__global__ __launch_bounds__(256) void prompt_attention_join_kernel(const KernelArgs A, int padded, int groups, int per_tile) {
   const PromptAttentionArgs& a = A.a;
-  const int rest = blockIdx.x / per_tile, part = blockIdx.x % per_tile;
+  __shared__ f32x4 sum_lds[256];
+  __shared__ f32x2 ml_lds[256 / 16];
+  const int rest = blockIdx.x / per_tile, piece = blockIdx.x % per_tile;
   Tile t;
   KernelArgs one = A;
   one.p.splits = 1;
   one.by_splits = FastDiv{0, -1};
   if (!find_tile(one, rest, &t) || t.b == a.B) return;
   const int lanes = padded <= 64 ? 16 : padded <= 128 ? 32 : 64;      // of a row
-  const int rows = 1 << A.p.row_shift;
-  const int at = part * (256 / lanes) + threadIdx.x / lanes, d = threadIdx.x % lanes * 4, row = t.first + at;
-  if (at >= rows || row >= t.rows || d >= a.D) return;
+  const int rows = 1 << A.p.row_shift, group = threadIdx.x / lanes, in_row = threadIdx.x % lanes, d = in_row * 4;
+  const int at = groups > 1 ? piece : piece * (256 / lanes) + group, row = t.first + at;
+  if (groups > 1 ? row >= t.rows : at >= rows || row >= t.rows || d >= a.D) return;      // (all lanes, where they meet below)
   const int tok = divided(row, A.by_group), hq = t.head * a.G + (row - tok * a.G);
   const int64_t slot = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits;
   const f32x2* const ml = (const f32x2*)((const char*)a.workspace + A.p.ml_at) + slot * rows + at;
-  const float* const parts = (const float*)((const char*)a.workspace + A.p.part_at) + (slot * rows + at) * padded + d;
-  const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
-  float top = sink;
-  for (int s = 0; s < A.p.splits; ++s) top = fmaxf(top, ml[s * rows][0]);
-  top = or_zero(top);
-  float total = exp2_fast(sink - top);
+  const float* const parts = (const float*)((const char*)a.workspace + A.p.part_at) + (slot * rows + at) * padded + (d < a.D ? d : 0);
+  const int first = groups > 1 ? group : 0;
+  float top = kNegInf;
+#pragma unroll 4
+  for (int s = first; s < A.p.splits; s += groups) top = fmaxf(top, ml[(int64_t)s * rows][0]);
+  float total = 0.0f;
   f32x4 o = {0, 0, 0, 0};
-  for (int s = 0; s < A.p.splits; ++s) {
-    const f32x2 x = ml[s * rows];
+#pragma unroll 4
+  for (int s = first; s < A.p.splits; s += groups) {
+    const f32x2 x = ml[(int64_t)s * rows];
     if (x[1] == 0.0f) continue;          // (a part that saw nothing has left no sums)
-    const float f = exp2_fast(x[0] - top);
+    const float f = exp2_fast(x[0] - or_zero(top));
     total += x[1] * f;
     o += f * *(const f32x4*)(parts + (int64_t)s * rows * padded);
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  if (groups > 1) {
+    sum_lds[threadIdx.x] = o;
+    if (in_row == 0) ml_lds[group] = f32x2{top, total};
+    __syncthreads();
+    if (group > 0 || d >= a.D) return;
+    float all = kNegInf;
+    for (int i = 0; i < groups; ++i) all = fmaxf(all, ml_lds[i][0]);
+    o = f32x4{0, 0, 0, 0};
+    total = 0.0f;
+    for (int i = 0; i < groups; ++i) {
+      const f32x2 x = ml_lds[i];
+      const float f = x[1] == 0.0f ? 0.0f : exp2_fast(x[0] - or_zero(all));
+      total += x[1] * f;
+      o += f * sum_lds[i * lanes + in_row];
+    }
+    top = all;
+  }
+  const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
+  const float ref = or_zero(fmaxf(top, sink)), fix = total == 0.0f ? 0.0f : exp2_fast(or_zero(top) - ref);
+  total = total * fix + exp2_fast(sink - ref);
+  const float inv = total == 0.0f ? 0.0f : fix / total;
   const int64_t out_row = (int64_t)(t.s0 + tok) * a.Hkv * a.G + hq;
   union { typename M::T e[4]; u32x2 u; } r;
 #pragma unroll
   for (int e = 0; e < 4; ++e) r.e[e] = (typename M::T)(o[e] * inv);
   *(u32x2*)((char*)a.out + (out_row * a.D + d) * 2) = r.u;
-  if (d == 0 && a.lse != nullptr) a.lse[out_row] = log_of_sum(top, total, a.sinks != nullptr ? a.sinks + hq : nullptr);
+  if (d == 0 && a.lse != nullptr) a.lse[out_row] = log_of_sum(ref, total, a.sinks != nullptr ? a.sinks + hq : nullptr);
 }
 
 int padded_width(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
@@ -1031,9 +1094,10 @@ void launch_width(const KernelArgs& A, hipStream_t stream) {
   }
   if (!few) hipLaunchKernelGGL((prompt_attention_kernel<M, FP8, DP>), grid, block, 0, stream, A);
   if (A.p.splits > 1) {
-    const int per_tile = rows / (256 / (DP <= 64 ? 16 : DP <= 128 ? 32 : 64));
+    const int lanes = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
+    const int groups = A.p.splits >= 16 ? 256 / lanes : 1, per_tile = groups > 1 ? rows : rows / (256 / lanes);
     hipLaunchKernelGGL((prompt_attention_join_kernel<M>), dim3((unsigned)((int64_t)A.p.slots * A.a.Hkv * per_tile)), block, 0,
-                       stream, A, DP, per_tile);
+                       stream, A, DP, groups, per_tile);
   }
 }
 
@@ -1073,7 +1137,7 @@ PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int
   // the workgroups of the longest ones ending last.
   const int64_t keys = std::max<int64_t>(1, (seen + kPromptKeys - 1) / kPromptKeys);
   const int64_t wanted = rows == kPromptFewRows ? 4096 : 1024;
-  const int64_t splits = std::max<int64_t>(1, std::min(keys / 4, wanted / tiles));
+  const int64_t splits = std::max<int64_t>(1, std::min({keys / 4, wanted / tiles, (int64_t)64}));
   p.share = (int)((keys + splits - 1) / splits);
   if (rows == kPromptFewRows) p.share = (p.share + 1) / 2 * 2;      // (two for each wavefront of two subs)
   p.splits = (int)((keys + p.share - 1) / p.share);
