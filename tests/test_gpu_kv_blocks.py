@@ -102,6 +102,29 @@ def test_one_token_calls_with_rows_of_a_padded_batch(hip_lib):
     c.append([4, 0, 6])
 
 
+def test_quotients_are_rounded_as_divisions(hip_lib):
+    """Scales of every kind of significand, all ones among them, over the types' range; values near the borders between
+    codes: a quotient that is off by its last bit would give another code there."""
+    g = torch.Generator().manual_seed(11)
+    n, D = 4096, 256
+    for dtype, low, high in ((BF16, -100, 100), (F16, -9, 4)):
+        size = torch.exp2(torch.randint(low, high, (n, 1, 1), generator=g).double()) * (1 + torch.rand((n, 1, 1), generator=g).double())
+        border = torch.randint(8, 16, (n, 1, D), generator=g).double() + 0.5        # between two significands of a code
+        x = size * border / 16 * torch.exp2(-torch.randint(0, 12, (n, 1, D), generator=g).double()) * (1 + 2e-3 * torch.randn((n, 1, D), generator=g).double())
+        x = (x * torch.sign(torch.randn((n, 1, D), generator=g).double())).to(dtype)
+        x[:, :, :1] = (448 * size).clamp(max=6e4 if dtype is F16 else 3e38).to(dtype)
+        c = Cache([n], 1, D, 16, 1)
+        lens, starts = torch.tensor([n], dtype=torch.int32, device=dev()), torch.tensor([0, n], dtype=torch.int32, device=dev())
+        rows = x.to(dev())
+        kv.kv_cache_append(rows, rows, c.k, c.v, c.table, lens, query_start=starts, k_scale=c.ks, v_scale=c.vs)
+        page, slot = c.table[0].long()[torch.arange(n, device=dev()) // 16], torch.arange(n, device=dev()) % 16
+        scale = x.float().abs().amax((1, 2)) / 448.0
+        assert torch.equal(c.ks[page, 0, slot].cpu(), scale)
+        want = (x.float() / scale[:, None, None]).clamp(-448, 448).to(FP8).view(torch.uint8)
+        for got in (c.k, c.v):
+            assert torch.equal(got.view(torch.uint8)[page, :, slot].cpu(), want)
+
+
 def test_zeros_and_tiny_values(hip_lib):
     c = Cache([40], 2, 64, 16, 8)
     zeros = [torch.zeros((3, 2, 64), dtype=BF16, device=dev()) for _ in range(2)]

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "kv_blocks.hpp"
 #include "kv_rows.hpp"
 
@@ -11,33 +13,102 @@ namespace {
 
 typedef kv_u32x4 u32x4;
 typedef kv_u32x2 u32x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 
 constexpr int kRowLoads = 4;     // pieces of new rows that a lane holds
 constexpr int kOldLoads = 4;     // pieces of older codes that it asks for at once
 
-// The largest magnitude among 8 values that is a finite number.
-__device__ __forceinline__ float finite_size(u32x4 x, bool bf16) {
-  float size = 0.0f;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+
+// The largest magnitudes of the lower and of the upper halves' 16-bit values, as their bits (which order as they do).
+__device__ __forceinline__ uint32_t larger_halves(uint32_t x, uint32_t y) {
+  union { uint32_t u; u16x2 v; } a, b;
+  a.u = x & 0x7FFF7FFFu;
+  b.u = y & 0x7FFF7FFFu;
+  a.v = __builtin_elementwise_max(a.v, b.v);
+  return a.u;
+}
+// ... with zeros for what is no finite number (an exponent of ones carries into the half's sign).
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x, bool bf16) {
+  const uint32_t bad = ((x & (bf16 ? 0x7F807F80u : 0x7C007C00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+  return x & ~((bad >> 15) * 0xFFFFu);
+}
+__device__ __forceinline__ uint32_t largest_halves(uint32_t size, u32x4 x) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float f = fabsf(f16_bits_to_f32(i & 1 ? x[i / 2] >> 16 : x[i / 2] & 0xFFFFu, bf16));
-    size = f < __builtin_inff() && f > size ? f : size;
-  }
+  for (int i = 0; i < 4; ++i) size = larger_halves(size, x[i]);
   return size;
+}
+__device__ __forceinline__ u32x4 finite_values(u32x4 x, bool bf16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = finite_halves(x[i], bf16);
+  return x;
+}
+__device__ __forceinline__ uint32_t larger_half(uint32_t size) { return max(size & 0xFFFFu, size >> 16); }
+__device__ __forceinline__ uint32_t infinity_of(bool bf16) { return bf16 ? 0x7F80u : 0x7C00u; }
+
+// Division by a block's scale.  With r the reciprocal, correctly rounded, and q = x r rounded, q + (x - q s) r is the
+// quotient, correctly rounded, unless the scale's significand is all ones (Markstein 1990) or the remainder leaves the
+// range of 32-bit floats: such scales are divided by.  (A code's rounding looks at quotients from 2^-11 on, so that
+// scales from 2^-80 to 2^80 keep all of it in range.)
+struct Scale {
+  float s, r;
+  bool simple;
+  __device__ __forceinline__ explicit Scale(float scale) {
+    // (a block of zeros has scale 0, and its codes are zeros)
+    s = scale > 0.0f ? scale : 1.0f;
+    r = 1.0f / s;
+    simple = s >= 0x1p-80f && s <= 0x1p80f && (__float_as_uint(s) & 0x7FFFFFu) != 0x7FFFFFu;
+  }
+  __device__ __forceinline__ float divided(float x) const {
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q);
+  }
+};
+__device__ __forceinline__ u32x2 codes_by(u32x4 x, const Scale& by, bool bf16) {
+  if (!by.simple) return e4m3_codes(x, by.s, bf16);
+  u32x2 codes;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = x[2 * i + j / 2];
+      const float v = f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu, bf16), q = by.divided(v);
+      f[j] = fabsf(v) < __builtin_inff() ? q : v;      // (an infinity and NaN as they are)
+    }
+    codes[i] = e4m3x4(f);
+  }
+  return codes;
+}
+
+// 8 codes times a factor, as codes.
+__device__ __forceinline__ u32x2 scaled_codes(u32x2 c, float factor) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[w], true);
+    const float f[4] = {p[0] * factor, p[1] * factor, q[0] * factor, q[1] * factor};
+    c[w] = e4m3x4(f);
+  }
+  return c;
 }
 
 // A block of positions has one scale for a head: s = max(s of its older positions, max |x| / 448 over its new
 // rows), codes the E4M3 values nearest to x / s.  Where s grows, the older codes c become those nearest to
 // c (s_old / s).
-// A wavefront takes the keys or the values of one block in one head: nobody else touches them, so that the
-// codes can be read, scaled and written back without an order among wavefronts.  Its lanes hold the
-// new rows' pieces of 8 values (up to 4 each; of larger blocks they are read again for the
-// second pass, from the cache).
-template <bool RAGGED>
-__global__ __launch_bounds__(256) void kv_quantise_kernel(const KvQuantiseArgs A, int bf16) {
+// A wavefront, or of larger blocks a workgroup, takes the keys or the values of one block in one head: nobody else
+// touches them, so that the codes can be read, scaled and written back without an order among them.  Its lanes hold the
+// new rows' pieces of 8 values (up to 4 each; of still larger blocks they are read again for the second pass, from the
+// cache).  Bound by a chain of dependent loads (the sequence, its length, its page, the block's scale) beside the rows',
+// and by the vector instructions of the codes.
+template <bool RAGGED, bool WORKGROUP>
+__global__ __launch_bounds__(256) void kv_quantise_kernel(const KvQuantiseArgs A, int bf16_) {
+  constexpr int kLanes = WORKGROUP ? 256 : 64;
+  __shared__ uint32_t size_lds[4];
   const KvAppendArgs& a = A.a;
-  const int lane = threadIdx.x & 63;
-  const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool bf16 = bf16_ != 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = WORKGROUP ? threadIdx.x : threadIdx.x & 63;
+  const int64_t at = WORKGROUP ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
   if (at >= (int64_t)A.slots * a.Hkv * 2) return;
   const int unit = (int)(at >> 1), is_v = (int)(at & 1);
   const int slot = divided(unit, A.by_heads), h = unit - slot * a.Hkv;
@@ -71,20 +142,36 @@ __global__ __launch_bounds__(256) void kv_quantise_kernel(const KvQuantiseArgs A
   };
   u32x4 x[kRowLoads];
 #pragma unroll
-  for (int i = 0; i < kRowLoads; ++i) x[i] = load(min(lane + 64 * i, n - 1));
+  for (int i = 0; i < kRowLoads; ++i) x[i] = load(min(lane + kLanes * i, n - 1));
   if ((uint32_t)page >= (uint32_t)a.num_pages) return;
   const int first_slot = begin - in_table * a.page_size;      // of the page
   float* const scale_at = (is_v ? A.v_scale : A.k_scale) + ((int64_t)page * a.Hkv + h) * A.blocks + divided(first_slot, A.by_block);
   const bool older = from > begin;
   const float before = older ? *scale_at : 0.0f;
 
-  float size = 0.0f;
+  // (the largest magnitude, and once more without what is no finite number where there is such a value)
+  auto largest = [&](bool finite) {
+    uint32_t size = 0;
 #pragma unroll
-  for (int i = 0; i < kRowLoads; ++i) size = fmaxf(size, finite_size(x[i], bf16 != 0));
-  for (int i = lane + 64 * kRowLoads; i < n; i += 64) size = fmaxf(size, finite_size(load(i), bf16 != 0));
+    for (int i = 0; i < kRowLoads; ++i) size = largest_halves(size, finite ? finite_values(x[i], bf16) : x[i]);
+    for (int i = lane + kLanes * kRowLoads; i < n; i += kLanes) {
+      const u32x4 y = load(i);
+      size = largest_halves(size, finite ? finite_values(y, bf16) : y);
+    }
+    size = larger_half(size);
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) size = fmaxf(size, __shfl_xor(size, d));
-  const float needed = size / 448.0f;
+    for (int d = 1; d < 64; d <<= 1) size = max(size, (uint32_t)__shfl_xor((int)size, d));
+    if constexpr (WORKGROUP) {
+      __syncthreads();      // (twice in a row: the first sizes have been read)
+      if ((threadIdx.x & 63) == 0) size_lds[wave] = size;
+      __syncthreads();
+      size = max(max(size_lds[0], size_lds[1]), max(size_lds[2], size_lds[3]));
+    }
+    return size;
+  };
+  uint32_t size = largest(false);
+  if (size >= infinity_of(bf16)) size = largest(true);
+  const float needed = f16_bits_to_f32(size, bf16) / 448.0f;
   const bool grows = older && !(before >= needed);
   const float scale = older && !grows ? before : needed;
 
@@ -95,110 +182,188 @@ __global__ __launch_bounds__(256) void kv_quantise_kernel(const KvQuantiseArgs A
   if (grows) {
     const float factor = before / scale;
     const int n_old = (from - begin) * pieces;
-    for (int i0 = lane; i0 < n_old; i0 += 64 * kOldLoads) {
+    for (int i0 = lane; i0 < n_old; i0 += kLanes * kOldLoads) {
       u32x2 c[kOldLoads];
 #pragma unroll
       for (int j = 0; j < kOldLoads; ++j) {
-        const int i = min(i0 + 64 * j, n_old - 1), row = divided(i, a.by_pieces);
+        const int i = min(i0 + kLanes * j, n_old - 1), row = divided(i, a.by_pieces);
         c[j] = *code_at(begin + row, i - row * pieces);
       }
 #pragma unroll
       for (int j = 0; j < kOldLoads; ++j) {
-        const int i = i0 + 64 * j, row = divided(i, a.by_pieces);
+        const int i = i0 + kLanes * j, row = divided(i, a.by_pieces);
         if (i >= n_old) break;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          typedef __attribute__((ext_vector_type(2))) float f32x2;
-          const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[j][w], false);
-          const f32x2 q = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[j][w], true);
-          const float f[4] = {p[0] * factor, p[1] * factor, q[0] * factor, q[1] * factor};
-          c[j][w] = e4m3x4(f);
-        }
-        *code_at(begin + row, i - row * pieces) = c[j];
+        *code_at(begin + row, i - row * pieces) = scaled_codes(c[j], factor);
       }
     }
   }
-  // (a block of zeros has scale 0, and its codes are zeros)
-  const float by = scale > 0.0f ? scale : 1.0f;
+  const Scale by(scale);
 #pragma unroll
   for (int i = 0; i < kRowLoads; ++i) {
-    const int j = lane + 64 * i, row = divided(j, a.by_pieces);
-    if (j < n) *code_at(from + row, j - row * pieces) = e4m3_codes(x[i], by, bf16 != 0);
+    const int j = lane + kLanes * i, row = divided(j, a.by_pieces);
+    if (j < n) *code_at(from + row, j - row * pieces) = codes_by(x[i], by, bf16);
   }
-  for (int j = lane + 64 * kRowLoads; j < n; j += 64) {
+  for (int j = lane + kLanes * kRowLoads; j < n; j += kLanes) {
     const int row = divided(j, a.by_pieces);
-    *code_at(from + row, j - row * pieces) = e4m3_codes(load(j), by, bf16 != 0);
+    *code_at(from + row, j - row * pieces) = codes_by(load(j), by, bf16);
   }
   if (lane == 0 && (grows || !older)) *scale_at = scale;
 }
 
-// ---- reading back ----------------------------------------------------------------------------------
-
-// A thread takes the same 8 values of a position's key and value in a head, as the append does.  Bound by the
-// rows read and written.
-template <bool FP8, bool BF16>
-__global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
-  const int per_token = a.Hkv * a.pieces;
-  const int first = (int)(blockIdx.x * 256 + (threadIdx.x & ~63)), idx = (int)(blockIdx.x * 256 + threadIdx.x);
-  if (first >= a.tokens * per_token) return;
-  const int t = divided(idx, a.by_token), rest = idx - t * per_token;
-  const int h = divided(rest, a.by_pieces), d = (rest - h * a.pieces) * 8;
-  const int there = min(t, a.tokens - 1);
-  int seq = there;
-  bool mine = true;          // the row belongs to a sequence
-  if (a.starts != nullptr) {
-    const int t0 = divided(first, a.by_token);
-    seq = last_not_above(a.B, t0, [&](int i) { return a.starts[i]; });
-    while (seq + 1 < a.B && a.starts[seq + 1] <= there) ++seq;
-    mine = there >= a.starts[seq] && there < a.starts[seq + 1];
+// Blocks of one position: a scale for each row, that nothing else touches.  A row's lanes (a power of two) take 8 values
+// each of its key and its value; rows one behind the other as the append's.  (By wavefronts for a block, as above,
+// 8191 tokens of 8 heads of 128 took 108 us.)
+__global__ __launch_bounds__(256) void kv_quantise_rows_kernel(const KvQuantiseArgs A, int bf16, int lanes, int lane_shift) {
+  const KvAppendArgs& a = A.a;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t first = idx - (threadIdx.x & 63);
+  if (first >= ((int64_t)a.tokens * a.Hkv << lane_shift)) return;
+  const int unit = (int)min(idx >> lane_shift, (int64_t)a.tokens * a.Hkv - 1), piece = threadIdx.x & (lanes - 1);
+  const bool real = idx >> lane_shift <= unit && piece < a.pieces;
+  const int t = divided(unit, A.by_heads), h = unit - t * a.Hkv, d = min(piece, a.pieces - 1) * 8;
+  const u32x4 k = *(const u32x4*)((const char*)a.k + ((int64_t)t * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2);
+  const u32x4 v = *(const u32x4*)((const char*)a.v + ((int64_t)t * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
+  uint32_t k_size = larger_half(largest_halves(0, finite_values(k, bf16 != 0)));
+  uint32_t v_size = larger_half(largest_halves(0, finite_values(v, bf16 != 0)));
+  for (int i = 1; i < lanes; i <<= 1) {
+    k_size = max(k_size, (uint32_t)__shfl_xor((int)k_size, i));
+    v_size = max(v_size, (uint32_t)__shfl_xor((int)v_size, i));
   }
-  if (t >= a.tokens) return;
+  const float ks = f16_bits_to_f32(k_size, bf16 != 0) / 448.0f, vs = f16_bits_to_f32(v_size, bf16 != 0) / 448.0f;
+  int seq = t;
+  if (a.starts != nullptr) {
+    seq = last_not_above(a.B, divided((int)(first >> lane_shift), A.by_heads), [&](int i) { return a.starts[i]; });
+    while (seq + 1 < a.B && a.starts[seq + 1] <= t) ++seq;
+    if (t < a.starts[seq]) return;
+  }
   const int len = a.lens[seq];
   const int pos = a.starts != nullptr ? len - a.starts[seq + 1] + t : len - 1;
-  int page = -1, in_table = 0;
-  if (mine && pos >= 0 && pos < len) {
-    in_table = divided(pos, a.by_page);
-    if (in_table < a.table_width) page = a.table[(int64_t)seq * a.table_stride + in_table];
+  if (!real || pos < 0 || pos >= len) return;
+  const int in_table = divided(pos, a.by_page);
+  if (in_table >= a.table_width) return;
+  const int page = a.table[(int64_t)seq * a.table_stride + in_table];
+  if ((uint32_t)page >= (uint32_t)a.num_pages) return;
+  const int slot = pos - in_table * a.page_size;
+  const int64_t to = (int64_t)page * a.page_stride + (int64_t)h * a.head_stride + (int64_t)slot * a.slot_stride + d;
+  *(u32x2*)((char*)a.k_cache + to) = codes_by(k, Scale(ks), bf16 != 0);
+  *(u32x2*)((char*)a.v_cache + to) = codes_by(v, Scale(vs), bf16 != 0);
+  if (piece == 0) {
+    const int64_t at = ((int64_t)page * a.Hkv + h) * A.blocks + slot;
+    A.k_scale[at] = ks;
+    A.v_scale[at] = vs;
   }
-  u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-  if ((uint32_t)page < (uint32_t)a.num_pages) {
-    const int slot = pos - in_table * a.page_size;
-    const int64_t from = (int64_t)page * a.page_stride + (int64_t)h * a.head_stride + (int64_t)slot * a.slot_stride + d;
-    if constexpr (!FP8) {
-      k = *(const u32x4*)((const char*)a.k_cache + from * 2);
-      v = *(const u32x4*)((const char*)a.v_cache + from * 2);
-    } else {
-      const u32x2 kc = *(const u32x2*)((const char*)a.k_cache + from), vc = *(const u32x2*)((const char*)a.v_cache + from);
-      const int64_t s = a.blocks == 0 ? h : ((int64_t)page * a.Hkv + h) * a.blocks + divided(slot, a.by_block);
-      const float ks = a.k_scale[s], vs = a.v_scale[s];
-      typedef __attribute__((ext_vector_type(2))) float f32x2;
-      auto pack = [](float x, float y) -> uint32_t {
-        if constexpr (BF16) {
-          union { __bf16 e[2]; uint32_t u; } c;
-          c.e[0] = (__bf16)x;
-          c.e[1] = (__bf16)y;
-          return c.u;
-        } else {
-          union { _Float16 e[2]; uint32_t u; } c;
-          c.e[0] = (_Float16)x;
-          c.e[1] = (_Float16)y;
-          return c.u;
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f32x2 k0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)kc[i], false), k1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)kc[i], true);
-        const f32x2 v0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[i], false), v1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)vc[i], true);
-        k[2 * i] = pack(k0[0] * ks, k0[1] * ks);
-        k[2 * i + 1] = pack(k1[0] * ks, k1[1] * ks);
-        v[2 * i] = pack(v0[0] * vs, v0[1] * vs);
-        v[2 * i + 1] = pack(v1[0] * vs, v1[1] * vs);
+}
+
+// ---- reading back ----------------------------------------------------------------------------------
+
+// 16 bytes of a row that are read: 8 values, or 16 codes as values of 16 bits in the other kinds.
+template <bool FP8, bool BF16>
+__device__ __forceinline__ void store_row(u32x4 x, float scale, char* to) {
+  if constexpr (!FP8) {
+    *(u32x4*)to = x;
+  } else {
+    auto pack = [](float x, float y) -> uint32_t {
+      if constexpr (BF16) {
+        union { __bf16 e[2]; uint32_t u; } c;
+        c.e[0] = (__bf16)x;
+        c.e[1] = (__bf16)y;
+        return c.u;
+      } else {
+        union { _Float16 e[2]; uint32_t u; } c;
+        c.e[0] = (_Float16)x;
+        c.e[1] = (_Float16)y;
+        return c.u;
       }
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      u32x4 y;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int c = (int)x[2 * i + j];
+        const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
+        y[2 * j] = pack(p[0] * scale, p[1] * scale);
+        y[2 * j + 1] = pack(q[0] * scale, q[1] * scale);
+      }
+      *(u32x4*)(to + 16 * i) = y;
     }
   }
-  if (!mine && !a.clear_rest) return;
-  *(u32x4*)((char*)a.k + ((int64_t)t * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2) = k;
-  *(u32x4*)((char*)a.v + ((int64_t)t * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2) = v;
+}
+
+// A workgroup takes `chunk` rows in all heads: a lane each looks up where they lie, then every thread reads 16 bytes
+// of a key and of a value in a head, four of each at a time.  Bound by the rows read and written.  (A thread for 8 values
+// with look-ups of its own took 116 us for 60001 positions of 8 heads of 128 in 8 bits, 369 MB.)
+template <bool FP8, bool BF16>
+__global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
+  constexpr int kAtOnce = 4;
+  __shared__ int64_t row_lds[kKvReadChunk], scale_lds[kKvReadChunk];     // (elements; -1: zeros, -2: left as it is)
+  const int tid = threadIdx.x, t0 = blockIdx.x * a.chunk;
+  const int rows = min(a.chunk, a.tokens - t0);
+  if (tid < 64) {
+    int seq = 0;
+    if (a.starts != nullptr) seq = last_not_above(a.B, t0, [&](int i) { return a.starts[i]; });
+    if (tid < rows) {
+      const int t = t0 + tid;
+      bool mine = true;          // the row belongs to a sequence
+      if (a.starts != nullptr) {
+        while (seq + 1 < a.B && a.starts[seq + 1] <= t) ++seq;
+        mine = t >= a.starts[seq] && t < a.starts[seq + 1];
+      } else {
+        seq = t;
+      }
+      int64_t row = mine || a.clear_rest ? -1 : -2, scale = 0;
+      const int len = a.lens[seq];
+      const int pos = a.starts != nullptr ? len - a.starts[seq + 1] + t : len - 1;
+      if (mine && pos >= 0 && pos < len) {
+        const int in_table = divided(pos, a.by_page);
+        const int page = in_table < a.table_width ? a.table[(int64_t)seq * a.table_stride + in_table] : -1;
+        if ((uint32_t)page < (uint32_t)a.num_pages) {
+          const int slot = pos - in_table * a.page_size;
+          row = (int64_t)page * a.page_stride + (int64_t)slot * a.slot_stride;
+          if (FP8 && a.blocks > 0) scale = (int64_t)page * a.Hkv * a.blocks + divided(slot, a.by_block);
+        }
+      }
+      row_lds[tid] = row;
+      scale_lds[tid] = scale;
+    }
+  }
+  __syncthreads();
+  constexpr int kElem = FP8 ? 1 : 2, kValues = 16 / kElem;
+  const int per_row = a.Hkv * a.pieces, n = rows * per_row;
+  for (int i0 = tid; i0 < n; i0 += 256 * kAtOnce) {
+    u32x4 k[kAtOnce], v[kAtOnce];
+    float ks[kAtOnce], vs[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + 256 * j;
+      k[j] = v[j] = u32x4{0, 0, 0, 0};
+      ks[j] = vs[j] = 1.0f;
+      if (i < n) {
+        const int r = divided(i, a.by_token), rest = i - r * per_row, h = divided(rest, a.by_pieces);
+        const int64_t row = row_lds[r];
+        if (row >= 0) {
+          const int64_t from = (row + (int64_t)h * a.head_stride) * kElem + (rest - h * a.pieces) * 16;
+          k[j] = *(const u32x4*)((const char*)a.k_cache + from);
+          v[j] = *(const u32x4*)((const char*)a.v_cache + from);
+          if constexpr (FP8) {
+            const int64_t s = a.blocks > 0 ? scale_lds[r] + (int64_t)h * a.blocks : h;
+            ks[j] = a.k_scale[s];
+            vs[j] = a.v_scale[s];
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + 256 * j;
+      if (i >= n) break;
+      const int r = divided(i, a.by_token), rest = i - r * per_row, h = divided(rest, a.by_pieces);
+      const int64_t d = (int64_t)(rest - h * a.pieces) * kValues;
+      if (row_lds[r] == -2) continue;
+      store_row<FP8, BF16>(k[j], ks[j], (char*)a.k + ((int64_t)(t0 + r) * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2);
+      store_row<FP8, BF16>(v[j], vs[j], (char*)a.v + ((int64_t)(t0 + r) * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
+    }
+  }
 }
 
 }  // namespace
@@ -210,25 +375,39 @@ void launch_kv_quantise(const KvQuantiseArgs& args, bool bf16, hipStream_t strea
   A.a.by_pieces = fast_div(A.a.pieces);
   A.by_block = fast_div(A.block);
   A.by_heads = fast_div(A.a.Hkv);
+  if (A.block == 1) {
+    int lanes = 1, shift = 0;
+    while (lanes < A.a.pieces) lanes *= 2, ++shift;
+    const int64_t threads = (int64_t)A.a.tokens * A.a.Hkv * lanes;
+    hipLaunchKernelGGL(kv_quantise_rows_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, A, (int)bf16, lanes,
+                       shift);
+    return;
+  }
   A.slots = (int)kv_quantise_slots(A.a.B, A.a.tokens, A.block, A.a.starts != nullptr);
-  const int64_t waves = (int64_t)A.slots * A.a.Hkv * 2;
-  const dim3 grid((unsigned)((waves + 3) / 4)), block(256);
-  if (A.a.starts != nullptr)
-    hipLaunchKernelGGL((kv_quantise_kernel<true>), grid, block, 0, stream, A, (int)bf16);
+  const int64_t units = (int64_t)A.slots * A.a.Hkv * 2;
+  const bool ragged = A.a.starts != nullptr, workgroup = ragged && A.block * A.a.pieces > 64 * kRowLoads;
+  const dim3 grid((unsigned)(workgroup ? units : (units + 3) / 4)), block(256);
+  if (workgroup)
+    hipLaunchKernelGGL((kv_quantise_kernel<true, true>), grid, block, 0, stream, A, (int)bf16);
+  else if (ragged)
+    hipLaunchKernelGGL((kv_quantise_kernel<true, false>), grid, block, 0, stream, A, (int)bf16);
   else
-    hipLaunchKernelGGL((kv_quantise_kernel<false>), grid, block, 0, stream, A, (int)bf16);
+    hipLaunchKernelGGL((kv_quantise_kernel<false, false>), grid, block, 0, stream, A, (int)bf16);
 }
 
 void launch_kv_read(const KvReadArgs& args, int kind, hipStream_t stream) {
   KvReadArgs a = args;
-  a.pieces = a.D / 8;
+  const bool fp8 = kind >= 2, b16 = kind % 2 == 0;
+  a.pieces = a.D * (fp8 ? 1 : 2) / 16;
+  const int per_row = a.Hkv * a.pieces;
   a.by_page = fast_div(a.page_size);
   a.by_pieces = fast_div(a.pieces);
-  a.by_token = fast_div(a.Hkv * a.pieces);
+  a.by_token = fast_div(per_row);
   a.by_block = fast_div(a.blocks > 0 ? a.block : 1);
-  const int64_t items = (int64_t)a.tokens * a.Hkv * a.pieces;
-  const dim3 grid((unsigned)((items + 255) / 256)), block(256);
-  const bool fp8 = kind >= 2, b16 = kind % 2 == 0;
+  // Work for every thread, and where there are rows enough for 2048 workgroups four times that and more.
+  const int least = std::max(1, 256 / per_row), most = std::max(1, std::min(kKvReadChunk, 8192 / per_row));
+  a.chunk = std::max(std::min(least, kKvReadChunk), std::min(most, a.tokens / 2048));
+  const dim3 grid((unsigned)((a.tokens + a.chunk - 1) / a.chunk)), block(256);
   if (!fp8)
     hipLaunchKernelGGL((kv_read_kernel<false, true>), grid, block, 0, stream, a);
   else if (b16)

@@ -41,9 +41,10 @@ struct KvReadArgs {
   int B, tokens, Hkv, D;
   bool clear_rest;          // rows that belong to no sequence become zeros
   // (set by the launcher)
-  int pieces;
+  int pieces, chunk;        // 16 bytes of a cached row; rows of a workgroup
   FastDiv by_page, by_pieces, by_token, by_block;
 };
+constexpr int kKvReadChunk = 64;
 void launch_kv_read(const KvReadArgs& a, int kind, hipStream_t stream);
 
 }  // namespace vk

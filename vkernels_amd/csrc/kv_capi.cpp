@@ -112,7 +112,7 @@ int append(const char* who, const void* k, const void* v, void* k_cache, void* v
     vk::KvQuantiseArgs A{};
     A.a = a;
     A.k_scale = k_scale; A.v_scale = v_scale; A.blocks = scale_blocks; A.block = page_size / scale_blocks;
-    if (vk::kv_quantise_slots(B, tokens, A.block, query_start != nullptr) > kThreads / 128 / 2 / Hkv)
+    if (vk::kv_quantise_slots(B, tokens, A.block, query_start != nullptr) > kThreads / 512 / 2 / Hkv)
       return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
     const hipError_t before = hipPeekAtLastError();
     vk::launch_kv_quantise(A, kind == VK_HIP_KV_FP8_BF16, static_cast<hipStream_t>(stream));
@@ -235,7 +235,8 @@ int vk_hip_kv_cache_read(const void* k_cache, const void* v_cache, const int32_t
   if (why == nullptr && (overlap(k_stride_t, k_stride_h) || overlap(v_stride_t, v_stride_h))) why = "rows of k and v must not overlap";
   if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
-  if ((int64_t)tokens * Hkv > kInt32 / D) return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
+  if ((int64_t)tokens * Hkv > kInt32 / D || tokens > kThreads / 512)
+    return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many values for one call");
   vk::KvReadArgs a{};
   a.k_cache = k_cache; a.v_cache = v_cache; a.table = block_table; a.lens = seq_lens; a.starts = query_start;
   a.k_scale = k_scale; a.v_scale = v_scale; a.k = k; a.v = v;
