@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_blocks.hpp"
 #include "kv_rows.hpp"
@@ -256,45 +257,40 @@ __global__ __launch_bounds__(256) void kv_quantise_rows_kernel(const KvQuantiseA
 
 // ---- reading back ----------------------------------------------------------------------------------
 
-// 16 bytes of a row that are read: 8 values, or 16 codes as values of 16 bits in the other kinds.
-template <bool FP8, bool BF16>
-__device__ __forceinline__ void store_row(u32x4 x, float scale, char* to) {
-  if constexpr (!FP8) {
-    *(u32x4*)to = x;
-  } else {
-    auto pack = [](float x, float y) -> uint32_t {
-      if constexpr (BF16) {
-        union { __bf16 e[2]; uint32_t u; } c;
-        c.e[0] = (__bf16)x;
-        c.e[1] = (__bf16)y;
-        return c.u;
-      } else {
-        union { _Float16 e[2]; uint32_t u; } c;
-        c.e[0] = (_Float16)x;
-        c.e[1] = (_Float16)y;
-        return c.u;
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      u32x4 y;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = (int)x[2 * i + j];
-        const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8(c, false), q = __builtin_amdgcn_cvt_pk_f32_fp8(c, true);
-        y[2 * j] = pack(p[0] * scale, p[1] * scale);
-        y[2 * j + 1] = pack(q[0] * scale, q[1] * scale);
-      }
-      *(u32x4*)(to + 16 * i) = y;
+// 8 values of a row that is read, as they are or codes as values of 16 bits.
+template <bool BF16>
+__device__ __forceinline__ u32x4 row_values(u32x4 x, float) { return x; }
+template <bool BF16>
+__device__ __forceinline__ u32x4 row_values(u32x2 codes, float scale) {
+  auto pack = [](float x, float y) -> uint32_t {
+    if constexpr (BF16) {
+      union { __bf16 e[2]; uint32_t u; } c;
+      c.e[0] = (__bf16)x;
+      c.e[1] = (__bf16)y;
+      return c.u;
+    } else {
+      union { _Float16 e[2]; uint32_t u; } c;
+      c.e[0] = (_Float16)x;
+      c.e[1] = (_Float16)y;
+      return c.u;
     }
+  };
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f32x2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[i], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes[i], true);
+    y[2 * i] = pack(p[0] * scale, p[1] * scale);
+    y[2 * i + 1] = pack(q[0] * scale, q[1] * scale);
   }
+  return y;
 }
 
-// A workgroup takes `chunk` rows in all heads: a lane each looks up where they lie, then every thread reads 16 bytes
+// A workgroup takes `chunk` rows in all heads: a lane each looks up where they lie, then every thread reads 8 values
 // of a key and of a value in a head, four of each at a time.  Bound by the rows read and written.  (A thread for 8 values
 // with look-ups of its own took 116 us for 60001 positions of 8 heads of 128 in 8 bits, 369 MB.)
 template <bool FP8, bool BF16>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
+  typedef std::conditional_t<FP8, u32x2, u32x4> Piece;
   constexpr int kAtOnce = 4;
   __shared__ int64_t row_lds[kKvReadChunk], scale_lds[kKvReadChunk];     // (elements; -1: zeros, -2: left as it is)
   const int tid = threadIdx.x, t0 = blockIdx.x * a.chunk;
@@ -328,23 +324,23 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
     }
   }
   __syncthreads();
-  constexpr int kElem = FP8 ? 1 : 2, kValues = 16 / kElem;
+  constexpr int kElem = FP8 ? 1 : 2;
   const int per_row = a.Hkv * a.pieces, n = rows * per_row;
   for (int i0 = tid; i0 < n; i0 += 256 * kAtOnce) {
-    u32x4 k[kAtOnce], v[kAtOnce];
+    Piece k[kAtOnce], v[kAtOnce];
     float ks[kAtOnce], vs[kAtOnce];
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int i = i0 + 256 * j;
-      k[j] = v[j] = u32x4{0, 0, 0, 0};
+      k[j] = v[j] = Piece{};
       ks[j] = vs[j] = 1.0f;
       if (i < n) {
         const int r = divided(i, a.by_token), rest = i - r * per_row, h = divided(rest, a.by_pieces);
         const int64_t row = row_lds[r];
         if (row >= 0) {
-          const int64_t from = (row + (int64_t)h * a.head_stride) * kElem + (rest - h * a.pieces) * 16;
-          k[j] = *(const u32x4*)((const char*)a.k_cache + from);
-          v[j] = *(const u32x4*)((const char*)a.v_cache + from);
+          const int64_t from = (row + (int64_t)h * a.head_stride + (rest - h * a.pieces) * 8) * kElem;
+          k[j] = *(const Piece*)((const char*)a.k_cache + from);
+          v[j] = *(const Piece*)((const char*)a.v_cache + from);
           if constexpr (FP8) {
             const int64_t s = a.blocks > 0 ? scale_lds[r] + (int64_t)h * a.blocks : h;
             ks[j] = a.k_scale[s];
@@ -358,10 +354,13 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvReadArgs a) {
       const int i = i0 + 256 * j;
       if (i >= n) break;
       const int r = divided(i, a.by_token), rest = i - r * per_row, h = divided(rest, a.by_pieces);
-      const int64_t d = (int64_t)(rest - h * a.pieces) * kValues;
+      const int d = (rest - h * a.pieces) * 8;
       if (row_lds[r] == -2) continue;
-      store_row<FP8, BF16>(k[j], ks[j], (char*)a.k + ((int64_t)(t0 + r) * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2);
-      store_row<FP8, BF16>(v[j], vs[j], (char*)a.v + ((int64_t)(t0 + r) * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
+      u32x4* const k_to = (u32x4*)((char*)a.k + ((int64_t)(t0 + r) * a.k_stride_t + (int64_t)h * a.k_stride_h + d) * 2);
+      u32x4* const v_to = (u32x4*)((char*)a.v + ((int64_t)(t0 + r) * a.v_stride_t + (int64_t)h * a.v_stride_h + d) * 2);
+      const u32x4 k_row = row_values<BF16>(k[j], ks[j]), v_row = row_values<BF16>(v[j], vs[j]);
+      *k_to = k_row;
+      *v_to = v_row;
     }
   }
 }
@@ -398,7 +397,7 @@ void launch_kv_quantise(const KvQuantiseArgs& args, bool bf16, hipStream_t strea
 void launch_kv_read(const KvReadArgs& args, int kind, hipStream_t stream) {
   KvReadArgs a = args;
   const bool fp8 = kind >= 2, b16 = kind % 2 == 0;
-  a.pieces = a.D * (fp8 ? 1 : 2) / 16;
+  a.pieces = a.D / 8;
   const int per_row = a.Hkv * a.pieces;
   a.by_page = fast_div(a.page_size);
   a.by_pieces = fast_div(a.pieces);

@@ -41,7 +41,7 @@ struct KvReadArgs {
   int B, tokens, Hkv, D;
   bool clear_rest;          // rows that belong to no sequence become zeros
   // (set by the launcher)
-  int pieces, chunk;        // 16 bytes of a cached row; rows of a workgroup
+  int pieces, chunk;        // 8 values of a row; rows of a workgroup
   FastDiv by_page, by_pieces, by_token, by_block;
 };
 constexpr int kKvReadChunk = 64;

@@ -58,13 +58,14 @@ __device__ __forceinline__ Piece<V> narrow(const float* x) {
 }
 
 // A wavefront takes heads of one token, a.rows at a time.  A lane has two pieces of V values of a row: those
-// whose values are each other's partners (V values at i and the V at i + R; of neighbouring pairs 2 V
-// values in a row), so that a pair never leaves its lane, and it has the same pieces of every row, so that its V
-// cosines and sines are loaded once.  The angles of a token are worked out once a wavefront, a lane for each
+// whose values are each other's partners (V values at i and the V at i + R; of neighbouring pairs any two), so that a
+// pair never leaves its lane, and it has the same pieces of every row, so that its V cosines and sines are loaded
+// once.  The angles of a token are worked out once a wavefront, a lane for each
 // frequency: the product in 64 bits, of which the whole turns go before it is cut to 32 (a position of 2^20
 // leaves 32 bits no more than an eighth of a radian at a frequency of 1).
-// Bound by the rows read and written.
-template <int V, bool BF16, bool PAIRS>
+// Bound by the rows read and written.  PAST: results of more bytes than the L2 caches hold go past them (8191 tokens,
+// 40 heads of 128, 168 MB: 43 us with stores through the caches, 35 past them).
+template <int V, bool BF16, bool PAIRS, bool PAST>
 __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_kernel(const QkNormRopeArgs a) {
   __shared__ __attribute__((aligned(16))) float cos_lds[kWaves][kMostFreqs], sin_lds[kWaves][kMostFreqs];
   const int lane = threadIdx.x & 63;
@@ -75,10 +76,11 @@ __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_kernel(const QkNormR
   const int freqs = a.turned / 2, heads = a.Hq + a.Hkv;
   const int unit = lane & (a.lanes - 1), sub = lane / a.lanes;
   const bool in_row = unit * 2 * V < a.D;
-  const bool turns = unit * V < freqs;
-  // where the lane's two pieces lie (lanes without any read the first ones)
-  const int at0 = !in_row ? 0 : PAIRS || !turns ? unit * 2 * V : unit * V;
-  const int at1 = !in_row ? V : PAIRS || !turns ? unit * 2 * V + V : unit * V + freqs;
+  // where the lane's two pieces lie (lanes without any read the first ones), and whether they turn
+  const bool beside = !PAIRS && unit * V >= freqs;
+  const int at0 = !in_row ? 0 : beside ? unit * 2 * V : unit * V;
+  const int at1 = !in_row ? V : PAIRS ? at0 + a.D / 2 : beside ? at0 + V : at0 + freqs;
+  const bool turns0 = PAIRS ? at0 < a.turned : !beside, turns1 = PAIRS ? at1 < a.turned : !beside;
 
   const int head0 = part * a.per_wave * a.rows;
   const int last = min(heads, head0 + a.per_wave * a.rows) - 1;
@@ -131,8 +133,10 @@ __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_kernel(const QkNormR
   float co[V], si[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    co[i] = turns ? cos_lds[wave][unit * V + i] : 1.0f;
-    si[i] = turns ? sin_lds[wave][unit * V + i] : 0.0f;
+    const int at = !PAIRS ? unit * V + i : i < V / 2 ? at0 / 2 + i : at1 / 2 + i - V / 2;
+    const bool turns = PAIRS && i >= V / 2 ? turns1 : turns0;
+    co[i] = turns ? cos_lds[wave][at] : 1.0f;
+    si[i] = turns ? sin_lds[wave][at] : 0.0f;
   }
 
   for (int i = 0; i < a.per_wave; ++i) {
@@ -159,25 +163,47 @@ __global__ __launch_bounds__(64 * kWaves) void qk_norm_rope_kernel(const QkNormR
       // (of halves a piece each, of neighbours both in one; values beside the pairs have cosine 1 and sine 0,
       // and a product with that 0 is none where the partner is infinite)
       const int p0 = PAIRS ? 2 * j : j, p1 = PAIRS ? 2 * j + 1 : V + j;
+      const bool turns = PAIRS && j >= V / 2 ? turns1 : turns0;
       o[p0] = turns ? v[p0] * co[j] - v[p1] * si[j] : v[p0];
       o[p1] = turns ? v[p1] * co[j] + v[p0] * si[j] : v[p1];
     }
     if (in_row && h <= last) {
       char* const row = (char*)row_of(h, (const char*)a.q_out, (const char*)a.k_out, a.qo_stride_t, a.qo_stride_h,
                                       a.ko_stride_t, a.ko_stride_h);
-      *(Piece<V>*)(row + at0 * 2) = narrow<V, BF16>(o);
-      *(Piece<V>*)(row + at1 * 2) = narrow<V, BF16>(o + V);
+      if constexpr (PAST) {
+        __builtin_nontemporal_store(narrow<V, BF16>(o), (Piece<V>*)(row + at0 * 2));
+        __builtin_nontemporal_store(narrow<V, BF16>(o + V), (Piece<V>*)(row + at1 * 2));
+      } else {
+        *(Piece<V>*)(row + at0 * 2) = narrow<V, BF16>(o);
+        *(Piece<V>*)(row + at1 * 2) = narrow<V, BF16>(o + V);
+      }
     }
   }
 }
 
-template <int V, bool BF16>
-void launch_pieces(const QkNormRopeArgs& a, bool pairs, hipStream_t stream) {
+template <int V, bool BF16, bool PAIRS>
+void launch_pieces(const QkNormRopeArgs& a, hipStream_t stream) {
   const dim3 grid((uint32_t)(((int64_t)a.T * a.waves + kWaves - 1) / kWaves)), block(64 * kWaves);
+  // (rows of 128 bytes and less, and pieces that lie side by side, would go past the caches as parts of lines: 64 values
+  // 30 us through them and 33 past, pairs in pieces side by side 36 and 39)
+  const bool past = (int64_t)a.T * (a.Hq + a.Hkv) * a.D * 2 > 32 << 20 && a.D >= 128 && (PAIRS || a.turned == a.D);
+  if constexpr (V == 8) {
+    if (past) {
+      hipLaunchKernelGGL((qk_norm_rope_kernel<V, BF16, PAIRS, true>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((qk_norm_rope_kernel<V, BF16, PAIRS, false>), grid, block, 0, stream, a);
+}
+
+template <bool BF16>
+void launch_type(const QkNormRopeArgs& a, bool pairs, int V, hipStream_t stream) {
   if (pairs)
-    hipLaunchKernelGGL((qk_norm_rope_kernel<V, BF16, true>), grid, block, 0, stream, a);
+    launch_pieces<8, BF16, true>(a, stream);
+  else if (V == 8)
+    launch_pieces<8, BF16, false>(a, stream);
   else
-    hipLaunchKernelGGL((qk_norm_rope_kernel<V, BF16, false>), grid, block, 0, stream, a);
+    launch_pieces<4, BF16, false>(a, stream);
 }
 
 }  // namespace
@@ -185,7 +211,7 @@ void launch_pieces(const QkNormRopeArgs& a, bool pairs, hipStream_t stream) {
 void launch_qk_norm_rope(const QkNormRopeArgs& args, bool bf16, bool pairs, hipStream_t stream) {
   QkNormRopeArgs a = args;
   // pieces of 8 values, or of 4 where the partners of 8 would not start on a piece
-  const int V = a.turned % 16 == 0 ? 8 : 4;
+  const int V = pairs || a.turned % 16 == 0 ? 8 : 4;
   const int units = a.D / (2 * V);
   a.lanes = 1;
   while (a.lanes < units) a.lanes *= 2;
@@ -198,11 +224,7 @@ void launch_qk_norm_rope(const QkNormRopeArgs& args, bool bf16, bool pairs, hipS
   a.waves = (times + a.per_wave - 1) / a.per_wave;
   a.by_waves = fast_div(a.waves);
   a.inv_width = 1.0f / (float)a.D;
-  if (V == 8) {
-    if (bf16) launch_pieces<8, true>(a, pairs, stream); else launch_pieces<8, false>(a, pairs, stream);
-  } else {
-    if (bf16) launch_pieces<4, true>(a, pairs, stream); else launch_pieces<4, false>(a, pairs, stream);
-  }
+  if (bf16) launch_type<true>(a, pairs, V, stream); else launch_type<false>(a, pairs, V, stream);
 }
 
 }  // namespace vk
