@@ -302,6 +302,17 @@ def test_nothing_to_read(hip_lib):
     assert bool((k == 0).all() and (v == 0).all())
 
 
+def test_a_backward_pass_is_an_error(hip_lib):
+    c = Cache([10], 2, 64, 16, 4)
+    wide = [torch.zeros(c.k.shape, dtype=BF16, device=dev(), requires_grad=True) for _ in range(2)]
+    lens = torch.tensor([5], dtype=torch.int32, device=dev())
+    k, v = kv.kv_cache_read(*wide, c.table, lens)
+    with pytest.raises(RuntimeError, match="kv_cache_read has no backward"):
+        (k.float().sum() + v.float().sum()).backward()
+    with torch.no_grad():
+        assert not kv.kv_cache_read(*wide, c.table, lens)[0].requires_grad
+
+
 def test_refusals(hip_lib):
     c = Cache([10, 10], 2, 64, 16, 4)
     lens = torch.tensor([3, 4], dtype=torch.int32, device=dev())

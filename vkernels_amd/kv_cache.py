@@ -178,17 +178,24 @@ def _rows(t):
     return t
 
 
-class _NoBackward(torch.autograd.Function):
-    """The results as they are; a backward pass that reaches them is an error instead of a gradient lost."""
+def _no_backward(name):
+    """A function that hands an operator's two results on as they are; a backward pass that reaches them is an error
+    instead of a gradient lost."""
 
-    @staticmethod
-    def forward(ctx, out, lse, *inputs):
-        return (out.view_as(out), None if lse is None else lse.view_as(lse))
+    class NoBackward(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, first, second, *inputs):
+            return first.view_as(first), None if second is None else second.view_as(second)
 
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError("paged_attention has no backward pass: it is an operator of inference "
-                           "(call it under torch.no_grad(), or detach what requires a gradient)")
+        @staticmethod
+        def backward(ctx, *grads):
+            raise RuntimeError(f"{name} has no backward pass: it is an operator of inference "
+                               "(call it under torch.no_grad(), or detach what requires a gradient)")
+
+    return NoBackward.apply
+
+
+_attention_result, _read_result = _no_backward("paged_attention"), _no_backward("kv_cache_read")
 
 
 def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_start=None, k_scale=None, v_scale=None):
@@ -218,7 +225,9 @@ def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_star
         _need(tokens == B, "without query_start there is one token for each sequence")
     k, v = _rows(k), _rows(v)
     ks, vs = k.stride(), v.stride()
-    k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
+    blocks = 0
+    if k_scale is not None or v_scale is not None:
+        k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
     name, more = ("vk_hip_kv_cache_append_ex", (blocks,)) if blocks else ("vk_hip_kv_cache_append", ())
     status = _fn(name)(
         k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
@@ -268,6 +277,8 @@ def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, 
         ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2], _stream(device))
     if status:
         _failed(status, "vk_hip_kv_cache_read")
+    if (k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled() and out is None:
+        k, v = _read_result(k, v, k_cache, v_cache)
     return k, v
 
 
@@ -322,7 +333,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
         if not _sums_ok(weight_sums, B, Hkv, max_len, device):
             raise ValueError("weight_sums must be float32 [B, Hkv, max_len or more] with contiguous rows on the cache's device")
         sums, (sums_b, sums_h, _) = weight_sums.data_ptr(), weight_sums.stride()
-    k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
+    blocks = 0
+    if k_scale is not None or v_scale is not None:
+        k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
     sink_at = None if sinks is None else _head_vector(sinks, Hq, "sinks", device)
     lse_at = None if lse is None else lse.data_ptr()
     qs, scale = q.stride(), D ** -0.5 if scale is None else scale
@@ -351,7 +364,7 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
         _failed(status, name)
     if ((q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
          sinks is not None and sinks.requires_grad) and torch.is_grad_enabled() and not own_out):
-        out, lse = _NoBackward.apply(out, lse, q, k_cache, v_cache, sinks)
+        out, lse = _attention_result(out, lse, q, k_cache, v_cache, sinks)
     return (out, lse) if return_lse else out
 
 

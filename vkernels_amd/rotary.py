@@ -13,7 +13,7 @@ import ctypes
 
 import torch
 
-from .kv_cache import _current_device, _failed, _need, _rows, _stream
+from .kv_cache import _current_device, _failed, _need, _no_backward, _rows, _stream
 from .vllm_experts import load_libvkernels_hip
 
 __all__ = ["qk_norm_rope"]
@@ -33,21 +33,11 @@ def _fn():
     return _fn_cache[0]
 
 
-class _NoBackward(torch.autograd.Function):
-    """The results as they are; a backward pass that reaches them is an error instead of a gradient lost."""
-
-    @staticmethod
-    def forward(ctx, q, k, *inputs):
-        return q.view_as(q), k.view_as(k)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError("qk_norm_rope has no backward pass: it is an operator of inference "
-                           "(call it under torch.no_grad(), or detach what requires a gradient)")
+_result = _no_backward("qk_norm_rope")
 
 
-def _weight(w, D, kind, device, name):
-    if not (w.shape == (D,) and w.dtype is kind and w.get_device() == device and (D == 1 or w.stride(0) == 1)):
+def _weight_at(w, D, of, device, name):
+    if not (w.shape == (D,) and w.dtype is of and w.get_device() == device and w.is_contiguous()):
         raise ValueError(f"{name} must be [D] contiguous on q's device, and both weights in float32 or in q's type")
     return w if w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
 
@@ -57,6 +47,22 @@ def _check_out(out, like, name):
     _need(out.shape == like.shape and out.dtype is like.dtype and out.get_device() == like.get_device() and s[2] == 1 and
           s[0] % 8 == 0 and s[1] % 8 == 0 and out.data_ptr() % 16 == 0,
           f"the result for {name} must be like {name}, with rows that start on 16 bytes")
+
+
+# The checks are one expression on the path that is taken (a decode step is short: the host's work per call
+# counts); _explain says which part of it did not hold.
+
+def _explain(q, k, positions, inv_freq):
+    _need(q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2],
+          "q and k must be [T, Hq, D] and [T, Hkv, D]")
+    _need(q.dtype in _KINDS and k.dtype is q.dtype, "q and k must both be bfloat16 or float16")
+    _need(all(t.get_device() == _current_device() for t in (q, k, positions, inv_freq)),
+          "the tensors must be on the current device")
+    _need(inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
+          inv_freq.shape[0] <= q.shape[2] // 2, "inv_freq must be up to D / 2 contiguous float32 values")
+    _need(positions.dtype is torch.int32 and (positions.numel() <= 1 or positions.stride(-1) == 1),
+          "positions must be int32 with contiguous rows")
+    _need(False, "q and k must have heads, and sizes below 2^31")
 
 
 def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps=1e-6, sections=None, pairs=False,
@@ -71,42 +77,35 @@ def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps
     the frequencies, in order, turn by each axis.
     Returns (q, k), new ones, or ``out`` (a pair of tensors, which may be q and k themselves).  q and k may be
     views of one tensor of any strides with D contiguous."""
-    device = q.get_device()
-    _need(q.dim() == 3 and k.dim() == 3 and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2],
-          "q and k must be [T, Hq, D] and [T, Hkv, D]")
-    T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    kind = _KINDS.get(q.dtype)
-    _need(kind is not None and k.dtype is q.dtype, "q and k must both be bfloat16 or float16")
-    _need(device >= 0 and device == _current_device() and k.get_device() == device and
-          positions.get_device() == device and inv_freq.get_device() == device,
-          "the tensors must be on the current device")
-    _need(T < 1 << 31 and Hq < 1 << 31 and Hkv < 1 << 31 and Hq > 0 and Hkv > 0 and D > 0,
-          "q and k must have heads, and sizes below 2^31")
-    _need(inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
-          inv_freq.shape[0] <= D // 2, "inv_freq must be up to D / 2 contiguous float32 values")
-    R = inv_freq.shape[0]
+    device, shape, k_shape, kind = q.get_device(), q.shape, k.shape, _KINDS.get(q.dtype)
+    if not (len(shape) == 3 and len(k_shape) == 3 and shape[0] == k_shape[0] and shape[2] == k_shape[2] and
+            kind is not None and k.dtype is q.dtype and device == _current_device() and k.get_device() == device and
+            positions.get_device() == device and inv_freq.get_device() == device and
+            inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
+            inv_freq.shape[0] <= shape[2] // 2 and positions.dtype is torch.int32 and
+            (positions.numel() <= 1 or positions.stride(-1) == 1) and
+            shape[1] > 0 and k_shape[1] > 0 and (shape[0] | shape[1] | k_shape[1]) <= 0x7FFFFFFF):
+        _explain(q, k, positions, inv_freq)
+    (T, Hq, D), Hkv, R = shape, k_shape[1], inv_freq.shape[0]
     if sections is None:
-        _need(positions.shape == (T,), "positions must be [T], or [axes, T] with sections")
+        if positions.shape != (T,):
+            raise ValueError("positions must be [T], or [axes, T] with sections")
         axes, axis_stride, c_sections = 1, 0, None
     else:
         axes = len(sections)
         _need(1 <= axes <= 4 and positions.shape == (axes, T), "positions must be [axes, T] with a section for each of up to 4 axes")
         _need(all(0 <= n <= R for n in sections) and sum(sections) == R, "sections must add up to the number of inv_freq")
         axis_stride, c_sections = positions.stride(0), (ctypes.c_int32 * axes)(*sections)
-    _need(positions.dtype is torch.int32 and (T <= 1 or positions.stride(-1) == 1),
-          "positions must be int32 with contiguous rows")
     weights_f32 = 0
-    if eps is None:
-        _need(q_weight is None and k_weight is None, "weights belong to the norm, which eps=None leaves out")
-    elif q_weight is not None or k_weight is not None:
+    if q_weight is not None or k_weight is not None:
+        _need(eps is not None, "weights belong to the norm, which eps=None leaves out")
         of = (q_weight if q_weight is not None else k_weight).dtype
         weights_f32 = int(of is torch.float32)
         of = torch.float32 if weights_f32 else q.dtype
-        q_weight = None if q_weight is None else _weight(q_weight, D, of, device, "q_weight")
-        k_weight = None if k_weight is None else _weight(k_weight, D, of, device, "k_weight")
-    wants_grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any(
-        w is not None and w.requires_grad for w in (q_weight, k_weight)))
+        q_weight = None if q_weight is None else _weight_at(q_weight, D, of, device, "q_weight")
+        k_weight = None if k_weight is None else _weight_at(k_weight, D, of, device, "k_weight")
+    wants_grad = (q.requires_grad or k.requires_grad or inv_freq.requires_grad or q_weight is not None and q_weight.requires_grad or
+                  k_weight is not None and k_weight.requires_grad) and torch.is_grad_enabled()
     if out is None:
         q_out, k_out = q.new_empty((T, Hq, D)), k.new_empty((T, Hkv, D))
     else:
@@ -125,5 +124,5 @@ def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps
     if status:
         _failed(status, "vk_hip_qk_norm_rope")
     if wants_grad and out is None:
-        q_out, k_out = _NoBackward.apply(q_out, k_out, *inputs, q_weight, k_weight)
+        q_out, k_out = _result(q_out, k_out, *inputs, inv_freq, q_weight, k_weight)
     return q_out, k_out
