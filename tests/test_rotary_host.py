@@ -33,7 +33,8 @@ def call():
     dict(axes=2, sections=LARGE), dict(q=None), dict(k=None), dict(q_out=None), dict(k_out=None), dict(positions=None),
     dict(inv_freq=None), dict(norm=0), dict(eps=-1e-6), dict(eps=float("nan")), dict(q_weight=P + 8), dict(k_weight=P + 4),
     dict(q=P + 8), dict(k_out=P + 2), dict(q_stride_t=516), dict(k_stride_h=68), dict(q_out_stride_h=60),
-    dict(q_stride_t=-512), dict(axis_stride=-4), dict(q_out_stride_t=0), dict(k_out_stride_h=0), dict(k_out_stride_h=32)])
+    dict(q_stride_t=-512), dict(axis_stride=-4), dict(q_out_stride_t=0), dict(k_out_stride_h=0), dict(k_out_stride_h=32),
+    dict(q_out_stride_t=64), dict(q_out_stride_t=504), dict(q_out_stride_t=64, q_out_stride_h=248), dict(k_out_stride_t=-128)])
 def test_invalid_arguments(call, bad):
     assert call(**bad) == ve.VK_ERROR_INVALID_ARGUMENT
     assert "vk_hip_qk_norm_rope" in ve.last_error(ve.load_libvkernels_hip())
@@ -42,7 +43,7 @@ def test_invalid_arguments(call, bad):
 def test_other_refusals(call):
     assert call(kind=2) == ve.VK_ERROR_UNSUPPORTED
     assert call(T=1 << 30) == ve.VK_ERROR_OUT_OF_RANGE
-    assert call(Hq=2147483647) == ve.VK_ERROR_OUT_OF_RANGE
+    assert call(T=1, Hq=2147483647) == ve.VK_ERROR_OUT_OF_RANGE
 
 
 def test_nothing_to_do(call):

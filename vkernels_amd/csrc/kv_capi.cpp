@@ -74,6 +74,15 @@ const char* rows_refusal(const void* k, const void* v, int64_t k_stride_t, int64
   return nullptr;
 }
 
+// Rows of D values that are written to: heads one behind the other within tokens, or tokens within heads.
+bool rows_overlap(int tokens, int heads, int D, int64_t by_t, int64_t by_h) {
+  if (by_t < 0 || by_h < 0) return true;
+  if (tokens <= 1 || heads <= 1) return (tokens > 1 && by_t < D) || (heads > 1 && by_h < D);
+  const bool heads_inside = by_h <= by_t;
+  const int64_t inner = heads_inside ? by_h : by_t, outer = heads_inside ? by_t : by_h, n = heads_inside ? heads : tokens;
+  return inner < D || outer / inner < n - 1 || outer - inner * (n - 1) < D;
+}
+
 const char* scales_refusal(int kind, const float* k_scale, const float* v_scale, int scale_blocks, int page_size) {
   if (elem_of(kind) == 1 && (k_scale == nullptr || v_scale == nullptr)) return "an 8-bit cache needs k_scale and v_scale";
   if (elem_of(kind) == 2 && (k_scale != nullptr || v_scale != nullptr)) return "k_scale and v_scale are for 8-bit caches";
@@ -229,10 +238,8 @@ int vk_hip_kv_cache_read(const void* k_cache, const void* v_cache, const int32_t
                                   table_width, table_stride, page_stride, head_stride, slot_stride);
   if (why == nullptr && (k == nullptr || v == nullptr)) why = "k/v must not be null";
   if (why == nullptr) why = rows_refusal(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h);
-  auto overlap = [tokens, Hkv, D](int64_t by_t, int64_t by_h) {
-    return by_t < 0 || by_h < 0 || (tokens > 1 && by_t < D) || (Hkv > 1 && by_h < D);
-  };
-  if (why == nullptr && (overlap(k_stride_t, k_stride_h) || overlap(v_stride_t, v_stride_h))) why = "rows of k and v must not overlap";
+  if (why == nullptr && (rows_overlap(tokens, Hkv, D, k_stride_t, k_stride_h) || rows_overlap(tokens, Hkv, D, v_stride_t, v_stride_h)))
+    why = "rows of k and v must not overlap";
   if (why == nullptr) why = scales_refusal(kind, k_scale, v_scale, scale_blocks, page_size);
   if (why != nullptr) return refuse(VK_ERROR_INVALID_ARGUMENT, who, why);
   if ((int64_t)tokens * Hkv > kInt32 / D || tokens > kThreads / 512)
@@ -427,11 +434,8 @@ int vk_hip_qk_norm_rope(const void* q, const void* k, const int32_t* positions, 
     why = "rows of q, k and the results must start on 16 bytes";
   if (why == nullptr && (q_stride_t < 0 || q_stride_h < 0 || k_stride_t < 0 || k_stride_h < 0 || axis_stride < 0))
     why = "strides must not be negative";
-  // (results hold every value once)
-  auto rows_overlap = [T, D](int heads, int64_t by_t, int64_t by_h) {
-    return (T > 1 && by_t < D) || (heads > 1 && by_h < D);
-  };
-  if (why == nullptr && (rows_overlap(Hq, q_out_stride_t, q_out_stride_h) || rows_overlap(Hkv, k_out_stride_t, k_out_stride_h)))
+  if (why == nullptr && (rows_overlap(T, Hq, D, q_out_stride_t, q_out_stride_h) ||
+                         rows_overlap(T, Hkv, D, k_out_stride_t, k_out_stride_h)))
     why = "rows of the results must not overlap";
   vk::QkNormRopeArgs a{};
   a.section_end[0] = turned / 2;

@@ -902,7 +902,8 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
     const float ref = or_zero(m) - kLift;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      union { typename W::T e[8]; typename W::V8 v; } p;
+      // (two 16-bit terms of each weight, 16 bits of it: the matrix cores have the time)
+      union { typename W::T e[8]; typename W::V8 v; } p, low;
 #pragma unroll
       for (int i = 0; i < 8; i += 4) {
         f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
@@ -913,7 +914,9 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
           const float w = exp2_fast(x[at] - ref);
           l += w;
           // (a scale that is not seen may be anything)
-          p.e[i + e] = (typename W::T)(!FP8 ? w : ((sees >> (at / 4 * 8 + at % 4)) & 1) ? w * f[e] : 0.0f);
+          const float scaled = !FP8 ? w : ((sees >> (at / 4 * 8 + at % 4)) & 1) ? w * f[e] : 0.0f;
+          p.e[i + e] = (typename W::T)scaled;
+          low.e[i + e] = (typename W::T)(scaled - (float)p.e[i + e]);
         }
       }
 #pragma unroll
@@ -930,7 +933,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
           both.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * F::kPitch));
           v = both.v;
         }
-        acc[i] = W::mfma(v, p.v, acc[i]);
+        acc[i] = W::mfma(v, low.v, W::mfma(v, p.v, acc[i]));
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
