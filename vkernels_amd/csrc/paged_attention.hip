@@ -178,7 +178,8 @@ struct Tile {
 // SCALES: an 8-bit cache's blocks of positions have scales of their own.  A lane loads the scale of one
 // position's keys or values with the tile; scores are multiplied by the keys', the weights by the values'
 // before they become 16-bit terms (in bf16 whatever the queries' type: codes are exact in it, and a weight
-// times a scale needs its range).
+// times a scale needs its range).  255 sequences of up to 8192 positions, 8 heads of 4 of 128, scales for 16 positions
+// each: 376 us for 2.35 GB, as with a scale for each head; one of 131071: 42 us for 269 MB, 6.3 TB/s.
 template <class M, bool FP8, int DP, bool P16, bool FULL, bool SCALES>
 __global__ __launch_bounds__(256, residents(DP)) void paged_attention_kernel(const KernelArgs A) {
   typedef Tile<M, FP8, DP> L;

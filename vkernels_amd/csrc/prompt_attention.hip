@@ -100,10 +100,12 @@ struct Layout {
   static constexpr int kPitch = kLanes * 16;                   // bytes of a row in LDS
   static constexpr int kTile = kPromptKeys * kPitch;
   static constexpr int kLds = 4 * kTile;                       // two buffers for keys, two for values
-  // Where in its row a piece of 16 bytes lies: exchanged by the row, so that 16 rows' pieces (keys) and 8 rows' pairs
-  // of pieces (values, for the transposed reads) spread over the banks.  Each is its own inverse.
+  // Where in its row a piece of 16 bytes lies: exchanged by the row (each exchange its own inverse), so that what is read at
+  // once spreads over the banks: one piece of 16 rows (keys), two neighbouring pairs of pieces of 4 rows (values, by the
+  // transposed reads).  No bank is asked for twice; with the pairs of two rows in one place a third of the cycles that
+  // LDS was busy were conflicts, which the time did not show.
   static __device__ __forceinline__ int key_turn(int row) { return DP <= 64 ? (row >> 1) & 7 : row & 15; }
-  static __device__ __forceinline__ int value_turn(int row) { return DP <= 64 ? (row >> 1) & 3 : row & 7; }
+  static __device__ __forceinline__ int value_turn(int row) { return DP <= 64 ? row & 2 : (row & 3) * 2; }
   static __device__ __forceinline__ int key_piece(int slot, int row) { return slot ^ key_turn(row); }
   static __device__ __forceinline__ int value_piece(int slot, int row) { return slot ^ (value_turn(row) * 2); }
 };
@@ -177,6 +179,11 @@ __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >
 // become 16-bit ones), a tile ahead, in two buffers each.  A wavefront takes 32 positions at a time and works out
 // the scores of the next 32 beside the weights of these, so that the matrix instructions run under the exponentials: the
 // tiles of keys are 32 positions on from those of values, and both are done with when a tile ends.
+// 4096 tokens over 16384 positions, 32 heads on 8 of 128: 1.02 ms, 945 TFLOP/s (a bf16 product of 8192^3 reaches 1379);
+// heads of 64: 1.19 ms for as many products, 810.  Matrix instructions take 45 % of the cycles, vector ones 53 %; without
+// the loads it is 0.89 ms, without the exponentials 1.05.  Keys and values through registers, no scores ahead: 1.21;
+// scores ahead in the compiler's own order: 1.24 (every read from LDS waited for), 1.08 by its scheduling groups.
+// Two chains of scores, reads 2 or 5 operands ahead, and priorities for either half change nothing or cost 2 %.
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(const KernelArgs A) {
   typedef Layout<DP> L;
@@ -674,8 +681,12 @@ struct FewLayout {
   static __device__ __forceinline__ int key_piece(int slot, int row) {
     return FP8 ? slot ^ code_turn(row) : L::key_piece(slot, row);
   }
+  // (codes of values are read two neighbouring pieces of rows 0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15, at once)
+  static __device__ __forceinline__ int value_code_turn(int row) {
+    return kLanes == 4 ? (row >> 3 & 1) * 2 : (row >> 1 & 1) * 2 + (row >> 3 & 1) * 4;
+  }
   static __device__ __forceinline__ int value_piece(int slot, int row) {
-    return FP8 ? slot ^ code_turn(row) : L::value_piece(slot, row);
+    return FP8 ? slot ^ value_code_turn(row) : L::value_piece(slot, row);
   }
   static __device__ __forceinline__ int value_pair(int pair, int row) { return pair ^ L::value_turn(row); }
 };
@@ -683,7 +694,9 @@ struct FewLayout {
 // The same for tiles of 32 rows: every wavefront has all of the rows and takes every fourth 32 positions, by itself.  Keys
 // and values go to the wavefront's own part of LDS as they are (8-bit codes become 16-bit values as they are read from
 // there), the next ones on their way while these are multiplied.  The wavefronts' results meet in LDS at the end, one
-// after the other.  Bound by the keys' and values' stream.
+// after the other.  Bound by latency: 5 tokens of 32 sequences of 1024 to 8192, 32 heads on 8 of 128 in 8 bits, 279 MB:
+// 95 us (2.9 TB/s) of which a workgroup's start, six dependent loads, and end are a third; one sequence of 131071: 68
+// (4.0 TB/s), in bf16 115 (4.7).  With tiles of 128 rows, one wavefront with all of them: 250.
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const KernelArgs A) {
   typedef std::conditional_t<FP8, Bf16, M> W;
@@ -1135,9 +1148,10 @@ PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int
   const int64_t tiles = (p.slots - 1) * (int64_t)Hkv;
   int64_t seen = max_len;
   if (window > 0) seen = std::min<int64_t>(max_len, (int64_t)window + rows + 16 + std::min(keep_first, max_len) + kPromptKeys);
-  // Shares of one size, so that all workgroups that have one work equally long (those behind a shorter sequence's end
-  // have none): shares by the sequence's own length took 108 us for 5 tokens over 1024 to 8192 positions of 32 sequences,
-  // the workgroups of the longest ones ending last.
+  // Shares of one size for all sequences (those behind a shorter one's end are empty; shares by a sequence's own length
+  // are no faster).  How many: 5 tokens over 1024 to 8192 positions of 32 sequences in 8 bits, 8 heads of 4, take 114 us
+  // with 1024 workgroups, 111 with 2048, 101 with 4096, 113 with 8192; 64 over the same, in tiles of 128 rows, 105 with
+  // 1024, 110 with 2048, 146 with 512.  At most 64, which one launch joins.
   const int64_t keys = std::max<int64_t>(1, (seen + kPromptKeys - 1) / kPromptKeys);
   const int64_t wanted = rows == kPromptFewRows ? 4096 : 1024;
   const int64_t splits = std::max<int64_t>(1, std::min({keys / 4, wanted / tiles, (int64_t)64}));

@@ -1,16 +1,19 @@
-"""The key-value cache of a decode step on torch device tensors: append, the attention of one
-new token over the paged cache, and eviction by accumulated attention weight.
+"""A paged key-value cache on torch device tensors: append, reading back, the attention of one or
+of several new tokens over it, and eviction by accumulated attention weight.
 
 A cache is two tensors [pages, Hkv, page_size, D] of any strides with D contiguous (a cache that is
 [pages, page_size, Hkv, D] in memory goes in as its ``transpose(1, 2)``), bf16, fp16 or
-float8_e4m3fn with a float32 scale for each head.  ``block_table`` [B, W] int32 names the page of
-every page_size positions of a sequence, ``seq_lens`` [B] int32 how many positions it has.  Every
+float8_e4m3fn with float32 scales: one for each head, [Hkv], or one for each block of positions of a
+page and head, [pages, Hkv, blocks], which append sets from what is written (the selection of an
+eviction moves rows between blocks, so it takes caches with a scale for each head alone).
+``block_table`` [B, W] int32 names the page of every page_size positions of a sequence,
+``seq_lens`` [B] int32 how many positions it has.  Every
 call is enqueued on the current stream of the tensors' device, with no host synchronisation; what it
 writes besides its arguments comes from torch's allocator, so calls on several streams do not share
 scratch and a call can be captured in a graph.
 
 These are operators of inference: no gradient passes through the cache, and a backward pass that comes to
-``paged_attention`` raises an error.
+their results raises an error.
 
 The entry points are additive: the reference keeps its cache outside this path.  Everything runs in
 ``libvkernels_hip.so``; there is no fallback.
