@@ -123,6 +123,18 @@ def test_a_refused_prompt_leaves_the_layer_as_it_was(hip_lib):
     assert torch.equal(before[0], layer.k_cache.view(torch.uint8)) and torch.equal(before[1], layer.scales["k_scale"])
 
 
+def test_queries_and_keys_of_two_types(hip_lib):
+    """Of an 8-bit cache with a scale for each head either 16-bit type is read and written."""
+    scale = torch.full((2,), 0.02, device=dev())
+    layer, normal, _ = _layer(cache_dtype=FP8, k_scale=scale, v_scale=scale)
+    q, k, v = normal(3, 4, 64).half(), normal(3, 2, 64), normal(3, 2, 64)
+    out = layer.attend(q, k, v)
+    want = aref.attention(q, layer.k_cache, layer.v_cache, layer.table, layer.lens_dev, torch.tensor([0, 1, 2, 3]),
+                          scale=64 ** -0.5, sinks=layer.sinks.cpu(), k_scale=scale.cpu(), v_scale=scale.cpu())
+    assert out.dtype is torch.float16
+    ref.assert_attention(out, None, want, torch.float16)
+
+
 def test_the_command_runs(hip_lib):
     for kw in (dict(rotary=True), dict(window=64, window_first=4, scale_blocks=1), dict(rotary=True, scale_blocks=16, window=100)):
         seconds, layer = _example("c0", 4, 150, 3, None, 8, 2, 64, **kw)

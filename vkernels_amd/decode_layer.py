@@ -75,7 +75,7 @@ class DecodeLayer:
         self.lens = [0] * sequences
         self.table = torch.full((sequences, width), -1, dtype=torch.int32, device=dev)
         self.lens_dev = torch.zeros(sequences, dtype=torch.int32, device=dev)
-        self.rotary, self.sees = rotary, dict(window=window, keep_first=window_first)
+        self.rotary, self.scale_blocks, self.sees = rotary, scale_blocks, dict(window=window, keep_first=window_first)
         self.positions = torch.zeros(sequences, dtype=torch.int32, device=dev)      # of the next tokens
         # only a cache that is evicted from needs to know what its positions were given
         self.sums = None if budget is None else torch.zeros((sequences, kv_heads, width * page_size), device=dev)
@@ -123,10 +123,12 @@ class DecodeLayer:
         self.lens_dev.copy_(torch.tensor(lens, dtype=torch.int32))
 
     def _turned(self, q, k, positions):
-        """Queries and keys as the attention and the cache take them; refused ahead of the cache, whose blocks' scales
-        grow with what is written."""
-        if q.shape != (k.shape[0], self.heads, self.head_dim) or q.dtype is not k.dtype:
-            raise ValueError("q must be [tokens, Hq, D] of k's type")
+        """Queries and keys as the attention and the cache take them.  What the attention would refuse of them where
+        blocks have scales, which grow with what is written, is refused ahead of the cache."""
+        if q.shape != (k.shape[0], self.heads, self.head_dim):
+            raise ValueError("q must be [tokens, Hq, D]")
+        if self.scale_blocks and q.dtype is not k.dtype:
+            raise ValueError("with scale_blocks q must be of k's type")
         if self.rotary is None:
             return q, k
         sections = self.rotary.get("sections")
