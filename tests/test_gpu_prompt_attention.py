@@ -302,3 +302,40 @@ def test_nothing_and_refusals(hip_lib):
     out = kv.paged_attention(q, *args[1:], **both)
     with pytest.raises(RuntimeError, match="no backward"):
         out.float().sum().backward()
+
+
+@pytest.mark.parametrize("D,q", [(64, F16), (128, F16), (192, F16), (128, BF16)])
+@pytest.mark.parametrize("new", [(3, 5), (200, 150)])
+@pytest.mark.parametrize("drop", [9, 17, 24, 30])
+@pytest.mark.parametrize("every", [0, 64, 1000])
+def test_weights_far_below_those_of_values_that_are_zero(hip_lib, D, q, new, drop, every):
+    """One position (or every so many) has nearly all of the weight and a value of zero: the others are the result."""
+    s = Prompt([8000, 6000], new, 1, 2, D, 16, 0, q=q)
+    large = torch.arange(s.table.shape[1] * 16) % every == 0 if every else torch.arange(s.table.shape[1] * 16) == 40
+    s.q.zero_()
+    s.k.zero_()
+    s.v.fill_(8.0)
+    s.q[..., 0] = 1.0
+    for b in range(2):
+        pages = s.table[b][s.table[b] >= 0].long()
+        at = large.view(-1, 16)[:len(pages)].to(dev())
+        k, v = s.k[pages], s.v[pages]           # [W, 1, 16, D]
+        k[..., 0] = torch.where(at[:, None], float(drop), 0.0).to(k.dtype)
+        v[at[:, None]] = 0.0
+        s.k[pages], s.v[pages] = k, v
+    out, lse = s.call(scale=1.0)
+    # scores are exact; a weight is rounded once to 16 bits and so is the result; the exponent's product with log2(e) is off by
+    # 2^-24 of up to 2^6, a move of the reference by 2^-22, twice for every large position; in fp16 a weight may also be off by
+    # 2^-18 of the largest among its 32 positions (which is 2^-7 or more, and a half step 2^-25 or less)
+    moves = 2 * (1 if not every else 8000 / every)
+    tol = 2 * torch.finfo(q).eps / 2 + 2.0 ** -18 + moves * 2.0 ** -22
+    row = 0
+    for b, (length, n) in enumerate(zip((8000, 6000), new)):
+        for p in range(length - n, length):
+            spikes = int(large[:p + 1].sum())
+            beside = 0 if q is BF16 else int((large[:8000].view(-1, 32).any(1).repeat_interleave(32) & ~large[:8000])[:p + 1].sum())
+            off = beside * min(math.exp(-drop), 2.0 ** -18) / ((p + 1 - spikes) * math.exp(-drop))
+            want = 8.0 * (p + 1 - spikes) * math.exp(-drop) / (spikes + (p + 1 - spikes) * math.exp(-drop))
+            got = out[row].double()
+            assert float((got - want).abs().max()) <= (tol + off) * want + 2.0 ** -25, (b, p)
+            row += 1

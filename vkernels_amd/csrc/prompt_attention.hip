@@ -23,6 +23,7 @@ namespace {
 
 using namespace attention;
 
+constexpr float kFall = 14.0f;      // weights stay 2^7 above the smallest fp16 value that has all its bits
 constexpr int kWaves = 4, kWaveRows = kPromptRows / kWaves;
 static_assert(kWaveRows == 32, "a wavefront's rows are the columns of a matrix instruction");
 
@@ -170,6 +171,28 @@ __device__ __forceinline__ float over_halves_sum(float x) {
 
 // Bits below n of 32.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
+// Brings the reference m of a row's weights to its largest new score where that passes it by kSlack; the sums are
+// relative to it.  (A row by itself: what it gives does not depend on the rows beside it.)
+// FALLS: down as well, where all new scores are more than kFall below.  Weights in fp16 end at 2^-24, and positions far below
+// one of large weight may be the whole result, where that one's value is small.  The sums take steps of up to 2^40 until
+// the weights' reaches 2^40: so they stay in range times any value.  What is still lost is 2^-18 of the largest weight among
+// a weight's own 32 positions (2^-7 or more in fp16, a half step at most 2^-25), and what is below 2^-60 of the row's.
+template <bool FALLS, int N>
+__device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&acc)[N]) {
+  // (one comparison for both sides)
+  const float middle = (kSlack - kFall) / 2;
+  if (!__any(FALLS ? fabsf(top - m - middle) > kSlack - middle : top > m + kSlack)) return;
+  float m_new = top > m + kSlack ? top : m;
+  if constexpr (FALLS) {
+    if (over_halves_max(l) < 0x1p40f && top < m - kFall && top > kNegInf) m_new = fmaxf(top, m - 40.0f);
+  }
+  const float fix = exp2_fast(m - or_zero(m_new));
+  m = m_new;
+  l *= fix;
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] *= fix;
+}
 
 // S^T = K q^T and O^T += V^T P^T, both 32 x 32 x 16 with the keys (the head's width) as rows and a wavefront's 32
 // rows as columns: a lane holds half of one row's scores, so that maximum, sum and rescaling stay in the lane and its
@@ -413,24 +436,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
     return over_halves_max(top);
   };
-  auto raise = [&](float top) {
-    if (__any(top > m + kSlack)) {
-      // (a row by itself: what it gives does not depend on the rows beside it)
-      const float m_new = top > m + kSlack ? top : m;
-      const float fix = exp2_fast(m - or_zero(m_new));
-      m = m_new;
-      l *= fix;
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) acc[i] *= fix;
-    }
-  };
+  auto follow_scores = [&](float top) { follow<std::is_same_v<W, F16>>(top, m, l, acc); };
 
   // The same where every row of the workgroup sees all of the sub and the scores need nothing but their factor: one
   // stretch of code in a fixed order, reads from LDS three operands ahead and the exponentials (then the next
   // scores' maximum) between the matrix instructions.  `top`: the largest scores, of the next sub afterwards.
   auto attend_whole = [&](int sub, const f32x16& x, f32x16& next, float& top) {
     constexpr int kSteps = DP / 16, kAhead = 3;
-    raise(top * to_log2);
+    follow_scores(top * to_log2);
     const float ref = or_zero(m) - kLift;
     union { typename W::T e[16]; typename W::V8 v[2]; } p;
     typename M::V8 k[kSteps];
@@ -505,7 +518,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
       }
     }
-    raise(largest(x) * c);
+    follow_scores(largest(x) * c);
     const float ref = or_zero(m) - kLift;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -904,14 +917,7 @@ __global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const Kern
 #pragma unroll
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
     top = over_halves_max(top);
-    if (__any(top > m + kSlack)) {
-      const float m_new = top > m + kSlack ? top : m;
-      const float fix = exp2_fast(m - or_zero(m_new));
-      m = m_new;
-      l *= fix;
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) acc[i] *= fix;
-    }
+    follow<std::is_same_v<W, F16>>(top, m, l, acc);
     const float ref = or_zero(m) - kLift;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
