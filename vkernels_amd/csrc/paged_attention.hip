@@ -757,7 +757,7 @@ __device__ __forceinline__ void add_weights(const KernelArgs& A, int block, int 
   const float* const scores = (const float*)((const char*)a.workspace + A.p.scores_at) +
                               (int64_t)bg * A.p.score_pitch * a.G;
   float* const to = a.sums + (int64_t)b * a.sums_stride_b + (int64_t)g * a.sums_stride_h;
-  const int place0 = at + threadIdx.x * 4;        // and 1024, 2048, 3072 behind it
+  const int place0 = at + threadIdx.x * 4;        // and PER - 1 more, 1024 apart
   // (16 bytes at a time where the sums' rows allow it and all four positions are seen)
   const bool wide = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
   auto all_seen = [&](int pos) { return wide && (pos >= span.lo || pos + 3 < span.first) && pos + 3 < span.len; };
