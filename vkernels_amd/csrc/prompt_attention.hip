@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     };
     for (int tile = tile_begin; tile < tile_end;) {
       // (heads of more than 128 do not have the registers)
-      if constexpr (DP <= 128) {
+      if constexpr (true) {
         if (plain) {
           float top = largest(even);
           for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
