@@ -70,6 +70,14 @@ def test_few_tokens_on_long_sequences(hip_lib, window, first, block, D, q):
     Prompt([5000, 1, 2200, 700, 0], [3, 1, 8, 20, 0], 2, 4, D, 16, block, q=q, seed=D, spare=1).check(window=window, keep_first=first, sinks=True)
 
 
+@pytest.mark.parametrize("window,first", [(0, 0), (300, 70)])
+@pytest.mark.parametrize("block,ps,D", [(16, 16, 256), (-1, 16, 160), (8, 24, 208), (1, 5, 240), (16, 16, 144), (16, 16, 192), (4, 16, 112)])
+@pytest.mark.parametrize("q", [BF16, F16])
+def test_few_tokens_over_codes_of_every_width(hip_lib, window, first, block, ps, D, q):
+    Prompt([3000, 1, 700, 90, 0], [3, 1, 8, 12, 0], 2, 4, D, ps, block, q=q, seed=D, spare=1).check(window=window, keep_first=first, sinks=True)
+    Prompt([300, 33, 64], [1, 2, 16], 1, 5, D, ps, block, q=q, seed=D + 1, layout="tokens").check(softcap=20.0)
+
+
 def test_parts_that_see_nothing(hip_lib):
     """Far more room than positions: shares behind every position, and sequences without any."""
     s = Prompt([40, 9, 0], [4, 9, 0], 1, 1, 64, 16, 0)

@@ -1,10 +1,11 @@
 // kv_capi.cpp — the extern "C" surface of the key-value cache's operators (declared in
 // include/vkernels_hip.h): argument checks and error state; the kernels are in
-// paged_attention.hip and kv_cache.hip.
+// kv_cache.hip, kv_blocks.hip, paged_attention.hip, prompt_attention.hip and qk_norm_rope.hip.
 #include "vkernels_hip.h"
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -140,7 +141,7 @@ float cap_of(float softcap) { return softcap >= 0x1p100f ? 0.0f : softcap > 0.0f
 // 4096 workgroups and one for every head more.)
 bool prompt_fits(int B, int tokens, int Hkv, int G, int D) {
   if (tokens > kInt32 / 4 / G || B > kInt32 / 4) return false;
-  return vk::prompt_attention_slots(B, tokens, G, D) <= kThreads / 512 / Hkv;
+  return vk::prompt_attention_slots(B, tokens, G, D, true) <= kThreads / 512 / Hkv;      // (in smaller tiles, if the cache's type says so)
 }
 
 // Attention of one new token of every sequence.
@@ -302,7 +303,10 @@ size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv,
                                                      int keep_first) {
   if (B <= 0 || tokens <= 0 || Hkv <= 0 || G <= 0 || D <= 0 || max_len < 0 || keep_first < 0) return 0;
   if (!prompt_fits(B, tokens, Hkv, G, D)) return 0;
-  return vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, window > 0 ? keep_first : 0).bytes;
+  auto bytes = [&](bool fp8) {
+    return vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, window > 0 ? keep_first : 0, fp8).bytes;
+  };
+  return std::max(bytes(false), bytes(true));      // (a cache of either type)
 }
 
 int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void* v_cache,
@@ -333,7 +337,7 @@ int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void
   if (max_len > kPositions || !prompt_fits(B, tokens, Hkv, G, D))
     return refuse(VK_ERROR_OUT_OF_RANGE, who, "too many sequences, tokens, heads and positions for one call");
   keep_first = window > 0 ? keep_first : 0;
-  const vk::PromptAttentionPlan plan = vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, keep_first);
+  const vk::PromptAttentionPlan plan = vk::prompt_attention_plan(B, tokens, Hkv, G, D, max_len, window, keep_first, elem_of(kind) == 1);
   if (plan.bytes > 0 && (workspace == nullptr || workspace_bytes < plan.bytes || !aligned(workspace, 16)))
     return refuse(VK_ERROR_INVALID_ARGUMENT, who,
                   "a workspace of vk_hip_paged_attention_prompt_workspace_bytes (16-byte aligned) is needed");

@@ -690,13 +690,15 @@ struct FewLayout {
   // (32 sequences of up to 8192, 8 heads of 128 in bf16: 163 us with one workgroup a CU, 138 so).
   static constexpr bool kDirect = FP8 || DP <= 64;
   static constexpr int kBuffers = kDirect ? 2 : 1;
-  static __device__ __forceinline__ int code_turn(int row) { return kLanes == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
+  static __device__ __forceinline__ int code_turn(int row) {
+    return kLanes == 4 ? (row >> 2) & 3 : kLanes == 8 ? (row >> 1) & 7 : row & 15;
+  }
   static __device__ __forceinline__ int key_piece(int slot, int row) {
     return FP8 ? slot ^ code_turn(row) : L::key_piece(slot, row);
   }
   // (codes of values are read two neighbouring pieces of rows 0 .. 3 and 8 .. 11, or 4 .. 7 and 12 .. 15, at once)
   static __device__ __forceinline__ int value_code_turn(int row) {
-    return kLanes == 4 ? (row >> 3 & 1) * 2 : (row >> 1 & 1) * 2 + (row >> 3 & 1) * 4;
+    return kLanes == 4 ? (row >> 3 & 1) * 2 : kLanes == 8 ? (row >> 1 & 1) * 2 + (row >> 3 & 1) * 4 : (row & 3) * 2 + (row >> 3 & 1) * 8;
   }
   static __device__ __forceinline__ int value_piece(int slot, int row) {
     return FP8 ? slot ^ value_code_turn(row) : L::value_piece(slot, row);
@@ -711,7 +713,7 @@ struct FewLayout {
 // 95 us (2.9 TB/s) of which a workgroup's start, six dependent loads, and end are a third; one sequence of 131071: 68
 // (4.0 TB/s), in bf16 115 (4.7).  With tiles of 128 rows, one wavefront with all of them: 250.
 template <class M, bool FP8, int DP>
-__global__ __launch_bounds__(256, 2) void prompt_attention_few_kernel(const KernelArgs A) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_few_kernel(const KernelArgs A) {
   typedef std::conditional_t<FP8, Bf16, M> W;
   typedef FewLayout<FP8, DP> F;
   constexpr int kSub = 32, kSumPitch = DP + 4;
@@ -1110,7 +1112,7 @@ void launch_width(const KernelArgs& A, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)A.p.slots * A.a.Hkv * A.p.splits)), block(256);
   const int rows = 1 << A.p.row_shift;
   bool few = false;
-  if constexpr (DP <= kPromptFewWidth) {
+  if constexpr (FP8 || DP <= kPromptFewWidth) {
     few = rows == kPromptFewRows;
     if (few) hipLaunchKernelGGL((prompt_attention_few_kernel<M, FP8, DP>), grid, block, 0, stream, A);
   }
@@ -1136,19 +1138,22 @@ void launch_kind(const KernelArgs& A, hipStream_t stream) {
 
 }  // namespace
 
-// Tiles of 32 rows where the sequences have no more on average.  (Wider heads do not have the registers.)
-static int row_shift_of(int B, int tokens, int G, int D) {
-  return D <= kPromptFewWidth && (int64_t)tokens * G <= (int64_t)kPromptFewRows * B ? 5 : 7;
+// Tiles of 32 rows where the sequences have no more on average; of wider 16-bit heads not (5 tokens of 32 sequences of up to
+// 4096, 8 heads of 4 of 256: 481 us against 208, 127 registers spilled; of 192 values 186 against 178.  In 8 bits over up
+// to 8192 267 against 485, and 223 against 436).
+static int row_shift_of(int B, int tokens, int G, int D, bool fp8) {
+  return (fp8 || D <= kPromptFewWidth) && (int64_t)tokens * G <= (int64_t)kPromptFewRows * B ? 5 : 7;
 }
 
-int64_t prompt_attention_slots(int B, int tokens, int G, int D) {
-  return ((int64_t)tokens * G >> row_shift_of(B, tokens, G, D)) + B + 1;
+int64_t prompt_attention_slots(int B, int tokens, int G, int D, bool fp8) {
+  return ((int64_t)tokens * G >> row_shift_of(B, tokens, G, D, fp8)) + B + 1;
 }
 
-PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first) {
+PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first,
+                                          bool fp8) {
   PromptAttentionPlan p{};
-  p.row_shift = row_shift_of(B, tokens, G, D);
-  p.slots = (int)prompt_attention_slots(B, tokens, G, D);
+  p.row_shift = row_shift_of(B, tokens, G, D, fp8);
+  p.slots = (int)prompt_attention_slots(B, tokens, G, D, fp8);
   const int rows = 1 << p.row_shift;
   // Where there are fewer tiles than the card holds workgroups, several share the positions of each.
   const int64_t tiles = (p.slots - 1) * (int64_t)Hkv;
@@ -1178,7 +1183,7 @@ PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int
 void launch_prompt_attention(const PromptAttentionArgs& a, int kind, hipStream_t stream) {
   KernelArgs A{};
   A.a = a;
-  A.p = prompt_attention_plan(a.B, a.tokens, a.Hkv, a.G, a.D, a.max_len, a.window, a.keep_first);
+  A.p = prompt_attention_plan(a.B, a.tokens, a.Hkv, a.G, a.D, a.max_len, a.window, a.keep_first, kind >= kKvFp8Bf16);
   A.by_page = fast_div(a.page_size);
   A.by_block = fast_div(a.scale_blocks > 0 ? a.page_size / a.scale_blocks : 1);
   A.by_group = fast_div(a.G);

@@ -12,7 +12,7 @@ namespace vk {
 constexpr int kPromptRows = 128;   // of a workgroup: a row is a query head of a token, the G heads of a key/value
                                    // head and a token one behind the other
 constexpr int kPromptFewRows = 32; // ... where sequences have few rows: the wavefronts share the positions instead
-constexpr int kPromptFewWidth = 128;   // ... and heads of no more values
+constexpr int kPromptFewWidth = 128;   // ... and heads of no more values, or an 8-bit cache
 constexpr int kPromptKeys = 64;    // positions a workgroup takes at a time
 
 struct PromptAttentionArgs {
@@ -43,8 +43,9 @@ struct PromptAttentionPlan {
   int share;                // kPromptKeys positions that each of them takes at most
   size_t ml_at, part_at, bytes;   // parts of the workspace
 };
-int64_t prompt_attention_slots(int B, int tokens, int G, int D);
-PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first);
+int64_t prompt_attention_slots(int B, int tokens, int G, int D, bool fp8);
+PromptAttentionPlan prompt_attention_plan(int B, int tokens, int Hkv, int G, int D, int max_len, int window, int keep_first,
+                                          bool fp8);
 void launch_prompt_attention(const PromptAttentionArgs& a, int kind, hipStream_t stream);
 
 }  // namespace vk
