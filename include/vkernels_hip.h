@@ -783,8 +783,8 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
  * above, token i is at p = L - n + i and sees positions j <= p, with a window those with j > p - window or
  * j < keep_first.  Scores, cap, sinks, scales, results and rows that see nothing as above; what is stored at a position
  * that a token does not see has no part in its row, NaN and infinities included.  Weights enter the product with
- * the values in 16 bits (bf16 with an 8-bit cache), rounded once, or as two such terms where rows are few (fp16: but
- * for 2^-18 of the largest weight among its 32 positions).  Rows that belong to no sequence become 0 (lse -inf)
+ * the values in the queries' type, rounded once, or where rows are few as two such terms, bf16's of an 8-bit cache
+ * (fp16: but for 2^-18 of the largest weight, times its scale, among its 32 positions).  Rows that belong to no sequence become 0 (lse -inf)
  * with clear_rest != 0 and else stay as they are.  The workspace is scratch of this call alone; 0 bytes: none is
  * needed.  Deterministic: no atomics on floating-point data. */
 size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,

@@ -29,7 +29,7 @@ class Prompt(Setup):
         out, lse = got if got is not None else self.call(**kw)
         torch.cuda.synchronize()
         # (bf16 has 8 significant bits, fp16 11)
-        bits = 11 if self.q.dtype is F16 and not self.block else 8
+        bits = 11 if self.q.dtype is F16 else 8
         want = aref.attention(self.q, self.k, self.v, self.table, self.lens, self.starts, k_scale=self.k_scale,
                               v_scale=self.v_scale, weight_bits=bits, **dict(kw, scale=kw.get("scale", self.D ** -0.5)))
         n = sum(self.new)

@@ -210,10 +210,13 @@ __device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&a
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(const KernelArgs A) {
   typedef Layout<DP> L;
-  typedef std::conditional_t<FP8, Bf16, M> W;      // what weights and values are multiplied in
+  // What values and weights, times a value's scale, are multiplied in: queries' type.  fp16 does not have every scale's range:
+  // there the reference of the weights follows weight times scale, kRanged.
+  typedef M W;
+  constexpr bool kRanged = FP8 && std::is_same_v<W, F16>;
   const PromptAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[L::kLds];
-  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][2][2 * kPromptKeys];   // as well
+  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][kRanged ? 3 : 2][2 * kPromptKeys];   // as well
   __shared__ int64_t row_lds[kWaves][2 * kPromptKeys];      // by the place mod 128
   __shared__ uint32_t any_bad;      // values that are no finite numbers have been left out
 
@@ -356,6 +359,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     const int at = (tile * kPromptKeys + kPromptKeys / 2 + lane) & (2 * kPromptKeys - 1);
     scale_lds[wave][0][at] = ks;
     scale_lds[wave][1][at] = vs;
+    // (beyond these a result of fp16 is 0, or no finite number; a scale that is not seen may be anything)
+    if constexpr (kRanged) scale_lds[wave][2][at] = vs == 0.0f ? 0.0f : fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -40.0f), 26.0f);
   };
   auto put_values = [&](int tile, uint64_t there) {
     const bool look = partial(walk.position(tile * kPromptKeys));
@@ -429,21 +434,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) acc[i] = W::mfma(read_values(sub, j, i), p, acc[i]);
   };
-  // The largest of a row's scores (both halves').
-  auto largest = [&](const f32x16& x) {
+  // What the reference follows of a sub's scores, c times which is in powers of two: the largest (of both halves).
+  auto largest = [&](int sub, const f32x16& x, float c) {
+    if constexpr (kRanged) {
+      float top = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 16; j += 4) {
+        const f32x4 f = scales_of(sub, 2, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, __builtin_fmaf(x[j + i], c, f[i]));
+      }
+      return over_halves_max(top);
+    }
     float top = x[0];
 #pragma unroll
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-    return over_halves_max(top);
+    return over_halves_max(top) * c;
   };
   auto follow_scores = [&](float top) { follow<std::is_same_v<W, F16>>(top, m, l, acc); };
 
   // The same where every row of the workgroup sees all of the sub and the scores need nothing but their factor: one
   // stretch of code in a fixed order, reads from LDS three operands ahead and the exponentials (then the next
-  // scores' maximum) between the matrix instructions.  `top`: the largest scores, of the next sub afterwards.
+  // scores' maximum) between the matrix instructions.  `top`: what the reference follows, of the next sub afterwards.
   auto attend_whole = [&](int sub, const f32x16& x, f32x16& next, float& top) {
     constexpr int kSteps = DP / 16, kAhead = 3;
-    follow_scores(top * to_log2);
+    follow_scores(top);
     const float ref = or_zero(m) - kLift;
     union { typename W::T e[16]; typename W::V8 v[2]; } p;
     typename M::V8 k[kSteps];
@@ -473,6 +488,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       __builtin_amdgcn_sched_barrier(0);
     }
     float most[2];
+    f32x4 range;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       acc[i % (DP / 32)] = W::mfma(v[i], p.v[i / (DP / 32)], acc[i % (DP / 32)]);
@@ -483,11 +499,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
           if (j % 4 == 0) f = scales_of(sub + 1, 0, j);
           next[j] *= f[j % 4];
         }
-        most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
+        float y = next[j];
+        if constexpr (kRanged) {
+          if (j % 4 == 0) range = scales_of(sub + 1, 2, j);
+          y = __builtin_fmaf(y, to_log2, range[j % 4]);
+        }
+        most[j & 1] = j < 2 ? y : fmaxf(most[j & 1], y);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    top = over_halves_max(fmaxf(most[0], most[1]));
+    top = over_halves_max(fmaxf(most[0], most[1])) * (kRanged ? 1.0f : to_log2);
   };
 
   // Positions of a sub, whose scores are in `x`, and the scores of the next one (skip_next: not those).
@@ -518,7 +539,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
       }
     }
-    follow_scores(largest(x) * c);
+    follow_scores(largest(sub, x, c));
     const float ref = or_zero(m) - kLift;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
@@ -578,7 +599,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       // (heads of more than 128 do not have the registers)
       if constexpr (true) {
         if (plain) {
-          float top = largest(even);
+          float top = largest(2 * tile, even, to_log2);
           for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
             ahead(tile);
             attend_whole(2 * tile, even, odd, top);
