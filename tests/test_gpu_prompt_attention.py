@@ -28,8 +28,8 @@ class Prompt(Setup):
         kw = dict(kw, sinks=self.sinks if sinks else None)
         out, lse = got if got is not None else self.call(**kw)
         torch.cuda.synchronize()
-        # (bf16 has 8 significant bits, fp16 11)
-        bits = 11 if self.q.dtype is F16 else 8
+        # (bf16 has 8 significant bits, fp16 11; weights of 8-bit caches are fp16)
+        bits = 11 if self.q.dtype is F16 or self.block else 8
         want = aref.attention(self.q, self.k, self.v, self.table, self.lens, self.starts, k_scale=self.k_scale,
                               v_scale=self.v_scale, weight_bits=bits, **dict(kw, scale=kw.get("scale", self.D ** -0.5)))
         n = sum(self.new)
@@ -76,6 +76,20 @@ def test_few_tokens_on_long_sequences(hip_lib, window, first, block, D, q):
 def test_few_tokens_over_codes_of_every_width(hip_lib, window, first, block, ps, D, q):
     Prompt([3000, 1, 700, 90, 0], [3, 1, 8, 12, 0], 2, 4, D, ps, block, q=q, seed=D, spare=1).check(window=window, keep_first=first, sinks=True)
     Prompt([300, 33, 64], [1, 2, 16], 1, 5, D, ps, block, q=q, seed=D + 1, layout="tokens").check(softcap=20.0)
+
+
+@pytest.mark.parametrize("new", [(200, 150), (3, 5)])
+@pytest.mark.parametrize("q,size", [(BF16, 2.0 ** -54), (BF16, 2.0 ** 60), (BF16, 1.0), (F16, 2.0 ** -6), (F16, 2.0 ** 5), (F16, -1.0)])
+@pytest.mark.parametrize("block", [-1, 4, 16])
+def test_value_scales_of_any_size(hip_lib, new, q, size, block):
+    """The weights' reference follows them: all far from 1, below it, blocks of zeros and blocks 2^12 apart."""
+    s = Prompt([700, 600], new, 2, 4, 128, 16, block, q=q, seed=5)
+    s.v_scale = s.v_scale * size
+    if block > 0:
+        kind = torch.randint(0, 3, s.v_scale.shape, generator=torch.Generator().manual_seed(1)).to(dev())
+        s.v_scale = torch.where(kind == 0, s.v_scale, torch.where(kind == 1, s.v_scale * 2.0 ** -12, 0.0))
+    s.check(sinks=True)
+    s.check(window=100, keep_first=20)
 
 
 def test_parts_that_see_nothing(hip_lib):

@@ -173,20 +173,24 @@ __device__ __forceinline__ float over_halves_sum(float x) {
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 
 // Brings the reference m of a row's weights to its largest new score where that passes it by kSlack; the sums are
-// relative to it.  (A row by itself: what it gives does not depend on the rows beside it.)
+// relative to it.  (A row by itself: what it gives does not depend on the rows beside it; of an 8-bit cache, where a tile that
+// all rows see is looked at by its largest score and scale, within rounding.)
 // FALLS: down as well, where all new scores are more than kFall below.  Weights in fp16 end at 2^-24, and positions far below
 // one of large weight may be the whole result, where that one's value is small.  The sums take steps of up to 2^40 until
 // the weights' reaches 2^40: so they stay in range times any value.  What is still lost is 2^-18 of the largest weight among
 // a weight's own 32 positions (2^-7 or more in fp16, a half step at most 2^-25), and what is below 2^-60 of the row's.
-template <bool FALLS, int N>
-__device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&acc)[N]) {
+// PEAK: the weighted sums are not bound by the weights' (their scales are on top), and the reference stays within 2^60 of its
+// highest place.
+template <bool FALLS, bool PEAK, int N>
+__device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&acc)[N], float& peak) {
   // (one comparison for both sides)
   const float middle = (kSlack - kFall) / 2;
   if (!__any(FALLS ? fabsf(top - m - middle) > kSlack - middle : top > m + kSlack)) return;
   float m_new = top > m + kSlack ? top : m;
   if constexpr (FALLS) {
-    if (over_halves_max(l) < 0x1p40f && top < m - kFall && top > kNegInf) m_new = fmaxf(top, m - 40.0f);
+    if (over_halves_max(l) < 0x1p40f && top < m - kFall && top > kNegInf && (!PEAK || m > peak - 20.0f)) m_new = fmaxf(top, m - 40.0f);
   }
+  if constexpr (PEAK) peak = fmaxf(peak, m_new);
   const float fix = exp2_fast(m - or_zero(m_new));
   m = m_new;
   l *= fix;
@@ -210,13 +214,14 @@ __device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&a
 template <class M, bool FP8, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(const KernelArgs A) {
   typedef Layout<DP> L;
-  // What values and weights, times a value's scale, are multiplied in: queries' type.  fp16 does not have every scale's range:
-  // there the reference of the weights follows weight times scale, kRanged.
-  typedef M W;
-  constexpr bool kRanged = FP8 && std::is_same_v<W, F16>;
+  // What values and weights are multiplied in.  Codes are exact in fp16, and weights times the values' scales have three bits
+  // more there than in bf16, whose errors would be larger than the result's own rounding (2.5e-3 against 1.7e-3 in bf16
+  // results, where fp16 weights leave 1.7e-3; 1.42 against 1.23 ms).  fp16 does not have every scale's range, so that the
+  // reference of the weights follows weight times scale.
+  typedef std::conditional_t<FP8, F16, M> W;
   const PromptAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[L::kLds];
-  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][kRanged ? 3 : 2][2 * kPromptKeys];   // as well
+  __shared__ __attribute__((aligned(16))) float scale_lds[FP8 ? kWaves : 1][3][2 * kPromptKeys];   // as well
   __shared__ int64_t row_lds[kWaves][2 * kPromptKeys];      // by the place mod 128
   __shared__ uint32_t any_bad;      // values that are no finite numbers have been left out
 
@@ -268,7 +273,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-  float m = kNegInf, l = 0.0f;
+  float m = kNegInf, l = 0.0f, peak = kNegInf;
   // (fp16 weights end at 2^-24: they are kept 2^7 above the reference, so that with the slack they reach 2^15)
   constexpr float kLift = std::is_same_v<W, F16> ? 7.0f : 0.0f;
 
@@ -301,6 +306,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   };
   u32x2 kreg[L::kLoads], vreg[L::kLoads];      // (8-bit caches)
   float ks = 1.0f, vs = 1.0f;
+  // The largest value scale (in powers of two) of the 32 positions behind an even sub, behind an odd one.
+  float range_of[2] = {0.0f, 0.0f};
   // A lane works out where its place's rows lie, for the wavefront's lanes that load them; which of the places there are.
   auto find_rows = [&](int tile, int entry) -> uint64_t {
     const int at_place = tile * kPromptKeys + kPromptKeys / 2 + lane, pos = walk.position(max(at_place, 0));
@@ -359,8 +366,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     const int at = (tile * kPromptKeys + kPromptKeys / 2 + lane) & (2 * kPromptKeys - 1);
     scale_lds[wave][0][at] = ks;
     scale_lds[wave][1][at] = vs;
-    // (beyond these a result of fp16 is 0, or no finite number; a scale that is not seen may be anything)
-    if constexpr (kRanged) scale_lds[wave][2][at] = vs == 0.0f ? 0.0f : fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -40.0f), 26.0f);
+    // (From 2^-60, 0 among them, to 2^60: a step of the reference from one end to the other stays within 32 bits, so that
+    // the sum of weights keeps positions whose values are 0.  A scale that is not seen may be anything.)
+    float range = fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -60.0f), 60.0f);
+    scale_lds[wave][2][at] = range;
+    // (the largest of 16 lanes by rotations within them)
+    auto with = [&](float other) { range = fmaxf(range, other); };
+    with(__uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(range), 0x128, 0xF, 0xF, false)));
+    with(__uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(range), 0x124, 0xF, 0xF, false)));
+    with(__uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(range), 0x122, 0xF, 0xF, false)));
+    with(__uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(range), 0x121, 0xF, 0xF, false)));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float most = fmaxf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(range), i * 32)),
+                               __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(range), i * 32 + 16)));
+      range_of[i] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(most)));
+    }
   };
   auto put_values = [&](int tile, uint64_t there) {
     const bool look = partial(walk.position(tile * kPromptKeys));
@@ -436,7 +457,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   };
   // What the reference follows of a sub's scores, c times which is in powers of two: the largest (of both halves).
   auto largest = [&](int sub, const f32x16& x, float c) {
-    if constexpr (kRanged) {
+    if constexpr (FP8) {
       float top = kNegInf;
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
@@ -451,7 +472,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
     return over_halves_max(top) * c;
   };
-  auto follow_scores = [&](float top) { follow<std::is_same_v<W, F16>>(top, m, l, acc); };
+  auto follow_scores = [&](float top) { follow<std::is_same_v<W, F16>, FP8>(top, m, l, acc, peak); };
 
   // The same where every row of the workgroup sees all of the sub and the scores need nothing but their factor: one
   // stretch of code in a fixed order, reads from LDS three operands ahead and the exponentials (then the next
@@ -488,7 +509,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       __builtin_amdgcn_sched_barrier(0);
     }
     float most[2];
-    f32x4 range;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       acc[i % (DP / 32)] = W::mfma(v[i], p.v[i / (DP / 32)], acc[i % (DP / 32)]);
@@ -499,16 +519,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
           if (j % 4 == 0) f = scales_of(sub + 1, 0, j);
           next[j] *= f[j % 4];
         }
-        float y = next[j];
-        if constexpr (kRanged) {
-          if (j % 4 == 0) range = scales_of(sub + 1, 2, j);
-          y = __builtin_fmaf(y, to_log2, range[j % 4]);
-        }
-        most[j & 1] = j < 2 ? y : fmaxf(most[j & 1], y);
+        most[j & 1] = j < 2 ? next[j] : fmaxf(most[j & 1], next[j]);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    top = over_halves_max(fmaxf(most[0], most[1])) * (kRanged ? 1.0f : to_log2);
+    top = __builtin_fmaf(over_halves_max(fmaxf(most[0], most[1])), to_log2, FP8 ? range_of[sub & 1] : 0.0f);
   };
 
   // Positions of a sub, whose scores are in `x`, and the scores of the next one (skip_next: not those).
@@ -940,7 +955,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_few_k
 #pragma unroll
     for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
     top = over_halves_max(top);
-    follow<std::is_same_v<W, F16>>(top, m, l, acc);
+    follow<std::is_same_v<W, F16>, false>(top, m, l, acc, m);
     const float ref = or_zero(m) - kLift;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
