@@ -785,7 +785,8 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
  * that a token does not see has no part in its row, NaN and infinities included.  Weights enter the product with
  * the values in the queries' type, of an 8-bit cache (times the values' scales) in fp16, rounded once, or where rows are
  * few as two 16-bit terms; in fp16 2^-18 of the largest weight (times the largest scale) among its 32 positions
- * may be lost.  Value scales are 0 or of sizes from 2^-60 to 2^60.  Rows that belong to no sequence become 0 (lse -inf) with clear_rest != 0 and else stay as they are.
+ * may be lost.  Rows that see a value scale outside of 2^-60 .. 2^60 (0 is none) have two bf16 terms a weight as well.  Rows
+ * that belong to no sequence become 0 (lse -inf) with clear_rest != 0 and else stay as they are.
  * The workspace is scratch of this call alone; 0 bytes: none is needed.  Deterministic: no atomics on floating-point
  * data. */
 size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,

@@ -24,6 +24,7 @@ namespace {
 using namespace attention;
 
 constexpr float kFall = 14.0f;      // weights stay 2^7 above the smallest fp16 value that has all its bits
+constexpr float kLeastScale = 0x1p-60f, kMostScale = 0x1p60f;      // of values, that fp16 weights follow
 constexpr int kWaves = 4, kWaveRows = kPromptRows / kWaves;
 static_assert(kWaveRows == 32, "a wavefront's rows are the columns of a matrix instruction");
 
@@ -217,7 +218,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   // What values and weights are multiplied in.  Codes are exact in fp16, and weights times the values' scales have three bits
   // more there than in bf16, whose errors would be larger than the result's own rounding (2.5e-3 against 1.7e-3 in bf16
   // results, where fp16 weights leave 1.7e-3; 1.42 against 1.23 ms).  fp16 does not have every scale's range, so that the
-  // reference of the weights follows weight times scale.
+  // reference of the weights follows weight times scale; rows that see scales outside 2^-60 .. 2^60 are worked on again.
   typedef std::conditional_t<FP8, F16, M> W;
   const PromptAttentionArgs& a = A.a;
   __shared__ __attribute__((aligned(16))) char lds[L::kLds];
@@ -715,6 +716,41 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   if (any_bad && tile_begin < tile_end) add_bad((typename M::T*)a.out + out_row * a.D);
 }
 
+// Does a row of the tile see a position whose value scale is outside of what fp16 weights follow?  (An infinite one or
+// NaN makes the row what it is either way.)
+__device__ __forceinline__ bool sees_far_scales(const KernelArgs& A, const Tile& t) {
+  const PromptAttentionArgs& a = A.a;
+  __shared__ uint32_t any_far;
+  if (threadIdx.x == 0) any_far = 0;
+  __syncthreads();
+  const int before = min(max(a.lens[t.b], 0), a.max_len) - t.tokens;
+  const int hi = before + divided(min(t.first + kPromptRows, t.rows) - 1, A.by_group) + 1;
+  const int begin = a.window > 0 ? max(before + divided(t.first, A.by_group), a.window - 1) - a.window + 1 : 0;
+  bool far = false;
+  auto look = [&](int64_t at) {
+    const float size = fabsf(a.v_scale[at]);
+    far |= size != 0.0f && (size < kLeastScale || size > kMostScale) && size < __builtin_inff();
+  };
+  if (a.scale_blocks == 0) {
+    look(t.head);
+  } else if (hi > 0) {
+    // The blocks of the first positions, then those of the window (all, without one).
+    const int32_t* const table = a.table + (int64_t)t.b * a.table_stride;
+    const int block = a.page_size / a.scale_blocks, lo = divided(begin, A.by_block);
+    const int first = a.keep_first > 0 ? min(lo, divided(a.keep_first - 1, A.by_block) + 1) : 0;
+    const int blocks = first + divided(hi - 1, A.by_block) + 1 - lo;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < blocks; i += 256) {
+      const int pos = (i < first ? i : lo + i - first) * block, in_table = divided(pos, A.by_page), id = table[in_table];
+      if ((uint32_t)id < (uint32_t)a.num_pages)
+        look(((int64_t)id * a.Hkv + t.head) * a.scale_blocks + divided(pos - in_table * a.page_size, A.by_block));
+    }
+  }
+  if (__any(far)) any_far = 1;
+  __syncthreads();
+  return any_far != 0;
+}
+
 // A wavefront's 32 positions in LDS: rows as they are in the cache, pieces of 16 bytes exchanged by the row (each exchange
 // its own inverse) so that 16 rows' pieces spread over the banks.
 template <bool FP8, int DP>
@@ -748,7 +784,10 @@ struct FewLayout {
 // after the other.  Bound by latency: 5 tokens of 32 sequences of 1024 to 8192, 32 heads on 8 of 128 in 8 bits, 279 MB:
 // 95 us (2.9 TB/s) of which a workgroup's start, six dependent loads, and end are a third; one sequence of 131071: 68
 // (4.0 TB/s), in bf16 115 (4.7).  With tiles of 128 rows, one wavefront with all of them: 250.
-template <class M, bool FP8, int DP>
+// AGAIN: behind tiles of 128 rows over an 8-bit cache, the rows that see a value scale outside of what the fp16 weights
+// there take (two bf16 terms take any), 32 of a tile's 128 after the other; without such a scale a workgroup only looks: 9 us
+// of the 1438 for 4096 tokens over 16384 positions in blocks of 16.
+template <class M, bool FP8, int DP, bool AGAIN>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_few_kernel(const KernelArgs A) {
   typedef std::conditional_t<FP8, Bf16, M> W;
   typedef FewLayout<FP8, DP> F;
@@ -769,312 +808,319 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_few_k
   Tile t;
   if (!find_tile(A, blockIdx.x, &t)) return;
   if (t.b == a.B) {
-    clear_rows(A, t);
+    if constexpr (!AGAIN) clear_rows(A, t);
     return;
   }
-  const int len = min(max(a.lens[t.b], 0), a.max_len), before = len - t.tokens;
-  const int row = min(t.first + n, t.rows - 1), tok = divided(row, A.by_group), g = row - tok * a.G;
-  const int place = before + tok;
-  const int tile_lo = before + divided(t.first, A.by_group);
-  const int tile_hi = before + divided(min(t.first + kPromptFewRows, t.rows) - 1, A.by_group);
-  auto low_of = [&](int place) { return a.window > 0 ? max(place, a.window - 1) - a.window : -1; };
-  const int low = low_of(place), hi = tile_hi + 1;
-  const Walk walk = walk_of(low_of(tile_lo) + 1, hi, a.keep_first);
-  const int subs = hi <= 0 ? 0 : (hi - walk.shift + kSub - 1) / kSub;
-  const int sub_begin = t.split * A.p.share * 2, sub_end = min(subs, sub_begin + A.p.share * 2);
-  if (sub_begin >= sub_end && A.p.splits > 1) {
-    // (a shorter sequence's)
-    const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
-    if (tid < kPromptFewRows) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + tid] = f32x2{kNegInf, 0.0f};
-    return;
-  }
-
-  typename M::V8 q[DP / 16];
-  {
-    const char* const from = (const char*)a.q + ((int64_t)(t.s0 + tok) * a.q_stride_t + (int64_t)(t.head * a.G + g) * a.q_stride_h) * 2;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      const int d = i * 16 + half * 8;
-      const u32x4 x = *(const u32x4*)(from + (d < a.D ? d : 0) * 2);
-      q[i] = as_v8<M>(d < a.D ? x : u32x4{0, 0, 0, 0});
+  if (AGAIN && !sees_far_scales(A, t)) return;
+  const int last_row = min(t.first + kPromptRows, t.rows);      // (AGAIN)
+  do {
+    const int len = min(max(a.lens[t.b], 0), a.max_len), before = len - t.tokens;
+    const int row = min(t.first + n, t.rows - 1), tok = divided(row, A.by_group), g = row - tok * a.G;
+    const int place = before + tok;
+    const int tile_lo = before + divided(t.first, A.by_group);
+    const int tile_hi = before + divided(min(t.first + kPromptFewRows, t.rows) - 1, A.by_group);
+    auto low_of = [&](int place) { return a.window > 0 ? max(place, a.window - 1) - a.window : -1; };
+    const int low = low_of(place), hi = tile_hi + 1;
+    const Walk walk = walk_of(low_of(tile_lo) + 1, hi, a.keep_first);
+    const int subs = hi <= 0 ? 0 : (hi - walk.shift + kSub - 1) / kSub;
+    const int sub_begin = t.split * A.p.share * 2, sub_end = min(subs, sub_begin + A.p.share * 2);
+    if (sub_begin >= sub_end && A.p.splits > 1) {
+      // (a shorter sequence's)
+      const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
+      if (tid < kPromptFewRows) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + tid] = f32x2{kNegInf, 0.0f};
+      return;
     }
-  }
-  const float to_log2 = (FP8 ? 1.0f : a.scale) * kLog2e;      // (8-bit keys: with the positions' scales)
-  const float cap_in = a.softcap > 0.0f ? 2.0f * to_log2 / a.softcap : 0.0f, cap_out = a.softcap * kLog2e;
-  constexpr float kLift = std::is_same_v<W, F16> ? 7.0f : 0.0f;
-  f32x16 acc[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-    for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
-  float m = kNegInf, l = 0.0f;
-  bool bad = false;             // this lane has left values out that are no finite numbers
 
-  const int32_t* const table = a.table + (int64_t)t.b * a.table_stride;
-  const int last_entry = divided(max(hi - 1, 0), A.by_page);
-  constexpr int kElem = FP8 ? 1 : 2;
-  const char* const kbase = (const char*)a.k_cache + (int64_t)t.head * a.head_stride * kElem;
-  const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
-  const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
-  const int slot = lane % F::kLanes, slot_row = lane / F::kLanes, row_bytes = a.D * kElem;
-  auto lds_keys = [&](int buf) { return (Lds)&lds.tiles[wave][buf][0][0]; };
-  auto lds_values = [&](int buf) { return (Lds)&lds.tiles[wave][buf][1][0]; };
-  // What lies behind a key's last value is zeros, once for all.
-  if (a.D < DP) {
+    typename M::V8 q[DP / 16];
+    {
+      const char* const from = (const char*)a.q + ((int64_t)(t.s0 + tok) * a.q_stride_t + (int64_t)(t.head * a.G + g) * a.q_stride_h) * 2;
 #pragma unroll
-    for (int i = 0; i < F::kLoads; ++i) {
-      const int r = slot_row + i * F::kRows;
-      if (F::key_piece(slot, r) * 16 >= row_bytes) {
-#pragma unroll
-        for (int b = 0; b < F::kBuffers; ++b) *(LdsPiece)(lds_keys(b) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+      for (int i = 0; i < DP / 16; ++i) {
+        const int d = i * 16 + half * 8;
+        const u32x4 x = *(const u32x4*)(from + (d < a.D ? d : 0) * 2);
+        q[i] = as_v8<M>(d < a.D ? x : u32x4{0, 0, 0, 0});
       }
     }
-  }
+    const float to_log2 = (FP8 ? 1.0f : a.scale) * kLog2e;      // (8-bit keys: with the positions' scales)
+    const float cap_in = a.softcap > 0.0f ? 2.0f * to_log2 / a.softcap : 0.0f, cap_out = a.softcap * kLog2e;
+    constexpr float kLift = std::is_same_v<W, F16> ? 7.0f : 0.0f;
+    f32x16 acc[DP / 32];
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[i][j] = 0.0f;
+    float m = kNegInf, l = 0.0f;
+    bool bad = false;             // this lane has left values out that are no finite numbers
 
-  auto ask = [&](int sub) { return table[min(divided(walk.position(sub * kSub) + n, A.by_page), last_entry)]; };
-  auto partial = [&](int pos0) {
-    return pos0 + kSub - 1 > tile_lo || (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kSub > a.keep_first);
-  };
-  u32x4 kreg[F::kLoads], vreg[F::kLoads];      // (those that do not go straight to LDS)
-  float scale_of = 0.0f;        // of position n's key, in the upper half its value
-  uint32_t loaded = 0;          // which positions of the loaded sub there are
-  auto fetch = [&](int sub, int entry, int buf) {
-    const int pos = walk.position(sub * kSub) + n, in_page = pos - divided(pos, A.by_page) * a.page_size;
-    const int id = pos < hi && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
-    loaded = (uint32_t)__ballot(id >= 0);
-    if (half == 0) row_lds[wave][n] = max(id, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
-    if constexpr (FP8) {
-      const int64_t s = a.scale_blocks == 0 ? t.head
-                                            : ((int64_t)max(id, 0) * a.Hkv + t.head) * a.scale_blocks + divided(in_page, A.by_block);
-      scale_of = id < 0 ? 0.0f : half == 0 ? a.k_scale[s] * a.scale : a.v_scale[s];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    int64_t at[F::kLoads];
-#pragma unroll
-    for (int i = 0; i < F::kLoads; ++i) at[i] = row_lds[wave][slot_row + i * F::kRows];
-#pragma unroll
-    for (int i = 0; i < F::kLoads; ++i) {
-      const int piece = F::key_piece(slot, slot_row + i * F::kRows) * 16;
-      if constexpr (!F::kDirect)
-        kreg[i] = *(const u32x4*)(kbase + at[i] + (piece < row_bytes ? piece : 0));
-      else if (piece < row_bytes)
-        dma16(kbase + at[i] + piece, lds_keys(buf) + i * F::kRows * F::kPitch);
-    }
-#pragma unroll
-    for (int i = 0; i < F::kLoads; ++i) {
-      const int piece = F::value_piece(slot, slot_row + i * F::kRows) * 16;
-      if constexpr (!F::kDirect)
-        vreg[i] = *(const u32x4*)(vbase + at[i] + (piece < row_bytes ? piece : 0));
-      else if (piece < row_bytes)
-        dma16(vbase + at[i] + piece, lds_values(buf) + i * F::kRows * F::kPitch);
-    }
-  };
-
-  const int quarter = (lane >> 4) & 1, l16 = lane & 15;
-  // (8-bit values are read 8 x 16 at a time, 16-bit ones 4 x 16)
-  const int value_row = FP8 ? half * 4 + (l16 >> 1) + (l16 >= 8 ? 4 : 0) : half * 4 + (l16 >> 2);
-  const int value_at = value_row * F::kPitch + (FP8 ? l16 & 1 : l16 & 3) * 8, key_row = n * F::kPitch;
-  int entry = 0;
-  if (sub_begin + wave < sub_end) {
-    fetch(sub_begin + wave, ask(sub_begin + wave), 0);
-    entry = ask(sub_begin + wave + kWaves);
-  }
-  int buf = 0;
-  for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
-    const int pos0 = walk.position(sub * kSub);
-    const uint32_t there = loaded;
-    const bool look = partial(pos0);
-    const Lds keys = lds_keys(buf), values = lds_values(buf);
-    buf ^= F::kBuffers - 1;
-    if constexpr (F::kDirect) {
-      __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
+    const int32_t* const table = a.table + (int64_t)t.b * a.table_stride;
+    const int last_entry = divided(max(hi - 1, 0), A.by_page);
+    constexpr int kElem = FP8 ? 1 : 2;
+    const char* const kbase = (const char*)a.k_cache + (int64_t)t.head * a.head_stride * kElem;
+    const char* const vbase = (const char*)a.v_cache + (int64_t)t.head * a.head_stride * kElem;
+    const int64_t page_bytes = a.page_stride * kElem, slot_bytes = a.slot_stride * kElem;
+    const int slot = lane % F::kLanes, slot_row = lane / F::kLanes, row_bytes = a.D * kElem;
+    auto lds_keys = [&](int buf) { return (Lds)&lds.tiles[wave][buf][0][0]; };
+    auto lds_values = [&](int buf) { return (Lds)&lds.tiles[wave][buf][1][0]; };
+    // What lies behind a key's last value is zeros, once for all.
+    if (a.D < DP) {
 #pragma unroll
       for (int i = 0; i < F::kLoads; ++i) {
         const int r = slot_row + i * F::kRows;
-        if (F::key_piece(slot, r) * 16 < row_bytes) *(LdsPiece)(keys + r * F::kPitch + slot * 16) = kreg[i];
-        *(LdsPiece)(values + r * F::kPitch + slot * 16) = vreg[i];
+        if (F::key_piece(slot, r) * 16 >= row_bytes) {
+#pragma unroll
+          for (int b = 0; b < F::kBuffers; ++b) *(LdsPiece)(lds_keys(b) + r * F::kPitch + slot * 16) = u32x4{0, 0, 0, 0};
+        }
       }
     }
-    if constexpr (FP8) scale_lds[wave][lane] = scale_of;
-    if (sub + kWaves < sub_end) {
-      fetch(sub + kWaves, entry, buf);
-      entry = ask(sub + 2 * kWaves);
-    }
-    if (look || there != ~0u) {
-      // Values as the product may have them.
-#pragma unroll
-      for (int i = 0; i < F::kLoads; ++i) {
-        const int r = slot_row + i * F::kRows;
-        const LdsPiece at = (LdsPiece)(values + r * F::kPitch + slot * 16);
-        u32x4 v = *at;
-        if (look && (FP8 ? drop_codes(v) : drop_others<W>(v)) && F::value_piece(slot, r) * 16 < row_bytes) bad = true;
-        *at = (there >> r) & 1 ? v : u32x4{0, 0, 0, 0};
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    f32x16 x;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
+
+    auto ask = [&](int sub) { return table[min(divided(walk.position(sub * kSub) + n, A.by_page), last_entry)]; };
+    auto partial = [&](int pos0) {
+      return pos0 + kSub - 1 > tile_lo || (a.window > 0 && pos0 <= low_of(tile_hi) && pos0 + kSub > a.keep_first);
+    };
+    u32x4 kreg[F::kLoads], vreg[F::kLoads];      // (those that do not go straight to LDS)
+    float scale_of = 0.0f;        // of position n's key, in the upper half its value
+    uint32_t loaded = 0;          // which positions of the loaded sub there are
+    auto fetch = [&](int sub, int entry, int buf) {
+      const int pos = walk.position(sub * kSub) + n, in_page = pos - divided(pos, A.by_page) * a.page_size;
+      const int id = pos < hi && (uint32_t)entry < (uint32_t)a.num_pages ? entry : -1;
+      loaded = (uint32_t)__ballot(id >= 0);
+      if (half == 0) row_lds[wave][n] = max(id, 0) * page_bytes + (uint32_t)in_page * (uint64_t)(uint32_t)slot_bytes;
       if constexpr (FP8) {
-        const u32x2 c = *(LdsCodes)(keys + key_row + F::key_piece(i, n) * 16 + half * 8);
-        x = M::mfma(fp8x8<M>(c[0], c[1]), q[i], x);
+        const int64_t s = a.scale_blocks == 0 ? t.head
+                                              : ((int64_t)max(id, 0) * a.Hkv + t.head) * a.scale_blocks + divided(in_page, A.by_block);
+        scale_of = id < 0 ? 0.0f : half == 0 ? a.k_scale[s] * a.scale : a.v_scale[s];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      int64_t at[F::kLoads];
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) at[i] = row_lds[wave][slot_row + i * F::kRows];
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) {
+        const int piece = F::key_piece(slot, slot_row + i * F::kRows) * 16;
+        if constexpr (!F::kDirect)
+          kreg[i] = *(const u32x4*)(kbase + at[i] + (piece < row_bytes ? piece : 0));
+        else if (piece < row_bytes)
+          dma16(kbase + at[i] + piece, lds_keys(buf) + i * F::kRows * F::kPitch);
+      }
+#pragma unroll
+      for (int i = 0; i < F::kLoads; ++i) {
+        const int piece = F::value_piece(slot, slot_row + i * F::kRows) * 16;
+        if constexpr (!F::kDirect)
+          vreg[i] = *(const u32x4*)(vbase + at[i] + (piece < row_bytes ? piece : 0));
+        else if (piece < row_bytes)
+          dma16(vbase + at[i] + piece, lds_values(buf) + i * F::kRows * F::kPitch);
+      }
+    };
+
+    const int quarter = (lane >> 4) & 1, l16 = lane & 15;
+    // (8-bit values are read 8 x 16 at a time, 16-bit ones 4 x 16)
+    const int value_row = FP8 ? half * 4 + (l16 >> 1) + (l16 >= 8 ? 4 : 0) : half * 4 + (l16 >> 2);
+    const int value_at = value_row * F::kPitch + (FP8 ? l16 & 1 : l16 & 3) * 8, key_row = n * F::kPitch;
+    int entry = 0;
+    if (sub_begin + wave < sub_end) {
+      fetch(sub_begin + wave, ask(sub_begin + wave), 0);
+      entry = ask(sub_begin + wave + kWaves);
+    }
+    int buf = 0;
+    for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
+      const int pos0 = walk.position(sub * kSub);
+      const uint32_t there = loaded;
+      const bool look = partial(pos0);
+      const Lds keys = lds_keys(buf), values = lds_values(buf);
+      buf ^= F::kBuffers - 1;
+      if constexpr (F::kDirect) {
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
       } else {
-        x = M::mfma(as_v8<M>(*(LdsPiece)(keys + key_row + F::key_piece(i * 2 + half, n) * 16)), q[i], x);
-      }
-    }
-
-    if constexpr (FP8) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) {
-        const f32x4 f = *(const f32x4*)&scale_lds[wave][j * 2 + half * 4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
-      }
-    }
-    if (a.softcap > 0.0f) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] = capped(x[j] * cap_in, cap_out);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] *= to_log2;
-    }
-    uint32_t sees = ~0u;
-    if (look || there != ~0u) {
-      sees = bits_below(place + 1 - pos0) & (~bits_below(low + 1 - pos0) | bits_below(a.keep_first - pos0)) & there;
-      sees >>= half * 4;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
-    }
-    float top = x[0];
-#pragma unroll
-    for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
-    top = over_halves_max(top);
-    follow<std::is_same_v<W, F16>, false>(top, m, l, acc, m);
-    const float ref = or_zero(m) - kLift;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      // (two 16-bit terms of each weight, 16 bits of it: the matrix cores have the time)
-      union { typename W::T e[8]; typename W::V8 v; } p, low;
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (FP8) f = *(const f32x4*)&scale_lds[wave][kSub + (j * 8 + i) * 2 + half * 4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at = j * 8 + i + e;
-          const float w = exp2_fast(x[at] - ref);
-          l += w;
-          // (a scale that is not seen may be anything)
-          const float scaled = !FP8 ? w : ((sees >> (at / 4 * 8 + at % 4)) & 1) ? w * f[e] : 0.0f;
-          p.e[i + e] = (typename W::T)scaled;
-          low.e[i + e] = (typename W::T)(scaled - (float)p.e[i + e]);
+        for (int i = 0; i < F::kLoads; ++i) {
+          const int r = slot_row + i * F::kRows;
+          if (F::key_piece(slot, r) * 16 < row_bytes) *(LdsPiece)(keys + r * F::kPitch + slot * 16) = kreg[i];
+          *(LdsPiece)(values + r * F::kPitch + slot * 16) = vreg[i];
         }
       }
+      if constexpr (FP8) scale_lds[wave][lane] = scale_of;
+      if (sub + kWaves < sub_end) {
+        fetch(sub + kWaves, entry, buf);
+        entry = ask(sub + 2 * kWaves);
+      }
+      if (look || there != ~0u) {
+        // Values as the product may have them.
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        typename W::V8 v;
+        for (int i = 0; i < F::kLoads; ++i) {
+          const int r = slot_row + i * F::kRows;
+          const LdsPiece at = (LdsPiece)(values + r * F::kPitch + slot * 16);
+          u32x4 v = *at;
+          if (look && (FP8 ? drop_codes(v) : drop_others<W>(v)) && F::value_piece(slot, r) * 16 < row_bytes) bad = true;
+          *at = (there >> r) & 1 ? v : u32x4{0, 0, 0, 0};
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      f32x16 x;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
         if constexpr (FP8) {
-          const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(
-              values + j * 16 * F::kPitch + value_at + F::value_piece(i * 2 + quarter, value_row) * 16));
-          v = fp8x8<W>((uint32_t)c[0], (uint32_t)c[1]);
+          const u32x2 c = *(LdsCodes)(keys + key_row + F::key_piece(i, n) * 16 + half * 8);
+          x = M::mfma(fp8x8<M>(c[0], c[1]), q[i], x);
         } else {
-          const Lds column = values + j * 16 * F::kPitch + value_at + F::value_pair(i * 2 + quarter, value_row) * 32;
-          union { i16x4 h[2]; typename W::V8 v; } both;
-          both.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
-          both.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * F::kPitch));
-          v = both.v;
+          x = M::mfma(as_v8<M>(*(LdsPiece)(keys + key_row + F::key_piece(i * 2 + half, n) * 16)), q[i], x);
         }
-        acc[i] = W::mfma(v, low.v, W::mfma(v, p.v, acc[i]));
       }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  }
 
-  // The four wavefronts' sums, relative to 2^ref each.
-  l = over_halves_sum(l);
-  const float ref = l == 0.0f ? kNegInf : or_zero(m) - kLift;
-  if (half == 0) ml_lds[wave][n] = f32x2{ref, l};
-  __syncthreads();
-  auto joined = [&](int r) {
-    float top = kNegInf, all = 0.0f;
+      if constexpr (FP8) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml_lds[w][r][0]);
-    const float at = or_zero(top);
+        for (int j = 0; j < 16; j += 4) {
+          const f32x4 f = *(const f32x4*)&scale_lds[wave][j * 2 + half * 4];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) all += ml_lds[w][r][1] * (ml_lds[w][r][1] == 0.0f ? 0.0f : exp2_fast(ml_lds[w][r][0] - at));
-    return f32x2{all == 0.0f ? kNegInf : at, all};
-  };
-  const float f = l == 0.0f ? 0.0f : exp2_fast(ref - or_zero(joined(n)[0]));
-  bad = __any(bad);
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (wave == w) {
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f32x4* const to = (f32x4*)&sums[n][i * 32 + j * 8 + half * 4];
-          f32x4 x = {acc[i][j * 4], acc[i][j * 4 + 1], acc[i][j * 4 + 2], acc[i][j * 4 + 3]};
-          x *= f;
-          *to = w == 0 ? x : *to + x;
+          for (int i = 0; i < 4; ++i) x[j + i] *= f[i];
         }
       }
-      if (bad) {
-        // What was left out, at the positions that a row sees (whatever its weight: an infinity stays one, or becomes NaN).
+      if (a.softcap > 0.0f) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = capped(x[j] * cap_in, cap_out);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] *= to_log2;
+      }
+      uint32_t sees = ~0u;
+      if (look || there != ~0u) {
+        sees = bits_below(place + 1 - pos0) & (~bits_below(low + 1 - pos0) | bits_below(a.keep_first - pos0)) & there;
+        sees >>= half * 4;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (!((sees >> (j / 4 * 8 + j % 4)) & 1)) x[j] = kNegInf;
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, x[j]);
+      top = over_halves_max(top);
+      follow<std::is_same_v<W, F16>, false>(top, m, l, acc, m);
+      const float ref = or_zero(m) - kLift;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // (two 16-bit terms of each weight, 16 bits of it: the matrix cores have the time)
+        union { typename W::T e[8]; typename W::V8 v; } p, low;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          f32x4 f = {1.0f, 1.0f, 1.0f, 1.0f};
+          if constexpr (FP8) f = *(const f32x4*)&scale_lds[wave][kSub + (j * 8 + i) * 2 + half * 4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int at = j * 8 + i + e;
+            const float w = exp2_fast(x[at] - ref);
+            l += w;
+            // (a scale that is not seen may be anything)
+            const float scaled = !FP8 ? w : ((sees >> (at / 4 * 8 + at % 4)) & 1) ? w * f[e] : 0.0f;
+            p.e[i + e] = (typename W::T)scaled;
+            low.e[i + e] = (typename W::T)(scaled - (float)p.e[i + e]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          typename W::V8 v;
+          if constexpr (FP8) {
+            const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(
+                values + j * 16 * F::kPitch + value_at + F::value_piece(i * 2 + quarter, value_row) * 16));
+            v = fp8x8<W>((uint32_t)c[0], (uint32_t)c[1]);
+          } else {
+            const Lds column = values + j * 16 * F::kPitch + value_at + F::value_pair(i * 2 + quarter, value_row) * 32;
+            union { i16x4 h[2]; typename W::V8 v; } both;
+            both.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)column);
+            both.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)(column + 8 * F::kPitch));
+            v = both.v;
+          }
+          acc[i] = W::mfma(v, low.v, W::mfma(v, p.v, acc[i]));
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+
+    // The four wavefronts' sums, relative to 2^ref each.
+    l = over_halves_sum(l);
+    const float ref = l == 0.0f ? kNegInf : or_zero(m) - kLift;
+    if (half == 0) ml_lds[wave][n] = f32x2{ref, l};
+    __syncthreads();
+    auto joined = [&](int r) {
+      float top = kNegInf, all = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) top = fmaxf(top, ml_lds[w][r][0]);
+      const float at = or_zero(top);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) all += ml_lds[w][r][1] * (ml_lds[w][r][1] == 0.0f ? 0.0f : exp2_fast(ml_lds[w][r][0] - at));
+      return f32x2{all == 0.0f ? kNegInf : at, all};
+    };
+    const float f = l == 0.0f ? 0.0f : exp2_fast(ref - or_zero(joined(n)[0]));
+    bad = __any(bad);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (wave == w) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4* const to = (f32x4*)&sums[n][i * 32 + j * 8 + half * 4];
+            f32x4 x = {acc[i][j * 4], acc[i][j * 4 + 1], acc[i][j * 4 + 2], acc[i][j * 4 + 3]};
+            x *= f;
+            *to = w == 0 ? x : *to + x;
+          }
+        }
+        if (bad) {
+          // What was left out, at the positions that a row sees (whatever its weight: an infinity stays one, or becomes NaN).
 #pragma unroll 1
-        for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
-          const int pos0 = walk.position(sub * kSub);
-          if (!partial(pos0)) continue;
+          for (int sub = sub_begin + wave; sub < sub_end; sub += kWaves) {
+            const int pos0 = walk.position(sub * kSub);
+            if (!partial(pos0)) continue;
 #pragma unroll 1
-          for (int pos = pos0; pos < min(pos0 + kSub, hi); ++pos) {
-            const int in_table = divided(pos, A.by_page), id = table[in_table];
-            if (!(pos <= place && (pos > low || pos < a.keep_first)) || (uint32_t)id >= (uint32_t)a.num_pages) continue;
-            const char* const from = vbase + (int64_t)id * page_bytes + (int64_t)(pos - in_table * a.page_size) * slot_bytes;
+            for (int pos = pos0; pos < min(pos0 + kSub, hi); ++pos) {
+              const int in_table = divided(pos, A.by_page), id = table[in_table];
+              if (!(pos <= place && (pos > low || pos < a.keep_first)) || (uint32_t)id >= (uint32_t)a.num_pages) continue;
+              const char* const from = vbase + (int64_t)id * page_bytes + (int64_t)(pos - in_table * a.page_size) * slot_bytes;
 #pragma unroll 1
-            for (int d = half * 4; d < a.D; d += d % 4 == 3 ? 5 : 1) {
-              union { uint16_t u; typename W::T t; } v;
-              if constexpr (FP8)
-                v.t = fp8x8<W>(((const uint8_t*)from)[d], 0)[0];
-              else
-                v.u = ((const uint16_t*)from)[d];
-              if (!finite<W>(v.u)) sums[n][d] += (float)v.t;
+              for (int d = half * 4; d < a.D; d += d % 4 == 3 ? 5 : 1) {
+                union { uint16_t u; typename W::T t; } v;
+                if constexpr (FP8)
+                  v.t = fp8x8<W>(((const uint8_t*)from)[d], 0)[0];
+                else
+                  v.u = ((const uint16_t*)from)[d];
+                if (!finite<W>(v.u)) sums[n][d] += (float)v.t;
+              }
             }
           }
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-  const int quads = a.D / 4;
-  const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
-  for (int i = tid; i < kPromptFewRows * quads; i += 256) {
-    const int r = i / quads, d = (i - r * quads) * 4, my_row = t.first + r;
-    if (my_row >= t.rows) break;
-    const f32x2 st = joined(r);
-    const f32x4 x = *(const f32x4*)&sums[r][d];
-    if (A.p.splits > 1) {
-      if (d == 0) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + r] = st;
-      *(f32x4*)((float*)((char*)a.workspace + A.p.part_at) + (part * kPromptFewRows + r) * DP + d) = x;
-    } else {
-      const int my_tok = divided(my_row, A.by_group), hq = t.head * a.G + (my_row - my_tok * a.G);
-      const int64_t out_row = (int64_t)(t.s0 + my_tok) * a.Hkv * a.G + hq;
-      const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
-      const float top = or_zero(fmaxf(st[0], sink)), fix = st[1] == 0.0f ? 0.0f : exp2_fast(st[0] - top);
-      const float total = st[1] * fix + exp2_fast(sink - top), inv = total == 0.0f ? 0.0f : fix / total;
-      union { typename M::T e[4]; u32x2 u; } o;
+    const int quads = a.D / 4;
+    const int64_t part = ((int64_t)t.slot * a.Hkv + t.head) * A.p.splits + t.split;
+    for (int i = tid; i < kPromptFewRows * quads; i += 256) {
+      const int r = i / quads, d = (i - r * quads) * 4, my_row = t.first + r;
+      if (my_row >= t.rows) break;
+      const f32x2 st = joined(r);
+      const f32x4 x = *(const f32x4*)&sums[r][d];
+      if (A.p.splits > 1) {
+        if (d == 0) ((f32x2*)((char*)a.workspace + A.p.ml_at))[part * kPromptFewRows + r] = st;
+        *(f32x4*)((float*)((char*)a.workspace + A.p.part_at) + (part * kPromptFewRows + r) * DP + d) = x;
+      } else {
+        const int my_tok = divided(my_row, A.by_group), hq = t.head * a.G + (my_row - my_tok * a.G);
+        const int64_t out_row = (int64_t)(t.s0 + my_tok) * a.Hkv * a.G + hq;
+        const float sink = a.sinks != nullptr ? a.sinks[hq] * kLog2e : kNegInf;
+        const float top = or_zero(fmaxf(st[0], sink)), fix = st[1] == 0.0f ? 0.0f : exp2_fast(st[0] - top);
+        const float total = st[1] * fix + exp2_fast(sink - top), inv = total == 0.0f ? 0.0f : fix / total;
+        union { typename M::T e[4]; u32x2 u; } o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o.e[e] = (typename M::T)(x[e] * inv);
-      *(u32x2*)((char*)a.out + (out_row * a.D + d) * 2) = o.u;
-      if (d == 0 && a.lse != nullptr) a.lse[out_row] = log_of_sum(top, total, a.sinks != nullptr ? a.sinks + hq : nullptr);
+        for (int e = 0; e < 4; ++e) o.e[e] = (typename M::T)(x[e] * inv);
+        *(u32x2*)((char*)a.out + (out_row * a.D + d) * 2) = o.u;
+        if (d == 0 && a.lse != nullptr) a.lse[out_row] = log_of_sum(top, total, a.sinks != nullptr ? a.sinks + hq : nullptr);
+      }
     }
-  }
+    // (the sums have been read when the next rows' keys come)
+    if constexpr (AGAIN) __syncthreads();
+    t.first += kPromptFewRows;
+  } while (AGAIN && t.first < last_row);
 }
 
 // Joins the parts of tiles whose positions several workgroups shared: a lane holds 4 values of a row.  Where there are many
@@ -1150,7 +1196,7 @@ void launch_width(const KernelArgs& A, hipStream_t stream) {
   bool few = false;
   if constexpr (FP8 || DP <= kPromptFewWidth) {
     few = rows == kPromptFewRows;
-    if (few) hipLaunchKernelGGL((prompt_attention_few_kernel<M, FP8, DP>), grid, block, 0, stream, A);
+    if (few) hipLaunchKernelGGL((prompt_attention_few_kernel<M, FP8, DP, false>), grid, block, 0, stream, A);
   }
   if (!few) hipLaunchKernelGGL((prompt_attention_kernel<M, FP8, DP>), grid, block, 0, stream, A);
   if (A.p.splits > 1) {
@@ -1158,6 +1204,15 @@ void launch_width(const KernelArgs& A, hipStream_t stream) {
     const int groups = A.p.splits >= 16 ? 256 / lanes : 1, per_tile = groups > 1 ? rows : rows / (256 / lanes);
     hipLaunchKernelGGL((prompt_attention_join_kernel<M>), dim3((unsigned)((int64_t)A.p.slots * A.a.Hkv * per_tile)), block, 0,
                        stream, A, DP, groups, per_tile);
+  }
+  if constexpr (FP8) {
+    if (few) return;
+    KernelArgs again = A;      // (a workgroup for every tile, with all of its positions)
+    again.p.splits = 1;
+    again.p.share = (A.a.max_len + kPromptKeys - 1) / kPromptKeys + 1;
+    again.by_splits = fast_div(1);
+    const dim3 tiles((unsigned)((int64_t)A.p.slots * A.a.Hkv));
+    hipLaunchKernelGGL((prompt_attention_few_kernel<M, FP8, DP, true>), tiles, block, 0, stream, again);
   }
 }
 
