@@ -779,14 +779,15 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
 
 /* Attention of several new tokens of every sequence over its cache, which holds them already: q, out
  * [tokens, Hq, D], lse [tokens, Hq], the tokens of sequence b rows query_start[b] .. query_start[b + 1] - 1
- * (query_start [B + 1] int32, from 0 on and not falling) and its last positions: with n of them and L as
+ * (query_start [B + 1] int32, not falling) and its last positions: with n of them and L as
  * above, token i is at p = L - n + i and sees positions j <= p, with a window those with j > p - window or
  * j < keep_first.  Scores, cap, sinks, scales, results and rows that see nothing as above; what is stored at a position
  * that a token does not see has no part in its row, NaN and infinities included.  Weights enter the product with
  * the values in the queries' type, of an 8-bit cache (times the values' scales) in fp16, rounded once, or where rows are
  * few as two 16-bit terms; in fp16 2^-18 of the largest weight (times the largest scale) among its 32 positions
  * may be lost.  Rows that see a value scale outside of 2^-60 .. 2^60 (0 is none) have two bf16 terms a weight as well.  Rows
- * that belong to no sequence become 0 (lse -inf) with clear_rest != 0 and else stay as they are.
+ * that belong to no sequence, in front of query_start[0] or behind query_start[B], become 0 (lse -inf) with
+ * clear_rest != 0 and else stay as they are.
  * The workspace is scratch of this call alone; 0 bytes: none is needed.  Deterministic: no atomics on floating-point
  * data. */
 size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,

@@ -36,11 +36,12 @@ struct KernelArgs {
 
 // What a workgroup works on.
 struct Tile {
-  int b;             // the sequence; B: rows behind the last one
+  int b;             // the sequence; B: behind the last one
   int slot, head, split;
   int s0, tokens;    // the sequence's first row of q, and how many it has
-  int first, rows;   // its first row of the tile, and rows of the sequence
+  int first, rows;   // its first row of the tile (negative: in front of the first sequence), and rows of the sequence
 };
+// False: the workgroup has no sequence's rows.
 __device__ __forceinline__ bool find_tile(const KernelArgs& A, int block, Tile* t) {
   const PromptAttentionArgs& a = A.a;
   // Key/value heads in neighbouring workgroups, which different XCDs take: with 8 heads each XCD's cache has one
@@ -59,21 +60,28 @@ __device__ __forceinline__ bool find_tile(const KernelArgs& A, int block, Tile* 
   t->tokens = (t->b < a.B ? max(start(t->b + 1), t->s0) : a.tokens) - t->s0;
   t->first = k << A.p.row_shift;
   t->rows = t->tokens * a.G;
-  return k >= 0 && t->first < t->rows;
+  return k >= 0 && t->first < t->rows && t->b < a.B;
 }
 
-// Rows that belong to no sequence.
+// Rows that belong to no sequence: those in front of the first one in the slots that lie there, what is left of them and
+// those behind the last one in the slots behind it (there is one always).
 __device__ __forceinline__ void clear_rows(const KernelArgs& A, const Tile& t) {
   const PromptAttentionArgs& a = A.a;
   if (!a.clear_rest || t.split > 0) return;
   const int pieces = a.D / 8;
-  for (int i = threadIdx.x; i < pieces << A.p.row_shift; i += 256) {
-    const int r = t.first + i / pieces, tok = divided(r, A.by_group);
-    if (r >= t.rows) break;
-    const int64_t row = ((int64_t)(t.s0 + tok) * a.Hkv + t.head) * a.G + (r - tok * a.G);
-    *(u32x4*)((char*)a.out + (row * a.D + i % pieces * 8) * 2) = u32x4{0, 0, 0, 0};
-    if (i % pieces == 0 && a.lse != nullptr) a.lse[row] = kNegInf;
-  }
+  auto clear = [&](int begin, int end) {
+    for (int i = threadIdx.x; i < (end - begin) * pieces; i += 256) {
+      const int r = begin + i / pieces, tok = divided(r, A.by_group);
+      const int64_t row = ((int64_t)tok * a.Hkv + t.head) * a.G + (r - tok * a.G);
+      *(u32x4*)((char*)a.out + (row * a.D + i % pieces * 8) * 2) = u32x4{0, 0, 0, 0};
+      if (i % pieces == 0 && a.lse != nullptr) a.lse[row] = kNegInf;
+    }
+  };
+  if (t.first < 0) clear(t.slot << A.p.row_shift, (t.slot + 1) << A.p.row_shift);
+  if (t.b < a.B) return;
+  const int front = min(max(a.starts[0], 0), a.tokens) * a.G, begin = t.s0 * a.G + t.first, end = a.tokens * a.G;
+  if (t.first == 0) clear(front & -(1 << A.p.row_shift), front);
+  clear(begin, min(begin + (1 << A.p.row_shift), end));
 }
 
 // The positions a tile sees, as a line of places: the first `split` of them the positions at the beginning, the
@@ -229,9 +237,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Tile t;
-  if (!find_tile(A, blockIdx.x, &t)) return;
   const int Hq = a.Hkv * a.G;
-  if (t.b == a.B) {
+  if (!find_tile(A, blockIdx.x, &t)) {
     clear_rows(A, t);
     return;
   }
@@ -806,8 +813,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_few_k
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Tile t;
-  if (!find_tile(A, blockIdx.x, &t)) return;
-  if (t.b == a.B) {
+  if (!find_tile(A, blockIdx.x, &t)) {
     if constexpr (!AGAIN) clear_rows(A, t);
     return;
   }
@@ -1135,7 +1141,7 @@ __global__ __launch_bounds__(256) void prompt_attention_join_kernel(const Kernel
   KernelArgs one = A;
   one.p.splits = 1;
   one.by_splits = FastDiv{0, -1};
-  if (!find_tile(one, rest, &t) || t.b == a.B) return;
+  if (!find_tile(one, rest, &t)) return;
   const int lanes = padded <= 64 ? 16 : padded <= 128 ? 32 : 64;      // of a row
   const int rows = 1 << A.p.row_shift, group = threadIdx.x / lanes, in_row = threadIdx.x % lanes, d = in_row * 4;
   const int at = groups > 1 ? piece : piece * (256 / lanes) + group, row = t.first + at;

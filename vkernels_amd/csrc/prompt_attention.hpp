@@ -38,7 +38,7 @@ struct PromptAttentionArgs {
 
 struct PromptAttentionPlan {
   int row_shift;            // a tile has 2^row_shift rows
-  int slots;                // places for the tiles of all sequences, and of the rows behind them
+  int slots;                // places for the tiles of all sequences, and of the rows in front of and behind them
   int splits;               // workgroups that share a tile's positions; more than 1: joined by a second launch
   int share;                // kPromptKeys positions that each of them takes at most
   size_t ml_at, part_at, bytes;   // parts of the workspace
