@@ -48,9 +48,10 @@ __device__ __forceinline__ uint32_t larger_half(uint32_t size) { return max(size
 __device__ __forceinline__ uint32_t infinity_of(bool bf16) { return bf16 ? 0x7F80u : 0x7C00u; }
 
 // Division by a block's scale.  With r the reciprocal, correctly rounded, and q = x r rounded, q + (x - q s) r is the
-// quotient, correctly rounded, unless the scale's significand is all ones (Markstein 1990) or the remainder leaves the
-// range of 32-bit floats: such scales are divided by.  (A code's rounding looks at quotients from 2^-11 on, so that
-// scales from 2^-80 to 2^80 keep all of it in range.)
+// quotient of an x that is not 0, correctly rounded, unless the scale's significand is all ones (Markstein 1990) or the
+// remainder leaves the range of 32-bit floats: such scales are divided by.  (A code's rounding looks at quotients from
+// 2^-11 on, so that scales from 2^-80 to 2^80 keep all of it in range.)
+constexpr int kZeroOrNoNumber = 0x267;      // of v_cmp_class: zeros, infinities and NaN of either sign
 struct Scale {
   float s, r;
   bool simple;
@@ -75,7 +76,7 @@ __device__ __forceinline__ u32x2 codes_by(u32x4 x, const Scale& by, bool bf16) {
     for (int j = 0; j < 4; ++j) {
       const uint32_t w = x[2 * i + j / 2];
       const float v = f16_bits_to_f32(j & 1 ? w >> 16 : w & 0xFFFFu, bf16), q = by.divided(v);
-      f[j] = fabsf(v) < __builtin_inff() ? q : v;      // (an infinity and NaN as they are)
+      f[j] = __builtin_amdgcn_classf(v, kZeroOrNoNumber) ? v : q;      // (as they are: of -0 the remainder loses the sign)
     }
     codes[i] = e4m3x4(f);
   }
