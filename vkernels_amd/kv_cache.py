@@ -13,7 +13,8 @@ writes besides its arguments comes from torch's allocator, so calls on several s
 scratch and a call can be captured in a graph.
 
 These are operators of inference: no gradient passes through the cache, and a backward pass that comes to
-their results raises an error.
+their results raises an error.  Results that the caller gives (``out``) cannot raise one later: the call is refused
+where one of its tensors wants a gradient, and so is every call whose tensors have forward-mode tangents.
 
 The entry points are additive: the reference keeps its cache outside this path.  Everything runs in
 ``libvkernels_hip.so``; there is no fallback.
@@ -24,6 +25,8 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .vllm_experts import last_error, load_libvkernels_hip
 
@@ -198,6 +201,22 @@ def _no_backward(name):
     return NoBackward.apply
 
 
+def _dual_level():
+    """0 or more where tensors may have tangents."""
+    return getattr(forward_ad, "_current_level", 0)
+
+
+def _refuse_derivatives(name, out, *inputs):
+    """Raises where a derivative would be lost: of what goes to results that the caller has given (`out`, or ()), whose
+    node is not this call's, and in forward mode."""
+    inputs = [t for t in inputs if t is not None]
+    if out and torch.is_grad_enabled() and any(t.requires_grad for t in (*out, *inputs)):
+        raise RuntimeError(f"{name} has no backward pass, and out= cannot say so later: call it under torch.no_grad(), or "
+                           "detach what requires a gradient")
+    if _dual_level() >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (*out, *inputs)):
+        raise RuntimeError(f"{name} has no derivative: it is an operator of inference")
+
+
 _attention_result, _read_result = _no_backward("paged_attention"), _no_backward("kv_cache_read")
 
 
@@ -272,6 +291,12 @@ def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, 
             _need(t.shape == (tokens, Hkv, D) and t.dtype is dtype and t.get_device() == device and s[2] == 1 and
                   s[0] % 8 == 0 and s[1] % 8 == 0 and t.data_ptr() % 16 == 0,
                   "out must be two [tokens, Hkv, D] on the cache's device with rows that start on 16 bytes")
+    inputs = k_cache, v_cache, k_scale, v_scale
+    wants_grad = torch.is_grad_enabled() and (
+        k_cache.requires_grad or v_cache.requires_grad or k_scale is not None and k_scale.requires_grad or
+        v_scale is not None and v_scale.requires_grad)
+    if out is not None or _dual_level() >= 0:
+        _refuse_derivatives("kv_cache_read", () if out is None else (k, v), *inputs)
     ks, vs = k.stride(), v.stride()
     k_scale, v_scale, blocks = _scales(k_scale, v_scale, pages, Hkv, ps, device)
     status = _fn("vk_hip_kv_cache_read")(
@@ -280,8 +305,10 @@ def kv_cache_read(k_cache, v_cache, block_table, seq_lens, *, query_start=None, 
         ks[0], ks[1], vs[0], vs[1], strides[0], strides[1], strides[2], _stream(device))
     if status:
         _failed(status, "vk_hip_kv_cache_read")
-    if (k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled() and out is None:
-        k, v = _read_result(k, v, k_cache, v_cache)
+    if out is not None:
+        increment_version((k, v))
+    elif wants_grad:
+        k, v = _read_result(k, v, *inputs)
     return k, v
 
 
@@ -324,7 +351,13 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
         keep_first = min(keep_first, max_len) if window else 0
     if not 0 <= max_len <= 0x7FFFFFFF:
         _int32(max_len=max_len)
-    q, own_out = _rows(q), out is not None
+    inputs, own_out = (q, k_cache, v_cache, sinks, k_scale, v_scale), out is not None
+    wants_grad = torch.is_grad_enabled() and (
+        q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or sinks is not None and sinks.requires_grad or
+        k_scale is not None and k_scale.requires_grad or v_scale is not None and v_scale.requires_grad)
+    if own_out or _dual_level() >= 0:
+        _refuse_derivatives("paged_attention", (out,) if own_out else (), *inputs)
+    q = _rows(q)
     if out is None:
         out = q.new_empty((rows, Hq, D))
     else:
@@ -365,9 +398,10 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
             _stream(device))
     if status:
         _failed(status, name)
-    if ((q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or
-         sinks is not None and sinks.requires_grad) and torch.is_grad_enabled() and not own_out):
-        out, lse = _attention_result(out, lse, q, k_cache, v_cache, sinks)
+    if own_out:
+        increment_version(out)
+    elif wants_grad:
+        out, lse = _attention_result(out, lse, *inputs)
     return (out, lse) if return_lse else out
 
 

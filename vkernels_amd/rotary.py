@@ -2,7 +2,8 @@
 token's position, in one pass over them.
 
 The call is enqueued on the current stream of the tensors' device, without host synchronisation, and can be
-captured in a graph.  It is an operator of inference: a backward pass that comes to it raises an error.
+captured in a graph.  It is an operator of inference: a backward pass that comes to it raises an error, and with
+results that the caller gives the call is refused where one of its tensors wants a gradient.
 
 The entry point is additive: the reference leaves queries and keys to its caller.  Everything runs in
 ``libvkernels_hip.so``; there is no fallback.
@@ -12,8 +13,9 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.graph import increment_version
 
-from .kv_cache import _current_device, _failed, _need, _no_backward, _rows, _stream
+from .kv_cache import _current_device, _dual_level, _failed, _need, _no_backward, _refuse_derivatives, _rows, _stream
 from .vllm_experts import load_libvkernels_hip
 
 __all__ = ["qk_norm_rope"]
@@ -104,15 +106,18 @@ def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps
         of = torch.float32 if weights_f32 else q.dtype
         q_weight = None if q_weight is None else _weight_at(q_weight, D, of, device, "q_weight")
         k_weight = None if k_weight is None else _weight_at(k_weight, D, of, device, "k_weight")
-    wants_grad = (q.requires_grad or k.requires_grad or inv_freq.requires_grad or q_weight is not None and q_weight.requires_grad or
-                  k_weight is not None and k_weight.requires_grad) and torch.is_grad_enabled()
+    inputs = q, k, inv_freq, q_weight, k_weight
+    wants_grad = torch.is_grad_enabled() and (
+        q.requires_grad or k.requires_grad or inv_freq.requires_grad or q_weight is not None and q_weight.requires_grad or
+        k_weight is not None and k_weight.requires_grad)
     if out is None:
         q_out, k_out = q.new_empty((T, Hq, D)), k.new_empty((T, Hkv, D))
     else:
         q_out, k_out = out
         _check_out(q_out, q, "q")
         _check_out(k_out, k, "k")
-    inputs = q, k
+    if out is not None or _dual_level() >= 0:
+        _refuse_derivatives("qk_norm_rope", () if out is None else (q_out, k_out), *inputs)
     q, k = _rows(q), _rows(k)
     qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
     status = _fn()(
@@ -123,6 +128,8 @@ def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps
         ko[0], ko[1], axis_stride, _stream(device))
     if status:
         _failed(status, "vk_hip_qk_norm_rope")
-    if wants_grad and out is None:
-        q_out, k_out = _result(q_out, k_out, *inputs, inv_freq, q_weight, k_weight)
+    if out is not None:
+        increment_version((q_out, k_out))
+    elif wants_grad:
+        q_out, k_out = _result(q_out, k_out, *inputs)
     return q_out, k_out
