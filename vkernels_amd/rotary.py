@@ -62,7 +62,7 @@ def _explain(q, k, positions, inv_freq):
           "the tensors must be on the current device")
     _need(inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
           inv_freq.shape[0] <= q.shape[2] // 2, "inv_freq must be up to D / 2 contiguous float32 values")
-    _need(positions.dtype is torch.int32 and (positions.numel() <= 1 or positions.stride(-1) == 1),
+    _need(positions.dtype is torch.int32 and (positions.stride()[-1:] == (1,) or q.shape[0] <= 1),
           "positions must be int32 with contiguous rows")
     _need(False, "q and k must have heads, and sizes below 2^31")
 
@@ -85,7 +85,7 @@ def qk_norm_rope(q, k, positions, inv_freq, *, q_weight=None, k_weight=None, eps
             positions.get_device() == device and inv_freq.get_device() == device and
             inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and
             inv_freq.shape[0] <= shape[2] // 2 and positions.dtype is torch.int32 and
-            (positions.numel() <= 1 or positions.stride(-1) == 1) and
+            (positions.stride()[-1:] == (1,) or shape[0] <= 1) and
             shape[1] > 0 and k_shape[1] > 0 and (shape[0] | shape[1] | k_shape[1]) <= 0x7FFFFFFF):
         _explain(q, k, positions, inv_freq)
     (T, Hq, D), Hkv, R = shape, k_shape[1], inv_freq.shape[0]
