@@ -93,7 +93,7 @@ def _need(ok, message):
 def _cache_ok(k_cache, v_cache, block_table, seq_lens, shape, strides, device, table, table_strides):
     return (v_cache.shape == shape and v_cache.stride() == strides and strides[3] == 1 and
             v_cache.dtype is k_cache.dtype and block_table.dtype is _INT32 and seq_lens.dtype is _INT32 and
-            table_strides[1] == 1 and seq_lens.shape == table[:1] and seq_lens.is_contiguous() and
+            (table_strides[1] == 1 or table[1] <= 1) and seq_lens.shape == table[:1] and seq_lens.is_contiguous() and
             v_cache.get_device() == device and block_table.get_device() == device and
             seq_lens.get_device() == device and device >= 0 and _current_device() == device and
             (shape[0] | shape[1] | shape[2] | table[0] | table[1] | table_strides[0]) <= 0x7FFFFFFF)
@@ -104,7 +104,8 @@ def _explain_cache(k_cache, v_cache, block_table, seq_lens):
           "k_cache and v_cache must be [pages, Hkv, page_size, D] alike")
     _need(k_cache.dtype == v_cache.dtype and k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1,
           "k_cache and v_cache must have one type and the same strides, rows of D values contiguous")
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.stride(1) == 1,
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and
+          (block_table.stride(1) == 1 or block_table.shape[1] <= 1),
           "block_table must be int32 [B, W] with contiguous rows")
     _need(seq_lens.dtype == torch.int32 and seq_lens.shape == block_table.shape[:1] and seq_lens.is_contiguous(),
           "seq_lens must be int32 [B], contiguous")
