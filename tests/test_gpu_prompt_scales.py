@@ -108,3 +108,43 @@ def test_infinite_scales_that_are_not_seen(hip_lib):
         s.v_scale[s.table[0, 0].long()] = value          # positions 0 .. 15
         out, lse = s.call(window=16)
         assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+
+
+@pytest.mark.parametrize("ps,block", [(24, 8), (16, 1), (16, 16), (5, 5)])
+@pytest.mark.parametrize("far", [0, 5, 400, 717, 899])
+@pytest.mark.parametrize("window,first", [(0, 0), (64, 6), (200, 0), (64, 500)])
+def test_one_block_far_from_the_others(hip_lib, ps, block, far, window, first):
+    """Wherever it lies: rows that see it are what the definition says, the others as if it were not there."""
+    s = Prompt([900, 130], [300, 70], 2, 4, 64, ps, block, seed=far + ps)
+    clean = s.call(window=window, keep_first=first)[0].double().cpu()
+    page = int(s.table[0, far // ps])
+    s.v_scale[page, :, far % ps // block] *= 2.0 ** 70
+    check(s, window=window, keep_first=first)
+    out = s.call(window=window, keep_first=first)[0].double().cpu()
+    begin, end = far // block * block, far // block * block + block
+    seen = torch.tensor([any(p <= place and (not window or p > place - window or p < first) for p in range(begin, min(end, 900)))
+                         for place in range(600, 900)] + [False] * 70)
+    # Both calls are within their weights' 2^-11 and their scores' rounding (64 2^-23 of products that sum up to some 10,
+    # twice: below 2^-11) of the largest value, and half a step of the result.
+    most = float((s.v.float().cpu().nan_to_num() * 0.3).abs().max())      # (scales are e^(0.7 x) / 60, codes up to some 240)
+    bound = 4 * 2.0 ** -11 * most + 2 * 2.0 ** -8 * clean.abs()
+    assert bool(((out - clean).abs() <= bound)[~seen].all())
+    assert not bool(seen.any()) or float(out[seen].abs().max()) > 2.0 ** 40
+
+
+def test_in_a_graph(hip_lib):
+    """Scales that come and go between replays of one captured call."""
+    s = Prompt([700, 600], (200, 150), 2, 4, 128, 16, 16)
+    ordinary = s.v_scale.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, lse = s.call(max_len=int(s.table.shape[1]) * 16)
+    for size in (1.0, 2.0 ** 80, 1.0, 2.0 ** -80, 0.5):
+        s.v_scale.copy_(ordinary * size)
+        out.fill_(math.nan)
+        graph.replay()
+        want = s.call(max_len=int(s.table.shape[1]) * 16)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        check(s)
