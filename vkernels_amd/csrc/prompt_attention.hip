@@ -619,21 +619,18 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
       }
     };
     for (int tile = tile_begin; tile < tile_end;) {
-      // (heads of more than 128 do not have the registers)
-      if constexpr (true) {
-        if (plain) {
-          float top = largest(2 * tile, even, to_log2);
-          for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
-            ahead(tile);
-            attend_whole(2 * tile, even, odd, top);
-            attend_whole(2 * tile + 1, odd, even, top);
-            if constexpr (FP8) {
-              put_keys(tile + 1);
-              put_values(tile + 1, there << 32 | first);
-            }
-            landed();
-            these = there << 32 | first;
+      if (plain) {
+        float top = largest(2 * tile, even, to_log2);
+        for (; tile + 1 < tile_end && these == ~0ull && !partial(walk.position(tile * kPromptKeys)) && !hidden(2 * tile + 2); ++tile) {
+          ahead(tile);
+          attend_whole(2 * tile, even, odd, top);
+          attend_whole(2 * tile + 1, odd, even, top);
+          if constexpr (FP8) {
+            put_keys(tile + 1);
+            put_values(tile + 1, there << 32 | first);
           }
+          landed();
+          these = there << 32 | first;
         }
       }
       ahead(tile);
