@@ -1,5 +1,5 @@
-"""GPU tests of results that the caller gives (out=) where gradients are wanted: refused, as no node can stand for the
-operator; and of what autograd sees of the tensors that are written."""
+"""GPU tests of results that the caller gives (out=) where gradients are wanted: refused, or an error in the backward pass
+that comes to them; and of what autograd sees of the tensors that are written."""
 from __future__ import annotations
 
 import pytest
@@ -66,28 +66,41 @@ def test_a_tensor_that_a_node_has_saved(hip_lib):
         rotate(q, k, out=(q, k))
 
 
-def test_reading_and_attention(hip_lib):
+def test_reading(hip_lib):
     s = Setup([40, 30], 2, 2, 64, 16, 0)
     wide = s.k.clone().requires_grad_()
-    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev())
-
-    def out():
-        return [torch.full((2, 2, 64), 3.0, dtype=BF16, device=dev()) for _ in range(2)]
-
-    room = out()
+    room = [torch.full((2, 2, 64), 3.0, dtype=BF16, device=dev()) for _ in range(2)]
     with pytest.raises(RuntimeError, match="kv_cache_read has no backward"):
         kv.kv_cache_read(wide, s.v, s.table, s.lens, out=room)
     with pytest.raises(RuntimeError, match="kv_cache_read has no backward"):
         kv.kv_cache_read(s.k, s.v, s.table, s.lens, out=[room[0], room[1].clone().requires_grad_()])
     assert bool((room[0] == 3).all() and (room[1] == 3).all())
-    q = s.q.clone().requires_grad_()
-    sinks = s.sinks.clone().requires_grad_()
+
+
+def test_attention(hip_lib):
+    s = Setup([40, 30], 2, 2, 64, 16, 0)
+    wide, q, sinks = (t.clone().requires_grad_() for t in (s.k, s.q, s.sinks))
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev())
     for more in (dict(), dict(query_start=starts), dict(return_lse=True)):
-        room = torch.full_like(s.q, 3.0)
+        leaf = rows(*s.q.shape, requires_grad=True)
         for args, kw in (((q, s.k, s.v), {}), ((s.q, wide, s.v), {}), ((s.q, s.k, wide), {}), ((s.q, s.k, s.v), dict(sinks=sinks)),
-                         ((s.q, s.k, s.v), dict(out=room.clone().requires_grad_()))):
-            with pytest.raises(RuntimeError, match="paged_attention has no backward"):
-                kv.paged_attention(*args, s.table, s.lens, **dict(more, out=room, **kw) if "out" not in kw else dict(more, **kw))
+                         ((s.q, s.k, s.v), dict(out=leaf * 2)), ((q, s.k, s.v), dict(out=rows(5, 4, 64)[2:4]))):
+            kw.setdefault("out", torch.full_like(s.q, 3.0))
+            with torch.no_grad():
+                want = kv.paged_attention(*args, s.table, s.lens, **dict(more, return_lse=True, **dict(kw, out=None)))
+            got = kv.paged_attention(*args, s.table, s.lens, **more, **kw)
+            got, lse = got if more.get("return_lse") else (got, None)
+            assert got is kw["out"] and got.requires_grad and torch.equal(got, want[0]) and (lse is None or torch.equal(lse, want[1]))
+            # (what is behind `out` is no input of the lse)
+            inputs_want = any(t.requires_grad for t in args) or "sinks" in kw
+            assert lse is None or lse.requires_grad == inputs_want
+            for result in (kw["out"], lse):
+                if result is not None and result.requires_grad:
+                    with pytest.raises(RuntimeError, match="paged_attention has no backward"):
+                        result.float().sum().backward()
+        room = torch.full_like(s.q, 3.0).requires_grad_()
+        with pytest.raises(RuntimeError, match="leaf"):
+            kv.paged_attention(s.q, s.k, s.v, s.table, s.lens, out=room, **more)
         assert bool((room == 3).all())
         with torch.no_grad():
             kv.paged_attention(q, s.k, s.v, s.table, s.lens, out=room, **more)

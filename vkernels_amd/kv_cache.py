@@ -13,8 +13,9 @@ writes besides its arguments comes from torch's allocator, so calls on several s
 scratch and a call can be captured in a graph.
 
 These are operators of inference: no gradient passes through the cache, and a backward pass that comes to
-their results raises an error.  Results that the caller gives (``out``) cannot raise one later: the call is refused
-where one of its tensors wants a gradient, and so is every call whose tensors have forward-mode tangents.
+their results raises an error, also where the caller gives them (``paged_attention``; ``kv_cache_read``, whose two may
+be parts of one tensor, refuses ``out`` where one of its tensors wants a gradient).  Tensors with forward-mode
+tangents are refused.
 
 The entry points are additive: the reference keeps its cache outside this path.  Everything runs in
 ``libvkernels_hip.so``; there is no fallback.
@@ -185,6 +186,11 @@ def _rows(t):
     return t
 
 
+def _backward_error(name):
+    return RuntimeError(f"{name} has no backward pass: it is an operator of inference "
+                        "(call it under torch.no_grad(), or detach what requires a gradient)")
+
+
 def _no_backward(name):
     """A function that hands an operator's two results on as they are; a backward pass that reaches them is an error
     instead of a gradient lost."""
@@ -196,10 +202,25 @@ def _no_backward(name):
 
         @staticmethod
         def backward(ctx, *grads):
-            raise RuntimeError(f"{name} has no backward pass: it is an operator of inference "
-                               "(call it under torch.no_grad(), or detach what requires a gradient)")
+            raise _backward_error(name)
 
     return NoBackward.apply
+
+
+def _no_backward_given(name):
+    """The same for one result that the caller has given, and that is written in place."""
+
+    class NoBackwardGiven(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, out, *inputs):
+            ctx.mark_dirty(out)
+            return out
+
+        @staticmethod
+        def backward(ctx, *grads):
+            raise _backward_error(name)
+
+    return NoBackwardGiven.apply
 
 
 def _dual_level():
@@ -219,6 +240,7 @@ def _refuse_derivatives(name, out, *inputs):
 
 
 _attention_result, _read_result = _no_backward("paged_attention"), _no_backward("kv_cache_read")
+_given_attention_result = _no_backward_given("paged_attention")
 
 
 def kv_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, *, query_start=None, k_scale=None, v_scale=None):
@@ -356,8 +378,8 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
     wants_grad = torch.is_grad_enabled() and (
         q.requires_grad or k_cache.requires_grad or v_cache.requires_grad or sinks is not None and sinks.requires_grad or
         k_scale is not None and k_scale.requires_grad or v_scale is not None and v_scale.requires_grad)
-    if own_out or _dual_level() >= 0:
-        _refuse_derivatives("paged_attention", (out,) if own_out else (), *inputs)
+    if _dual_level() >= 0:
+        _refuse_derivatives("paged_attention", (), *inputs, out)
     q = _rows(q)
     if out is None:
         out = q.new_empty((rows, Hq, D))
@@ -376,6 +398,13 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
     sink_at = None if sinks is None else _head_vector(sinks, Hq, "sinks", device)
     lse_at = None if lse is None else lse.data_ptr()
     qs, scale = q.stride(), D ** -0.5 if scale is None else scale
+    if own_out:
+        # (ahead of the launch: what autograd does not let be written in place is an error, and nothing has run)
+        wants_grad = wants_grad or torch.is_grad_enabled() and out.requires_grad
+        if wants_grad:
+            _given_attention_result(out, *inputs)
+        else:
+            increment_version(out)
     if query_start is None:
         size = _bytes("vk_hip_paged_attention_workspace_bytes_ex", kind, B, Hkv, G, D, max_len, window, keep_first,
                       sums is not None)
@@ -399,10 +428,11 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
             _stream(device))
     if status:
         _failed(status, name)
-    if own_out:
-        increment_version(out)
-    elif wants_grad:
-        out, lse = _attention_result(out, lse, *inputs)
+    if wants_grad:
+        if not own_out:
+            out, lse = _attention_result(out, lse, *inputs)
+        elif lse is not None:
+            lse, _ = _attention_result(lse, None, *inputs)
     return (out, lse) if return_lse else out
 
 
