@@ -788,8 +788,8 @@ int vk_hip_paged_attention_ex(const void* q, const void* k_cache, const void* v_
  * may be lost.  Rows that see a value scale outside of 2^-60 .. 2^60 (0 is none) have two bf16 terms a weight as well.  Rows
  * that belong to no sequence, in front of query_start[0] or behind query_start[B], become 0 (lse -inf) with
  * clear_rest != 0 and else stay as they are.
- * The workspace is scratch of this call alone; 0 bytes: none is needed.  Deterministic: no atomics on floating-point
- * data. */
+ * The workspace is scratch of this call alone; 0 bytes: none is needed.  out overlaps no input.  Deterministic: no atomics on
+ * floating-point data. */
 size_t vk_hip_paged_attention_prompt_workspace_bytes(int B, int tokens, int Hkv, int G, int D, int max_len, int window,
                                                      int keep_first);
 int vk_hip_paged_attention_prompt(const void* q, const void* k_cache, const void* v_cache,

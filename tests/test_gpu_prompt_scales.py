@@ -148,3 +148,12 @@ def test_in_a_graph(hip_lib):
         torch.cuda.synchronize()
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
         check(s)
+
+
+def test_results_in_the_queries_place(hip_lib):
+    """Tiles that are worked on again read their queries again."""
+    s = Prompt([700, 600], (200, 150), 2, 4, 64, 16, 16)
+    s.v_scale = s.v_scale * 2.0 ** 80
+    want = s.call()
+    got = s.call(out=s.q)
+    assert got[0] is s.q and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

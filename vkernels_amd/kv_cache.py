@@ -386,6 +386,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, query_start=N
     else:
         _need(out.shape == q.shape and out.dtype is q.dtype and out.is_contiguous() and out.get_device() == device,
               "out must be contiguous and like q")
+        # (tiles whose scales are far from 1 read their queries a second time, behind the first results)
+        if query_start is not None and kind >= 2 and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+            q = q.clone()
     lse = q.new_empty((rows, Hq), dtype=torch.float32) if return_lse else None
     sums, sums_b, sums_h = None, 0, 0
     if weight_sums is not None:
