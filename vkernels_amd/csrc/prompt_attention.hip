@@ -217,7 +217,8 @@ __device__ __forceinline__ void follow(float top, float& m, float& l, f32x16 (&a
 // tiles of keys are 32 positions on from those of values, and both are done with when a tile ends.
 // 4096 tokens over 16384 positions, 32 heads on 8 of 128: 1.02 ms, 945 TFLOP/s (a bf16 product of 8192^3 reaches 1379);
 // heads of 64: 1.19 ms for as many products, 810.  Matrix instructions take 45 % of the cycles, vector ones 53 %; without
-// the loads it is 0.89 ms, without the exponentials 1.05.  Keys and values through registers, no scores ahead: 1.21;
+// the loads it is 0.89 ms, without the exponentials 1.05: these are hidden, loads are an eighth, and what keeps the
+// rest above the products' 0.70 is not known.  Keys and values through registers, no scores ahead: 1.21;
 // scores ahead in the compiler's own order: 1.24 (every read from LDS waited for), 1.08 by its scheduling groups.
 // Two chains of scores, reads 2 or 5 operands ahead, and priorities for either half change nothing or cost 2 %.
 template <class M, bool FP8, int DP>

@@ -35,8 +35,9 @@ class DecodeLayer:
     ``w_router`` [hidden, experts] are bf16.  With a ``budget`` a sequence whose cache has grown to
     ``budget + slack`` positions is cut back to ``budget``: its first ``keep_first``, its latest
     ``keep_last`` and those that have been given the most weight (position encodings go into the keys
-    before they are stored).  ``pages`` bounds the cache; pages that an eviction empties serve other
-    sequences.
+    before they are stored).  Decode steps alone count weight: an eviction ranks a prompt's positions by what the
+    steps behind it have given them, and not by what the prompt's own tokens have.  ``pages`` bounds the cache; pages
+    that an eviction empties serve other sequences.
 
     ``rotary`` are the arguments of qk_norm_rope besides queries, keys and positions (``inv_freq`` and what else a
     model has): every token is turned by the number of its sequence's tokens in front of it, on all axes alike.
